@@ -19,6 +19,21 @@ LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), LIB_NAME)
 EN_F32, EN_F16, EN_BF16 = 0, 1, 2
 _DTYPE_TAG = {torch.float32: EN_F32, torch.float16: EN_F16, torch.bfloat16: EN_BF16}
 
+
+class NormRotary(ctypes.Structure):
+    """``en_norm_rotary``"""
+    _fields_ = [("cos", c_void_p), ("sin", c_void_p), ("q_weight", c_void_p), ("k_weight", c_void_p), ("table_rows", c_int),
+                ("rotary_dim", c_int), ("interleaved", c_int), ("eps", c_float)]
+
+
+class Kv8Cache(ctypes.Structure):
+    """``en_kv8_cache``"""
+    _fields_ = [("k_pages", c_void_p), ("v_pages", c_void_p), ("k_scales", c_void_p), ("v_scales", c_void_p), ("k_tail", c_void_p),
+                ("v_tail", c_void_p), ("page_table", c_void_p), ("code_strides", c_int64 * 4), ("scale_strides", c_int64 * 4),
+                ("num_pages", c_int), ("page_size", c_int), ("max_pages_per_seq", c_int), ("batch", c_int), ("head_num", c_int),
+                ("size_per_head", c_int), ("code", c_int), ("dtype", c_int)]
+
+
 # name -> (restype, argtypes); must list every symbol the header declares
 SIGNATURES = {
     "en_version": (c_int, []),
@@ -79,6 +94,13 @@ SIGNATURES = {
                                          [c_int] * 5 + [c_void_p]),
     "en_block_decode_workspace_bytes": (c_int64, [c_int] * 3 + [c_int64, c_int]),
     "en_block_decode": (c_int, [c_void_p] * 2),
+    "en_qk_norm_rotary": (c_int, [c_void_p] * 6 + [c_int, c_int64] + [c_int] * 3 + [c_void_p, c_void_p, c_int, c_void_p]),
+    "en_kv_append_paged_rotary": (c_int, [c_void_p] * 8 + [c_int] * 7 + [c_void_p] * 3 + [c_int, c_void_p, c_void_p]),
+    "en_kv8_fill": (c_int, [c_void_p] * 4 + [c_int64, c_int] + [c_void_p] * 3),
+    "en_kv8_append": (c_int, [c_void_p] * 6 + [c_int] + [c_void_p] * 4),
+    "en_kv8_read": (c_int, [c_void_p] * 3 + [c_int] + [c_void_p] * 3),
+    "en_decode_attn_kv8_workspace_bytes": (c_int64, [c_int] * 5),
+    "en_decode_attn_kv8": (c_int, [c_void_p] * 4 + [c_int, c_float, c_void_p, c_int64, c_void_p]),
     "en_copy_bytes": (c_int, [c_void_p, c_void_p, c_int64, c_void_p]),
     "en_stream_yardstick": (c_int, [c_void_p, c_void_p, c_int64, c_int, c_int, c_void_p]),
     "en_prefix_yardstick": (c_int, [c_void_p, c_void_p, c_void_p] + [c_int] * 7 + [c_void_p]),

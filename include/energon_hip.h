@@ -445,6 +445,77 @@ typedef struct en_block_decode_args {
 int64_t en_block_decode_workspace_bytes(int batch, int head_num, int size_per_head, int64_t mlp_width, int cache_len);
 int en_block_decode(const en_block_decode_args *args, en_stream_t stream);
 
+/* ---- rotary positions, norms of heads, and a K/V cache in 8 bits -------------------------------------------
+ * No counterpart in the reference, whose models learn their positions and keep K and V as they were projected. */
+
+/* What a head's row goes through on its way, in fp32 and rounded once: y = x * rsqrt(mean(x^2) + eps) * weight where there is a
+ * weight ([size_per_head], of the rows' dtype), then the rotation of the first rotary_dim channels by the row's position,
+ * (a, b) -> (a cos - b sin, b cos + a sin) with a, b = channels i and i + rotary_dim / 2 (interleaved: 2i and 2i + 1).
+ * cos, sin: [table_rows, rotary_dim / 2] fp32, or NULL with rotary_dim 0.  A position outside the table makes the rotated
+ * channels of its row NaN. */
+typedef struct en_norm_rotary {
+  const float *cos, *sin;
+  const void *q_weight, *k_weight;       /* each may be NULL */
+  int32_t table_rows, rotary_dim, interleaved;
+  float eps;
+} en_norm_rotary;
+
+/* Queries and keys of packed tokens, [tokens, heads, size_per_head] each, into q_out and k_out (which may be q and k).  strides:
+ * (token, head) in elements of q, k, q_out, k_out.  A token's position is its place in its sequence (cu_seqlens
+ * [batch + 1]), or positions[token] where that is given (cu_seqlens may then be NULL); tokens behind the last sequence are left
+ * out.  k may be NULL with k_heads 0.  size_per_head at most 256. */
+int en_qk_norm_rotary(const void *q, const void *k, void *q_out, void *k_out, const int32_t *cu_seqlens, const int32_t *positions,
+                      int batch, int64_t tokens, int q_heads, int k_heads, int size_per_head, const int64_t *strides,
+                      const en_norm_rotary *how, int dtype, en_stream_t stream);
+
+/* en_kv_append_paged with that on the way: q [batch, q_heads, size_per_head] into q_out (contiguous), k_new into its page, both as of
+ * position kv_lens[b]; v_new is copied.  strides: (sequence, head) in elements of q, k_new, v_new; pool_strides as there. */
+int en_kv_append_paged_rotary(const void *q, const void *k_new, const void *v_new, void *q_out, void *k_pool, void *v_pool,
+                              const int32_t *kv_lens, const int32_t *page_table, int batch, int q_heads, int k_heads,
+                              int max_pages_per_seq, int page_size, int num_pages, int size_per_head, const int64_t *strides,
+                              const int64_t *pool_strides, const en_norm_rotary *how, int dtype, int32_t *overflow,
+                              en_stream_t stream);
+
+/* A K/V cache in 8 bits.  The positions of a sequence are taken in blocks of EN_KV8_BLOCK.  A full block lies in a page
+ * (page_table[b, position / page_size], page_size a power of two, at least EN_KV8_BLOCK): its keys as codes k_pages[page, head, position,
+ * channel], its values as codes v_pages[page, head, block, channel, position in the block], with one fp32 scale for the block and
+ * head of each.  The positions behind the last full block stay in 16 bits in k_tail [batch, head, EN_KV8_BLOCK, channel] and v_tail
+ * [batch, head, channel, EN_KV8_BLOCK].  A block is quantized once, when it is full: with a its largest magnitude and M the
+ * largest code (127; 448), scale = a / M and code = round(x * (M / a)) in fp32, to nearest even; scale and codes are 0 where
+ * a < 2^-100, and the scale is NaN where a value is not finite.  A page id outside the pool reads as zeros and is not written. */
+#define EN_KV8_BLOCK 16
+enum en_kv8_code { EN_KV8_INT8 = 0, EN_KV8_E4M3 = 1 };
+typedef struct en_kv8_cache {
+  void *k_pages, *v_pages;               /* 16-byte aligned */
+  float *k_scales, *v_scales;
+  void *k_tail, *v_tail;                 /* contiguous, 16-byte aligned */
+  const int32_t *page_table;             /* [batch, max_pages_per_seq] */
+  int64_t code_strides[4];               /* bytes: k page, k head, v page, v head; multiples of 16, page strides below 2^32 */
+  int64_t scale_strides[4];              /* elements, the same order; below 2^32 */
+  int32_t num_pages, page_size, max_pages_per_seq, batch, head_num, size_per_head;   /* head size a multiple of 16, at most 128 */
+  int32_t code, dtype;                   /* en_kv8_code; EN_F16 or EN_BF16 of the tails and of what is written and read */
+} en_kv8_cache;
+
+/* Prompts: rows cu_seqlens[b] + p of k and v ([tokens, head_num, size_per_head] by strides (token, head) of k, of v) become the positions
+ * p < min(length, max_seq_len) of sequence b; rows from `tokens` on are not read.  overflow, if given, counts positions that had no page. */
+int en_kv8_fill(const void *k, const void *v, const en_kv8_cache *cache, const int32_t *cu_seqlens, int64_t tokens, int max_seq_len,
+                const int64_t *strides, int32_t *overflow, en_stream_t stream);
+/* A decode step: en_kv_append_paged_rotary into this cache.  q may be NULL with q_heads 0.  A sequence whose position kv_lens[b] has no
+ * page keeps its cache, loses the new row and is counted in overflow. */
+int en_kv8_append(const void *q, const void *k_new, const void *v_new, void *q_out, const en_kv8_cache *cache,
+                  const int32_t *kv_lens, int q_heads, const int64_t *strides, const en_norm_rotary *how, int32_t *overflow,
+                  en_stream_t stream);
+/* Positions first[b] + s (first NULL: s), s < seq_len, of every sequence back in 16 bits: k_out, v_out [batch, head_num, seq_len,
+ * size_per_head]; zeros from kv_lens[b] on. */
+int en_kv8_read(const en_kv8_cache *cache, const int32_t *kv_lens, const int32_t *first, int seq_len, void *k_out, void *v_out,
+                en_stream_t stream);
+/* Decode attention: ctx[b, h] = softmax(scale * <q[b, h], K>) V over the kv_lens[b] cached positions of key head h / (q_heads /
+ * head_num); zeros for an empty sequence.  q, ctx: contiguous [batch, q_heads, size_per_head].  workspace:
+ * en_decode_attn_kv8_workspace_bytes, 16-byte aligned; its contents need not be kept or cleared. */
+int64_t en_decode_attn_kv8_workspace_bytes(int batch, int q_heads, int head_num, int capacity, int size_per_head);
+int en_decode_attn_kv8(const void *q, void *ctx, const en_kv8_cache *cache, const int32_t *kv_lens, int q_heads, float scale,
+                       void *workspace, int64_t workspace_bytes, en_stream_t stream);
+
 /* ---- measurement helper ------------------------------------------------- */
 
 /* The whole step in one call: depad, transpose_pad, QK^T, scale_mask_softmax, PV,
