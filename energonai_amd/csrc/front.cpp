@@ -583,6 +583,239 @@ bool fits_int(std::initializer_list<int64_t> values) {
   return true;
 }
 
+// en_norm_rotary of (cos, sin) or None, two gains or None, eps and the pairing, for rows of D channels like `x`.
+bool norm_rotary(PyObject *rotary, PyObject *q_weight, PyObject *k_weight, PyObject *eps, PyObject *interleaved, const Tensor &x, int64_t D,
+                 en_norm_rotary &out) {
+  int il;
+  out = en_norm_rotary{};
+  if (!number(eps, out.eps) || !flag(interleaved, il)) return false;
+  out.interleaved = il;
+  if (rotary != Py_None) {
+    if (!PyTuple_CheckExact(rotary) || PyTuple_GET_SIZE(rotary) != 2) return false;
+    const Tensor *c = plain_contiguous(PyTuple_GET_ITEM(rotary, 0)), *s = plain_contiguous(PyTuple_GET_ITEM(rotary, 1));
+    if (!c || !s || c->dim() != 2 || c->sizes() != s->sizes() || c->scalar_type() != at::kFloat || s->scalar_type() != at::kFloat ||
+        c->device() != x.device() || s->device() != x.device() || 2 * c->size(1) > D || !fits_int({c->size(0)}))
+      return false;
+    out.cos = c->data_ptr<float>();
+    out.sin = s->data_ptr<float>();
+    out.table_rows = (int32_t)c->size(0);
+    out.rotary_dim = (int32_t)(2 * c->size(1));
+  }
+  auto gain = [&](PyObject *o, const void *&p) {
+    if (o == Py_None) return true;
+    const Tensor *w = plain_contiguous(o);
+    if (!w || w->numel() != D || w->scalar_type() != x.scalar_type() || w->device() != x.device()) return false;
+    p = w->data_ptr();
+    return true;
+  };
+  return gain(q_weight, out.q_weight) && gain(k_weight, out.k_weight);
+}
+
+// qk_norm_rotary(q, k, batch, SeqInfo, rotary, q_weight, k_weight, eps, interleaved) -> (q, k) or None
+PyObject *qk_norm_rotary(PyObject *const *a) {
+  const Tensor *q = plain_rows(a[0], 3), *k = plain_rows(a[1], 3);
+  int64_t batch;
+  if (!q || !k || modes_on() || !whole(a[2], batch) || batch < 1) Py_RETURN_NONE;
+  const int64_t T = q->size(0), Hq = q->size(1), Hk = k->size(1), D = q->size(2);
+  const int tag = known_tag(*q);
+  en_norm_rotary how;
+  Lens info;
+  if (tag < 0 || k->size(0) != T || k->size(2) != D || k->scalar_type() != q->scalar_type() || k->device() != q->device() ||
+      !fits_int({Hq, Hk, D, batch}) || !lens_of(a[3], *q, batch, true, info) || !norm_rotary(a[4], a[5], a[6], a[7], a[8], *q, D, how))
+    Py_RETURN_NONE;
+  const c10::DeviceGuard guard(q->device());
+  order_stream(a[3], *q);
+  const Tensor q_out = at::empty(q->sizes(), q->options()), k_out = at::empty(k->sizes(), k->options());
+  const int64_t strides[8] = {q->stride(0), q->stride(1), k->stride(0), k->stride(1), Hq * D, D, Hk * D, D};
+  const void *q_p = q->data_ptr(), *k_p = k->data_ptr();
+  void *qo_p = q_out.data_ptr(), *ko_p = k_out.data_ptr();
+  const int32_t *cu = i32(*info.cu);
+  const hipStream_t stream = stream_of(*q);
+  check(without_gil([&] {
+          return en_qk_norm_rotary(q_p, k_p, qo_p, ko_p, cu, nullptr, (int)batch, T, (int)Hq, (int)Hk, (int)D, strides, &how, tag, stream);
+        }), "qk_norm_rotary");
+  return tuple({q_out, k_out});
+}
+
+// The rows of a decode step: [B, H, D] of k_new and v_new, [B, Hq, D] of q, of one type on one device.
+bool step_rows(const Tensor *q, const Tensor *k, const Tensor *v, int64_t B, int64_t H, int64_t D, at::ScalarType type, const Tensor &home,
+               int64_t (&strides)[6]) {
+  if (!q || !k || !v) return false;
+  const int64_t rows[3] = {B, H, D};
+  if (k->sizes() != c10::IntArrayRef(rows) || v->sizes() != c10::IntArrayRef(rows) || q->size(0) != B || q->size(2) != D) return false;
+  int i = 0;
+  for (const Tensor *t : {q, k, v}) {
+    if (t->scalar_type() != type || t->device() != home.device()) return false;
+    strides[i++] = t->stride(0);
+    strides[i++] = t->stride(1);
+  }
+  return true;
+}
+bool counter(PyObject *o, const Tensor &home, int32_t *&p) {
+  p = nullptr;
+  if (o == Py_None) return true;
+  const Tensor *t = plain_contiguous(o);
+  if (!t || t->scalar_type() != at::kInt || t->device() != home.device()) return false;
+  p = t->data_ptr<int32_t>();
+  return true;
+}
+
+// kv_pages_append_rotary(q, k_new, v_new, k_pool, v_pool, SeqInfo, page_table, rotary, q_weight, k_weight, eps, interleaved, overflow) -> q or None
+PyObject *kv_pages_append_rotary(PyObject *const *a) {
+  const Tensor *q = plain_rows(a[0], 3), *kn = plain_rows(a[1], 3), *vn = plain_rows(a[2], 3), *kp = plain_rows(a[3], 4), *vp = plain_rows(a[4], 4);
+  if (!q || !kp || !vp || modes_on()) Py_RETURN_NONE;
+  const int64_t N = kp->size(0), H = kp->size(1), P = kp->size(2), D = kp->size(3), B = q->size(0), Hq = q->size(1);
+  const int tag = known_tag(*kp);
+  int64_t strides[6];
+  int32_t *over;
+  en_norm_rotary how;
+  Lens info;
+  if (tag < 0 || vp->sizes() != kp->sizes() || vp->strides() != kp->strides() || vp->scalar_type() != kp->scalar_type() || vp->device() != kp->device() ||
+      !fits_int({N, H, P, D, B, Hq}) || !step_rows(q, kn, vn, B, H, D, kp->scalar_type(), *kp, strides) || !lens_of(a[5], *kp, B, false, info) ||
+      !norm_rotary(a[7], a[8], a[9], a[10], a[11], *q, D, how) || !counter(a[12], *kp, over))
+    Py_RETURN_NONE;
+  const Tensor *table = page_table(a[6], *kp, B);
+  if (!table) Py_RETURN_NONE;
+  const c10::DeviceGuard guard(kp->device());
+  order_stream(a[5], *kp);
+  const Tensor out = at::empty(q->sizes(), q->options());
+  const int64_t pool[3] = {kp->stride(0), kp->stride(1), kp->stride(2)}, pages = table->size(1);
+  const void *q_p = q->data_ptr(), *kn_p = kn->data_ptr(), *vn_p = vn->data_ptr();
+  void *out_p = out.data_ptr(), *kp_p = kp->data_ptr(), *vp_p = vp->data_ptr();
+  const int32_t *lens_p = i32(*info.lens), *table_p = i32(*table);
+  const hipStream_t stream = stream_of(*kp);
+  check(without_gil([&] {
+          return en_kv_append_paged_rotary(q_p, kn_p, vn_p, out_p, kp_p, vp_p, lens_p, table_p, (int)B, (int)Hq, (int)H, (int)pages, (int)P, (int)N,
+                                           (int)D, strides, pool, &how, tag, over, stream);
+        }), "kv_pages_append_rotary");
+  return THPVariable_Wrap(out);
+}
+
+// en_kv8_cache of the seven tensors of a cache; `home`: one of them.
+bool kv8_cache(PyObject *o, en_kv8_cache &c, const Tensor *&home) {
+  if ((!PyTuple_Check(o) && !PyList_CheckExact(o)) || PySequence_Fast_GET_SIZE(o) != 7) return false;
+  const Tensor *t[7];
+  for (int i = 0; i < 7; ++i) {
+    t[i] = i < 4 ? plain(PySequence_Fast_GET_ITEM(o, i)) : plain_contiguous(PySequence_Fast_GET_ITEM(o, i));
+    if (!t[i] || t[i]->device() != t[0]->device()) return false;
+  }
+  const Tensor &kp = *t[0], &vp = *t[1], &ks = *t[2], &vs = *t[3], &kt = *t[4], &vt = *t[5], &table = *t[6];
+  const at::ScalarType code = kp.scalar_type(), type = kt.scalar_type();
+  if ((code != at::kChar && code != at::kFloat8_e4m3fn) || vp.scalar_type() != code || (type != at::kHalf && type != at::kBFloat16) ||
+      vt.scalar_type() != type || ks.scalar_type() != at::kFloat || vs.scalar_type() != at::kFloat || table.scalar_type() != at::kInt ||
+      kp.dim() != 4 || table.dim() != 2)
+    return false;
+  constexpr int64_t blk = EN_KV8_BLOCK;
+  const int64_t N = kp.size(0), H = kp.size(1), P = kp.size(2), D = kp.size(3), B = table.size(0), blocks = P / blk;
+  const int64_t v_shape[5] = {N, H, blocks, D, blk}, s_shape[3] = {N, H, blocks}, kt_shape[4] = {B, H, blk, D}, vt_shape[4] = {B, H, D, blk};
+  if (P % blk || vp.sizes() != c10::IntArrayRef(v_shape) || ks.sizes() != c10::IntArrayRef(s_shape) || vs.sizes() != c10::IntArrayRef(s_shape) ||
+      kt.sizes() != c10::IntArrayRef(kt_shape) || vt.sizes() != c10::IntArrayRef(vt_shape) || kp.stride(3) != 1 || kp.stride(2) != D ||
+      vp.stride(4) != 1 || vp.stride(3) != blk || vp.stride(2) != D * blk || (blocks > 1 && (ks.stride(2) != 1 || vs.stride(2) != 1)) ||
+      !fits_int({N, H, P, D, B, table.size(1)}))
+    return false;
+  c = en_kv8_cache{kp.data_ptr(), vp.data_ptr(), ks.data_ptr<float>(), vs.data_ptr<float>(), kt.data_ptr(), vt.data_ptr(), i32(table),
+                   {kp.stride(0), kp.stride(1), vp.stride(0), vp.stride(1)}, {ks.stride(0), ks.stride(1), vs.stride(0), vs.stride(1)},
+                   (int32_t)N, (int32_t)P, (int32_t)table.size(1), (int32_t)B, (int32_t)H, (int32_t)D,
+                   code == at::kChar ? EN_KV8_INT8 : EN_KV8_E4M3, type == at::kHalf ? EN_F16 : EN_BF16};
+  home = t[4];
+  return true;
+}
+
+// kv8_pages_fill(k_src, v_src, cache, batch, max_seq_len, SeqInfo, overflow) -> True or None
+PyObject *kv8_pages_fill(PyObject *const *a) {
+  const Tensor *k = plain_rows(a[0], 3), *v = plain_rows(a[1], 3), *home;
+  en_kv8_cache c;
+  int64_t batch, S;
+  int32_t *over;
+  Lens info;
+  if (!k || !v || modes_on() || !kv8_cache(a[2], c, home) || !whole(a[3], batch) || batch != c.batch || !whole(a[4], S) || !fits_int({S}) ||
+      !lens_of(a[5], *home, batch, true, info) || !counter(a[6], *home, over))
+    Py_RETURN_NONE;
+  for (const Tensor *t : {k, v})
+    if (t->size(0) != k->size(0) || t->size(1) != c.head_num || t->size(2) != c.size_per_head || t->scalar_type() != home->scalar_type() || t->device() != home->device())
+      Py_RETURN_NONE;
+  const c10::DeviceGuard guard(home->device());
+  order_stream(a[5], *home);
+  const int64_t strides[4] = {k->stride(0), k->stride(1), v->stride(0), v->stride(1)}, tokens = k->size(0);
+  const void *k_p = k->data_ptr(), *v_p = v->data_ptr();
+  const int32_t *cu = i32(*info.cu);
+  const hipStream_t stream = stream_of(*home);
+  check(without_gil([&] { return en_kv8_fill(k_p, v_p, &c, cu, tokens, (int)S, strides, over, stream); }), "kv8_pages_fill");
+  Py_RETURN_TRUE;
+}
+
+// kv8_pages_append(q, k_new, v_new, cache, SeqInfo, rotary, q_weight, k_weight, eps, interleaved, overflow) -> q or None
+PyObject *kv8_pages_append(PyObject *const *a) {
+  const Tensor *q = plain_rows(a[0], 3), *kn = plain_rows(a[1], 3), *vn = plain_rows(a[2], 3), *home;
+  en_kv8_cache c;
+  int64_t strides[6];
+  int32_t *over;
+  en_norm_rotary how;
+  Lens info;
+  if (!q || modes_on() || !kv8_cache(a[3], c, home) || !fits_int({q->size(1)}) ||
+      !step_rows(q, kn, vn, c.batch, c.head_num, c.size_per_head, home->scalar_type(), *home, strides) || !lens_of(a[4], *home, c.batch, false, info) ||
+      !norm_rotary(a[5], a[6], a[7], a[8], a[9], *q, c.size_per_head, how) || !counter(a[10], *home, over))
+    Py_RETURN_NONE;
+  const c10::DeviceGuard guard(home->device());
+  order_stream(a[4], *home);
+  const Tensor out = at::empty(q->sizes(), q->options());
+  const void *q_p = q->data_ptr(), *kn_p = kn->data_ptr(), *vn_p = vn->data_ptr();
+  void *out_p = out.data_ptr();
+  const int32_t *lens_p = i32(*info.lens);
+  const int Hq = (int)q->size(1);
+  const hipStream_t stream = stream_of(*home);
+  check(without_gil([&] { return en_kv8_append(q_p, kn_p, vn_p, out_p, &c, lens_p, Hq, strides, &how, over, stream); }), "kv8_pages_append");
+  return THPVariable_Wrap(out);
+}
+
+// kv8_pages_read(cache, SeqInfo, max_seq_len, first or None) -> (k, v) or None
+PyObject *kv8_pages_read(PyObject *const *a) {
+  const Tensor *home, *first = nullptr;
+  en_kv8_cache c;
+  int64_t S;
+  Lens info;
+  if (modes_on() || !kv8_cache(a[0], c, home) || !lens_of(a[1], *home, c.batch, false, info) || !whole(a[2], S) || !fits_int({S})) Py_RETURN_NONE;
+  if (a[3] != Py_None) {
+    first = plain_contiguous(a[3]);
+    if (!first || first->numel() != c.batch || first->scalar_type() != at::kInt || first->device() != home->device()) Py_RETURN_NONE;
+  }
+  const c10::DeviceGuard guard(home->device());
+  order_stream(a[1], *home);
+  const int64_t shape[4] = {c.batch, c.head_num, S, c.size_per_head};
+  const Tensor k = at::empty(shape, home->options()), v = at::empty(shape, home->options());
+  void *k_p = k.data_ptr(), *v_p = v.data_ptr();
+  const int32_t *lens_p = i32(*info.lens), *first_p = first ? i32(*first) : nullptr;
+  const hipStream_t stream = stream_of(*home);
+  check(without_gil([&] { return en_kv8_read(&c, lens_p, first_p, (int)S, k_p, v_p, stream); }), "kv8_pages_read");
+  return tuple({k, v});
+}
+
+// decode_attn_kv8(q, cache, SeqInfo, scale or None) -> ctx or None
+PyObject *decode_attn_kv8(PyObject *const *a) {
+  const Tensor *q = plain_contiguous(a[0]), *home;
+  en_kv8_cache c;
+  Lens info;
+  if (!q || modes_on() || !kv8_cache(a[1], c, home) || !lens_of(a[2], *home, c.batch, false, info)) Py_RETURN_NONE;
+  const int64_t B = c.batch, D = c.size_per_head, Hq = q->dim() >= 3 ? q->size(1) : 0;
+  float scale = (float)std::pow((double)D, -0.5);
+  if (q->dim() < 3 || q->size(0) != B || q->size(-1) != D || q->numel() != B * Hq * D || Hq < c.head_num || Hq % c.head_num || !fits_int({Hq}) ||
+      q->scalar_type() != home->scalar_type() || q->device() != home->device() || reinterpret_cast<uintptr_t>(q->data_ptr()) % 16 ||
+      (a[3] != Py_None && !number(a[3], scale)) || !fits_int({(int64_t)c.max_pages_per_seq * c.page_size}))
+    Py_RETURN_NONE;
+  const c10::DeviceGuard guard(q->device());
+  order_stream(a[2], *q);
+  const int64_t need = en_decode_attn_kv8_workspace_bytes((int)B, (int)Hq, c.head_num, c.max_pages_per_seq * c.page_size, (int)D);
+  const Tensor out = at::empty({B, Hq, 1, D}, q->options());
+  Tensor ws;
+  if (need > 0) ws = at::empty({need}, q->options().dtype(at::kByte));
+  const void *q_p = q->data_ptr();
+  void *out_p = out.data_ptr(), *ws_p = need > 0 ? ws.data_ptr() : nullptr;
+  const int32_t *lens_p = i32(*info.lens);
+  const hipStream_t stream = stream_of(*q);
+  check(without_gil([&] { return en_decode_attn_kv8(q_p, out_p, &c, lens_p, (int)Hq, scale, ws_p, need, stream); }), "decode_attn_kv8");
+  return THPVariable_Wrap(out);
+}
+
 // depad(src, SeqInfo, batch, left_padded, total) -> packed rows or None
 PyObject *depad(PyObject *const *a) {
   const Tensor *src = plain_contiguous(a[0]);
@@ -1024,6 +1257,12 @@ PyMethodDef kMethods[] = {
     EN_FAST(layer_norm, 6, "layer_norm_forward of plain operands, or None"),
     EN_FAST(kv_pages_append, 7, "kv_pages_append of plain operands, or None"),
     EN_FAST(decode_attn_paged, 6, "decode_attn_paged of plain operands, or None"),
+    EN_FAST(qk_norm_rotary, 9, "qk_norm_rotary of plain operands, or None"),
+    EN_FAST(kv_pages_append_rotary, 13, "kv_pages_append_rotary of plain operands, or None"),
+    EN_FAST(kv8_pages_fill, 7, "kv8_pages_fill of plain operands, or None"),
+    EN_FAST(kv8_pages_append, 11, "kv8_pages_append of plain operands, or None"),
+    EN_FAST(kv8_pages_read, 4, "kv8_pages_read of plain operands, or None"),
+    EN_FAST(decode_attn_kv8, 4, "decode_attn_kv8 of plain operands, or None"),
     EN_FAST(depad, 5, "depad of plain operands, or None"),
     EN_FAST(transpose_pad, 6, "transpose_pad of plain operands, or None"),
     EN_FAST(transpose_depad, 7, "transpose_depad of plain operands, or None"),

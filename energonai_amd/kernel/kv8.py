@@ -18,7 +18,7 @@ from typing import NamedTuple, Optional
 import torch
 
 from .. import _lib
-from ..seqinfo import seq_info
+from ..seqinfo import SeqInfo, seq_info
 from .attention import _overflow
 from .rotary import _new_rows, _rows, norm_rotary
 
@@ -99,6 +99,8 @@ def kv8_pages_fill(k_src, v_src, cache, batch_size: int, max_seq_len: int, seq_l
     ``s < min(len[b], max_seq_len)`` of sequence ``b``: full blocks into the pages that ``page_table`` names, the rest into the tails.  Positions whose
     page id lies outside the pool are not written and counted in ``overflow``."""
     who = "kv8_pages_fill"
+    if type(seq_len_list) is SeqInfo and _lib.front.kv8_pages_fill(k_src, v_src, cache, batch_size, max_seq_len, seq_len_list, overflow):
+        return
     c = _cache(cache, who)
     kt, device = cache[4], cache[4].device
     for t, n in ((k_src, "k_src"), (v_src, "v_src")):
@@ -126,6 +128,10 @@ def kv8_pages_append(q, k_new, v_new, cache, kv_len_list, rotary=None, *, q_weig
     complete into its page.  Returns the normed, rotated queries (``q`` may be ``None``: then nothing).  The caller advances the lengths
     afterwards.  A sequence whose position has no page keeps its cache, loses the new rows and is counted in ``overflow``."""
     who = "kv8_pages_append"
+    if q is not None and type(kv_len_list) is SeqInfo:
+        turned = _lib.front.kv8_pages_append(q, k_new, v_new, cache, kv_len_list, rotary, q_weight, k_weight, eps, interleaved, overflow)
+        if turned is not None:
+            return turned
     c = _cache(cache, who)
     kt, device = cache[4], cache[4].device
     Hq, qs = _new_rows(who, q, k_new, v_new, c.batch, c.head_num, c.size_per_head, kt.dtype, device)
@@ -148,6 +154,10 @@ def kv8_pages_read(cache, kv_len_list, max_seq_len: int, *, first: Optional[torc
     ``kv_len[b]`` on: what a prompt that goes on from a cached one attends to, or what a swapped-out sequence keeps.  ``first`` is int32 ``[B]``
     (``None``: 0)."""
     who = "kv8_pages_read"
+    if out is None and type(kv_len_list) is SeqInfo:
+        pair = _lib.front.kv8_pages_read(cache, kv_len_list, max_seq_len, first)
+        if pair is not None:
+            return pair
     c = _cache(cache, who)
     kt, device = cache[4], cache[4].device
     info = _lens(who, kv_len_list, c.batch, device)
@@ -183,6 +193,10 @@ def decode_attn_kv8(q, cache, kv_len_list, *, scale: Optional[float] = None, out
     neighbouring query heads sharing a key head; ``[B,Hq,1,D]``, zeros for an empty sequence.  ``scale`` defaults to
     ``size_per_head ** -0.5``.  ``workspace``: any tensor of ``decode_attn_kv8_workspace_bytes`` bytes (``None``: a temporary)."""
     who = "decode_attn_kv8"
+    if out is None and workspace is None and type(kv_len_list) is SeqInfo:
+        ctx = _lib.front.decode_attn_kv8(q, cache, kv_len_list, scale)
+        if ctx is not None:
+            return ctx
     c = _cache(cache, who)
     device = cache[4].device
     _lib.require_gpu(q, "q", contiguous=False)

@@ -16,7 +16,7 @@ from typing import Optional, Tuple
 import torch
 
 from .. import _lib
-from ..seqinfo import seq_info
+from ..seqinfo import SeqInfo, seq_info
 from .attention import _overflow, _page_table, _pool
 
 
@@ -69,6 +69,10 @@ def qk_norm_rotary(q, k, batch_size: int, seq_len_list, rotary=None, *, q_weight
     channels NaN.  Rows behind the last sequence are left as they are (with ``positions`` every row is a token).  Returns new ``(q, k)``,
     or writes into the two tensors ``out`` names, which may be ``q`` and ``k`` themselves.  ``k`` may be ``None``."""
     who = "qk_norm_rotary"
+    if type(seq_len_list) is SeqInfo and out is None and positions is None:
+        pair = _lib.front.qk_norm_rotary(q, k, batch_size, seq_len_list, rotary, q_weight, k_weight, eps, interleaved)
+        if pair is not None:
+            return pair
     _rows(q, "q", who)
     T, Hq, D = q.shape
     tensors = [q]
@@ -132,6 +136,11 @@ def kv_pages_append_rotary(q, k_new, v_new, k_pool, v_pool, kv_len_list, page_ta
     their pages normed and rotated, the values as they are, and the normed, rotated queries ``[B,Hq,D]`` are returned (``Hq`` may
     be any number).  All operands may be strided views of one projection.  A sequence without a page for its next position is handled as there."""
     who = "kv_pages_append_rotary"
+    if type(kv_len_list) is SeqInfo:
+        turned = _lib.front.kv_pages_append_rotary(q, k_new, v_new, k_pool, v_pool, kv_len_list, page_table, rotary, q_weight, k_weight, eps,
+                                                   interleaved, overflow)
+        if turned is not None:
+            return turned
     ps = _pool(k_pool, "k_pool")
     if _pool(v_pool, "v_pool") != ps or k_pool.shape != v_pool.shape or k_pool.dtype != v_pool.dtype or k_pool.device != v_pool.device:
         raise RuntimeError(f"{who}: K and V must share shapes, strides, dtype and device")
