@@ -15,6 +15,8 @@
 // The probabilities are rounded to the cache's 16-bit type for the second product (half a step, 2^-12 or 2^-9, each; the first product's operands
 // are exact), relative to a reference m_o that follows score + log2(value scale), so that their products with the scale neither
 // vanish nor overflow in fp16; the sum of the softmax takes them in fp32 relative to the scores' own maximum m_s.
+#include <type_traits>
+
 #include "kv8_common.hip.h"
 
 namespace en {
@@ -28,9 +30,17 @@ typedef short i16x4 __attribute__((ext_vector_type(4)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int kTile = 4 * kBlk;               // positions of a tile
-constexpr int kWaves = 2048;                  // of the launch: two a SIMD, and what of the registers they leave holds loads in flight
+#ifndef KW
+#define KW 2048
+#endif
+constexpr int kWaves = KW;                  // of the launch: two a SIMD, and what of the registers they leave holds loads in flight
 constexpr int kQueries = 16;                  // columns of a tile: queries that share one pass
 constexpr float kRaise = 8.f;                 // log2
+constexpr int kTeam = 8;                      // waves of a workgroup that takes one unit
+#ifndef TC
+#define TC 1024
+#endif
+constexpr int kTeamCapacity = TC;
 
 template <int DT> struct Mma;
 template <> struct Mma<EN_F16> {
@@ -98,6 +108,13 @@ struct Kv8AttnArgs {
   int rows;                     // min(G, kQueries)
 };
 
+// The length of a sequence that the whole wave asks for, as a scalar load: as a vector load, waiting for it would be waiting for the
+// keys and values that are on their way.
+__device__ __forceinline__ int kv8_wave_len(const Kv8 &c, const int32_t *lens, int b) {
+  typedef const __attribute__((address_space(4))) int32_t *scalar_t;
+  const int n = *(scalar_t)(uintptr_t)(lens + __builtin_amdgcn_readfirstlane(b));
+  return min(max(n, 0), (c.max_pages << c.lg_blocks) * kBlk);
+}
 __device__ __forceinline__ int kv8_tiles(int n) { return max(1, (n / kBlk + 3) / 4); }
 
 // The tiles of all units in a row: per sequence its key heads' (and chunks'), one unit behind the other.
@@ -177,237 +194,395 @@ template <int NT> struct Kv8State {
   __device__ __forceinline__ float ratio() const { return m_s > -INFINITY ? __builtin_amdgcn_exp2f(m_s - m_o) : 0.f; }
 };
 
-template <int DT, int CODE, int NT>
-__global__ __launch_bounds__(kBlock, 2) void decode_attn_kv8_kernel(Kv8AttnArgs a) {
+// What a partial result of maximum m and sum l is multiplied by where the largest maximum is `top`: 0 for one without positions, and for one
+// whose sum is NaN a number, so that it stays.
+__device__ __forceinline__ float share_weight(float m, float l, float top) {
+  return m > -INFINITY ? __builtin_amdgcn_exp2f(m - top) : l == 0.f ? 0.f : 1.f;
+}
+// Four channels of a row of sum l; zeros where there was no position.
+template <int DT> __device__ __forceinline__ void write_row(typename Elem<DT>::T *out, float l, const f32x4 &o) {
+  typedef Elem<DT> E;
+  const float by = l > 0.f ? 1.f / l : l;
+  Pack<typename E::T, 4> y;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) y.v[e] = E::from_float(l == 0.f ? 0.f : o[e] * by);
+  store_pack<typename E::T, 4>(out, y);
+}
+
+// A place in the row of all tiles: sequence, unit of it (key head and run of queries), tile.
+struct Kv8At {
+  int b, n, tiles, tile;
+  int h, chunk;
+};
+
+// The keys of four rows (4t .. 4t + 3 of each of four blocks) a lane as the first product wants them: 16 channels of row l % 16, run c of 64.
+// Rows of 128 codes are whole cache lines, and 16 lanes x 4 of 16 bytes take half of each of 16: both halves of eight rows in one
+// load instead (lanes 8.. of 16 take the other half of rows 0..7, and the first half of rows 8..15 in the second load), and the
+// halves back in place by a rotation in the registers.  (Bytes as they lie: the 1031 MB of 128 sequences 190 us, so 179.)
+__device__ __forceinline__ uint32_t eight_away(uint32_t v) { return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x128, 0xF, 0xF, true); }
+__device__ __forceinline__ void halves_in_place(uint4 &x, uint4 &y, bool low) {
+  const uint4 a = x, b = y;
+  x = make_uint4(low ? a.x : b.x, low ? a.y : b.y, low ? a.z : b.z, low ? a.w : b.w);
+  y = make_uint4(eight_away(low ? b.x : a.x), eight_away(low ? b.y : a.y), eight_away(low ? b.z : a.z), eight_away(low ? b.w : a.w));
+}
+
+// Runs of 16 channels of which a team's results go through LDS at once: all, or four where they would be more than 64 KB.
+__host__ __device__ constexpr int kv8_team_tiles(int rows, int nt) { return rows > 8 && nt > 4 ? 4 : nt; }
+
+// TEAM 1: every wave by itself, a run of plan.quota tiles.  TEAM 8: the waves of a workgroup take the tiles of one unit in turn and
+// put their results together in LDS.
+template <int DT, int CODE, int NT, int TEAM>
+__global__ __launch_bounds__(TEAM == 1 ? kBlock : TEAM * kWave, 2) void decode_attn_kv8_kernel(Kv8AttnArgs a) {
   typedef Elem<DT> E;
   typedef typename E::T T;
   typedef Mma<DT> M;
   constexpr int D = NT * 16, NC = (D + 63) / 64;            // runs of 64 channels: 16 a lane
+  constexpr bool kWholeLines = D == 128;
   const int lane = threadIdx.x % kWave, col = lane % 16, g = lane / 16;
-  const uint32_t wave = __builtin_amdgcn_readfirstlane(blockIdx.x * (kBlock / kWave) + threadIdx.x / kWave);
-  const Kv8Plan plan = kv8_plan(a, lane);
-  const uint32_t x0 = wave * plan.quota;
-  if (x0 >= plan.all) return;
-  uint32_t left = min(plan.quota, plan.all - x0);
-  int b;
-  uint32_t before;
-  kv8_find(a, plan, x0, lane, b, before);
-  b = __builtin_amdgcn_readfirstlane(b);
-  before = __builtin_amdgcn_readfirstlane(before);
-  int n = kv8_len(a.c, a.lens, b), tiles = kv8_tiles(n);
-  uint32_t unit = (x0 - before) / (uint32_t)tiles;
-  int tile = (int)(x0 - before - unit * tiles);
-  bool first_segment = true;
-
-  while (true) {
-    const int h = (int)unit / a.chunks, chunk = (int)unit - h * a.chunks;
-    const int queries = min(kQueries, a.G - chunk * kQueries);
-    const int end = (int)min((uint32_t)tiles, tile + left);          // tiles [tile, end) of this unit are this wave's
-    const int begin = tile, blocks = n / kBlk;
-    const int64_t q_row = ((int64_t)b * a.c.H + h) * a.G + chunk * kQueries;
-
-    // the queries: column l % 16, channels 64 c + 16 g .. of run c
-    uint4 q[NC][2];
-    {
-      const T *row = reinterpret_cast<const T *>(a.q) + (q_row + min(col, queries - 1)) * D;
-#pragma unroll
-      for (int c = 0; c < NC; ++c) {
-        const int ch = 64 * c + 16 * g;
-        const bool in = col < queries && ch < D;
-        const uint4 *p = reinterpret_cast<const uint4 *>(row + (ch < D ? ch : 0));
-        const uint4 zero = make_uint4(0, 0, 0, 0), x = p[0], y = p[1];
-        q[c][0] = in ? x : zero;
-        q[c][1] = in ? y : zero;
-      }
-    }
-    Kv8State<NT> st;
-    st.clear();
-
-    // Page ids of a tile: of the block whose rows this lane loads as keys, and of the one whose positions it loads as values.
-    auto pages = [&](int t, int &kid, int &vid) {
-      const int kb = 4 * t + (col >> 2), vb = 4 * t + g;
-      kid = kb < blocks ? kv8_page(a.c, b, kb) : -1;
-      vid = vb < blocks ? kv8_page(a.c, b, vb) : -1;
-    };
-    // Lanes without a page load what lies at the pool's start, and take zeros.
-    uint4 kr[4][NC], vr[NT];
-    float ks, vs;
-    auto load_keys = [&](int t, int kid) {
-      const int blk = kv8_block_in_page(a.c, 4 * t + (col >> 2));
-      const uint8_t *p = kid >= 0 ? kv8_k_block(a.c, kid, h, blk, D) + (col & 3) * D : a.c.kp;
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int c = 0; c < NC; ++c) {
-          const int ch = 64 * c + 16 * g < D ? 64 * c + 16 * g : 0;      // past the head: any channels, their queries are zeros
-          kr[i][c] = load16<true>(kid >= 0 ? p + 4 * i * D + ch : p);
-        }
-    };
-    auto load_values = [&](int t, int vid) {
-      const int blk = kv8_block_in_page(a.c, 4 * t + g);
-      const uint8_t *p = vid >= 0 ? kv8_v_block(a.c, vid, h, blk, D) + col * kBlk : a.c.vp;
-#pragma unroll
-      for (int i = 0; i < NT; ++i) vr[i] = load16<true>(vid >= 0 ? p + i * 16 * kBlk : p);
-      ks = a.c.ks[vid >= 0 ? kv8_k_scale(a.c, vid, h, blk) : 0];
-      vs = a.c.vs[vid >= 0 ? kv8_v_scale(a.c, vid, h, blk) : 0];
-    };
-
-    int kid, vid, next_kid, next_vid;
-    pages(begin, kid, vid);
-    load_keys(begin, kid);
-    load_values(begin, vid);
-    pages(begin + 1, next_kid, next_vid);
-    for (int t = begin; t < end; ++t) {
-      int after_kid, after_vid;
-      pages(t + 2, after_kid, after_vid);
-      const bool whole = __ballot(kid < 0 || vid < 0) == 0;      // uniform: most tiles have all their pages
-      f32x4 s[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) s[i] = f32x4{0.f, 0.f, 0.f, 0.f};
-      if (!whole && kid < 0) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-#pragma unroll
-          for (int c = 0; c < NC; ++c) kr[i][c] = make_uint4(0, 0, 0, 0);
-      }
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int c = 0; c < NC; ++c) {
-          uint4 lo, hi;
-          widen16<DT, CODE>(kr[i][c], lo, hi);
-          s[i] = M::k32(lo, q[c][0], s[i]);
-          s[i] = M::k32(hi, q[c][1], s[i]);
-        }
-      __builtin_amdgcn_sched_barrier(0);
-      if (t + 1 < end) load_keys(t + 1, next_kid);
-      __builtin_amdgcn_sched_barrier(0);
-
-      if (!whole && vid < 0) {
-        ks = vs = 0.f;
-#pragma unroll
-        for (int i = 0; i < NT; ++i) vr[i] = make_uint4(0, 0, 0, 0);
-      }
-      const float by = ks * a.c_exp;
-      const bool in = 4 * t + g < blocks;
-      float top = -INFINITY;
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          s[i][e] = in ? s[i][e] * by : -INFINITY;
-          top = fmaxf(top, s[i][e]);
-        }
-      st.raise(top, fmaxf(__builtin_amdgcn_logf(fabsf(vs)), -126.f));
-      const float base = st.base(), f = vs * st.ratio();
-      uint32_t p[8];
+  const uint32_t member = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  const uint32_t wave = blockIdx.x * (kBlock / kWave) + member;
+  const uint32_t units = a.c.H * a.chunks;
+  uint32_t left;                 // tiles that are this wave's
+  Kv8At at;
+  if constexpr (TEAM == 1) {
+    const Kv8Plan plan = kv8_plan(a, lane);
+    const uint32_t x0 = wave * plan.quota;
+    if (x0 >= plan.all) return;
+    left = min(plan.quota, plan.all - x0);
+    uint32_t before;
+    kv8_find(a, plan, x0, lane, at.b, before);
+    at.b = __builtin_amdgcn_readfirstlane(at.b);
+    before = __builtin_amdgcn_readfirstlane(before);
+    at.n = kv8_wave_len(a.c, a.lens, at.b);
+    at.tiles = kv8_tiles(at.n);
+    const uint32_t unit = (x0 - before) / (uint32_t)at.tiles;
+    at.tile = (int)(x0 - before - unit * at.tiles);
+    at.h = (int)(unit / (uint32_t)a.chunks);
+    at.chunk = (int)unit - at.h * a.chunks;
+  } else {
+    at.b = blockIdx.x / units;
+    const uint32_t unit = blockIdx.x - (uint32_t)at.b * units;
+    at.h = (int)(unit / (uint32_t)a.chunks);
+    at.chunk = (int)unit - at.h * a.chunks;
+    at.n = kv8_wave_len(a.c, a.lens, at.b);
+    at.tiles = kv8_tiles(at.n);
+    at.tile = (int)member;
+    left = at.tiles > (int)member ? (uint32_t)(at.tiles - member + TEAM - 1) / TEAM : 0u;
+  }
+  // The tile behind; `ahead` of this wave's are left from there on, and where there are none it stays.
+  auto advance = [&](Kv8At &x, uint32_t ahead) {
+    if (ahead <= 1) return;
+    x.tile += TEAM;
+    if (TEAM > 1 || x.tile < x.tiles) return;
+    x.tile = 0;
+    if (++x.chunk < a.chunks) return;
+    x.chunk = 0;
+    if (++x.h < a.c.H) return;
+    x.h = 0;
+    ++x.b;
+    x.n = kv8_wave_len(a.c, a.lens, x.b);
+    x.tiles = kv8_tiles(x.n);
+  };
+  // Pages of a tile: of the block whose rows this lane loads as keys, and of the one whose positions it loads as values.  As the table has
+  // them: what depends on them comes a tile later, and nothing waits here for the loads of keys and values in between (the ids
+  // looked at where they are loaded, every tile waited for all loads: 128 sequences' 1031 MB 186 us, so KKK).
+  const int last_page = max(a.c.max_pages - 1, 0);
+  auto pages = [&](const Kv8At &x, int &kid, int &vid) {
+    const int32_t *row = a.c.table + (int64_t)x.b * a.c.max_pages;
+    kid = row[min((4 * x.tile + (col >> 2)) >> a.c.lg_blocks, last_page)];
+    vid = row[min((4 * x.tile + g) >> a.c.lg_blocks, last_page)];
+  };
+  // The id, or -1 for a block that is none of the sequence's or has no page.
+  auto checked = [&](const Kv8At &x, int block, int id) {
+    return 4 * x.tile + block < x.n / kBlk && (unsigned)id < (unsigned)a.c.num_pages ? id : -1;
+  };
+  // Lanes without a page load from the first one, and take zeros.
+  uint4 kr[4][NC], vr[NT];
+  float next_ks, next_vs;
+  auto load_keys = [&](const Kv8At &x, int kid) {
+    const uint8_t *p = kv8_k_block(a.c, max(kid, 0), x.h, kv8_block_in_page(a.c, 4 * x.tile + (col >> 2)), D) + (col & 3) * D + 16 * g;
+    if constexpr (kWholeLines) {
+      // rows of lanes 0..7 first, blocks 0 and 1; then those of lanes 8..15
+      const int other = (int)eight_away((uint32_t)max(kid, 0));
+      const uint8_t *p2 = kv8_k_block(a.c, other, x.h, kv8_block_in_page(a.c, 4 * x.tile + ((col ^ 8) >> 2)), D) + (col & 3) * D + 16 * g + 64;
+      const uint8_t *first = col < 8 ? p : p2, *second = col < 8 ? p2 : p;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        float e4[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          e4[e] = __builtin_amdgcn_exp2f(s[i][e] - base);
-          st.l += e4[e];
-        }
-        p[2 * i] = M::two(e4[0] * f, e4[1] * f);
-        p[2 * i + 1] = M::two(e4[2] * f, e4[3] * f);
+        kr[i][0] = load16<true>(first + 4 * i * D);
+        kr[i][1] = load16<true>(second + 4 * i * D);
       }
-      const uint4 p_lo = make_uint4(p[0], p[1], p[2], p[3]), p_hi = make_uint4(p[4], p[5], p[6], p[7]);
-#pragma unroll
-      for (int i = 0; i < NT; ++i) {
-        uint4 lo, hi;
-        widen16<DT, CODE>(vr[i], lo, hi);
-        st.o[i] = M::k32(lo, p_lo, st.o[i]);
-        st.o[i] = M::k32(hi, p_hi, st.o[i]);
-      }
-      __builtin_amdgcn_sched_barrier(0);
-      if (t + 1 < end) load_values(t + 1, next_vid);
-      __builtin_amdgcn_sched_barrier(0);
-      kid = next_kid;
-      vid = next_vid;
-      next_kid = after_kid;
-      next_vid = after_vid;
-    }
-
-    const int in_tail = n % kBlk;
-    if (end == tiles && in_tail) {
-      // the positions behind the last full block, 16 bits as they are: row i of the one key tile is position i
-      const int64_t at = ((int64_t)b * a.c.H + h) * kBlk * D;
-      const T *kt = reinterpret_cast<const T *>(a.c.kt) + at + col * D;
-      f32x4 s = {0.f, 0.f, 0.f, 0.f};
+    } else {
 #pragma unroll
       for (int c = 0; c < NC; ++c) {
-        const int ch = 64 * c + 16 * g < D ? 64 * c + 16 * g : 0;
-        const uint4 *p = reinterpret_cast<const uint4 *>(kt + ch);
-        s = M::k32(p[0], q[c][0], s);
-        s = M::k32(p[1], q[c][1], s);
+        const uint8_t *pc = p + (64 * c + 16 * g < D ? 64 * c : -16 * g);      // past the head: any channels, their queries are zeros
+#pragma unroll
+        for (int i = 0; i < 4; ++i) kr[i][c] = load16<true>(pc + 4 * i * D);
       }
-      float top = -INFINITY;
+    }
+  };
+  auto load_scales = [&](const Kv8At &x, int vid) {
+    const int blk = kv8_block_in_page(a.c, 4 * x.tile + g);
+    next_ks = a.c.ks[kv8_k_scale(a.c, max(vid, 0), x.h, blk)];
+    next_vs = a.c.vs[kv8_v_scale(a.c, max(vid, 0), x.h, blk)];
+  };
+  auto load_values = [&](const Kv8At &x, int vid) {
+    const uint8_t *p = kv8_v_block(a.c, max(vid, 0), x.h, kv8_block_in_page(a.c, 4 * x.tile + g), D) + col * kBlk;
+#pragma unroll
+    for (int i = 0; i < NT; ++i) vr[i] = load16<true>(p + i * 16 * kBlk);
+  };
+  // The queries of a unit: column l % 16, channels 64 c + 16 g .. of run c.
+  uint4 q[NC][2];
+  auto load_queries = [&](const Kv8At &x) {
+    const int queries = min(kQueries, a.G - x.chunk * kQueries);
+    const T *row = reinterpret_cast<const T *>(a.q) + ((((int64_t)x.b * a.c.H + x.h) * a.G + x.chunk * kQueries) + min(col, queries - 1)) * D;
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+      const int ch = 64 * c + 16 * g;
+      const uint4 *p = reinterpret_cast<const uint4 *>(row + (ch < D ? ch : 0));
+      const uint4 zero = make_uint4(0, 0, 0, 0), lo = p[0], hi = p[1];
+      q[c][0] = col < queries && ch < D ? lo : zero;
+      q[c][1] = col < queries && ch < D ? hi : zero;
+    }
+  };
+
+  Kv8State<NT> st;
+  st.clear();
+  // One tile whose keys and values are on their way; `next` follows it, its loads are issued as registers become free
+  // (without a branch around them: past one, the waits for what was loaded before no longer leave them out).
+  auto step = [&](const Kv8At &x, int kid, int vid, const Kv8At &next, int next_kid, int next_vid, auto more) {
+    if constexpr (kWholeLines) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) halves_in_place(kr[i][0], kr[i][1], col < 8);
+    }
+    const bool whole = __ballot(kid < 0 || vid < 0) == 0;      // uniform: most tiles have all their pages
+    f32x4 s[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) s[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+    if (!whole && kid < 0) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int c = 0; c < NC; ++c) kr[i][c] = make_uint4(0, 0, 0, 0);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int c = 0; c < NC; ++c) {
+        uint4 lo, hi;
+        widen16<DT, CODE>(kr[i][c], lo, hi);
+        s[i] = M::k32(lo, q[c][0], s[i]);
+        s[i] = M::k32(hi, q[c][1], s[i]);
+      }
+    float ks = next_ks, vs = next_vs;
+    asm volatile("" : "+v"(ks), "+v"(vs));         // here, while the loads into their registers are still to come
+    __builtin_amdgcn_sched_barrier(0);
+    if constexpr (more.value) {
+      load_keys(next, next_kid);
+      load_scales(next, next_vid);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+
+    if (!whole && vid < 0) {
+      ks = vs = 0.f;
+#pragma unroll
+      for (int i = 0; i < NT; ++i) vr[i] = make_uint4(0, 0, 0, 0);
+    }
+    const float by = ks * a.c_exp;
+    const bool in = 4 * x.tile + g < x.n / kBlk;
+    float top = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        s[e] = 4 * g + e < in_tail ? s[e] * a.c_exp : -INFINITY;
-        top = fmaxf(top, s[e]);
+        s[i][e] = in ? s[i][e] * by : -INFINITY;
+        top = fmaxf(top, s[i][e]);
       }
-      st.raise(top, 0.f);
-      const float base = st.base(), f = st.ratio();
+    st.raise(top, fmaxf(__builtin_amdgcn_logf(fabsf(vs)), -126.f));
+    const float base = st.base(), f = vs * st.ratio();
+    uint32_t p[8];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
       float e4[4];
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        e4[e] = __builtin_amdgcn_exp2f(s[e] - base);
+        e4[e] = __builtin_amdgcn_exp2f(s[i][e] - base);
         st.l += e4[e];
       }
-      const uint2 pp = make_uint2(M::two(e4[0] * f, e4[1] * f), M::two(e4[2] * f, e4[3] * f));
-      const uint16_t *vt = reinterpret_cast<const uint16_t *>(a.c.vt) + at + col * kBlk + 4 * g;
-      // rows behind the last position may hold anything
-      const uint32_t m0 = (4 * g < in_tail ? 0xffffu : 0u) | (4 * g + 1 < in_tail ? 0xffff0000u : 0u),
-                     m1 = (4 * g + 2 < in_tail ? 0xffffu : 0u) | (4 * g + 3 < in_tail ? 0xffff0000u : 0u);
+      p[2 * i] = M::two(e4[0] * f, e4[1] * f);
+      p[2 * i + 1] = M::two(e4[2] * f, e4[3] * f);
+    }
+    const uint4 p_lo = make_uint4(p[0], p[1], p[2], p[3]), p_hi = make_uint4(p[4], p[5], p[6], p[7]);
 #pragma unroll
-      for (int i = 0; i < NT; ++i) {
-        const uint2 w = *reinterpret_cast<const uint2 *>(vt + i * 16 * kBlk);
-        st.o[i] = M::k16(make_uint2(w.x & m0, w.y & m1), pp, st.o[i]);
+    for (int i = 0; i < NT; ++i) {
+      uint4 lo, hi;
+      widen16<DT, CODE>(vr[i], lo, hi);
+      st.o[i] = M::k32(lo, p_lo, st.o[i]);
+      st.o[i] = M::k32(hi, p_hi, st.o[i]);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    if constexpr (more.value) load_values(next, next_vid);
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  // The positions behind the last full block, 16 bits as they are: row i of the one key tile is position i.
+  auto tail = [&](const Kv8At &x) {
+    const int in_tail = x.n % kBlk;
+    const int64_t from = ((int64_t)x.b * a.c.H + x.h) * kBlk * D;
+    const T *kt = reinterpret_cast<const T *>(a.c.kt) + from + col * D;
+    f32x4 s = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+      const int ch = 64 * c + 16 * g < D ? 64 * c + 16 * g : 0;
+      const uint4 *p = reinterpret_cast<const uint4 *>(kt + ch);
+      s = M::k32(p[0], q[c][0], s);
+      s = M::k32(p[1], q[c][1], s);
+    }
+    float top = -INFINITY;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      s[e] = 4 * g + e < in_tail ? s[e] * a.c_exp : -INFINITY;
+      top = fmaxf(top, s[e]);
+    }
+    st.raise(top, 0.f);
+    const float base = st.base(), f = st.ratio();
+    float e4[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      e4[e] = __builtin_amdgcn_exp2f(s[e] - base);
+      st.l += e4[e];
+    }
+    const uint2 pp = make_uint2(M::two(e4[0] * f, e4[1] * f), M::two(e4[2] * f, e4[3] * f));
+    const uint16_t *vt = reinterpret_cast<const uint16_t *>(a.c.vt) + from + col * kBlk + 4 * g;
+    // rows behind the last position may hold anything
+    const uint32_t m0 = (4 * g < in_tail ? 0xffffu : 0u) | (4 * g + 1 < in_tail ? 0xffff0000u : 0u),
+                   m1 = (4 * g + 2 < in_tail ? 0xffffu : 0u) | (4 * g + 3 < in_tail ? 0xffff0000u : 0u);
+#pragma unroll
+    for (int i = 0; i < NT; ++i) {
+      const uint2 w = *reinterpret_cast<const uint2 *>(vt + i * 16 * kBlk);
+      st.o[i] = M::k16(make_uint2(w.x & m0, w.y & m1), pp, st.o[i]);
+    }
+  };
+
+  Kv8At next = at, later;
+  int kid, vid, raw_kid, raw_vid;      // of the tile; of the next one, as the table has them
+  if (TEAM == 1 || left > 0) {
+    pages(at, kid, vid);
+    advance(next, left);
+    pages(next, raw_kid, raw_vid);
+    kid = checked(at, col >> 2, kid);
+    vid = checked(at, g, vid);
+    load_keys(at, kid);
+    load_scales(at, vid);
+    load_values(at, vid);
+    load_queries(at);
+  }
+  int begin = at.tile;
+  bool first_segment = true;
+  auto turn = [&](auto more) {
+    later = next;
+    advance(later, left - 1);
+    int next_kid = checked(next, col >> 2, raw_kid), next_vid = checked(next, g, raw_vid);
+    asm volatile("" : "+v"(next_kid), "+v"(next_vid));
+    __builtin_amdgcn_sched_barrier(0);
+    pages(later, raw_kid, raw_vid);
+    __builtin_amdgcn_sched_barrier(0);
+    step(at, kid, vid, next, next_kid, next_vid, more);
+    --left;
+    if constexpr (TEAM == 1) {
+      const bool done = at.tile + 1 == at.tiles;
+      if (!more.value || done) {
+        // the end of the unit, or of this wave's part of it; the loads of the next unit's first tile are on their way
+        if (done && at.n % kBlk) tail(at);
+        const int queries = min(kQueries, a.G - at.chunk * kQueries);
+        const int64_t q_row = ((int64_t)at.b * a.c.H + at.h) * a.G + at.chunk * kQueries;
+        const float l = over_blocks_sum(st.l);
+        const float back = st.m_s > -INFINITY ? __builtin_amdgcn_exp2f(st.m_o - st.m_s) : 0.f;
+        if (begin == 0 && done) {
+          const float by = l > 0.f ? back / l : (l == l ? 0.f : l);
+          if (col < queries) {
+            T *out = reinterpret_cast<T *>(a.ctx) + (q_row + col) * D + 4 * g;
+#pragma unroll
+            for (int i = 0; i < NT; ++i) {
+              Pack<T, 4> w;
+#pragma unroll
+              for (int e = 0; e < 4; ++e) w.v[e] = E::from_float(l == 0.f ? 0.f : st.o[i][e] * by);
+              store_pack<T, 4>(out + 16 * i, w);
+            }
+          }
+        } else if (col < queries) {
+          const int64_t slot = ((int64_t)wave * 2 + (first_segment ? 0 : 1)) * a.rows + col;
+          float *out = a.part_o + slot * D + 4 * g;
+#pragma unroll
+          for (int i = 0; i < NT; ++i) *reinterpret_cast<f32x4 *>(out + 16 * i) = st.o[i] * back;
+          if (g == 0) a.part_ml[slot] = make_float2(st.m_s, l);
+        }
+        st.clear();
+        first_segment = false;
+        begin = 0;
+        if constexpr (more.value) load_queries(next);
       }
     }
+    at = next;
+    kid = next_kid;
+    vid = next_vid;
+    next = later;
+  };
+  while (left > 1) turn(std::true_type{});
+  if (left > 0) turn(std::false_type{});
 
+  if constexpr (TEAM > 1) {
+    extern __shared__ __align__(16) float s_part[];          // m and l [TEAM][rows] each, then [TEAM][rows][16 tiles]
+    const int rows = a.rows, queries = min(kQueries, a.G - at.chunk * kQueries);
+    const int tiles = kv8_team_tiles(rows, NT), width = tiles * 16;      // channels of 16 that go through LDS at a time
+    float *s_m = s_part, *s_l = s_m + TEAM * rows, *s_o = s_l + TEAM * rows;
+    // the tail goes to the wave that has the fewest tiles, or no more than the others
+    if (at.n % kBlk && member == (uint32_t)(at.tiles % TEAM)) {
+      load_queries(at);
+      tail(at);
+    }
     const float l = over_blocks_sum(st.l);
     const float back = st.m_s > -INFINITY ? __builtin_amdgcn_exp2f(st.m_o - st.m_s) : 0.f;
-    if (begin == 0 && end == tiles) {
-      const float by = l > 0.f ? back / l : (l == l ? 0.f : l);
-      if (col < queries) {
-        T *out = reinterpret_cast<T *>(a.ctx) + (q_row + col) * D + 4 * g;
-#pragma unroll
-        for (int i = 0; i < NT; ++i) {
-          Pack<T, 4> w;
-#pragma unroll
-          for (int e = 0; e < 4; ++e) w.v[e] = E::from_float(l == 0.f ? 0.f : st.o[i][e] * by);
-          store_pack<T, 4>(out + 16 * i, w);
-        }
-      }
-    } else if (col < queries) {
-      const int64_t slot = ((int64_t)wave * 2 + (first_segment ? 0 : 1)) * a.rows + col;
-      float *out = a.part_o + slot * D + 4 * g;
-#pragma unroll
-      for (int i = 0; i < NT; ++i) *reinterpret_cast<f32x4 *>(out + 16 * i) = st.o[i] * back;
-      if (g == 0) a.part_ml[slot] = make_float2(st.m_s, l);
+    const int64_t q_row = ((int64_t)at.b * a.c.H + at.h) * a.G + at.chunk * kQueries;
+    if (col < queries && g == 0) {
+      s_m[member * rows + col] = st.m_s;
+      s_l[member * rows + col] = l;
     }
-
-    left -= (uint32_t)(end - begin);
-    if (left == 0) return;
-    first_segment = false;
-    tile = 0;
-    if (++unit == plan.units) {
-      unit = 0;
-      ++b;
-      n = kv8_len(a.c, a.lens, b);
-      tiles = kv8_tiles(n);
+    for (int t0 = 0; t0 < NT; t0 += tiles) {
+      if (t0) __syncthreads();
+      if (col < queries) {
+#pragma unroll
+        for (int i = 0; i < NT; ++i)
+          if (i >= t0 && i < t0 + tiles) *reinterpret_cast<f32x4 *>(s_o + (member * rows + col) * width + (i - t0) * 16 + 4 * g) = st.o[i] * back;
+      }
+      __syncthreads();
+      const int per_row = min(tiles, NT - t0) * 4;
+      for (int i = threadIdx.x; i < queries * per_row; i += TEAM * kWave) {
+        const int r = i / per_row, d = i % per_row * 4;
+        float m = -INFINITY, sum = 0.f;
+        f32x4 o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int w = 0; w < TEAM; ++w) m = fmaxf(m, s_m[w * rows + r]);
+#pragma unroll
+        for (int w = 0; w < TEAM; ++w) {
+          const float f = share_weight(s_m[w * rows + r], s_l[w * rows + r], m);
+          sum += s_l[w * rows + r] * f;
+          o += *reinterpret_cast<const f32x4 *>(s_o + (w * rows + r) * width + d) * f;
+        }
+        write_row<DT>(reinterpret_cast<T *>(a.ctx) + (q_row + r) * D + t0 * 16 + d, sum, o);
+      }
     }
   }
 }
 
-// Combines the partial results of the units that several waves had tiles of: four channels a lane, the waves' shares in turn.
+// Combines the partial results of the units that several waves had tiles of.  A workgroup takes a unit's rows: 32 lanes four channels each,
+// eight groups of lanes.  Few shares: a group takes a row.  Many (one sequence of 8 key heads: 256 each): the groups take every
+// eighth share of a row, and their results go through LDS; what counts then is how many are on their way at once, eight a lane.
+constexpr int kCombineLanes = 32, kCombineGroups = kBlock / kCombineLanes, kAhead = 8;
+
 template <int DT>
 __global__ __launch_bounds__(kBlock) void decode_attn_kv8_combine_kernel(Kv8AttnArgs a, int D) {
-  typedef Elem<DT> E;
-  typedef typename E::T T;
+  typedef typename Elem<DT>::T T;
+  __shared__ f32x4 s_o[kCombineGroups][kCombineLanes];
+  __shared__ float s_m[kCombineGroups], s_l[kCombineGroups];
   const int lane = threadIdx.x % kWave;
   const Kv8Plan plan = kv8_plan(a, lane);
   const int b = blockIdx.x / plan.units;
@@ -421,43 +596,73 @@ __global__ __launch_bounds__(kBlock) void decode_attn_kv8_combine_kernel(Kv8Attn
   const int h = (int)unit / a.chunks, chunk = (int)unit - h * a.chunks;
   const int queries = min(kQueries, a.G - chunk * kQueries);
   const bool from_start = x0 == w0 * plan.quota;            // the first wave's run begins with this unit
-  for (int i = threadIdx.x; i < queries * (D / 4); i += kBlock) {
-    const int r = i / (D / 4), d = i % (D / 4) * 4;
-    float m = -INFINITY, l = 0.f;
-    f32x4 o = {0.f, 0.f, 0.f, 0.f};
-    constexpr int kAhead = 4;
-    for (uint32_t w = w0; w <= w1; w += kAhead) {
+  const int group = threadIdx.x / kCombineLanes, d = threadIdx.x % kCombineLanes * 4;
+  T *out = reinterpret_cast<T *>(a.ctx) + (((int64_t)b * a.c.H + h) * a.G + chunk * kQueries) * D + d;
+  // what the shares w, w + step, .. of row r combine to
+  auto gather = [&](int r, uint32_t w, uint32_t step, float &m, float &l, f32x4 &o) {
+    m = -INFINITY;
+    l = 0.f;
+    o = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (; w <= w1; w += kAhead * step) {
       float2 ml[kAhead];
       f32x4 v[kAhead];
 #pragma unroll
       for (int j = 0; j < kAhead; ++j) {
-        const uint32_t x = min(w + j, w1);
+        const uint32_t x = min(w + j * step, w1);
         const int64_t slot = ((int64_t)x * 2 + (x == w0 && !from_start ? 1 : 0)) * a.rows + r;
         ml[j] = a.part_ml[slot];
-        v[j] = *reinterpret_cast<const f32x4 *>(a.part_o + slot * D + d);
-        if (w + j > w1) ml[j].x = -INFINITY;
+        v[j] = *reinterpret_cast<const f32x4 *>(a.part_o + slot * D + (d < D ? d : 0));
       }
       float top = m;
 #pragma unroll
-      for (int j = 0; j < kAhead; ++j) top = fmaxf(top, ml[j].x);
-      if (top == -INFINITY) continue;
-      const float keep = __builtin_amdgcn_exp2f(m - top);
+      for (int j = 0; j < kAhead; ++j)
+        if (w + j * step <= w1) top = fmaxf(top, ml[j].x);
+      const float keep = share_weight(m, l, top);
       l *= keep;
       o *= keep;
 #pragma unroll
       for (int j = 0; j < kAhead; ++j) {
-        if (w + j > w1) continue;
-        const float f = __builtin_amdgcn_exp2f(ml[j].x - top);
+        if (w + j * step > w1) continue;
+        const float f = share_weight(ml[j].x, ml[j].y, top);
         l += ml[j].y * f;
         o += v[j] * f;
       }
       m = top;
     }
-    const float by = l > 0.f ? 1.f / l : (l == l ? 0.f : l);
-    Pack<T, 4> y;
+  };
+  float m, l;
+  f32x4 o;
+  if (w1 - w0 < 2 * kAhead) {
+    const int r = blockIdx.y * kCombineGroups + group;
+    if (r < queries && d < D) {
+      gather(r, w0, 1, m, l, o);
+      write_row<DT>(out + r * D, l, o);
+    }
+    return;
+  }
+  for (int r = blockIdx.y; r < queries; r += gridDim.y) {
+    gather(r, w0 + group, kCombineGroups, m, l, o);
+    if (r != (int)blockIdx.y) __syncthreads();              // the row before has been read
+    s_o[group][threadIdx.x % kCombineLanes] = o;
+    if (threadIdx.x % kCombineLanes == 0) {
+      s_m[group] = m;
+      s_l[group] = l;
+    }
+    __syncthreads();
+    if (group == 0 && d < D) {
+      float top = -INFINITY;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) y.v[e] = E::from_float(l == 0.f ? 0.f : o[e] * by);
-    store_pack<T, 4>(reinterpret_cast<T *>(a.ctx) + (((int64_t)b * a.c.H + h) * a.G + chunk * kQueries + r) * D + d, y);
+      for (int j = 0; j < kCombineGroups; ++j) top = fmaxf(top, s_m[j]);
+      l = 0.f;
+      o = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int j = 0; j < kCombineGroups; ++j) {
+        const float f = share_weight(s_m[j], s_l[j], top);
+        l += s_l[j] * f;
+        o += s_o[j][d / 4] * f;
+      }
+      write_row<DT>(out + r * D, l, o);
+    }
   }
 }
 
@@ -482,6 +687,7 @@ extern "C" int en_decode_attn_kv8(const void *q, void *ctx, const en_kv8_cache *
   const int64_t capacity = (int64_t)cache->max_pages_per_seq * cache->page_size;
   if (workspace_bytes < en_decode_attn_kv8_workspace_bytes(cache->batch, q_heads, cache->head_num, (int)capacity, cache->size_per_head)) return EN_ERR_SHAPE;
   Kv8AttnArgs a{kv8_args(cache), q, ctx, kv_lens, q_heads / cache->head_num, 0, scale * 1.4426950408889634f, kWaves, nullptr, nullptr, 0};
+  if (capacity == 0) a.c.table = kv_lens;      // no row of the table to look at: any word, which names no position
   a.chunks = (int)ceil_div(a.G, kQueries);
   a.rows = a.G < kQueries ? a.G : kQueries;
   const int64_t units = (int64_t)cache->batch * cache->head_num * a.chunks;
@@ -490,18 +696,22 @@ extern "C" int en_decode_attn_kv8(const void *q, void *ctx, const en_kv8_cache *
   a.part_o = reinterpret_cast<float *>(workspace);
   a.part_ml = reinterpret_cast<float2 *>(a.part_o + rows * cache->size_per_head);
   const hipStream_t s = (hipStream_t)stream;
-  const unsigned grid = kWaves / (kBlock / kWave);
+  const bool team = capacity <= kTeamCapacity;
+  auto launch = [&](auto dt, auto code, auto nt) {
+    constexpr int DT = decltype(dt)::value, CODE = decltype(code)::value, NT = decltype(nt)::value;
+    if (team) decode_attn_kv8_kernel<DT, CODE, NT, kTeam><<<(unsigned)units, kTeam * kWave, kTeam * a.rows * (kv8_team_tiles(a.rows, NT) * 16 + 2) * 4, s>>>(a);
+    else decode_attn_kv8_kernel<DT, CODE, NT, 1><<<kWaves / (kBlock / kWave), kBlock, 0, s>>>(a);
+  };
   auto heads = [&](auto dt, auto code) {
-    constexpr int DT = decltype(dt)::value, CODE = decltype(code)::value;
     switch (cache->size_per_head) {
-      case 16: decode_attn_kv8_kernel<DT, CODE, 1><<<grid, kBlock, 0, s>>>(a); break;
-      case 32: decode_attn_kv8_kernel<DT, CODE, 2><<<grid, kBlock, 0, s>>>(a); break;
-      case 48: decode_attn_kv8_kernel<DT, CODE, 3><<<grid, kBlock, 0, s>>>(a); break;
-      case 64: decode_attn_kv8_kernel<DT, CODE, 4><<<grid, kBlock, 0, s>>>(a); break;
-      case 80: decode_attn_kv8_kernel<DT, CODE, 5><<<grid, kBlock, 0, s>>>(a); break;
-      case 96: decode_attn_kv8_kernel<DT, CODE, 6><<<grid, kBlock, 0, s>>>(a); break;
-      case 112: decode_attn_kv8_kernel<DT, CODE, 7><<<grid, kBlock, 0, s>>>(a); break;
-      default: decode_attn_kv8_kernel<DT, CODE, 8><<<grid, kBlock, 0, s>>>(a); break;
+      case 16: launch(dt, code, std::integral_constant<int, 1>{}); break;
+      case 32: launch(dt, code, std::integral_constant<int, 2>{}); break;
+      case 48: launch(dt, code, std::integral_constant<int, 3>{}); break;
+      case 64: launch(dt, code, std::integral_constant<int, 4>{}); break;
+      case 80: launch(dt, code, std::integral_constant<int, 5>{}); break;
+      case 96: launch(dt, code, std::integral_constant<int, 6>{}); break;
+      case 112: launch(dt, code, std::integral_constant<int, 7>{}); break;
+      default: launch(dt, code, std::integral_constant<int, 8>{}); break;
     }
   };
   auto codes = [&](auto dt) {
@@ -511,8 +721,11 @@ extern "C" int en_decode_attn_kv8(const void *q, void *ctx, const en_kv8_cache *
   if (cache->dtype == EN_F16) codes(std::integral_constant<int, EN_F16>{});
   else codes(std::integral_constant<int, EN_BF16>{});
   EN_RETURN_IF_LAUNCH_FAILED();
-  if (cache->dtype == EN_F16) decode_attn_kv8_combine_kernel<EN_F16><<<(unsigned)units, kBlock, 0, s>>>(a, cache->size_per_head);
-  else decode_attn_kv8_combine_kernel<EN_BF16><<<(unsigned)units, kBlock, 0, s>>>(a, cache->size_per_head);
+  if (team) return EN_OK;
+  // rows of a unit in workgroups of their own where units are few; where units are many, each has few shares
+  const dim3 shares((unsigned)units, units >= 512 ? (unsigned)ceil_div(a.rows, kCombineGroups) : (unsigned)a.rows);
+  if (cache->dtype == EN_F16) decode_attn_kv8_combine_kernel<EN_F16><<<shares, kBlock, 0, s>>>(a, cache->size_per_head);
+  else decode_attn_kv8_combine_kernel<EN_BF16><<<shares, kBlock, 0, s>>>(a, cache->size_per_head);
   EN_RETURN_IF_LAUNCH_FAILED();
   return EN_OK;
 }
