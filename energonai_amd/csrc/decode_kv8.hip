@@ -30,10 +30,7 @@ typedef short i16x4 __attribute__((ext_vector_type(4)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int kTile = 4 * kBlk;               // positions of a tile
-#ifndef KW
-#define KW 2048
-#endif
-constexpr int kWaves = KW;                  // of the launch: two a SIMD, and what of the registers they leave holds loads in flight
+constexpr int kWaves = 1024;                  // of the launch: one a SIMD, whose loads of the next tile cover the latency by themselves
 constexpr int kQueries = 16;                  // columns of a tile: queries that share one pass
 constexpr float kRaise = 8.f;                 // log2
 constexpr int kTeam = 8;                      // waves of a workgroup that takes one unit
@@ -102,7 +99,7 @@ struct Kv8AttnArgs {
   const int32_t *lens;
   int G, chunks;                // queries of a key head, and the runs of kQueries they are taken in
   float c_exp;                  // scale * log2(e)
-  uint32_t waves;
+  uint32_t *first_tile;         // [B] of a sequence, in the row of all tiles; behind them the tiles of a wave's run
   float *part_o;                // [2 waves][rows][D]
   float2 *part_ml;              // [2 waves][rows]
   int rows;                     // min(G, kQueries)
@@ -118,44 +115,15 @@ __device__ __forceinline__ int kv8_wave_len(const Kv8 &c, const int32_t *lens, i
 __device__ __forceinline__ int kv8_tiles(int n) { return max(1, (n / kBlk + 3) / 4); }
 
 // The tiles of all units in a row: per sequence its key heads' (and chunks'), one unit behind the other.
-struct Kv8Plan {
-  uint32_t units, all, quota;    // units a sequence; tiles; tiles a wave
-};
-__device__ __forceinline__ uint32_t wave_sum(uint32_t v) {
+__device__ __forceinline__ uint32_t wave_prefix(uint32_t v, int lane) {
 #pragma unroll
-  for (int m = 1; m < kWave; m *= 2) v += (uint32_t)__shfl_xor((int)v, m, kWave);
+  for (int m = 1; m < kWave; m *= 2) {
+    const uint32_t up = (uint32_t)__shfl_up((int)v, m, kWave);
+    v += lane >= m ? up : 0u;
+  }
   return v;
 }
-__device__ __forceinline__ Kv8Plan kv8_plan(const Kv8AttnArgs &a, int lane) {
-  uint32_t sum = 0;
-  for (int b = lane; b < a.c.B; b += kWave) sum += kv8_tiles(kv8_len(a.c, a.lens, b));
-  Kv8Plan p;
-  p.units = a.c.H * a.chunks;
-  p.all = __builtin_amdgcn_readfirstlane(wave_sum(sum)) * p.units;
-  p.quota = (p.all + a.waves - 1) / a.waves;
-  return p;
-}
-// Sequence that tile x belongs to, and the tiles before that sequence.
-__device__ __forceinline__ void kv8_find(const Kv8AttnArgs &a, const Kv8Plan &p, uint32_t x, int lane, int &b, uint32_t &before) {
-  before = 0;
-  for (int b0 = 0;; b0 += kWave) {
-    uint32_t incl = b0 + lane < a.c.B ? kv8_tiles(kv8_len(a.c, a.lens, b0 + lane)) * p.units : 0u;
-    const uint32_t mine = incl;
-#pragma unroll
-    for (int m = 1; m < kWave; m *= 2) {
-      const uint32_t up = (uint32_t)__shfl_up((int)incl, m, kWave);
-      incl += lane >= m ? up : 0u;
-    }
-    const uint64_t past = __ballot(before + incl > x);
-    if (past || b0 + kWave >= a.c.B) {
-      const int l = past ? __builtin_ctzll(past) : kWave - 1;
-      b = b0 + l;
-      before += (uint32_t)__builtin_amdgcn_readlane((int)(incl - mine), l);
-      return;
-    }
-    before += (uint32_t)__builtin_amdgcn_readlane((int)incl, kWave - 1);
-  }
-}
+__device__ __forceinline__ uint32_t lane_value(uint32_t v, int lane) { return (uint32_t)__builtin_amdgcn_readlane((int)v, lane); }
 
 __device__ __forceinline__ float over_blocks_max(float v) {
   v = fmaxf(v, __shfl_xor(v, 16, kWave));
@@ -232,7 +200,7 @@ __host__ __device__ constexpr int kv8_team_tiles(int rows, int nt) { return rows
 // TEAM 1: every wave by itself, a run of plan.quota tiles.  TEAM 8: the waves of a workgroup take the tiles of one unit in turn and
 // put their results together in LDS.
 template <int DT, int CODE, int NT, int TEAM>
-__global__ __launch_bounds__(TEAM == 1 ? kBlock : TEAM * kWave, 2) void decode_attn_kv8_kernel(Kv8AttnArgs a) {
+__global__ __launch_bounds__(TEAM == 1 ? kBlock : TEAM * kWave, TEAM == 1 ? 1 : 2) void decode_attn_kv8_kernel(Kv8AttnArgs a) {
   typedef Elem<DT> E;
   typedef typename E::T T;
   typedef Mma<DT> M;
@@ -242,23 +210,44 @@ __global__ __launch_bounds__(TEAM == 1 ? kBlock : TEAM * kWave, 2) void decode_a
   const uint32_t member = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const uint32_t wave = blockIdx.x * (kBlock / kWave) + member;
   const uint32_t units = a.c.H * a.chunks;
-  uint32_t left;                 // tiles that are this wave's
+  uint32_t left, x = 0;          // tiles that are this wave's, and the first of those that are left
   Kv8At at;
   if constexpr (TEAM == 1) {
-    const Kv8Plan plan = kv8_plan(a, lane);
-    const uint32_t x0 = wave * plan.quota;
-    if (x0 >= plan.all) return;
-    left = min(plan.quota, plan.all - x0);
-    uint32_t before;
-    kv8_find(a, plan, x0, lane, at.b, before);
-    at.b = __builtin_amdgcn_readfirstlane(at.b);
-    before = __builtin_amdgcn_readfirstlane(before);
-    at.n = kv8_wave_len(a.c, a.lens, at.b);
-    at.tiles = kv8_tiles(at.n);
+    // lengths of the first 64 sequences stay in a register: few batches have more
+    const int len0 = lane < a.c.B ? kv8_len(a.c, a.lens, lane) : 0;
+    const uint32_t incl0 = wave_prefix(lane < a.c.B ? kv8_tiles(len0) * units : 0u, lane);
+    uint32_t all = lane_value(incl0, kWave - 1);
+    for (int b0 = kWave; b0 < a.c.B; b0 += kWave)
+      all += lane_value(wave_prefix(b0 + lane < a.c.B ? kv8_tiles(kv8_len(a.c, a.lens, b0 + lane)) * units : 0u, lane), kWave - 1);
+    const uint32_t quota = (all + kWaves - 1) / kWaves, x0 = wave * quota;
+    if (x0 >= all) return;
+    left = min(quota, all - x0);
+    // the sequence of tile x0: the first whose tiles end past it
+    int len = len0;
+    uint32_t incl = incl0, before = 0;
+    at.b = 0;
+    while (true) {
+      const uint64_t past = __ballot(before + incl > x0);
+      if (past) {
+        const int l = __builtin_ctzll(past);
+        at.b += l;
+        at.n = (int)lane_value((uint32_t)len, l);
+        at.tiles = kv8_tiles(at.n);
+        before += lane_value(incl, l) - at.tiles * units;
+        break;
+      }
+      before += lane_value(incl, kWave - 1);
+      at.b += kWave;
+      len = at.b + lane < a.c.B ? kv8_len(a.c, a.lens, at.b + lane) : 0;
+      incl = wave_prefix(at.b + lane < a.c.B ? kv8_tiles(len) * units : 0u, lane);
+    }
     const uint32_t unit = (x0 - before) / (uint32_t)at.tiles;
     at.tile = (int)(x0 - before - unit * at.tiles);
     at.h = (int)(unit / (uint32_t)a.chunks);
     at.chunk = (int)unit - at.h * a.chunks;
+    // for the combine launch: the run's length, and each sequence's first tile, from the wave that comes to it
+    if (wave == 0 && lane == 0) a.first_tile[a.c.B] = quota;
+    x = x0;
   } else {
     at.b = blockIdx.x / units;
     const uint32_t unit = blockIdx.x - (uint32_t)at.b * units;
@@ -477,6 +466,11 @@ __global__ __launch_bounds__(TEAM == 1 ? kBlock : TEAM * kWave, 2) void decode_a
   }
   int begin = at.tile;
   bool first_segment = true;
+  // a sequence's first tile is where its first unit begins
+  auto note = [&](const Kv8At &y, uint32_t tile) {
+    if (TEAM == 1 && y.tile == 0 && y.h == 0 && y.chunk == 0 && lane == 0) a.first_tile[y.b] = tile;
+  };
+  if (left > 0) note(at, x);
   auto turn = [&](auto more) {
     later = next;
     advance(later, left - 1);
@@ -518,9 +512,13 @@ __global__ __launch_bounds__(TEAM == 1 ? kBlock : TEAM * kWave, 2) void decode_a
         st.clear();
         first_segment = false;
         begin = 0;
-        if constexpr (more.value) load_queries(next);
+        if constexpr (more.value) {
+          load_queries(next);
+          note(next, x + 1);
+        }
       }
     }
+    ++x;
     at = next;
     kid = next_kid;
     vid = next_vid;
@@ -583,19 +581,13 @@ __global__ __launch_bounds__(kBlock) void decode_attn_kv8_combine_kernel(Kv8Attn
   typedef typename Elem<DT>::T T;
   __shared__ f32x4 s_o[kCombineGroups][kCombineLanes];
   __shared__ float s_m[kCombineGroups], s_l[kCombineGroups];
-  const int lane = threadIdx.x % kWave;
-  const Kv8Plan plan = kv8_plan(a, lane);
-  const int b = blockIdx.x / plan.units;
-  const uint32_t unit = blockIdx.x - (uint32_t)b * plan.units;
-  uint32_t sum = 0;
-  for (int i = lane; i < b; i += kWave) sum += kv8_tiles(kv8_len(a.c, a.lens, i));
-  const uint32_t tiles = kv8_tiles(kv8_len(a.c, a.lens, b));
-  const uint32_t x0 = __builtin_amdgcn_readfirstlane(wave_sum(sum)) * plan.units + unit * tiles, x1 = x0 + tiles;
-  const uint32_t w0 = x0 / plan.quota, w1 = (x1 - 1) / plan.quota;
+  const uint32_t units = a.c.H * a.chunks, b = blockIdx.x / units, unit = blockIdx.x - b * units, quota = a.first_tile[a.c.B];
+  const uint32_t tiles = kv8_tiles(kv8_len(a.c, a.lens, (int)b)), x0 = a.first_tile[b] + unit * tiles, x1 = x0 + tiles;
+  const uint32_t w0 = x0 / quota, w1 = (x1 - 1) / quota;
   if (w0 == w1) return;                                     // one wave had it whole
   const int h = (int)unit / a.chunks, chunk = (int)unit - h * a.chunks;
   const int queries = min(kQueries, a.G - chunk * kQueries);
-  const bool from_start = x0 == w0 * plan.quota;            // the first wave's run begins with this unit
+  const bool from_start = x0 == w0 * quota;            // the first wave's run begins with this unit
   const int group = threadIdx.x / kCombineLanes, d = threadIdx.x % kCombineLanes * 4;
   T *out = reinterpret_cast<T *>(a.ctx) + (((int64_t)b * a.c.H + h) * a.G + chunk * kQueries) * D + d;
   // what the shares w, w + step, .. of row r combine to
@@ -674,7 +666,8 @@ using namespace en;
 
 extern "C" int64_t en_decode_attn_kv8_workspace_bytes(int batch, int q_heads, int head_num, int capacity, int size_per_head) {
   if (batch < 1 || head_num < 1 || q_heads < head_num || q_heads % head_num || capacity < 0 || size_per_head < 1) return 0;
-  return kv8_part_rows(q_heads, head_num) * (4 * (int64_t)size_per_head + 8);
+  if (capacity <= kTeamCapacity) return 0;
+  return kv8_part_rows(q_heads, head_num) * (4 * (int64_t)size_per_head + 8) + 4 * ((int64_t)batch + 1);
 }
 
 extern "C" int en_decode_attn_kv8(const void *q, void *ctx, const en_kv8_cache *cache, const int32_t *kv_lens, int q_heads, float scale,
@@ -682,11 +675,13 @@ extern "C" int en_decode_attn_kv8(const void *q, void *ctx, const en_kv8_cache *
   if (const int bad = check_kv8(cache)) return bad;
   if (q_heads < cache->head_num || q_heads % cache->head_num) return EN_ERR_SHAPE;
   if (cache->batch == 0) return EN_OK;
-  if (!q || !ctx || !kv_lens || !workspace) return EN_ERR_NULL;
+  if (!q || !ctx || !kv_lens) return EN_ERR_NULL;
   if (!aligned_to(q, 16) || !aligned_to(ctx, 16) || !aligned_to(workspace, 16)) return EN_ERR_ALIGN;
   const int64_t capacity = (int64_t)cache->max_pages_per_seq * cache->page_size;
+  const bool team = capacity <= kTeamCapacity;
+  if (!team && !workspace) return EN_ERR_NULL;
   if (workspace_bytes < en_decode_attn_kv8_workspace_bytes(cache->batch, q_heads, cache->head_num, (int)capacity, cache->size_per_head)) return EN_ERR_SHAPE;
-  Kv8AttnArgs a{kv8_args(cache), q, ctx, kv_lens, q_heads / cache->head_num, 0, scale * 1.4426950408889634f, kWaves, nullptr, nullptr, 0};
+  Kv8AttnArgs a{kv8_args(cache), q, ctx, kv_lens, q_heads / cache->head_num, 0, scale * 1.4426950408889634f, nullptr, nullptr, nullptr, 0};
   if (capacity == 0) a.c.table = kv_lens;      // no row of the table to look at: any word, which names no position
   a.chunks = (int)ceil_div(a.G, kQueries);
   a.rows = a.G < kQueries ? a.G : kQueries;
@@ -695,8 +690,8 @@ extern "C" int en_decode_attn_kv8(const void *q, void *ctx, const en_kv8_cache *
   const int64_t rows = kv8_part_rows(q_heads, cache->head_num);
   a.part_o = reinterpret_cast<float *>(workspace);
   a.part_ml = reinterpret_cast<float2 *>(a.part_o + rows * cache->size_per_head);
+  a.first_tile = reinterpret_cast<uint32_t *>(a.part_ml + rows);
   const hipStream_t s = (hipStream_t)stream;
-  const bool team = capacity <= kTeamCapacity;
   auto launch = [&](auto dt, auto code, auto nt) {
     constexpr int DT = decltype(dt)::value, CODE = decltype(code)::value, NT = decltype(nt)::value;
     if (team) decode_attn_kv8_kernel<DT, CODE, NT, kTeam><<<(unsigned)units, kTeam * kWave, kTeam * a.rows * (kv8_team_tiles(a.rows, NT) * 16 + 2) * 4, s>>>(a);

@@ -183,7 +183,8 @@ def kv8_pages_read(cache, kv_len_list, max_seq_len: int, *, first: Optional[torc
 
 
 def decode_attn_kv8_workspace_bytes(batch_size: int, q_heads: int, head_num: int, capacity: int, size_per_head: int) -> int:
-    """Bytes of the buffer through which ``decode_attn_kv8`` passes partial results."""
+    """Bytes of the buffer through which ``decode_attn_kv8`` passes its plan and partial results (0: caches of this capacity, in positions a
+    sequence, need none)."""
     return int(_lib.fn.en_decode_attn_kv8_workspace_bytes(int(batch_size), int(q_heads), int(head_num), int(capacity), int(size_per_head)))
 
 
@@ -226,5 +227,5 @@ def decode_attn_kv8(q, cache, kv_len_list, *, scale: Optional[float] = None, out
     scale = float(D) ** -0.5 if scale is None else float(scale)
     with _lib.device_guard(q):
         _lib.check(_lib.fn.en_decode_attn_kv8(q_.data_ptr(), out.data_ptr(), ctypes.byref(c), info.lens.data_ptr(), Hq, scale,
-                                              workspace.data_ptr(), workspace.numel() * workspace.element_size(), _lib.stream_of(q)), who)
+                                              _lib.ptr(workspace) or None, workspace.numel() * workspace.element_size(), _lib.stream_of(q)), who)
     return out

@@ -511,7 +511,8 @@ int en_kv8_read(const en_kv8_cache *cache, const int32_t *kv_lens, const int32_t
                 en_stream_t stream);
 /* Decode attention: ctx[b, h] = softmax(scale * <q[b, h], K>) V over the kv_lens[b] cached positions of key head h / (q_heads /
  * head_num); zeros for an empty sequence.  q, ctx: contiguous [batch, q_heads, size_per_head].  workspace:
- * en_decode_attn_kv8_workspace_bytes, 16-byte aligned; its contents need not be kept or cleared. */
+ * en_decode_attn_kv8_workspace_bytes (may be 0, then NULL), 16-byte aligned; its contents need not be kept or cleared, but calls that may
+ * run at the same time need one each. */
 int64_t en_decode_attn_kv8_workspace_bytes(int batch, int q_heads, int head_num, int capacity, int size_per_head);
 int en_decode_attn_kv8(const void *q, void *ctx, const en_kv8_cache *cache, const int32_t *kv_lens, int q_heads, float scale,
                        void *workspace, int64_t workspace_bytes, en_stream_t stream);

@@ -369,6 +369,48 @@ def test_long_and_ragged_with_wide_offsets():
     assert torch.equal(k[0].cpu(), held.held(ks[0]).float().to(BF16)) and torch.equal(v[1, :, :37].cpu(), held.held(vs[1]).float().to(BF16))
 
 
+@pytest.mark.parametrize("dtype,code,Hq,H,D,B,lo,hi", [
+    (F16, I8, 16, 8, 64, 3, 30000, 40000),           # shares of several tiles, taken as waves come to the end of theirs
+    (BF16, E4, 40, 40, 128, 30, 0, 2100),            # several units a share
+    (BF16, I8, 8, 1, 128, 1, 70001, 70001),          # hundreds of shares a unit
+    (F16, E4, 34, 2, 80, 70, 1000, 1600),            # two runs of queries a key head; more sequences than lanes
+])
+def test_attention_shares(dtype, code, Hq, H, D, B, lo, hi):
+    """Sequences cut into many shares against float64, on the GPU (the oracle on some of the heads), and the same bits again."""
+    K = _K()
+    announce("decode_attn_kv8 shares", dtype, code, Hq, H, D, B, lo, hi)
+    g = torch.Generator().manual_seed(B + hi)
+    lens = torch.randint(lo, hi + 1, (B,), generator=g).tolist()
+    P = 64
+    cache = list(K.kv8_pages(sum(n // P + 1 for n in lens), B, H, P, D, hi // P + 2, dtype, "cuda", code))
+    table = torch.full(cache[6].shape, -1, dtype=torch.int32)
+    ids = torch.randperm(cache[0].shape[0], generator=g).tolist()
+    for b, n in enumerate(lens):
+        for pi in range(-(-n // P)):
+            table[b, pi] = ids.pop()
+    cache[6] = table.cuda()
+    gg = torch.Generator(device="cuda").manual_seed(1)
+    kv = torch.randn(sum(lens), 2 * H, D, generator=gg, device="cuda", dtype=dtype)
+    at = torch.tensor(lens, dtype=torch.int32).cuda()
+    K.kv8_pages_fill(kv[:, :H], kv[:, H:], cache, B, max(lens), at)
+    q = 2 * torch.randn(B, Hq, 1, D, generator=gg, device="cuda", dtype=dtype)
+    got = K.decode_attn_kv8(q, cache, at)
+    assert torch.equal(got, K.decode_attn_kv8(q, cache, at))
+    half = torch.finfo(dtype).eps / 2
+    k, v = K.kv8_pages_read(cache, at, max(lens))                       # rounded to the type: K and V again half a step off
+    for b in range(0, B, max(1, B // 6)):
+        n = lens[b]
+        kb, vb = k[b, :, :n].double(), v[b, :, :n].double()
+        qb = q[b, :, 0].double().view(H, -1, D)
+        p = torch.softmax(qb @ kb.transpose(-1, -2) * D ** -0.5, -1)
+        want, size = p @ vb, p @ vb.abs()
+        # a key half a step off moves a score by that of sum |q k|, at most 40 here (2 x 128 products of N(0,1) / sqrt(128), by 3): in the mean it is far less,
+        # and it is the root of the sum of squares that counts: sqrt(sum (q k)^2) / sqrt(D) half, under 8 half
+        tol = half * (size + want.abs()) + half * size + 8 * half * size
+        off = ((got[b, :, 0].double().view(want.shape) - want).abs() - tol).max()
+        assert n == 0 or off <= 0, (b, n, float(off))
+
+
 @pytest.mark.parametrize("seed", range(8))
 def test_attention_random(seed):
     K = _K()
@@ -484,7 +526,7 @@ def test_refusals():
         with pytest.raises(RuntimeError):
             K.decode_attn_kv8(bad, good, at)
     with pytest.raises(RuntimeError):
-        K.decode_attn_kv8(q, good, at, workspace=torch.zeros(16, dtype=torch.uint8, device="cuda"))
+        K.decode_attn_kv8(q, make(max_pages_per_seq=1000), at, workspace=torch.zeros(16, dtype=torch.uint8, device="cuda"))
     with pytest.raises(RuntimeError):
         K.decode_attn_kv8(q, good, at, out=q.float())
     with pytest.raises(RuntimeError):

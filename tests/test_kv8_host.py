@@ -77,8 +77,8 @@ def test_norm_and_rotation_refuse():
 def test_cache_calls_refuse():
     fn = _lib().fn
     six, four = (ctypes.c_int64 * 6)(*[128, 64] * 3), (ctypes.c_int64 * 4)(*[128, 64] * 2)
-    ws = fn.en_decode_attn_kv8_workspace_bytes(3, 4, 2, 64, 64)
-    assert ws > 0 and fn.en_decode_attn_kv8_workspace_bytes(3, 5, 2, 64, 64) == 0
+    ws = fn.en_decode_attn_kv8_workspace_bytes(3, 4, 2, 1 << 16, 64)
+    assert ws > 0 and fn.en_decode_attn_kv8_workspace_bytes(3, 5, 2, 1 << 16, 64) == fn.en_decode_attn_kv8_workspace_bytes(3, 4, 2, 64, 64) == 0
     how = _how()
 
     def calls(c):
@@ -105,8 +105,9 @@ def test_cache_calls_refuse():
     assert fn.en_kv8_read(c, PTR, None, -1, PTR, PTR, None) == SHAPE and fn.en_kv8_read(c, PTR, None, 4, PTR + 8, PTR, None) == ALIGN
     for hq in (0, 1, 3, 5):
         assert fn.en_decode_attn_kv8(PTR, PTR, c, PTR, hq, 1.0, PTR, ws, None) == SHAPE
-    assert fn.en_decode_attn_kv8(PTR, PTR, c, PTR, 4, 1.0, None, ws, None) == NULL
-    assert fn.en_decode_attn_kv8(PTR, PTR, c, PTR, 4, 1.0, PTR, ws - 1, None) == SHAPE
+    long = ctypes.byref(_cache(max_pages_per_seq=1 << 11))
+    assert fn.en_decode_attn_kv8(PTR, PTR, long, PTR, 4, 1.0, None, ws, None) == NULL
+    assert fn.en_decode_attn_kv8(PTR, PTR, long, PTR, 4, 1.0, PTR, ws - 1, None) == SHAPE
     assert fn.en_decode_attn_kv8(PTR + 2, PTR, c, PTR, 4, 1.0, PTR, ws, None) == ALIGN
 
 
