@@ -112,6 +112,8 @@ __device__ __forceinline__ int kv8_wave_len(const Kv8 &c, const int32_t *lens, i
   const int n = *(scalar_t)(uintptr_t)(lens + __builtin_amdgcn_readfirstlane(b));
   return min(max(n, 0), (c.max_pages << c.lg_blocks) * kBlk);
 }
+// What a unit counts in the row of tiles beside its tiles: its tail, the softmax's end and the output.
+constexpr int kUnitCost = 1;
 __device__ __forceinline__ int kv8_tiles(int n) { return max(1, (n / kBlk + 3) / 4); }
 
 // The tiles of all units in a row: per sequence its key heads' (and chunks'), one unit behind the other.
@@ -181,6 +183,7 @@ template <int DT> __device__ __forceinline__ void write_row(typename Elem<DT>::T
 struct Kv8At {
   int b, n, tiles, tile;
   int h, chunk;
+  uint32_t x;                    // its place, in tiles and units' ends
 };
 
 // The keys of four rows (4t .. 4t + 3 of each of four blocks) a lane as the first product wants them: 16 channels of row l % 16, run c of 64.
@@ -210,18 +213,18 @@ __global__ __launch_bounds__(TEAM == 1 ? kBlock : TEAM * kWave, TEAM == 1 ? 1 : 
   const uint32_t member = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const uint32_t wave = blockIdx.x * (kBlock / kWave) + member;
   const uint32_t units = a.c.H * a.chunks;
-  uint32_t left, x = 0;          // tiles that are this wave's, and the first of those that are left
+  uint32_t end = 0;              // of this wave's run
   Kv8At at;
   if constexpr (TEAM == 1) {
     // lengths of the first 64 sequences stay in a register: few batches have more
     const int len0 = lane < a.c.B ? kv8_len(a.c, a.lens, lane) : 0;
-    const uint32_t incl0 = wave_prefix(lane < a.c.B ? kv8_tiles(len0) * units : 0u, lane);
+    const uint32_t incl0 = wave_prefix(lane < a.c.B ? (kv8_tiles(len0) + kUnitCost) * units : 0u, lane);
     uint32_t all = lane_value(incl0, kWave - 1);
     for (int b0 = kWave; b0 < a.c.B; b0 += kWave)
-      all += lane_value(wave_prefix(b0 + lane < a.c.B ? kv8_tiles(kv8_len(a.c, a.lens, b0 + lane)) * units : 0u, lane), kWave - 1);
+      all += lane_value(wave_prefix(b0 + lane < a.c.B ? (kv8_tiles(kv8_len(a.c, a.lens, b0 + lane)) + kUnitCost) * units : 0u, lane), kWave - 1);
     const uint32_t quota = (all + kWaves - 1) / kWaves, x0 = wave * quota;
     if (x0 >= all) return;
-    left = min(quota, all - x0);
+    end = min(x0 + quota, all);
     // the sequence of tile x0: the first whose tiles end past it
     int len = len0;
     uint32_t incl = incl0, before = 0;
@@ -233,21 +236,21 @@ __global__ __launch_bounds__(TEAM == 1 ? kBlock : TEAM * kWave, TEAM == 1 ? 1 : 
         at.b += l;
         at.n = (int)lane_value((uint32_t)len, l);
         at.tiles = kv8_tiles(at.n);
-        before += lane_value(incl, l) - at.tiles * units;
+        before += lane_value(incl, l) - (at.tiles + kUnitCost) * units;
         break;
       }
       before += lane_value(incl, kWave - 1);
       at.b += kWave;
       len = at.b + lane < a.c.B ? kv8_len(a.c, a.lens, at.b + lane) : 0;
-      incl = wave_prefix(at.b + lane < a.c.B ? kv8_tiles(len) * units : 0u, lane);
+      incl = wave_prefix(at.b + lane < a.c.B ? (kv8_tiles(len) + kUnitCost) * units : 0u, lane);
     }
-    const uint32_t unit = (x0 - before) / (uint32_t)at.tiles;
-    at.tile = (int)(x0 - before - unit * at.tiles);
+    const uint32_t unit = (x0 - before) / (uint32_t)(at.tiles + kUnitCost);
+    at.tile = (int)(x0 - before - unit * (at.tiles + kUnitCost));
     at.h = (int)(unit / (uint32_t)a.chunks);
     at.chunk = (int)unit - at.h * a.chunks;
     // for the combine launch: the run's length, and each sequence's first tile, from the wave that comes to it
     if (wave == 0 && lane == 0) a.first_tile[a.c.B] = quota;
-    x = x0;
+    at.x = x0;
   } else {
     at.b = blockIdx.x / units;
     const uint32_t unit = blockIdx.x - (uint32_t)at.b * units;
@@ -256,22 +259,31 @@ __global__ __launch_bounds__(TEAM == 1 ? kBlock : TEAM * kWave, TEAM == 1 ? 1 : 
     at.n = kv8_wave_len(a.c, a.lens, at.b);
     at.tiles = kv8_tiles(at.n);
     at.tile = (int)member;
-    left = at.tiles > (int)member ? (uint32_t)(at.tiles - member + TEAM - 1) / TEAM : 0u;
+    at.x = 0;
   }
-  // The tile behind; `ahead` of this wave's are left from there on, and where there are none it stays.
-  auto advance = [&](Kv8At &x, uint32_t ahead) {
-    if (ahead <= 1) return;
-    x.tile += TEAM;
-    if (TEAM > 1 || x.tile < x.tiles) return;
-    x.tile = 0;
-    if (++x.chunk < a.chunks) return;
-    x.chunk = 0;
-    if (++x.h < a.c.H) return;
-    x.h = 0;
-    ++x.b;
-    x.n = kv8_wave_len(a.c, a.lens, x.b);
-    x.tiles = kv8_tiles(x.n);
+  auto past = [&](const Kv8At &c) { return TEAM == 1 ? c.x >= end : c.tile >= c.tiles; };
+  // The next unit's first tile, where it is still this wave's.
+  auto next_unit = [&](Kv8At &c) {
+    c.x += c.tiles + kUnitCost - c.tile;
+    if (c.x >= end) return;
+    c.tile = 0;
+    if (++c.chunk < a.chunks) return;
+    c.chunk = 0;
+    if (++c.h < a.c.H) return;
+    c.h = 0;
+    ++c.b;
+    c.n = kv8_wave_len(a.c, a.lens, c.b);
+    c.tiles = kv8_tiles(c.n);
   };
+  auto advance = [&](Kv8At &c) {
+    if (past(c)) return;
+    c.tile += TEAM;
+    if constexpr (TEAM == 1) {
+      ++c.x;
+      if (c.tile == c.tiles) next_unit(c);
+    }
+  };
+  if (TEAM == 1 && at.tile >= at.tiles) next_unit(at);      // the run begins with a unit's end
   // Pages of a tile: of the block whose rows this lane loads as keys, and of the one whose positions it loads as values.  As the table has
   // them: what depends on them comes a tile later, and nothing waits here for the loads of keys and values in between (the ids
   // looked at where they are loaded, every tile waited for all loads: 128 sequences' 1031 MB 186 us, so KKK).
@@ -319,8 +331,8 @@ __global__ __launch_bounds__(TEAM == 1 ? kBlock : TEAM * kWave, TEAM == 1 ? 1 : 
 #pragma unroll
     for (int i = 0; i < NT; ++i) vr[i] = load16<true>(p + i * 16 * kBlk);
   };
-  // The queries of a unit: column l % 16, channels 64 c + 16 g .. of run c.
-  uint4 q[NC][2];
+  // The queries of a unit: column l % 16, channels 64 c + 16 g .. of run c.  Columns and channels that are none are zeros.
+  uint4 q[NC][2], next_q[NC][2];
   auto load_queries = [&](const Kv8At &x) {
     const int queries = min(kQueries, a.G - x.chunk * kQueries);
     const T *row = reinterpret_cast<const T *>(a.q) + ((((int64_t)x.b * a.c.H + x.h) * a.G + x.chunk * kQueries) + min(col, queries - 1)) * D;
@@ -328,9 +340,18 @@ __global__ __launch_bounds__(TEAM == 1 ? kBlock : TEAM * kWave, TEAM == 1 ? 1 : 
     for (int c = 0; c < NC; ++c) {
       const int ch = 64 * c + 16 * g;
       const uint4 *p = reinterpret_cast<const uint4 *>(row + (ch < D ? ch : 0));
-      const uint4 zero = make_uint4(0, 0, 0, 0), lo = p[0], hi = p[1];
-      q[c][0] = col < queries && ch < D ? lo : zero;
-      q[c][1] = col < queries && ch < D ? hi : zero;
+      next_q[c][0] = p[0];
+      next_q[c][1] = p[1];
+    }
+  };
+  auto take_queries = [&](const Kv8At &x) {
+    const int queries = min(kQueries, a.G - x.chunk * kQueries);
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+      const bool in = col < queries && 64 * c + 16 * g < D;
+      const uint4 zero = make_uint4(0, 0, 0, 0);
+      q[c][0] = in ? next_q[c][0] : zero;
+      q[c][1] = in ? next_q[c][1] : zero;
     }
   };
 
@@ -413,17 +434,28 @@ __global__ __launch_bounds__(TEAM == 1 ? kBlock : TEAM * kWave, TEAM == 1 ? 1 : 
     __builtin_amdgcn_sched_barrier(0);
   };
   // The positions behind the last full block, 16 bits as they are: row i of the one key tile is position i.
-  auto tail = [&](const Kv8At &x) {
-    const int in_tail = x.n % kBlk;
+  uint4 tail_k[NC][2];
+  uint2 tail_v[NT];
+  auto load_tail = [&](const Kv8At &x) {
     const int64_t from = ((int64_t)x.b * a.c.H + x.h) * kBlk * D;
     const T *kt = reinterpret_cast<const T *>(a.c.kt) + from + col * D;
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+      const uint4 *p = reinterpret_cast<const uint4 *>(kt + (64 * c + 16 * g < D ? 64 * c + 16 * g : 0));
+      tail_k[c][0] = p[0];
+      tail_k[c][1] = p[1];
+    }
+    const uint16_t *vt = reinterpret_cast<const uint16_t *>(a.c.vt) + from + col * kBlk + 4 * g;
+#pragma unroll
+    for (int i = 0; i < NT; ++i) tail_v[i] = *reinterpret_cast<const uint2 *>(vt + i * 16 * kBlk);
+  };
+  auto tail = [&](const Kv8At &x) {
+    const int in_tail = x.n % kBlk;
     f32x4 s = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
-      const int ch = 64 * c + 16 * g < D ? 64 * c + 16 * g : 0;
-      const uint4 *p = reinterpret_cast<const uint4 *>(kt + ch);
-      s = M::k32(p[0], q[c][0], s);
-      s = M::k32(p[1], q[c][1], s);
+      s = M::k32(tail_k[c][0], q[c][0], s);
+      s = M::k32(tail_k[c][1], q[c][1], s);
     }
     float top = -INFINITY;
 #pragma unroll
@@ -440,22 +472,18 @@ __global__ __launch_bounds__(TEAM == 1 ? kBlock : TEAM * kWave, TEAM == 1 ? 1 : 
       st.l += e4[e];
     }
     const uint2 pp = make_uint2(M::two(e4[0] * f, e4[1] * f), M::two(e4[2] * f, e4[3] * f));
-    const uint16_t *vt = reinterpret_cast<const uint16_t *>(a.c.vt) + from + col * kBlk + 4 * g;
     // rows behind the last position may hold anything
     const uint32_t m0 = (4 * g < in_tail ? 0xffffu : 0u) | (4 * g + 1 < in_tail ? 0xffff0000u : 0u),
                    m1 = (4 * g + 2 < in_tail ? 0xffffu : 0u) | (4 * g + 3 < in_tail ? 0xffff0000u : 0u);
 #pragma unroll
-    for (int i = 0; i < NT; ++i) {
-      const uint2 w = *reinterpret_cast<const uint2 *>(vt + i * 16 * kBlk);
-      st.o[i] = M::k16(make_uint2(w.x & m0, w.y & m1), pp, st.o[i]);
-    }
+    for (int i = 0; i < NT; ++i) st.o[i] = M::k16(make_uint2(tail_v[i].x & m0, tail_v[i].y & m1), pp, st.o[i]);
   };
 
   Kv8At next = at, later;
   int kid, vid, raw_kid, raw_vid;      // of the tile; of the next one, as the table has them
-  if (TEAM == 1 || left > 0) {
+  if (!past(at)) {
     pages(at, kid, vid);
-    advance(next, left);
+    advance(next);
     pages(next, raw_kid, raw_vid);
     kid = checked(at, col >> 2, kid);
     vid = checked(at, g, vid);
@@ -463,26 +491,30 @@ __global__ __launch_bounds__(TEAM == 1 ? kBlock : TEAM * kWave, TEAM == 1 ? 1 : 
     load_scales(at, vid);
     load_values(at, vid);
     load_queries(at);
+    take_queries(at);
   }
   int begin = at.tile;
   bool first_segment = true;
   // a sequence's first tile is where its first unit begins
-  auto note = [&](const Kv8At &y, uint32_t tile) {
-    if (TEAM == 1 && y.tile == 0 && y.h == 0 && y.chunk == 0 && lane == 0) a.first_tile[y.b] = tile;
+  auto note = [&](const Kv8At &c) {
+    if (TEAM == 1 && c.tile == 0 && c.h == 0 && c.chunk == 0 && lane == 0) a.first_tile[c.b] = c.x;
   };
-  if (left > 0) note(at, x);
   auto turn = [&](auto more) {
     later = next;
-    advance(later, left - 1);
+    advance(later);
     int next_kid = checked(next, col >> 2, raw_kid), next_vid = checked(next, g, raw_vid);
     asm volatile("" : "+v"(next_kid), "+v"(next_vid));
     __builtin_amdgcn_sched_barrier(0);
     pages(later, raw_kid, raw_vid);
+    const bool done = TEAM == 1 && at.tile + 1 == at.tiles;
+    if (done) {
+      // what a unit's end and the next one's beginning need is sent for a tile before
+      if (at.n % kBlk) load_tail(at);
+      if constexpr (more.value) load_queries(next);
+    }
     __builtin_amdgcn_sched_barrier(0);
     step(at, kid, vid, next, next_kid, next_vid, more);
-    --left;
     if constexpr (TEAM == 1) {
-      const bool done = at.tile + 1 == at.tiles;
       if (!more.value || done) {
         // the end of the unit, or of this wave's part of it; the loads of the next unit's first tile are on their way
         if (done && at.n % kBlk) tail(at);
@@ -513,19 +545,21 @@ __global__ __launch_bounds__(TEAM == 1 ? kBlock : TEAM * kWave, TEAM == 1 ? 1 : 
         first_segment = false;
         begin = 0;
         if constexpr (more.value) {
-          load_queries(next);
-          note(next, x + 1);
+          take_queries(next);
+          note(next);
         }
       }
     }
-    ++x;
     at = next;
     kid = next_kid;
     vid = next_vid;
     next = later;
   };
-  while (left > 1) turn(std::true_type{});
-  if (left > 0) turn(std::false_type{});
+  if (!past(at)) {
+    note(at);
+    while (!past(next)) turn(std::true_type{});
+    turn(std::false_type{});
+  }
 
   if constexpr (TEAM > 1) {
     extern __shared__ __align__(16) float s_part[];          // m and l [TEAM][rows] each, then [TEAM][rows][16 tiles]
@@ -534,7 +568,9 @@ __global__ __launch_bounds__(TEAM == 1 ? kBlock : TEAM * kWave, TEAM == 1 ? 1 : 
     float *s_m = s_part, *s_l = s_m + TEAM * rows, *s_o = s_l + TEAM * rows;
     // the tail goes to the wave that has the fewest tiles, or no more than the others
     if (at.n % kBlk && member == (uint32_t)(at.tiles % TEAM)) {
+      load_tail(at);
       load_queries(at);
+      take_queries(at);
       tail(at);
     }
     const float l = over_blocks_sum(st.l);
@@ -582,12 +618,12 @@ __global__ __launch_bounds__(kBlock) void decode_attn_kv8_combine_kernel(Kv8Attn
   __shared__ f32x4 s_o[kCombineGroups][kCombineLanes];
   __shared__ float s_m[kCombineGroups], s_l[kCombineGroups];
   const uint32_t units = a.c.H * a.chunks, b = blockIdx.x / units, unit = blockIdx.x - b * units, quota = a.first_tile[a.c.B];
-  const uint32_t tiles = kv8_tiles(kv8_len(a.c, a.lens, (int)b)), x0 = a.first_tile[b] + unit * tiles, x1 = x0 + tiles;
+  const uint32_t tiles = kv8_tiles(kv8_len(a.c, a.lens, (int)b)), x0 = a.first_tile[b] + unit * (tiles + kUnitCost), x1 = x0 + tiles;
   const uint32_t w0 = x0 / quota, w1 = (x1 - 1) / quota;
   if (w0 == w1) return;                                     // one wave had it whole
   const int h = (int)unit / a.chunks, chunk = (int)unit - h * a.chunks;
   const int queries = min(kQueries, a.G - chunk * kQueries);
-  const bool from_start = x0 == w0 * quota;            // the first wave's run begins with this unit
+  const bool from_start = x0 - w0 * quota <= kUnitCost;     // the first wave's run begins with this unit, or the end of the one before
   const int group = threadIdx.x / kCombineLanes, d = threadIdx.x % kCombineLanes * 4;
   T *out = reinterpret_cast<T *>(a.ctx) + (((int64_t)b * a.c.H + h) * a.G + chunk * kQueries) * D + d;
   // what the shares w, w + step, .. of row r combine to
@@ -686,7 +722,7 @@ extern "C" int en_decode_attn_kv8(const void *q, void *ctx, const en_kv8_cache *
   a.chunks = (int)ceil_div(a.G, kQueries);
   a.rows = a.G < kQueries ? a.G : kQueries;
   const int64_t units = (int64_t)cache->batch * cache->head_num * a.chunks;
-  if (units * ceil_div(capacity + kTile, kTile) >= INT32_MAX) return EN_ERR_SHAPE;
+  if (units * (ceil_div(capacity + kTile, kTile) + kUnitCost) >= INT32_MAX) return EN_ERR_SHAPE;
   const int64_t rows = kv8_part_rows(q_heads, cache->head_num);
   a.part_o = reinterpret_cast<float *>(workspace);
   a.part_ml = reinterpret_cast<float2 *>(a.part_o + rows * cache->size_per_head);
