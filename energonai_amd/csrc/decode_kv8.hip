@@ -30,14 +30,17 @@ typedef short i16x4 __attribute__((ext_vector_type(4)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int kTile = 4 * kBlk;               // positions of a tile
-constexpr int kWaves = 1024;                  // of the launch: one a SIMD, whose loads of the next tile cover the latency by themselves
+constexpr int kWaves = 1024;                  // of the launch: one a SIMD, whose loads of the next tile cover the latency by themselves.  Twice
+                                              // as many leave twice the partial results: 32 of up to 2000, 32 / 8 x 128 19.9 -> 25.5 us, 128 of up to 4000 104 -> 107
 constexpr int kQueries = 16;                  // columns of a tile: queries that share one pass
 constexpr float kRaise = 8.f;                 // log2
 constexpr int kTeam = 8;                      // waves of a workgroup that takes one unit
-#ifndef TC
-#define TC 1024
-#endif
-constexpr int kTeamCapacity = TC;
+constexpr int kTeamCapacity = 1024, kTeamUnits = 512;
+// One launch of a workgroup a unit where they are all resident at once and a unit is at most two tiles a wave; otherwise runs, which any lengths
+// leave equal, and a second launch.  us, runs / a workgroup a unit, 64 positions a page: 1 sequence of 100, 12 heads x 64 8.0 / 4.7;
+// 32 of up to 500, 12 x 64 11.3 / 8.2; 32 of up to 1000, 32 / 8 x 128 15.5 / 13.4, of up to 2000 19.5 / 20.2; 8 of up to 1000 11.7 / 12.2; 1 of
+// 2000 10.3 / 18.1.  More units: 64 of up to 250, 40 x 128 30.1 / 44.6, of up to 1000 71 / 82.
+inline bool kv8_team(int64_t units, int64_t capacity) { return units <= kTeamUnits && capacity <= kTeamCapacity; }
 
 template <int DT> struct Mma;
 template <> struct Mma<EN_F16> {
@@ -702,7 +705,7 @@ using namespace en;
 
 extern "C" int64_t en_decode_attn_kv8_workspace_bytes(int batch, int q_heads, int head_num, int capacity, int size_per_head) {
   if (batch < 1 || head_num < 1 || q_heads < head_num || q_heads % head_num || capacity < 0 || size_per_head < 1) return 0;
-  if (capacity <= kTeamCapacity) return 0;
+  if (kv8_team((int64_t)batch * head_num * ceil_div(q_heads / head_num, kQueries), capacity)) return 0;
   return kv8_part_rows(q_heads, head_num) * (4 * (int64_t)size_per_head + 8) + 4 * ((int64_t)batch + 1);
 }
 
@@ -714,7 +717,7 @@ extern "C" int en_decode_attn_kv8(const void *q, void *ctx, const en_kv8_cache *
   if (!q || !ctx || !kv_lens) return EN_ERR_NULL;
   if (!aligned_to(q, 16) || !aligned_to(ctx, 16) || !aligned_to(workspace, 16)) return EN_ERR_ALIGN;
   const int64_t capacity = (int64_t)cache->max_pages_per_seq * cache->page_size;
-  const bool team = capacity <= kTeamCapacity;
+  const bool team = kv8_team((int64_t)cache->batch * cache->head_num * ceil_div(q_heads / cache->head_num, kQueries), capacity);
   if (!team && !workspace) return EN_ERR_NULL;
   if (workspace_bytes < en_decode_attn_kv8_workspace_bytes(cache->batch, q_heads, cache->head_num, (int)capacity, cache->size_per_head)) return EN_ERR_SHAPE;
   Kv8AttnArgs a{kv8_args(cache), q, ctx, kv_lens, q_heads / cache->head_num, 0, scale * 1.4426950408889634f, nullptr, nullptr, nullptr, 0};
