@@ -167,14 +167,15 @@ struct Kv8AppendArgs {
   int32_t *overflow;
 };
 
-// One row of up to 128 channels through norm and rotation, a pair a lane, from `in` to `out` and, if given, `copy`.
+// One row of up to 128 channels through norm and rotation, a pair a lane, from `in` to `out` and, if given, `copy`.  In 64 bits: a key that is
+// held in 8 bits is rounded twice, and of a decode step's few rows the arithmetic is not what counts (64 sequences, 48 heads x 128 KKK us, in 32 KKK).
 template <int DT, bool IL, typename T>
 __device__ __forceinline__ void turn_row(const RotaryHow &how, const T *in, int pos, const void *weight, T *out, T *copy, int lane) {
   RotaryRow<DT, 1, kWave, 1, IL> row;
   RotaryTurn<1, kWave, 1, IL> turn;
   row.load(how, in, lane);
   turn.load(how, pos, lane);
-  norm_and_turn(how, row, turn, weight, lane);
+  norm_and_turn<double>(how, row, turn, weight, lane);
   store_row<false>(how, row, out, lane);
   if (copy) store_row<false>(how, row, copy, lane);
 }
@@ -391,7 +392,7 @@ extern "C" int en_kv8_append(const void *q, const void *k_new, const void *v_new
     if (!aligned_to(p, 2)) return EN_ERR_ALIGN;
   const int64_t units = (int64_t)cache->batch * (q_heads + 2 * (int64_t)cache->head_num);
   if (units > INT32_MAX) return EN_ERR_SHAPE;
-  const Kv8AppendArgs a{kv8_args(cache), rotary_how(how, cache->size_per_head), q, k_new, v_new, q_out, kv_lens, strides[0], strides[1], strides[2],
+  const Kv8AppendArgs a{kv8_args(cache), rotary_how(how, cache->size_per_head, 1), q, k_new, v_new, q_out, kv_lens, strides[0], strides[1], strides[2],
                         strides[3], strides[4], strides[5], q_heads, how->interleaved != 0, (uint32_t)units, overflow};
   with_kv8_form(cache, [&](auto dt, auto code, auto d) {
     kv8_append_kernel<decltype(dt)::value, decltype(code)::value, decltype(d)::value>

@@ -32,7 +32,7 @@ __device__ __forceinline__ int sequence_of(const int32_t *cu, int batch, int t) 
 }
 
 // HPG heads of one token a lane group: its table rows are read once for them, and their loads are in flight together.
-template <int DT, int VEC, int LPR, int NP, bool IL, int HPG, bool NT>
+template <int DT, int VEC, int LPR, int NP, bool IL, int HPG, bool NT, bool NTL = false>
 __global__ __launch_bounds__(kBlock) void qk_norm_rotary_kernel(RotaryRowsArgs a) {
   typedef typename Elem<DT>::T T;
   typedef RotaryRow<DT, VEC, LPR, NP, IL> Row;
@@ -55,7 +55,7 @@ __global__ __launch_bounds__(kBlock) void qk_norm_rotary_kernel(RotaryRowsArgs a
   const int64_t in_head = which ? a.in_head[1] : a.in_head[0], out_head = which ? a.out_head[1] : a.out_head[0];
   Row rows[HPG];
 #pragma unroll
-  for (int h = 0; h < HPG; ++h) rows[h].load(a.how, in + min(first + h, heads - 1) * in_head, lane);
+  for (int h = 0; h < HPG; ++h) rows[h].template load<NTL>(a.how, in + min(first + h, heads - 1) * in_head, lane);
   RotaryTurn<VEC, LPR, NP, IL> turn;
   turn.load(a.how, pos, lane);
   const void *weight = which ? a.how.k_weight : a.how.q_weight;
@@ -127,8 +127,6 @@ __global__ __launch_bounds__(kBlock) void kv_append_paged_rotary_kernel(RotaryAp
   if (live) store_row<false>(a.how, turned ? moved : row, out, lane);
 }
 
-static int64_t byte_size(int64_t rows, int heads, int D, int es) { return rows * heads * D * es; }
-
 }  // namespace en
 
 using namespace en;
@@ -148,15 +146,16 @@ extern "C" int en_qk_norm_rotary(const void *q, const void *k, void *q_out, void
   const int64_t rows = tokens * (q_heads + k_heads);
   const bool many = rows >= kManyRows;
   const int hpg = many ? 4 : 1;
-  RotaryRowsArgs a{rotary_how(how, size_per_head), {q, k}, {q_out, k_out}, {strides[0], strides[2]}, {strides[1], strides[3]},
+  const bool il = how->interleaved != 0;
+  const RotaryForm form = rotary_form(size_per_head, how->rotary_dim, il, dtype);
+  RotaryRowsArgs a{rotary_how(how, size_per_head, form.vec), {q, k}, {q_out, k_out}, {strides[0], strides[2]}, {strides[1], strides[3]},
                    {strides[4], strides[6]}, {strides[5], strides[7]}, {q_heads, k_heads},
                    {(int)ceil_div(q_heads, hpg), (int)ceil_div(k_heads, hpg)}, cu_seqlens, positions, batch, 0, 0};
   const int64_t groups = tokens * (a.parts[0] + a.parts[1]);
   if (groups > INT32_MAX) return EN_ERR_SHAPE;
   a.tokens = (uint32_t)tokens;
   a.groups = (uint32_t)groups;
-  const bool il = how->interleaved != 0, nt = byte_size(tokens, q_heads + k_heads, size_per_head, es) >= kStreamStoreBytes;
-  const RotaryForm form = rotary_form(size_per_head, how->rotary_dim, il, dtype);
+  const int64_t bytes = tokens * (q_heads + k_heads) * size_per_head * es;
   const hipStream_t s = (hipStream_t)stream;
   auto launch = [&](auto dt) {
     constexpr int DT = decltype(dt)::value;
@@ -165,8 +164,9 @@ extern "C" int en_qk_norm_rotary(const void *q, const void *k, void *q_out, void
       constexpr bool IL = decltype(inter)::value;
       const unsigned grid = (unsigned)ceil_div(groups, kBlock / LPR);
       if (!many) qk_norm_rotary_kernel<DT, VEC, LPR, NP, IL, 1, false><<<grid, kBlock, 0, s>>>(a);
-      else if (!nt) qk_norm_rotary_kernel<DT, VEC, LPR, NP, IL, 4, false><<<grid, kBlock, 0, s>>>(a);
-      else qk_norm_rotary_kernel<DT, VEC, LPR, NP, IL, 4, true><<<grid, kBlock, 0, s>>>(a);
+      else if (bytes < kStreamStoreBytes) qk_norm_rotary_kernel<DT, VEC, LPR, NP, IL, 4, false><<<grid, kBlock, 0, s>>>(a);
+      else if (bytes < kStreamLoadBytes) qk_norm_rotary_kernel<DT, VEC, LPR, NP, IL, 4, true><<<grid, kBlock, 0, s>>>(a);
+      else qk_norm_rotary_kernel<DT, VEC, LPR, NP, IL, 4, true, true><<<grid, kBlock, 0, s>>>(a);
     });
   };
   const bool known = dtype == EN_F32 ? launch(Int<EN_F32>{}) : dtype == EN_F16 ? launch(Int<EN_F16>{}) : launch(Int<EN_BF16>{});
@@ -190,11 +190,11 @@ extern "C" int en_kv_append_paged_rotary(const void *q, const void *k_new, const
   if (batch == 0) return EN_OK;
   const int64_t rows = (int64_t)batch * (q_heads + 2 * (int64_t)k_heads);
   if (rows > INT32_MAX) return EN_ERR_SHAPE;
-  const RotaryAppendArgs a{rotary_how(how, size_per_head), q, k_new, v_new, q_out, k_pool, v_pool, kv_lens, page_table,
-                           strides[0], strides[1], strides[2], strides[3], strides[4], strides[5], pool_strides[0], pool_strides[1],
-                           pool_strides[2], batch, q_heads, k_heads, max_pages_per_seq, page_size, num_pages, (uint32_t)rows, overflow};
   const bool il = how->interleaved != 0;
   const RotaryForm form = rotary_form(size_per_head, how->rotary_dim, il, dtype);
+  const RotaryAppendArgs a{rotary_how(how, size_per_head, form.vec), q, k_new, v_new, q_out, k_pool, v_pool, kv_lens, page_table,
+                           strides[0], strides[1], strides[2], strides[3], strides[4], strides[5], pool_strides[0], pool_strides[1],
+                           pool_strides[2], batch, q_heads, k_heads, max_pages_per_seq, page_size, num_pages, (uint32_t)rows, overflow};
   const hipStream_t s = (hipStream_t)stream;
   auto launch = [&](auto dt) {
     constexpr int DT = decltype(dt)::value;

@@ -1,8 +1,9 @@
 // One head's row on its way from the projection: RMS norm over its channels and rotation by its position, in registers.
 //
 // A row of D channels is taken by LPR lanes, NP units each; a unit is two vectors of VEC channels, a and b, that hold both channels
-// of every pair they have a part in, so that the rotation needs no other lane: channels u VEC .. and R/2 + u VEC .. of the rotated part,
-// or neighbouring vectors (of the rest of the row, and wherever pairs are neighbouring channels).  Only the norm's sum crosses lanes.
+// of every pair they have a part in, so that the rotation needs no other lane: channels u VEC .. and R/2 + u VEC .. of the rotated part; where
+// pairs are neighbouring channels, and in the rest of the row, any two, and those are taken whose neighbours the neighbouring lanes take, so
+// that a load fills cache lines (4 prompts of 8000, 80 heads x 128, neighbouring pairs 357 -> KKK us).  Only the norm's sum crosses lanes.
 // VEC is the largest of 8 (16-bit rows), 4, 2, 1 that divides R/2 and D (interleaved: R and D), a property of the head alone:
 // loads and stores take any element's address.
 #pragma once
@@ -30,10 +31,10 @@ template <> struct LooseType<4, 8> { typedef u32x2_by4 type; };
 template <> struct LooseType<4, 16> { typedef u32x4_by4 type; };
 
 // VEC elements at an address aligned to one of them.
-template <typename T, int VEC>
+template <typename T, int VEC, bool NT = false>
 __device__ __forceinline__ Pack<T, VEC> load_loose(const T *p) {
   typedef typename LooseType<sizeof(T), sizeof(T) * VEC>::type W;
-  const W w = *reinterpret_cast<const W *>(p);
+  const W w = NT ? __builtin_nontemporal_load(reinterpret_cast<const W *>(p)) : *reinterpret_cast<const W *>(p);
   Pack<T, VEC> r;
   __builtin_memcpy(&r, &w, sizeof(r));
   return r;
@@ -51,6 +52,7 @@ struct RotaryHow {
   const float *cos, *sin;
   const void *q_weight, *k_weight;
   int rows, R, D;
+  int rest;             // half the vectors behind the rotated part, rounded up: how far apart the two of a unit there are
   float eps;
 };
 
@@ -62,23 +64,24 @@ template <int DT, int VEC, int LPR, int NP, bool IL> struct RotaryRow {
 
   // First channel of vector `half` of unit u; D or more where the row has none.
   __device__ static __forceinline__ int channel(const RotaryHow &w, int u, int half) {
-    if (IL) return VEC == 1 ? 2 * u + half : (2 * u + half) * VEC;
+    if (IL) return VEC == 1 ? 2 * u + half : (u + half * LPR * NP) * VEC;
     const int turned = w.R / 2 / VEC;
     if (u < turned) return u * VEC + half * (w.R / 2);
-    return w.R + (2 * (u - turned) + half) * VEC;
+    return u - turned < w.rest ? w.R + (u - turned + half * w.rest) * VEC : w.D;
   }
-  __device__ __forceinline__ void load(const RotaryHow &w, const T *row, int lane) {
+  template <bool NT = false> __device__ __forceinline__ void load(const RotaryHow &w, const T *row, int lane) {
 #pragma unroll
     for (int i = 0; i < NP; ++i)
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
         const int c = channel(w, lane + i * LPR, half);
-        raw[i][half] = load_loose<T, VEC>(row + (c < w.D ? c : 0));
+        raw[i][half] = load_loose<T, VEC, NT>(row + (c < w.D ? c : 0));
       }
   }
 };
 
-// The cos and sin of a lane's units at one position: f[0] cos, f[1] sin, VEC pairs a unit (interleaved: VEC of the unit's two vectors).
+// The cos and sin of a lane's units at one position: f[0] cos, f[1] sin.  VEC pairs a unit; of neighbouring pairs, the first half of them
+// is the first vector's.
 template <int VEC, int LPR, int NP, bool IL> struct RotaryTurn {
   float f[NP][2][VEC];
 
@@ -86,39 +89,50 @@ template <int VEC, int LPR, int NP, bool IL> struct RotaryTurn {
     const bool in = (uint64_t)pos < (uint64_t)w.rows;
     const int half_dim = w.R / 2;
     const int64_t at = (in ? pos : 0) * half_dim;
+    constexpr int PER = IL && VEC > 1 ? VEC / 2 : VEC, N = PER < 4 ? PER : 4;      // pairs a vector; R is made of vectors
 #pragma unroll
-    for (int i = 0; i < NP; ++i) {
-      const int first = (lane + i * LPR) * VEC;        // first pair of the unit: VEC pairs, contiguous in either form
+    for (int i = 0; i < NP; ++i)
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) {
-        f[i][0][e] = 1.f;
-        f[i][1][e] = 0.f;
-      }
-      if (first < half_dim) {
-        constexpr int N = IL && VEC > 1 ? VEC / 2 : VEC < 4 ? VEC : 4;      // what R is made of
+      for (int e = 0; e < VEC; e += N) {
+        const int u = lane + i * LPR, first = PER == VEC ? u * VEC + e : (u + (e / PER) * LPR * NP) * PER + e % PER;
+        const bool turned = first < half_dim;
+        const Pack<float, N> c = turned ? load_loose<float, N>(w.cos + at + first) : Pack<float, N>{},
+                             s = turned ? load_loose<float, N>(w.sin + at + first) : Pack<float, N>{};
 #pragma unroll
-        for (int e = 0; e < VEC; e += N) {
-          if (first + e >= half_dim) break;            // a unit of neighbouring pairs whose second vector is not rotated
-          const Pack<float, N> c = load_loose<float, N>(w.cos + at + first + e), s = load_loose<float, N>(w.sin + at + first + e);
-#pragma unroll
-          for (int j = 0; j < N; ++j) {
-            f[i][0][e + j] = in ? c.v[j] : __builtin_nanf("");
-            f[i][1][e + j] = in ? s.v[j] : __builtin_nanf("");
-          }
+        for (int j = 0; j < N; ++j) {
+          f[i][0][e + j] = in ? c.v[j] : __builtin_nanf("");
+          f[i][1][e + j] = in ? s.v[j] : __builtin_nanf("");
         }
       }
-    }
   }
 };
 
-// y of the row in `r`, in place.  Called by all lanes of the wave.
-template <int DT, int VEC, int LPR, int NP, bool IL>
+__device__ __forceinline__ float fused(float a, float b, float c) { return __builtin_fmaf(a, b, c); }
+__device__ __forceinline__ double fused(double a, double b, double c) { return __builtin_fma(a, b, c); }
+template <int DT> __device__ __forceinline__ typename Elem<DT>::T round_to(float v) { return Elem<DT>::from_float(v); }
+// From 64 bits by way of 32, rounded there to odd: the second rounding is then the only one.
+template <int DT> __device__ __forceinline__ typename Elem<DT>::T round_to(double v) {
+  const float f = (float)v;
+  uint32_t u = __float_as_uint(f);
+  const double back = (double)f;
+  if (back != v && v == v && f != 0.f && !(u & 1)) u += (back < v) == (f > 0.f) ? 1 : -1;      // towards v, which lies between f and its odd neighbour
+  return Elem<DT>::from_float(__uint_as_float(u));
+}
+template <int WIDTH> __device__ __forceinline__ float lanes_sum(float v) { return group_allreduce<OpSum, WIDTH>(v); }
+template <int WIDTH> __device__ __forceinline__ double lanes_sum(double v) {
+#pragma unroll
+  for (int m = 1; m < WIDTH; m *= 2) v += __shfl_xor(v, m, kWave);
+  return v;
+}
+
+// y of the row in `r`, in place, computed in A.  Called by all lanes of the wave.
+template <typename A = float, int DT, int VEC, int LPR, int NP, bool IL>
 __device__ __forceinline__ void norm_and_turn(const RotaryHow &w, RotaryRow<DT, VEC, LPR, NP, IL> &r, const RotaryTurn<VEC, LPR, NP, IL> &turn,
                                               const void *weight, int lane) {
   typedef Elem<DT> E;
   typedef typename E::T T;
   typedef RotaryRow<DT, VEC, LPR, NP, IL> Row;
-  float x[NP][2][VEC];
+  A x[NP][2][VEC];
 #pragma unroll
   for (int i = 0; i < NP; ++i)
 #pragma unroll
@@ -126,7 +140,7 @@ __device__ __forceinline__ void norm_and_turn(const RotaryHow &w, RotaryRow<DT, 
 #pragma unroll
       for (int e = 0; e < VEC; ++e) x[i][half][e] = E::to_float(r.raw[i][half].v[e]);
   if (weight) {
-    float s = 0.f;
+    A s = 0;
 #pragma unroll
     for (int i = 0; i < NP; ++i)
 #pragma unroll
@@ -134,8 +148,7 @@ __device__ __forceinline__ void norm_and_turn(const RotaryHow &w, RotaryRow<DT, 
         if (Row::channel(w, lane + i * LPR, half) < w.D)
 #pragma unroll
           for (int e = 0; e < VEC; ++e) s += x[i][half][e] * x[i][half][e];
-    s = group_allreduce<OpSum, LPR>(s);
-    const float inv = 1.0f / sqrtf(s / (float)w.D + w.eps);
+    const A inv = A(1) / sqrt(lanes_sum<LPR>(s) / A(w.D) + A(w.eps));
 #pragma unroll
     for (int i = 0; i < NP; ++i)
 #pragma unroll
@@ -143,7 +156,7 @@ __device__ __forceinline__ void norm_and_turn(const RotaryHow &w, RotaryRow<DT, 
         const int c = Row::channel(w, lane + i * LPR, half);
         const Pack<T, VEC> g = load_loose<T, VEC>(reinterpret_cast<const T *>(weight) + (c < w.D ? c : 0));
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) x[i][half][e] *= inv * E::to_float(g.v[e]);
+        for (int e = 0; e < VEC; ++e) x[i][half][e] = x[i][half][e] * inv * A(E::to_float(g.v[e]));
       }
   }
 #pragma unroll
@@ -154,24 +167,24 @@ __device__ __forceinline__ void norm_and_turn(const RotaryHow &w, RotaryRow<DT, 
 #pragma unroll
         for (int e = 0; e < VEC; e += 2) {
           const bool turned = Row::channel(w, lane + i * LPR, half) < w.R;      // the others stay what they are, infinities too
-          const float c = turn.f[i][0][(half * VEC + e) / 2], s = turn.f[i][1][(half * VEC + e) / 2];
-          const float a = x[i][half][e], b = x[i][half][e + 1];
-          x[i][half][e] = turned ? __builtin_fmaf(a, c, -(b * s)) : a;
-          x[i][half][e + 1] = turned ? __builtin_fmaf(b, c, a * s) : b;
+          const A c = turn.f[i][0][(half * VEC + e) / 2], s = turn.f[i][1][(half * VEC + e) / 2];
+          const A a = x[i][half][e], b = x[i][half][e + 1];
+          x[i][half][e] = turned ? fused(a, c, -(b * s)) : a;
+          x[i][half][e + 1] = turned ? fused(b, c, a * s) : b;
         }
     } else {
 #pragma unroll
       for (int e = 0; e < VEC; ++e) {
         const bool turned = (lane + i * LPR) * VEC < w.R / 2;
-        const float a = x[i][0][e], b = x[i][1][e];
-        x[i][0][e] = turned ? __builtin_fmaf(a, turn.f[i][0][e], -(b * turn.f[i][1][e])) : a;
-        x[i][1][e] = turned ? __builtin_fmaf(b, turn.f[i][0][e], a * turn.f[i][1][e]) : b;
+        const A a = x[i][0][e], b = x[i][1][e], c = turn.f[i][0][e], s = turn.f[i][1][e];
+        x[i][0][e] = turned ? fused(a, c, -(b * s)) : a;
+        x[i][1][e] = turned ? fused(b, c, a * s) : b;
       }
     }
 #pragma unroll
     for (int half = 0; half < 2; ++half)
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) r.raw[i][half].v[e] = E::from_float(x[i][half][e]);
+      for (int e = 0; e < VEC; ++e) r.raw[i][half].v[e] = round_to<DT>(x[i][half][e]);
   }
 }
 
@@ -209,8 +222,10 @@ inline int check_rotary(const en_norm_rotary *how, int D) {
   if (!aligned_to(how->cos, 4) || !aligned_to(how->sin, 4)) return EN_ERR_ALIGN;
   return EN_OK;
 }
-inline RotaryHow rotary_how(const en_norm_rotary *how, int D) {
-  return RotaryHow{how->cos, how->sin, how->q_weight, how->k_weight, how->table_rows, how->rotary_dim, D, how->eps};
+// `vec`: the form's vector.
+inline RotaryHow rotary_how(const en_norm_rotary *how, int D, int vec) {
+  return RotaryHow{how->cos, how->sin, how->q_weight, how->k_weight, how->table_rows, how->rotary_dim, D,
+                   (int)ceil_div(D - how->rotary_dim, 2 * vec), how->eps};
 }
 
 // Calls f(VEC, LPR, NP, interleaved) as integral constants for the form of this head; false where there is none.

@@ -194,7 +194,7 @@ def test_fill_without_pages_and_strided():
     (F16, E4, 5, 1, 112, 14, False, True), (F16, I8, 2, 2, 16, 16, True, False),
 ])
 def test_append_turns(dtype, code, Hq, H, D, R, il, norm):
-    """The rows of qk_norm_rotary at the lengths, in the tails and, where they complete a block, in the pages."""
+    """Queries and keys normed and turned to the nearest number of their type; keys in the tails and, where they complete a block, in the pages."""
     K = _K()
     announce("kv8 append turns", dtype, code, Hq, H, D, R, il, norm)
     g = torch.Generator().manual_seed(D)
@@ -212,16 +212,14 @@ def test_append_turns(dtype, code, Hq, H, D, R, il, norm):
     rot = K.rotary_table(100, R)
     at = torch.tensor(lens, dtype=torch.int32).cuda()
     kw = dict(q_weight=gains[0], k_weight=gains[1], interleaved=il)
-    want_q, turned = K.qk_norm_rotary(q, k, B, None, rot, positions=at, **kw)
     got = K.kv8_pages_append(q, k, v, dev, at, rot, **kw)
-    # the norm's sum is taken over other lanes than there: a step of the type at most, and so a code
-    step = torch.finfo(dtype).eps
-    near = lambda a, b: bool(((a.float() - b.float()).abs() <= step * b.float().abs() + 2.0 ** -24).all())  # noqa: E731
-    assert near(got, want_q) if norm else torch.equal(got, want_q)
+    turned = torch.stack([dev[4][b, :, lens[b] % 16] for b in range(B)])
+    for y, r, w in ((got, q, gains[0]), (turned, k, gains[1])):
+        want, size = ref.norm_rotary(r.cpu(), at.cpu().long(), tuple(t.cpu() for t in rot), None if w is None else w.cpu(), 1e-6, il)
+        # computed in 64 bits: half a step of the type, and of its smallest numbers
+        assert bool(((y.double().cpu() - want).abs() <= torch.finfo(dtype).eps / 2 * want.abs() + 2.0 ** -40 * size + (2.0 ** -25 if dtype == F16 else 0.0)).all())
     for b in range(B):
         n = lens[b]
-        assert near(dev[4][b, :, n % 16], turned[b]) if norm else torch.equal(dev[4][b, :, n % 16], turned[b])
-        turned[b] = dev[4][b, :, n % 16]
         ref.put(cache, b, torch.cat((ks[b], turned[b].cpu()[:, None]), 1), torch.cat((vs[b], v[b].cpu()[:, None]), 1))
         if n % 16 == 15:                               # the tail keeps its last row
             cache[4][b, :, 15], cache[5][b, :, :, 15] = turned[b].cpu(), v[b].cpu()
