@@ -9,7 +9,9 @@
 namespace en {
 
 // Two 16-bit elements as a word, at any element's address.
-template <typename T> __device__ __forceinline__ uint32_t load_two(const T *p) { return __builtin_bit_cast(uint32_t, load_loose<T, 2>(p)); }
+template <typename T, bool NT = false> __device__ __forceinline__ uint32_t load_two(const T *p) {
+  return __builtin_bit_cast(uint32_t, load_loose<T, 2, NT>(p));
+}
 template <int DT> __device__ __forceinline__ float low_value(uint32_t w) {
   return Elem<DT>::to_float(__builtin_bit_cast(typename Elem<DT>::T, (uint16_t)w));
 }
@@ -61,6 +63,22 @@ template <int D> struct ValueBlock {
   __device__ static __forceinline__ int first(int lane) { return lane / kLanes * kEach; }
 };
 
+// The same of a tail, which has the positions of a channel side by side.
+template <int D> __device__ __forceinline__ void value_rows(const uint16_t *tail, int lane, uint32_t (&raw)[ValueBlock<D>::kEach]) {
+  typedef ValueBlock<D> V;
+  const uint16_t *from = tail + 2 * V::pair(lane) * kBlk + V::first(lane);
+#pragma unroll
+  for (int i = 0; i < V::kEach; i += 8) {
+    const uint4 lo = *reinterpret_cast<const uint4 *>(from + i), hi = *reinterpret_cast<const uint4 *>(from + kBlk + i);
+    const uint32_t l[4] = {lo.x, lo.y, lo.z, lo.w}, u[4] = {hi.x, hi.y, hi.z, hi.w};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      raw[i + 2 * e] = (l[e] & 0xffffu) | u[e] << 16;
+      raw[i + 2 * e + 1] = l[e] >> 16 | (u[e] & 0xffff0000u);
+    }
+  }
+}
+
 template <int DT, int CODE, int D>
 __device__ __forceinline__ void put_value_block(const ValueBlock<D> &v, uint8_t *codes, float *scale, int lane) {
   typedef ValueBlock<D> V;
@@ -100,7 +118,7 @@ struct Kv8FillArgs {
 };
 
 // Grid: blocks of the longest sequence (its last may be a tail) x 2 heads (keys, values) x sequences; four waves a workgroup.
-template <int DT, int CODE, int D>
+template <int DT, int CODE, int D, bool NT>
 __global__ __launch_bounds__(kBlock) void kv8_fill_kernel(Kv8FillArgs a) {
   typedef typename Elem<DT>::T T;
   const int lane = threadIdx.x % kWave, unit = blockIdx.y * (kBlock / kWave) + threadIdx.x / kWave;
@@ -115,17 +133,21 @@ __global__ __launch_bounds__(kBlock) void kv8_fill_kernel(Kv8FillArgs a) {
   const int64_t step = is_v ? a.v_token : a.k_token;
   src += (int64_t)(start + j * kBlk) * step;
   const int64_t tail = ((int64_t)b * H + h) * kBlk * D;
-  const int id = kv8_page(a.c, b, j), blk = kv8_block_in_page(a.c, j);
-  if (id < 0) {
-    if (!is_v && h == 0 && lane == 0 && a.overflow) atomicAdd(a.overflow, rows);
-    return;
-  }
+  const int blk = kv8_block_in_page(a.c, j);
+  int id;
+  // the rows are on their way before the page is asked for
+  auto no_page = [&]() {
+    id = kv8_page(a.c, b, j);
+    if (id < 0 && !is_v && h == 0 && lane == 0 && a.overflow) atomicAdd(a.overflow, rows);
+    return id < 0;
+  };
   if (!is_v) {
     typedef KeyBlock<D> K;
     K k;
 #pragma unroll
     for (int i = 0; i < K::kEach; ++i)
-      k.raw[i] = __builtin_bit_cast(uint4, load_loose<T, 8>(src + min(K::row(i, lane), rows - 1) * step + K::channel(i, lane)));
+      k.raw[i] = __builtin_bit_cast(uint4, load_loose<T, 8, NT>(src + min(K::row(i, lane), rows - 1) * step + K::channel(i, lane)));
+    if (no_page()) return;
     if (rows == kBlk) {
       put_key_block<DT, CODE, D>(k, kv8_k_block(a.c, id, h, blk, D), a.c.ks + kv8_k_scale(a.c, id, h, blk), lane);
     } else {
@@ -138,7 +160,8 @@ __global__ __launch_bounds__(kBlock) void kv8_fill_kernel(Kv8FillArgs a) {
     typedef ValueBlock<D> V;
     V v;
 #pragma unroll
-    for (int i = 0; i < V::kEach; ++i) v.raw[i] = load_two<T>(src + min(V::first(lane) + i, rows - 1) * step + 2 * V::pair(lane));
+    for (int i = 0; i < V::kEach; ++i) v.raw[i] = load_two<T, NT>(src + min(V::first(lane) + i, rows - 1) * step + 2 * V::pair(lane));
+    if (no_page()) return;
     if (rows == kBlk) {
       put_value_block<DT, CODE, D>(v, kv8_v_block(a.c, id, h, blk, D), a.c.vs + kv8_v_scale(a.c, id, h, blk), lane);
     } else if (V::has(lane)) {
@@ -234,16 +257,7 @@ __global__ __launch_bounds__(kBlock) void kv8_append_kernel(Kv8AppendArgs a) {
     uint16_t *vt = reinterpret_cast<uint16_t *>(a.c.vt) + tail + 2 * V::pair(lane) * kBlk;
     V v;
     if (full) {
-#pragma unroll
-      for (int i = 0; i < V::kEach; i += 8) {
-        const uint4 lo = *reinterpret_cast<const uint4 *>(vt + V::first(lane) + i), hi = *reinterpret_cast<const uint4 *>(vt + kBlk + V::first(lane) + i);
-        const uint32_t l[4] = {lo.x, lo.y, lo.z, lo.w}, u[4] = {hi.x, hi.y, hi.z, hi.w};
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          v.raw[i + 2 * e] = (l[e] & 0xffffu) | u[e] << 16;
-          v.raw[i + 2 * e + 1] = l[e] >> 16 | (u[e] & 0xffff0000u);
-        }
-      }
+      value_rows<D>(reinterpret_cast<const uint16_t *>(a.c.vt) + tail, lane, v.raw);
       if (V::first(lane) + V::kEach == kBlk) v.raw[V::kEach - 1] = now;
     }
     if (V::has(lane) && V::first(lane) == 0) {
@@ -264,7 +278,7 @@ struct Kv8ReadArgs {
 };
 
 // Grid: blocks that seq_len positions can touch x 2 heads x sequences; a wave a block, its rows written where they fall into the range.
-template <int DT, int CODE, int D>
+template <int DT, int CODE, int D, bool NT>
 __global__ __launch_bounds__(kBlock) void kv8_read_kernel(Kv8ReadArgs a) {
   typedef Elem<DT> E;
   typedef typename E::T T;
@@ -307,7 +321,7 @@ __global__ __launch_bounds__(kBlock) void kv8_read_kernel(Kv8ReadArgs a) {
       } else if (r < there && there < kBlk) {
         w = *reinterpret_cast<const uint4 *>(reinterpret_cast<const T *>(a.c.kt) + tail + r * D + c);
       }
-      if (K::has(i, lane) && r >= lo && r < hi) *reinterpret_cast<uint4 *>(out + (int64_t)r * D + c) = w;
+      if (K::has(i, lane) && r >= lo && r < hi) store16<NT>(out + (int64_t)r * D + c, w);
     }
   } else {
     typedef ValueBlock<D> V;
@@ -327,13 +341,21 @@ __global__ __launch_bounds__(kBlock) void kv8_read_kernel(Kv8ReadArgs a) {
         row[i + 3] = two(Codes<CODE>::template value<3>(w0), Codes<CODE>::template value<3>(w1));
       }
     } else {
-      const uint16_t *vt = reinterpret_cast<const uint16_t *>(a.c.vt) + tail + 2 * c * kBlk + p0;
 #pragma unroll
-      for (int i = 0; i < V::kEach; ++i) row[i] = p0 + i < there && there < kBlk ? vt[i] | (uint32_t)vt[kBlk + i] << 16 : 0u;
+      for (int i = 0; i < V::kEach; ++i) row[i] = 0;
+      if (there > 0 && there < kBlk) {
+        value_rows<D>(reinterpret_cast<const uint16_t *>(a.c.vt) + tail, lane, row);
+#pragma unroll
+        for (int i = 0; i < V::kEach; ++i) row[i] = p0 + i < there ? row[i] : 0u;
+      }
     }
 #pragma unroll
     for (int i = 0; i < V::kEach; ++i)
-      if (V::has(lane) && p0 + i >= lo && p0 + i < hi) *reinterpret_cast<uint32_t *>(out + (int64_t)(p0 + i) * D + 2 * c) = row[i];
+      if (V::has(lane) && p0 + i >= lo && p0 + i < hi) {
+        uint32_t *to = reinterpret_cast<uint32_t *>(out + (int64_t)(p0 + i) * D + 2 * c);
+        if constexpr (NT) __builtin_nontemporal_store(row[i], to);
+        else *to = row[i];
+      }
   }
 }
 
@@ -374,7 +396,9 @@ extern "C" int en_kv8_fill(const void *k, const void *v, const en_kv8_cache *cac
   const dim3 grid((unsigned)ceil_div(max_seq_len, kBlk), (unsigned)ceil_div(2 * (int64_t)cache->head_num, kBlock / kWave), (unsigned)cache->batch);
   if (grid.y > 65535) return EN_ERR_SHAPE;
   with_kv8_form(cache, [&](auto dt, auto code, auto d) {
-    kv8_fill_kernel<decltype(dt)::value, decltype(code)::value, decltype(d)::value><<<grid, kBlock, 0, (hipStream_t)stream>>>(a);
+    constexpr int DT = decltype(dt)::value, CODE = decltype(code)::value, D = decltype(d)::value;
+    if (4 * tokens * cache->head_num * D >= kStreamLoadBytes) kv8_fill_kernel<DT, CODE, D, true><<<grid, kBlock, 0, (hipStream_t)stream>>>(a);
+    else kv8_fill_kernel<DT, CODE, D, false><<<grid, kBlock, 0, (hipStream_t)stream>>>(a);
   });
   EN_RETURN_IF_LAUNCH_FAILED();
   return EN_OK;
@@ -414,7 +438,9 @@ extern "C" int en_kv8_read(const en_kv8_cache *cache, const int32_t *kv_lens, co
                   (unsigned)cache->batch);
   if (grid.y > 65535) return EN_ERR_SHAPE;
   with_kv8_form(cache, [&](auto dt, auto code, auto d) {
-    kv8_read_kernel<decltype(dt)::value, decltype(code)::value, decltype(d)::value><<<grid, kBlock, 0, (hipStream_t)stream>>>(a);
+    constexpr int DT = decltype(dt)::value, CODE = decltype(code)::value, D = decltype(d)::value;
+    if (4ll * cache->batch * cache->head_num * seq_len * D >= kStreamStoreBytes) kv8_read_kernel<DT, CODE, D, true><<<grid, kBlock, 0, (hipStream_t)stream>>>(a);
+    else kv8_read_kernel<DT, CODE, D, false><<<grid, kBlock, 0, (hipStream_t)stream>>>(a);
   });
   EN_RETURN_IF_LAUNCH_FAILED();
   return EN_OK;

@@ -74,57 +74,56 @@ struct RotaryAppendArgs {
   const int32_t *lens, *table;
   int64_t q_sb, q_sh, k_sb, k_sh, v_sb, v_sh, p_page, p_head, p_row;
   int B, Hq, Hk, max_pages, page, num_pages;
-  uint32_t rows;                // B * (Hq + 2 Hk)
+  int parts_q, parts_k;
+  uint32_t groups;              // B * (parts_q + 2 parts_k)
   int32_t *overflow;
 };
 
-// One row a lane group: a decode step has few rows, and what counts is that all of them are on their way at once.
-template <int DT, int VEC, int LPR, int NP, bool IL>
+// HPG rows of one sequence and kind a lane group: one while a decode step's rows are few and what counts is that all of them are on their
+// way at once, two where they are many and each group's cos and sin are as much to load as a row.
+template <int DT, int VEC, int LPR, int NP, bool IL, int HPG>
 __global__ __launch_bounds__(kBlock) void kv_append_paged_rotary_kernel(RotaryAppendArgs a) {
   typedef typename Elem<DT>::T T;
   typedef RotaryRow<DT, VEC, LPR, NP, IL> Row;
   const int lane = threadIdx.x % LPR;
-  const uint32_t group = blockIdx.x * (kBlock / LPR) + threadIdx.x / LPR, g = min(group, a.rows - 1);
-  const int per = a.Hq + 2 * a.Hk, b = (int)(g / per);
-  int h = (int)(g - (uint32_t)b * per);
+  const uint32_t group = blockIdx.x * (kBlock / LPR) + threadIdx.x / LPR, g = min(group, a.groups - 1);
+  const int per = a.parts_q + 2 * a.parts_k, b = (int)(g / per);
+  int part = (int)(g - (uint32_t)b * per);
+  const bool is_q = part < a.parts_q;
+  part -= is_q ? 0 : a.parts_q;
+  const bool is_v = !is_q && part >= a.parts_k;
+  part -= is_v ? a.parts_k : 0;
+  const int first = part * HPG, heads = is_q ? a.Hq : a.Hk;
+  const T *in = is_q ? reinterpret_cast<const T *>(a.q) + b * a.q_sb : is_v ? reinterpret_cast<const T *>(a.v) + b * a.v_sb
+                                                                           : reinterpret_cast<const T *>(a.k) + b * a.k_sb;
+  const int64_t in_head = is_q ? a.q_sh : is_v ? a.v_sh : a.k_sh, out_head = is_q ? a.how.D : a.p_head;
+  Row rows[HPG];
+#pragma unroll
+  for (int h = 0; h < HPG; ++h) rows[h].load(a.how, in + min(first + h, heads - 1) * in_head, lane);
   const int pos = a.lens[b];
-  const T *in;
+  const void *weight = is_q ? a.how.q_weight : is_v ? nullptr : a.how.k_weight;
   T *out;
-  bool live = group < a.rows;
-  const void *weight = nullptr;
-  bool turned = true;
-  if (h < a.Hq) {
-    in = reinterpret_cast<const T *>(a.q) + b * a.q_sb + h * a.q_sh;
-    out = reinterpret_cast<T *>(a.q_out) + ((int64_t)b * a.Hq + h) * a.how.D;
-    weight = a.how.q_weight;
+  bool live = group < a.groups;
+  if (is_q) {
+    out = reinterpret_cast<T *>(a.q_out) + (int64_t)b * a.Hq * a.how.D;
   } else {
-    h -= a.Hq;
-    const bool is_v = h >= a.Hk;
-    h -= is_v ? a.Hk : 0;
     const int pi = pos >= 0 ? pos / a.page : a.max_pages;
     const int id = pi < a.max_pages ? a.table[(int64_t)b * a.max_pages + pi] : -1;
     if ((unsigned)id >= (unsigned)a.num_pages) {
-      if (live && !is_v && h == 0 && lane == 0 && a.overflow) atomicAdd(a.overflow, 1);
+      if (live && !is_v && first == 0 && lane == 0 && a.overflow) atomicAdd(a.overflow, 1);
       live = false;
     }
-    const int64_t at = live ? id * a.p_page + h * a.p_head + (pos - (int64_t)pi * a.page) * a.p_row : 0;
-    if (is_v) {
-      in = reinterpret_cast<const T *>(a.v) + b * a.v_sb + h * a.v_sh;
-      out = reinterpret_cast<T *>(a.v_pool) + at;
-      turned = false;
-    } else {
-      in = reinterpret_cast<const T *>(a.k) + b * a.k_sb + h * a.k_sh;
-      out = reinterpret_cast<T *>(a.k_pool) + at;
-      weight = a.how.k_weight;
-    }
+    out = reinterpret_cast<T *>(is_v ? a.v_pool : a.k_pool) + (live ? id * a.p_page + (pos - (int64_t)pi * a.page) * a.p_row : 0);
   }
-  Row row;
-  row.load(a.how, in, lane);
-  RotaryTurn<VEC, LPR, NP, IL> turn;
-  turn.load(a.how, pos, lane);
-  Row moved = row;
-  norm_and_turn(a.how, moved, turn, weight, lane);
-  if (live) store_row<false>(a.how, turned ? moved : row, out, lane);
+  if (!is_v) {
+    RotaryTurn<VEC, LPR, NP, IL> turn;
+    turn.load(a.how, pos, lane);
+#pragma unroll
+    for (int h = 0; h < HPG; ++h) norm_and_turn(a.how, rows[h], turn, weight, lane);
+  }
+#pragma unroll
+  for (int h = 0; h < HPG; ++h)
+    if (live && first + h < heads) store_row<false>(a.how, rows[h], out + (first + h) * out_head, lane);
 }
 
 }  // namespace en
@@ -192,16 +191,21 @@ extern "C" int en_kv_append_paged_rotary(const void *q, const void *k_new, const
   if (rows > INT32_MAX) return EN_ERR_SHAPE;
   const bool il = how->interleaved != 0;
   const RotaryForm form = rotary_form(size_per_head, how->rotary_dim, il, dtype);
-  const RotaryAppendArgs a{rotary_how(how, size_per_head, form.vec), q, k_new, v_new, q_out, k_pool, v_pool, kv_lens, page_table,
+  const int hpg = rows >= kManyRows / 2 ? 2 : 1;
+  RotaryAppendArgs a{rotary_how(how, size_per_head, form.vec), q, k_new, v_new, q_out, k_pool, v_pool, kv_lens, page_table,
                            strides[0], strides[1], strides[2], strides[3], strides[4], strides[5], pool_strides[0], pool_strides[1],
-                           pool_strides[2], batch, q_heads, k_heads, max_pages_per_seq, page_size, num_pages, (uint32_t)rows, overflow};
+                           pool_strides[2], batch, q_heads, k_heads, max_pages_per_seq, page_size, num_pages,
+                           (int)ceil_div(q_heads, hpg), (int)ceil_div(k_heads, hpg), 0, overflow};
+  const int64_t groups = batch * (a.parts_q + 2 * (int64_t)a.parts_k);
+  a.groups = (uint32_t)groups;
   const hipStream_t s = (hipStream_t)stream;
   auto launch = [&](auto dt) {
     constexpr int DT = decltype(dt)::value;
     return with_rotary_form<DT>(form, il, [&](auto vec, auto lpr, auto np, auto inter) {
       constexpr int LPR = decltype(lpr)::value;
-      kv_append_paged_rotary_kernel<DT, decltype(vec)::value, LPR, decltype(np)::value, decltype(inter)::value>
-          <<<(unsigned)ceil_div(rows, kBlock / LPR), kBlock, 0, s>>>(a);
+      const unsigned grid = (unsigned)ceil_div(groups, kBlock / LPR);
+      if (hpg == 1) kv_append_paged_rotary_kernel<DT, decltype(vec)::value, LPR, decltype(np)::value, decltype(inter)::value, 1><<<grid, kBlock, 0, s>>>(a);
+      else kv_append_paged_rotary_kernel<DT, decltype(vec)::value, LPR, decltype(np)::value, decltype(inter)::value, 2><<<grid, kBlock, 0, s>>>(a);
     });
   };
   const bool known = dtype == EN_F32 ? launch(Int<EN_F32>{}) : dtype == EN_F16 ? launch(Int<EN_F16>{}) : launch(Int<EN_BF16>{});
