@@ -14,12 +14,12 @@ from typing import Optional
 import torch
 from torch import nn
 
-from ..kernel import (attn_fused_varlen, attn_pv, attn_qk, decode_attn, decode_pv, decode_qk, depad, repad, scale_mask_softmax,
-                      transpose_depad)
+from ..kernel import (attn_fused_varlen, attn_pv, attn_qk, decode_attn, decode_pv, decode_qk, depad, qk_norm_rotary, repad, rotary_table,
+                      scale_mask_softmax, transpose_depad)
 from ..kernel.attention import kv_cache_fill
 from ..seqinfo import SeqInfo, seq_info
 from .gemm import project
-from .kv_cache import KVCache, OutputHistory, PagedKVCache, start_history
+from .kv_cache import KVCache, OutputHistory, PagedKVCache, PagedKVCache8, start_history
 
 
 def lens_from_mask(attention_mask: torch.Tensor) -> torch.Tensor:
@@ -30,10 +30,18 @@ def lens_from_mask(attention_mask: torch.Tensor) -> torch.Tensor:
 
 
 class MultiHeadAttention1D(nn.Module):
+    """``rotary_dim`` channels of every query and key head are rotated by position (0: none; ``rotary_interleaved``: pairs of neighbouring
+    channels), ``qk_norm`` adds an RMS norm of each head before that, with a gain for queries and one for keys, and ``kv_cache_dtype``
+    (``torch.int8`` or ``torch.float8_e4m3fn``) keeps the cache in 8 bits, in pages."""
+
+    # what is not there in a module saved before there was a choice
+    rotary_dim, rotary_base, rotary_interleaved, qk_norm, kv_cache_dtype, turned = 0, 10000.0, False, False, None, False
+
     def __init__(self, hidden_size: int, num_heads: int, bias: bool = True, dtype: torch.dtype = torch.float16,
                  max_seq_len: int = 512, fused_qkv: bool = True, is_decoder: bool = True, disable_past_cache=False,
                  left_padded: Optional[bool] = None, kv_page_size: Optional[int] = None,
-                 kv_pool_pages: Optional[int] = None) -> None:
+                 kv_pool_pages: Optional[int] = None, rotary_dim: int = 0, rotary_base: float = 10000.0, rotary_interleaved: bool = False,
+                 qk_norm: bool = False, qk_norm_eps: float = 1e-6, kv_cache_dtype: Optional[torch.dtype] = None) -> None:
         super().__init__()
         if hidden_size % num_heads != 0:
             raise ValueError(f"{hidden_size} is not divisible by {num_heads}")
@@ -54,6 +62,21 @@ class MultiHeadAttention1D(nn.Module):
             self.key_ = nn.Linear(hidden_size, hidden_size, bias=bias, dtype=dtype)
             self.value_ = nn.Linear(hidden_size, hidden_size, bias=bias, dtype=dtype)
         self.dense = nn.Linear(hidden_size, hidden_size, bias=True, dtype=dtype)
+        if rotary_dim < 0 or rotary_dim % 2 or rotary_dim > self.attention_head_size:
+            raise ValueError(f"rotary_dim = {rotary_dim} must be even and at most the head size {self.attention_head_size}")
+        self.rotary_dim, self.rotary_base, self.rotary_interleaved = int(rotary_dim), float(rotary_base), bool(rotary_interleaved)
+        self.qk_norm, self.qk_norm_eps = bool(qk_norm), float(qk_norm_eps)
+        if qk_norm:
+            self.query_norm = nn.Parameter(torch.ones(self.attention_head_size, dtype=dtype))
+            self.key_norm = nn.Parameter(torch.ones(self.attention_head_size, dtype=dtype))
+        self.turned = bool(rotary_dim or qk_norm)         # queries and keys are not used as they are projected
+        self._rotary_tables = {}                          # device -> (cos, sin)
+        if kv_cache_dtype is not None:
+            if kv_cache_dtype not in (torch.int8, torch.float8_e4m3fn) or dtype not in (torch.float16, torch.bfloat16) \
+                    or self.attention_head_size % 16 or self.attention_head_size > 128:
+                raise ValueError("kv_cache_dtype must be torch.int8 or torch.float8_e4m3fn, of a float16 or bfloat16 module with heads of 16, 32, .. 128 channels")
+            kv_page_size = kv_page_size or 64
+        self.kv_cache_dtype = kv_cache_dtype
         # None: one [B,H,max_seq_len,D] buffer per cache; a page size: pages of a pool (PagedKVCache)
         self.kv_page_size = kv_page_size
         self.kv_pool_pages = kv_pool_pages
@@ -73,6 +96,23 @@ class MultiHeadAttention1D(nn.Module):
         v = project(self.value_, x).view(rows, H, D)
         return q, k, v, None
 
+    def _rotary(self, device, positions: int):
+        """The module's ``(cos, sin)`` on ``device``, for at least ``positions`` positions: as many as a cache can hold."""
+        if not self.rotary_dim:
+            return None
+        page = self.kv_page_size or 1
+        rows = (self.max_seq_len + page - 1) // page * page
+        if positions > rows:
+            raise RuntimeError(f"the batch is padded to {positions} positions but the rotation was planned for max_seq_len = {self.max_seq_len}")
+        tables = self._rotary_tables.get(device)
+        if tables is None:
+            tables = self._rotary_tables[device] = rotary_table(rows, self.rotary_dim, self.rotary_base, device)
+        return tables
+
+    def _turn_how(self) -> dict:
+        norms = (self.query_norm.detach(), self.key_norm.detach()) if self.qk_norm else (None, None)
+        return dict(q_weight=norms[0], k_weight=norms[1], eps=self.qk_norm_eps if self.qk_norm else 0.0, interleaved=self.rotary_interleaved)
+
     # ---- attention over packed tokens --------------------------------------------------------
     def forward_packed(self, x: torch.Tensor, info: SeqInfo, batch_size: int, max_seq_len: int,
                        fill_cache: bool = False) -> torch.Tensor:
@@ -80,6 +120,9 @@ class MultiHeadAttention1D(nn.Module):
         H, D = self.num_heads, self.attention_head_size
         T = x.numel() // self.hidden_size
         q, k, v, kvq = self._project(x)
+        if self.turned:
+            q, k = qk_norm_rotary(q, k, batch_size, info, self._rotary(x.device, max_seq_len), **self._turn_how())
+            kvq = None
         if x.dtype in (torch.float16, torch.bfloat16):
             ctx = attn_fused_varlen(q, k, v, batch_size, max_seq_len, info, scale=self.scaling,
                                     causal=self.is_decoder)
@@ -105,13 +148,18 @@ class MultiHeadAttention1D(nn.Module):
             raise RuntimeError(f"the batch is padded to {max_seq_len} positions but the K/V cache was planned for "
                                f"max_seq_len = {self.max_seq_len}")
         src = k if kvq is None else kvq
-        if self.kv_page_size:
+        if self.kv_cache_dtype is not None:
+            cache = PagedKVCache8(batch_size, H, self.max_seq_len, D, src.dtype, src.device, page_size=self.kv_page_size,
+                                  pool_pages=self.kv_pool_pages, code_dtype=self.kv_cache_dtype)
+        elif self.kv_page_size:
             cache = PagedKVCache(batch_size, H, self.max_seq_len, D, src.dtype, src.device,
                                  page_size=self.kv_page_size, pool_pages=self.kv_pool_pages)
         else:
             cache = KVCache(batch_size, H, self.max_seq_len, D, src.dtype, src.device, zeroed=False)
         if kvq is not None:
             cache.fill(kvq, kvq, info, 0, H, longest=max_seq_len)
+        elif self.kv_cache_dtype is not None:
+            cache.fill(k, v, info, longest=max_seq_len)
         else:
             cache.fill(k.contiguous(), v.contiguous(), info, longest=max_seq_len)
         self.kv_cache = cache       # only now: rows and lengths of a cache that was not filled are whatever the memory held
@@ -125,7 +173,10 @@ class MultiHeadAttention1D(nn.Module):
         B = last.shape[0]
         cache = self.kv_cache
         q, k, v, _ = self._project(last)
-        cache.append(k, v)
+        if self.turned:
+            q = cache.append_rotary(q, k, v, self._rotary(last.device, 0), **self._turn_how())
+        else:
+            cache.append(k, v)
         ctx = cache.attend(q, self.scaling)      # [B,H,1,D], one pass over the caches
         return project(self.dense, ctx.view(B, 1, self.hidden_size))
 

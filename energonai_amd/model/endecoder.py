@@ -34,7 +34,8 @@ class Block1D(nn.Module):
                  layernorm_epsilon: float = 1e-5, dtype: torch.dtype = torch.float16, bias: bool = True,
                  apply_post_layernorm: bool = False, max_seq_len: int = 512, fused_qkv: bool = True,
                  is_decoder: bool = True, disable_past_cache=False, kv_page_size: Optional[int] = None,
-                 kv_pool_pages: Optional[int] = None) -> None:
+                 kv_pool_pages: Optional[int] = None, rotary_dim: int = 0, rotary_base: float = 10000.0, rotary_interleaved: bool = False,
+                 qk_norm: bool = False, qk_norm_eps: float = 1e-6, kv_cache_dtype: Optional[torch.dtype] = None) -> None:
         super().__init__()
         self.apply_post_layernorm = apply_post_layernorm
         self.disable_past_cache = disable_past_cache
@@ -42,7 +43,9 @@ class Block1D(nn.Module):
         self.attn = MultiHeadAttention1D(hidden_size=hidden_size, num_heads=num_heads, bias=bias, dtype=dtype,
                                          max_seq_len=max_seq_len, fused_qkv=fused_qkv, is_decoder=is_decoder,
                                          disable_past_cache=disable_past_cache, kv_page_size=kv_page_size,
-                                         kv_pool_pages=kv_pool_pages)
+                                         kv_pool_pages=kv_pool_pages, rotary_dim=rotary_dim, rotary_base=rotary_base,
+                                         rotary_interleaved=rotary_interleaved, qk_norm=qk_norm, qk_norm_eps=qk_norm_eps,
+                                         kv_cache_dtype=kv_cache_dtype)
         self.norm2 = LayerNorm(hidden_size, eps=layernorm_epsilon, dtype=dtype)
         self.mlp = MLP1D(hidden_size=hidden_size, mlp_ratio=mlp_ratio, activation=activation, dtype=dtype, bias=bias,
                          disable_past_cache=disable_past_cache)
@@ -64,11 +67,11 @@ class Block1D(nn.Module):
         return s1 + self.mlp.forward_rows(h2)
 
     def _plain(self, attn, mlp) -> bool:
-        """True where nothing that the general form of a pre-LN block asks is out of the ordinary: the package's own modules, no
-        gradients, autocast or tuned GEMMs asked for, no global hooks, no modes that want to see the projections."""
+        """True where nothing that the general form of a pre-LN block asks is out of the ordinary: the package's own modules, queries
+        and keys as they are projected, no gradients, autocast or tuned GEMMs asked for, no global hooks, no modes that want to see the projections."""
         m = self._modules
         return not (type(self)._rows is not Block1D._rows or "_rows" in self.__dict__ or type(attn) is not MultiHeadAttention1D
-                    or type(m.get("norm1")) is not LayerNorm or type(m.get("norm2")) is not LayerNorm or not attn.fused_qkv
+                    or type(m.get("norm1")) is not LayerNorm or type(m.get("norm2")) is not LayerNorm or not attn.fused_qkv or attn.turned
                     or torch.is_grad_enabled() or torch.is_autocast_enabled() or gemm_tuning()
                     or _has_any_global_hook() or _dispatch_modes() or (_function_modes() and _modes_active()))
 

@@ -14,7 +14,8 @@ from typing import Optional
 
 import torch
 
-from ..kernel import decode_attn, decode_attn_paged, kv_cache_append, kv_cache_fill, kv_pages_append, kv_pages_fill, repad
+from ..kernel import (decode_attn, decode_attn_kv8, decode_attn_paged, kv8_pages, kv8_pages_append, kv8_pages_fill, kv_cache_append,
+                      kv_cache_fill, kv_pages_append, kv_pages_append_rotary, kv_pages_fill, qk_norm_rotary, repad)
 from ..kernel.attention import kv_cache_start
 from ..seqinfo import SeqInfo
 
@@ -73,6 +74,14 @@ class KVCache:
         kv_cache_append(k_new, v_new, self.k, self.v, self.info)
         self.lens.add_(1)
 
+    def append_rotary(self, q: torch.Tensor, k_new: torch.Tensor, v_new: torch.Tensor, rotary, **how) -> torch.Tensor:
+        """``append`` of keys normed and rotated by their position on the way; returns the queries, the same done to them (see
+        ``kernel.qk_norm_rotary`` for ``rotary`` and ``how``)."""
+        self.prepare_append()
+        q, k_new = qk_norm_rotary(q, k_new, self.batch_size, None, rotary, positions=self.lens, **how)
+        self.append(k_new, v_new.contiguous())
+        return q
+
     def attend(self, q: torch.Tensor, scale: float) -> torch.Tensor:
         """Attention of one new query per sequence over the cached positions: ``[B,H,1,D]``."""
         return decode_attn(q, self.k, self.v, self.info, scale=scale)
@@ -96,9 +105,7 @@ class PagedKVCache:
         self.page_size = page_size
         self.max_pages = (max_seq_len + page_size - 1) // page_size
         self.pool_pages = batch_size * self.max_pages if pool_pages is None else int(pool_pages)
-        self.k = torch.zeros((self.pool_pages, head_num, page_size, size_per_head), dtype=dtype, device=device)
-        self.v = torch.zeros_like(self.k)
-        self.table = torch.full((batch_size, self.max_pages), -1, dtype=torch.int32, device=device)
+        self._allocate(batch_size, head_num, size_per_head, dtype, device)
         self.lens = torch.zeros(batch_size, dtype=torch.int32, device=device)
         self.info = SeqInfo(self.lens, None, batch_size, None, self.lens)
         self.batch_size = batch_size
@@ -106,6 +113,11 @@ class PagedKVCache:
         self._free = list(range(self.pool_pages - 1, -1, -1))
         self._pages = [[] for _ in range(batch_size)]
         self._host_lens = [0] * batch_size
+
+    def _allocate(self, batch_size: int, head_num: int, size_per_head: int, dtype, device) -> None:
+        self.k = torch.zeros((self.pool_pages, head_num, self.page_size, size_per_head), dtype=dtype, device=device)
+        self.v = torch.zeros_like(self.k)
+        self.table = torch.full((batch_size, self.max_pages), -1, dtype=torch.int32, device=device)
 
     def pages_in_use(self) -> int:
         return self.pool_pages - len(self._free)
@@ -156,10 +168,13 @@ class PagedKVCache:
                 self.release(b)
         self._assign([(b, (n + P - 1) // P) for b, n in enumerate(lens_host)])
         bound = self.max_seq_len if longest is None else min(int(longest), self.max_seq_len)
-        kv_pages_fill(k_src, self.k, self.batch_size, bound, info, self.table, k_head_first)
-        kv_pages_fill(v_src, self.v, self.batch_size, bound, info, self.table, v_head_first)
+        self._fill_pages(k_src, v_src, bound, info, k_head_first, v_head_first)
         self.lens.copy_(info.lens)
         self._host_lens = lens_host
+
+    def _fill_pages(self, k_src, v_src, bound: int, info: SeqInfo, k_head_first: int, v_head_first: int) -> None:
+        kv_pages_fill(k_src, self.k, self.batch_size, bound, info, self.table, k_head_first)
+        kv_pages_fill(v_src, self.v, self.batch_size, bound, info, self.table, v_head_first)
 
     @property
     def page_table(self):
@@ -183,8 +198,51 @@ class PagedKVCache:
         self.lens.add_(1)
         self.appended()
 
+    def append_rotary(self, q: torch.Tensor, k_new: torch.Tensor, v_new: torch.Tensor, rotary, **how) -> torch.Tensor:
+        """See ``KVCache.append_rotary``; here it is one launch."""
+        self.prepare_append()
+        q = kv_pages_append_rotary(q, k_new, v_new, self.k, self.v, self.info, self.table, rotary, **how)
+        self.lens.add_(1)
+        self.appended()
+        return q
+
     def attend(self, q: torch.Tensor, scale: float) -> torch.Tensor:
         return decode_attn_paged(q, self.k, self.v, self.info, self.table, scale=scale)
+
+
+class PagedKVCache8(PagedKVCache):
+    """``PagedKVCache`` in 8 bits (int8 or float8_e4m3fn), with a scale for each block of 16 positions and head and each sequence's
+    unfinished block in 16 bits (``kernel.KV8Pages``): half the memory, and half the bytes a decode step reads.  fp16 and bf16 models, heads of
+    16, 32, .. 128 channels."""
+
+    def __init__(self, batch_size: int, head_num: int, max_seq_len: int, size_per_head: int, dtype, device, page_size: int = 64,
+                 pool_pages: Optional[int] = None, code_dtype=torch.int8):
+        self.code_dtype = code_dtype
+        super().__init__(batch_size, head_num, max_seq_len, size_per_head, dtype, device, page_size, pool_pages)
+
+    def _allocate(self, batch_size: int, head_num: int, size_per_head: int, dtype, device) -> None:
+        self.pages = kv8_pages(self.pool_pages, batch_size, head_num, self.page_size, size_per_head, self.max_pages, dtype, device, self.code_dtype)
+        self.head_num, self.table = head_num, self.pages.page_table
+
+    def _fill_pages(self, k_src, v_src, bound: int, info: SeqInfo, k_head_first: int, v_head_first: int) -> None:
+        kv8_pages_fill(k_src[:, k_head_first:k_head_first + self.head_num], v_src[:, v_head_first:v_head_first + self.head_num], self.pages,
+                       self.batch_size, bound, info)
+
+    def append(self, k_new: torch.Tensor, v_new: torch.Tensor) -> None:
+        self.prepare_append()
+        kv8_pages_append(None, k_new, v_new, self.pages, self.info)
+        self.lens.add_(1)
+        self.appended()
+
+    def append_rotary(self, q: torch.Tensor, k_new: torch.Tensor, v_new: torch.Tensor, rotary, **how) -> torch.Tensor:
+        self.prepare_append()
+        q = kv8_pages_append(q, k_new, v_new, self.pages, self.info, rotary, **how)
+        self.lens.add_(1)
+        self.appended()
+        return q
+
+    def attend(self, q: torch.Tensor, scale: float) -> torch.Tensor:
+        return decode_attn_kv8(q, self.pages, self.info, scale=scale)
 
 
 class OutputHistory:
