@@ -611,28 +611,33 @@ bool norm_rotary(PyObject *rotary, PyObject *q_weight, PyObject *k_weight, PyObj
   return gain(q_weight, out.q_weight) && gain(k_weight, out.k_weight);
 }
 
-// qk_norm_rotary(q, k, batch, SeqInfo, rotary, q_weight, k_weight, eps, interleaved) -> (q, k) or None
+// qk_norm_rotary(q, k, batch, SeqInfo or None, positions or None, rotary, q_weight, k_weight, eps, interleaved) -> (q, k) or None
 PyObject *qk_norm_rotary(PyObject *const *a) {
   const Tensor *q = plain_rows(a[0], 3), *k = plain_rows(a[1], 3);
   int64_t batch;
-  if (!q || !k || modes_on() || !whole(a[2], batch) || batch < 1) Py_RETURN_NONE;
+  if (!q || !k || modes_on() || !whole(a[2], batch) || batch < 0) Py_RETURN_NONE;
   const int64_t T = q->size(0), Hq = q->size(1), Hk = k->size(1), D = q->size(2);
   const int tag = known_tag(*q);
   en_norm_rotary how;
   Lens info;
+  const bool placed = a[4] != Py_None;
+  const Tensor *positions = placed ? plain_contiguous(a[4]) : nullptr;
+  if (placed ? !positions || positions->numel() != T || positions->scalar_type() != at::kInt || positions->device() != q->device()
+             : !fits_int({batch}) || !lens_of(a[3], *q, batch, true, info))
+    Py_RETURN_NONE;
   if (tag < 0 || k->size(0) != T || k->size(2) != D || k->scalar_type() != q->scalar_type() || k->device() != q->device() ||
-      !fits_int({Hq, Hk, D, batch}) || !lens_of(a[3], *q, batch, true, info) || !norm_rotary(a[4], a[5], a[6], a[7], a[8], *q, D, how))
+      !fits_int({Hq, Hk, D, batch + 1}) || !norm_rotary(a[5], a[6], a[7], a[8], a[9], *q, D, how))
     Py_RETURN_NONE;
   const c10::DeviceGuard guard(q->device());
-  order_stream(a[3], *q);
+  if (!placed) order_stream(a[3], *q);
   const Tensor q_out = at::empty(q->sizes(), q->options()), k_out = at::empty(k->sizes(), k->options());
   const int64_t strides[8] = {q->stride(0), q->stride(1), k->stride(0), k->stride(1), Hq * D, D, Hk * D, D};
   const void *q_p = q->data_ptr(), *k_p = k->data_ptr();
   void *qo_p = q_out.data_ptr(), *ko_p = k_out.data_ptr();
-  const int32_t *cu = i32(*info.cu);
+  const int32_t *cu = placed ? nullptr : i32(*info.cu), *at = placed ? i32(*positions) : nullptr;
   const hipStream_t stream = stream_of(*q);
   check(without_gil([&] {
-          return en_qk_norm_rotary(q_p, k_p, qo_p, ko_p, cu, nullptr, (int)batch, T, (int)Hq, (int)Hk, (int)D, strides, &how, tag, stream);
+          return en_qk_norm_rotary(q_p, k_p, qo_p, ko_p, cu, at, (int)batch, T, (int)Hq, (int)Hk, (int)D, strides, &how, tag, stream);
         }), "qk_norm_rotary");
   return tuple({q_out, k_out});
 }
@@ -1257,7 +1262,7 @@ PyMethodDef kMethods[] = {
     EN_FAST(layer_norm, 6, "layer_norm_forward of plain operands, or None"),
     EN_FAST(kv_pages_append, 7, "kv_pages_append of plain operands, or None"),
     EN_FAST(decode_attn_paged, 6, "decode_attn_paged of plain operands, or None"),
-    EN_FAST(qk_norm_rotary, 9, "qk_norm_rotary of plain operands, or None"),
+    EN_FAST(qk_norm_rotary, 10, "qk_norm_rotary of plain operands, or None"),
     EN_FAST(kv_pages_append_rotary, 13, "kv_pages_append_rotary of plain operands, or None"),
     EN_FAST(kv8_pages_fill, 7, "kv8_pages_fill of plain operands, or None"),
     EN_FAST(kv8_pages_append, 11, "kv8_pages_append of plain operands, or None"),

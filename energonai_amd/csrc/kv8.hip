@@ -393,7 +393,8 @@ extern "C" int en_kv8_fill(const void *k, const void *v, const en_kv8_cache *cac
   if (!k || !v || !cu_seqlens || !strides) return EN_ERR_NULL;
   if (!aligned_to(k, 2) || !aligned_to(v, 2)) return EN_ERR_ALIGN;
   const Kv8FillArgs a{kv8_args(cache), k, v, strides[0], strides[1], strides[2], strides[3], cu_seqlens, max_seq_len, tokens, overflow};
-  const dim3 grid((unsigned)ceil_div(max_seq_len, kBlk), (unsigned)ceil_div(2 * (int64_t)cache->head_num, kBlock / kWave), (unsigned)cache->batch);
+  const dim3 grid((unsigned)ceil_div(tokens < max_seq_len ? tokens : max_seq_len, kBlk), (unsigned)ceil_div(2 * (int64_t)cache->head_num, kBlock / kWave),
+                  (unsigned)cache->batch);
   if (grid.y > 65535) return EN_ERR_SHAPE;
   with_kv8_form(cache, [&](auto dt, auto code, auto d) {
     constexpr int DT = decltype(dt)::value, CODE = decltype(code)::value, D = decltype(d)::value;

@@ -35,10 +35,10 @@ __device__ __forceinline__ int kv8_page(const Kv8 &c, int b, int j) {
 __device__ __forceinline__ int kv8_block_in_page(const Kv8 &c, int j) { return j & ((1 << c.lg_blocks) - 1); }
 
 __device__ __forceinline__ uint8_t *kv8_k_block(const Kv8 &c, int id, int h, int blk, int D) {
-  return c.kp + (uint64_t)(uint32_t)id * c.kp_page + (uint64_t)(uint32_t)h * c.kp_head + blk * kBlk * D;
+  return c.kp + (uint64_t)(uint32_t)id * c.kp_page + (uint64_t)(uint32_t)h * c.kp_head + (uint64_t)(uint32_t)blk * (kBlk * D);
 }
 __device__ __forceinline__ uint8_t *kv8_v_block(const Kv8 &c, int id, int h, int blk, int D) {
-  return c.vp + (uint64_t)(uint32_t)id * c.vp_page + (uint64_t)(uint32_t)h * c.vp_head + blk * kBlk * D;
+  return c.vp + (uint64_t)(uint32_t)id * c.vp_page + (uint64_t)(uint32_t)h * c.vp_head + (uint64_t)(uint32_t)blk * (kBlk * D);
 }
 __device__ __forceinline__ int64_t kv8_k_scale(const Kv8 &c, int id, int h, int blk) {
   return (int64_t)((uint64_t)(uint32_t)id * c.ks_page + (uint64_t)(uint32_t)h * c.ks_head) + blk;
@@ -101,7 +101,8 @@ inline int check_kv8(const en_kv8_cache *c) {
   if (c->batch < 0 || c->head_num < 1 || c->num_pages < 1 || c->max_pages_per_seq < 0 || c->page_size < kBlk || (c->page_size & (c->page_size - 1)) ||
       c->size_per_head < 16 || c->size_per_head > 128 || c->size_per_head % 16 || (int64_t)c->max_pages_per_seq * c->page_size > INT32_MAX - kBlk)
     return EN_ERR_SHAPE;
-  if (!c->k_pages || !c->v_pages || !c->k_scales || !c->v_scales || !c->k_tail || !c->v_tail || !c->page_table) return EN_ERR_NULL;
+  if (!c->k_pages || !c->v_pages || !c->k_scales || !c->v_scales || !c->k_tail || !c->v_tail || (!c->page_table && c->max_pages_per_seq > 0 && c->batch > 0))
+    return EN_ERR_NULL;
   for (const void *p : {(const void *)c->k_pages, (const void *)c->v_pages, (const void *)c->k_tail, (const void *)c->v_tail})
     if (!aligned_to(p, 16)) return EN_ERR_ALIGN;
   for (const void *p : {(const void *)c->k_scales, (const void *)c->v_scales, (const void *)c->page_table})

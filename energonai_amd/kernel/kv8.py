@@ -9,6 +9,10 @@ history in the projection's type (energonai/model/attention.py:61-71).
 
 Heads of 16, 32, .. 128 channels, fp16 and bf16, pages of a power of two of at least 16 positions.  A page id outside the pool reads as
 zeros and is not written.
+
+A tail belongs to its sequence's place in the batch, as the row of ``page_table`` does, and holds the positions behind the last full block
+alone: a sequence that moves to another place takes both along, and a length may go back to no less than the last multiple of 16 it has
+passed (shorter: the sequence is filled again, for instance from ``kv8_pages_read``).
 """
 from __future__ import annotations
 
@@ -216,8 +220,6 @@ def decode_attn_kv8(q, cache, kv_len_list, *, scale: Optional[float] = None, out
         _lib.require_gpu(out, "out")
         if out.numel() != B * Hq * D or out.dtype != q.dtype or out.device != device:
             raise RuntimeError(f"{who}: out must be a contiguous [B,Hq,1,D] tensor of q's dtype on its device")
-    if B == 0:
-        return out
     need = decode_attn_kv8_workspace_bytes(B, Hq, c.head_num, c.max_pages_per_seq * c.page_size, D)
     if workspace is None:
         workspace = torch.empty(need, dtype=torch.uint8, device=device)

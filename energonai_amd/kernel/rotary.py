@@ -38,6 +38,26 @@ def _rows(t, name: str, who: str) -> torch.Tensor:
     return t
 
 
+def _span(t: torch.Tensor):
+    return t.data_ptr(), t.data_ptr() + (1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride()))) * t.element_size() if t.numel() else t.data_ptr()
+
+
+def _not_over(who: str, inputs, outs) -> None:
+    """Refuses results that would be written over rows still to be read: each may be its own input, or lie apart from all of them."""
+    for o in outs:
+        if any(n > 1 and s < o.shape[2] for n, s in zip(o.shape[:2], o.stride()[:2])):
+            raise RuntimeError(f"{who}: the rows of out must not overlap")
+    for i, o in enumerate(outs):
+        if o.data_ptr() == inputs[i].data_ptr() and o.stride() == inputs[i].stride():
+            continue
+        for t in inputs:
+            (a0, a1), (b0, b1) = _span(o), _span(t)
+            if a0 < b1 and b0 < a1:
+                raise RuntimeError(f"{who}: out must be q and k themselves or lie apart from them")
+    if len(outs) == 2 and outs[0].data_ptr() == outs[1].data_ptr() and outs[0].numel() and outs[1].numel():
+        raise RuntimeError(f"{who}: the two results must not share memory")
+
+
 def norm_rotary(who: str, like: torch.Tensor, rotary, q_weight, k_weight, eps, interleaved) -> _lib.NormRotary:
     """``en_norm_rotary`` of the arguments these calls share; ``like``: rows of the head size, type and device they are for."""
     D = like.shape[-1]
@@ -69,8 +89,8 @@ def qk_norm_rotary(q, k, batch_size: int, seq_len_list, rotary=None, *, q_weight
     channels NaN.  Rows behind the last sequence are left as they are (with ``positions`` every row is a token).  Returns new ``(q, k)``,
     or writes into the two tensors ``out`` names, which may be ``q`` and ``k`` themselves.  ``k`` may be ``None``."""
     who = "qk_norm_rotary"
-    if type(seq_len_list) is SeqInfo and out is None and positions is None:
-        pair = _lib.front.qk_norm_rotary(q, k, batch_size, seq_len_list, rotary, q_weight, k_weight, eps, interleaved)
+    if out is None and k is not None and (positions is not None or type(seq_len_list) is SeqInfo):
+        pair = _lib.front.qk_norm_rotary(q, k, batch_size, seq_len_list, positions, rotary, q_weight, k_weight, eps, interleaved)
         if pair is not None:
             return pair
     _rows(q, "q", who)
@@ -90,6 +110,7 @@ def qk_norm_rotary(q, k, batch_size: int, seq_len_list, rotary=None, *, q_weight
         if len(outs) != len(tensors) or any(_rows(o, "out", who).shape != t.shape or o.dtype != t.dtype or o.device != t.device
                                             for o, t in zip(outs, tensors)):
             raise RuntimeError(f"{who}: out must be a pair of tensors of q's and k's shapes, dtype and device")
+        _not_over(who, tensors, outs)
     info = None
     if positions is None:
         info = seq_info(seq_len_list, batch_size, q.device)

@@ -487,6 +487,36 @@ def test_two_captured_steps_and_streams():
     assert torch.equal(on_s, step(b))
 
 
+def test_nothing_cached():
+    """No sequences, no pages, no positions, sequences of length zero between others: nothing is read, zeros come back."""
+    K = _K()
+    announce("kv8, nothing cached")
+    H, D = 2, 64
+    none = K.kv8_pages(1, 3, H, 16, D, 0, F16, "cuda")
+    zero = torch.zeros(3, dtype=torch.int32, device="cuda")
+    many = torch.tensor([0, 5, 1 << 30], dtype=torch.int32, device="cuda")
+    q = torch.randn(3, 4, 1, D, device="cuda", dtype=F16)
+    over = torch.zeros(1, dtype=torch.int32, device="cuda")
+    x = torch.randn(3, H, D, device="cuda", dtype=F16)
+    for lens in (zero, many):
+        assert bool((K.decode_attn_kv8(q, none, lens) == 0).all())
+        assert all(bool((t == 0).all()) for t in K.kv8_pages_read(none, lens, 20))
+        K.kv8_pages_append(None, x, x, none, lens, overflow=over.zero_())
+        assert int(over) == 3
+    K.kv8_pages_fill(x, x, none, 3, 4, torch.tensor([1, 0, 2], dtype=torch.int32, device="cuda"), overflow=over.zero_())
+    assert int(over) == 3 and all(bool((t == 0).all()) for t in none[:6])
+    big = K.kv8_pages(4, 3, H, 16, D, 5000, F16, "cuda")              # capacity for the second form of the attention, no page, no position
+    assert bool((K.decode_attn_kv8(q, big, zero) == 0).all())
+    empty = K.kv8_pages(1, 0, H, 16, D, 2, F16, "cuda")
+    for call in (lambda: K.decode_attn_kv8(q[:0], empty, zero[:0]), lambda: K.kv8_pages_read(empty, zero[:0], 3)):
+        with pytest.raises(RuntimeError):                             # a batch of no sequences has no lengths, here as anywhere in the package
+            call()
+    assert K.kv8_pages_read(big, zero, 0)[0].shape == (3, H, 0, D)
+    one = K.rotary_table(4, D)
+    for t in K.qk_norm_rotary(x[:0], x[:0], 3, zero, one):
+        assert t.shape == (0, H, D)
+
+
 def test_refusals():
     K = _K()
     announce("kv8 refusals")

@@ -87,6 +87,7 @@ def test_cache_calls_refuse():
                 fn.en_kv8_read(c, PTR, None, 4, PTR, PTR, None), fn.en_decode_attn_kv8(PTR, PTR, c, PTR, 4, 1.0, PTR, ws, None)]
     assert calls(_cache(batch=0)) == [0] * 4
     assert calls(None) == [NULL] * 4
+    assert calls(_cache(batch=0, page_table=None)) == [0] * 4 and calls(_cache(page_table=None)) == [NULL] * 4
     for n in ("k_pages", "v_pages", "k_scales", "v_scales", "k_tail", "v_tail", "page_table"):
         assert calls(_cache(**{n: None})) == [NULL] * 4, n
     for kw in (dict(num_pages=0), dict(page_size=8), dict(page_size=48), dict(max_pages_per_seq=-1), dict(batch=-1), dict(head_num=0), dict(size_per_head=40),
