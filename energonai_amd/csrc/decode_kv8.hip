@@ -36,11 +36,18 @@ constexpr int kQueries = 16;                  // columns of a tile: queries that
 constexpr float kRaise = 8.f;                 // log2
 constexpr int kTeam = 8;                      // waves of a workgroup that takes one unit
 constexpr int kTeamCapacity = 1024, kTeamUnits = 512;
-// One launch of a workgroup a unit where they are all resident at once and a unit is at most two tiles a wave; otherwise runs, which any lengths
-// leave equal, and a second launch.  us, runs / a workgroup a unit, 64 positions a page: 1 sequence of 100, 12 heads x 64 8.0 / 4.7;
-// 32 of up to 500, 12 x 64 11.3 / 8.2; 32 of up to 1000, 32 / 8 x 128 15.5 / 13.4, of up to 2000 19.5 / 20.2; 8 of up to 1000 11.7 / 12.2; 1 of
-// 2000 10.3 / 18.1.  More units: 64 of up to 250, 40 x 128 30.1 / 44.6, of up to 1000 71 / 82.
-inline bool kv8_team(int64_t units, int64_t capacity) { return units <= kTeamUnits && capacity <= kTeamCapacity; }
+constexpr int kWholeCapacity = 256;
+// How units are dealt: runs of tiles, equal whatever the lengths are, at the cost of a second launch; a workgroup a unit, where they are all
+// resident at once and a unit is at most two tiles a wave; or whole units to the waves in turn, where units are many and lengths cannot differ by
+// much.  us, pages of 64: runs / a workgroup a unit: 1 sequence of 100, 12 heads x 64 8.0 / 4.7; 32 of up to 500, 12 x 64 11.3 / 8.2;
+// 32 of up to 1000, 32 / 8 x 128 15.5 / 13.4, of up to 2000 19.5 / 20.2; 8 of up to 1000 11.7 / 12.2; 1 of 2000 10.3 / 18.1; 64 of up to 250,
+// 40 x 128 30.1 / 44.6.  Runs / whole units: 66 of 1, 128 / 8 x 80 9.3 / 6.6; 64 of up to 60, 40 x 128 19.7 / 17.0; 256 of up to 100, 8 x 128
+// 22.8 / 16.5; 64 of up to 250, 40 x 128 31.3 / 30.5, of up to 500 42.9 / 47.3; 20 of up to 500, 32 x 128 18.3 / 20.3; 40 of up to 2000 64 / 96.
+enum class Deal { kTeam, kWhole, kRuns };
+inline Deal kv8_deal(int64_t units, int64_t capacity) {
+  if (units <= kTeamUnits) return capacity <= kTeamCapacity ? Deal::kTeam : Deal::kRuns;
+  return capacity <= kWholeCapacity ? Deal::kWhole : Deal::kRuns;
+}
 
 template <int DT> struct Mma;
 template <> struct Mma<EN_F16> {
@@ -106,6 +113,7 @@ struct Kv8AttnArgs {
   float *part_o;                // [2 waves][rows][D]
   float2 *part_ml;              // [2 waves][rows]
   int rows;                     // min(G, kQueries)
+  int whole;                    // waves take whole units, every kWaves-th
 };
 
 // The length of a sequence that the whole wave asks for, as a scalar load: as a vector load, waiting for it would be waiting for the
@@ -187,6 +195,7 @@ struct Kv8At {
   int b, n, tiles, tile;
   int h, chunk;
   uint32_t x;                    // its place, in tiles and units' ends
+  uint32_t u;                    // the unit's among all, where waves take whole units
 };
 
 // The keys of four rows (4t .. 4t + 3 of each of four blocks) a lane as the first product wants them: 16 channels of row l % 16, run c of 64.
@@ -220,7 +229,23 @@ __global__ __launch_bounds__(TEAM == 1 ? kBlock : TEAM * kWave, TEAM == 1 ? 1 : 
   const uint32_t units = a.c.H * a.chunks;
   uint32_t end = 0;              // of this wave's run
   Kv8At at;
-  if constexpr (TEAM == 1) {
+  // The first tile of unit u of all.
+  auto place = [&](Kv8At &c, uint32_t u) {
+    c.u = u;
+    c.b = (int)(u / units);
+    const uint32_t unit = u - (uint32_t)c.b * units;
+    c.h = (int)(unit / (uint32_t)a.chunks);
+    c.chunk = (int)unit - c.h * a.chunks;
+    c.n = kv8_wave_len(a.c, a.lens, c.b);
+    c.tiles = kv8_tiles(c.n);
+    c.tile = 0;
+  };
+  if (TEAM == 1 && a.whole) {
+    if (wave >= units * a.c.B) return;
+    end = 0xffffffffu;           // a place that none of its tiles has
+    place(at, wave);
+    at.x = 0;
+  } else if constexpr (TEAM == 1) {
     // lengths of the first 64 sequences stay in a register: few batches have more
     const int len0 = lane < a.c.B ? kv8_len(a.c, a.lens, lane) : 0;
     const uint32_t incl0 = wave_prefix(lane < a.c.B ? (kv8_tiles(len0) + kUnitCost) * units : 0u, lane);
@@ -256,19 +281,20 @@ __global__ __launch_bounds__(TEAM == 1 ? kBlock : TEAM * kWave, TEAM == 1 ? 1 : 
     // for the combine launch: the run's length, and each sequence's first tile, from the wave that comes to it
     if (wave == 0 && lane == 0) a.first_tile[a.c.B] = quota;
     at.x = x0;
+    at.u = 0;
   } else {
-    at.b = blockIdx.x / units;
-    const uint32_t unit = blockIdx.x - (uint32_t)at.b * units;
-    at.h = (int)(unit / (uint32_t)a.chunks);
-    at.chunk = (int)unit - at.h * a.chunks;
-    at.n = kv8_wave_len(a.c, a.lens, at.b);
-    at.tiles = kv8_tiles(at.n);
+    place(at, blockIdx.x);
     at.tile = (int)member;
     at.x = 0;
   }
   auto past = [&](const Kv8At &c) { return TEAM == 1 ? c.x >= end : c.tile >= c.tiles; };
   // The next unit's first tile, where it is still this wave's.
   auto next_unit = [&](Kv8At &c) {
+    if (a.whole) {
+      if (c.u + kWaves >= units * a.c.B) c.x = end;
+      else place(c, c.u + kWaves);
+      return;
+    }
     c.x += c.tiles + kUnitCost - c.tile;
     if (c.x >= end) return;
     c.tile = 0;
@@ -502,7 +528,7 @@ __global__ __launch_bounds__(TEAM == 1 ? kBlock : TEAM * kWave, TEAM == 1 ? 1 : 
   bool first_segment = true;
   // a sequence's first tile is where its first unit begins
   auto note = [&](const Kv8At &c) {
-    if (TEAM == 1 && c.tile == 0 && c.h == 0 && c.chunk == 0 && lane == 0) a.first_tile[c.b] = c.x;
+    if (TEAM == 1 && !a.whole && c.tile == 0 && c.h == 0 && c.chunk == 0 && lane == 0) a.first_tile[c.b] = c.x;
   };
   auto turn = [&](auto more) {
     later = next;
@@ -707,7 +733,7 @@ using namespace en;
 
 extern "C" int64_t en_decode_attn_kv8_workspace_bytes(int batch, int q_heads, int head_num, int capacity, int size_per_head) {
   if (batch < 1 || head_num < 1 || q_heads < head_num || q_heads % head_num || capacity < 0 || size_per_head < 1) return 0;
-  if (kv8_team((int64_t)batch * head_num * ceil_div(q_heads / head_num, kQueries), capacity)) return 0;
+  if (kv8_deal((int64_t)batch * head_num * ceil_div(q_heads / head_num, kQueries), capacity) != Deal::kRuns) return 0;
   return kv8_part_rows(q_heads, head_num) * (4 * (int64_t)size_per_head + 8) + 4 * ((int64_t)batch + 1);
 }
 
@@ -719,11 +745,13 @@ extern "C" int en_decode_attn_kv8(const void *q, void *ctx, const en_kv8_cache *
   if (!q || !ctx || !kv_lens) return EN_ERR_NULL;
   if (!aligned_to(q, 16) || !aligned_to(ctx, 16) || !aligned_to(workspace, 16)) return EN_ERR_ALIGN;
   const int64_t capacity = (int64_t)cache->max_pages_per_seq * cache->page_size;
-  const bool team = kv8_team((int64_t)cache->batch * cache->head_num * ceil_div(q_heads / cache->head_num, kQueries), capacity);
-  if (!team && !workspace) return EN_ERR_NULL;
+  const Deal deal = kv8_deal((int64_t)cache->batch * cache->head_num * ceil_div(q_heads / cache->head_num, kQueries), capacity);
+  const bool team = deal == Deal::kTeam;
+  if (deal == Deal::kRuns && !workspace) return EN_ERR_NULL;
   if (workspace_bytes < en_decode_attn_kv8_workspace_bytes(cache->batch, q_heads, cache->head_num, (int)capacity, cache->size_per_head)) return EN_ERR_SHAPE;
-  Kv8AttnArgs a{kv8_args(cache), q, ctx, kv_lens, q_heads / cache->head_num, 0, scale * 1.4426950408889634f, nullptr, nullptr, nullptr, 0};
+  Kv8AttnArgs a{kv8_args(cache), q, ctx, kv_lens, q_heads / cache->head_num, 0, scale * 1.4426950408889634f, nullptr, nullptr, nullptr, 0, 0};
   if (capacity == 0) a.c.table = kv_lens;      // no row of the table to look at: any word, which names no position
+  a.whole = deal == Deal::kWhole;
   a.chunks = (int)ceil_div(a.G, kQueries);
   a.rows = a.G < kQueries ? a.G : kQueries;
   const int64_t units = (int64_t)cache->batch * cache->head_num * a.chunks;
@@ -757,7 +785,7 @@ extern "C" int en_decode_attn_kv8(const void *q, void *ctx, const en_kv8_cache *
   if (cache->dtype == EN_F16) codes(std::integral_constant<int, EN_F16>{});
   else codes(std::integral_constant<int, EN_BF16>{});
   EN_RETURN_IF_LAUNCH_FAILED();
-  if (team) return EN_OK;
+  if (deal != Deal::kRuns) return EN_OK;
   // rows of a unit in workgroups of their own where units are few; where units are many, each has few shares
   const dim3 shares((unsigned)units, units >= 512 ? (unsigned)ceil_div(a.rows, kCombineGroups) : (unsigned)a.rows);
   if (cache->dtype == EN_F16) decode_attn_kv8_combine_kernel<EN_F16><<<shares, kBlock, 0, s>>>(a, cache->size_per_head);
