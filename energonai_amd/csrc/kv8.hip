@@ -185,25 +185,48 @@ struct Kv8AppendArgs {
   void *q_out;
   const int32_t *lens;
   int64_t q_sb, q_sh, k_sb, k_sh, v_sb, v_sh;
-  int Hq, interleaved;
-  uint32_t units;                     // B * (Hq + 2 H)
+  int Hq, parts_q, interleaved;
+  uint32_t units;                     // B * (parts_q + 2 H)
   int32_t *overflow;
 };
 
-// One row of up to 128 channels through norm and rotation, a pair a lane, from `in` to `out` and, if given, `copy`.  In 64 bits: a key that is
-// held in 8 bits is rounded twice, and of a decode step's few rows the arithmetic is not what counts (64 sequences, 48 heads x 128 KKK us, in 32 KKK).
-template <int DT, bool IL, typename T>
-__device__ __forceinline__ void turn_row(const RotaryHow &how, const T *in, int pos, const void *weight, T *out, T *copy, int lane) {
-  RotaryRow<DT, 1, kWave, 1, IL> row;
+// A row of up to 128 channels, a pair a lane.
+template <int DT, bool IL> using PairRow = RotaryRow<DT, 1, kWave, 1, IL>;
+
+// Up to kTurned heads of q of one sequence.
+constexpr int kTurned = 4;
+template <int DT, bool IL>
+__device__ __forceinline__ void turn_queries(const Kv8AppendArgs &a, int b, int first, int pos, int lane) {
+  typedef typename Elem<DT>::T T;
+  PairRow<DT, IL> rows[kTurned];
+#pragma unroll
+  for (int h = 0; h < kTurned; ++h) rows[h].load(a.how, reinterpret_cast<const T *>(a.q) + b * a.q_sb + min(first + h, a.Hq - 1) * a.q_sh, lane);
+  RotaryTurn<1, kWave, 1, IL> turn;
+  turn.load(a.how, pos, lane);
+#pragma unroll
+  for (int h = 0; h < kTurned; ++h) norm_and_turn(a.how, rows[h], turn, a.how.q_weight, lane);
+#pragma unroll
+  for (int h = 0; h < kTurned; ++h)
+    if (first + h < a.Hq) store_row<false>(a.how, rows[h], reinterpret_cast<T *>(a.q_out) + ((int64_t)b * a.Hq + first + h) * a.how.D, lane);
+}
+// A key head's new row, from `in` to the tail's row `out` and, if given, `copy`.  In 64 bits: a key that is held in 8 bits is rounded twice,
+// and of a decode step's few rows the arithmetic is not what counts (64 sequences of 8 heads x 128: no difference to be seen).
+// `has_page` is asked behind the loads.  False: nothing is written.
+template <int DT, bool IL, typename T, typename F>
+__device__ __forceinline__ bool turn_key(const RotaryHow &how, const T *in, int pos, T *out, T *copy, int lane, F &&has_page) {
+  PairRow<DT, IL> row;
   RotaryTurn<1, kWave, 1, IL> turn;
   row.load(how, in, lane);
   turn.load(how, pos, lane);
-  norm_and_turn<double>(how, row, turn, weight, lane);
+  if (!has_page()) return false;
+  norm_and_turn<double>(how, row, turn, how.k_weight, lane);
   store_row<false>(how, row, out, lane);
   if (copy) store_row<false>(how, row, copy, lane);
+  return true;
 }
 
-// A wave a row: of q, into q_out; of a key or value head, into the tail and, where it completes the block, the block into its page.
+// A wave takes a few rows of q, into q_out, or the row of a key or value head, into the tail and, where that completes the block, the block
+// into its page.
 template <int DT, int CODE, int D>
 __global__ __launch_bounds__(kBlock) void kv8_append_kernel(Kv8AppendArgs a) {
   typedef typename Elem<DT>::T T;
@@ -211,33 +234,33 @@ __global__ __launch_bounds__(kBlock) void kv8_append_kernel(Kv8AppendArgs a) {
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), lane = threadIdx.x % kWave, H = a.c.H;
   const uint32_t unit = blockIdx.x * (kBlock / kWave) + wave;
   if (unit >= a.units) return;
-  const int per = a.Hq + 2 * H, b = (int)(unit / per);
+  const int per = a.parts_q + 2 * H, b = (int)(unit / per);
   int h = (int)(unit - (uint32_t)b * per);
   const int pos = a.lens[b];
-  if (h < a.Hq) {
-    const T *in = reinterpret_cast<const T *>(a.q) + b * a.q_sb + h * a.q_sh;
-    T *out = reinterpret_cast<T *>(a.q_out) + ((int64_t)b * a.Hq + h) * D;
-    if (a.interleaved) turn_row<DT, true>(a.how, in, pos, a.how.q_weight, out, (T *)nullptr, lane);
-    else turn_row<DT, false>(a.how, in, pos, a.how.q_weight, out, (T *)nullptr, lane);
+  if (h < a.parts_q) {
+    if (a.interleaved) turn_queries<DT, true>(a, b, h * kTurned, pos, lane);
+    else turn_queries<DT, false>(a, b, h * kTurned, pos, lane);
     return;
   }
-  h -= a.Hq;
+  h -= a.parts_q;
   const bool is_v = h >= H;
   h -= is_v ? H : 0;
   const int j = pos >> 4, slot = pos & (kBlk - 1);
-  const int id = pos >= 0 ? kv8_page(a.c, b, j) : -1, blk = kv8_block_in_page(a.c, j);
-  if (id < 0) {
-    if (!is_v && h == 0 && lane == 0 && a.overflow) atomicAdd(a.overflow, 1);
-    return;
-  }
+  const int blk = kv8_block_in_page(a.c, j);
+  int id = -1;
+  auto has_page = [&]() {
+    id = pos >= 0 ? kv8_page(a.c, b, j) : -1;
+    if (id < 0 && !is_v && h == 0 && lane == 0 && a.overflow) atomicAdd(a.overflow, 1);
+    return id >= 0;
+  };
   const bool full = slot == kBlk - 1;
   const int64_t tail = ((int64_t)b * H + h) * kBlk * D;
   if (!is_v) {
     const T *in = reinterpret_cast<const T *>(a.k) + b * a.k_sb + h * a.k_sh;
     T *kt = reinterpret_cast<T *>(a.c.kt) + tail, *copy = full ? s_row[wave] : nullptr;
-    if (a.interleaved) turn_row<DT, true>(a.how, in, pos, a.how.k_weight, kt + slot * D, copy, lane);
-    else turn_row<DT, false>(a.how, in, pos, a.how.k_weight, kt + slot * D, copy, lane);
-    if (!full) return;
+    if (!(a.interleaved ? turn_key<DT, true>(a.how, in, pos, kt + slot * D, copy, lane, has_page)
+                        : turn_key<DT, false>(a.how, in, pos, kt + slot * D, copy, lane, has_page)) || !full)
+      return;
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
     __builtin_amdgcn_wave_barrier();               // one wave: its LDS accesses are in order
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
@@ -255,6 +278,7 @@ __global__ __launch_bounds__(kBlock) void kv8_append_kernel(Kv8AppendArgs a) {
     typedef ValueBlock<D> V;
     const uint32_t now = load_two<T>(reinterpret_cast<const T *>(a.v) + b * a.v_sb + h * a.v_sh + 2 * V::pair(lane));
     uint16_t *vt = reinterpret_cast<uint16_t *>(a.c.vt) + tail + 2 * V::pair(lane) * kBlk;
+    if (!has_page()) return;
     V v;
     if (full) {
       value_rows<D>(reinterpret_cast<const uint16_t *>(a.c.vt) + tail, lane, v.raw);
@@ -415,10 +439,11 @@ extern "C" int en_kv8_append(const void *q, const void *k_new, const void *v_new
   if (!k_new || !v_new || !kv_lens || !strides || (q_heads && (!q || !q_out))) return EN_ERR_NULL;
   for (const void *p : {q, k_new, v_new, (const void *)q_out, how->q_weight, how->k_weight})
     if (!aligned_to(p, 2)) return EN_ERR_ALIGN;
-  const int64_t units = (int64_t)cache->batch * (q_heads + 2 * (int64_t)cache->head_num);
+  const int parts_q = (int)ceil_div(q_heads, kTurned);
+  const int64_t units = (int64_t)cache->batch * (parts_q + 2 * (int64_t)cache->head_num);
   if (units > INT32_MAX) return EN_ERR_SHAPE;
   const Kv8AppendArgs a{kv8_args(cache), rotary_how(how, cache->size_per_head, 1), q, k_new, v_new, q_out, kv_lens, strides[0], strides[1], strides[2],
-                        strides[3], strides[4], strides[5], q_heads, how->interleaved != 0, (uint32_t)units, overflow};
+                        strides[3], strides[4], strides[5], q_heads, parts_q, how->interleaved != 0, (uint32_t)units, overflow};
   with_kv8_form(cache, [&](auto dt, auto code, auto d) {
     kv8_append_kernel<decltype(dt)::value, decltype(code)::value, decltype(d)::value>
         <<<(unsigned)ceil_div(units, kBlock / kWave), kBlock, 0, (hipStream_t)stream>>>(a);
