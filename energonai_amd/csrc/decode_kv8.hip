@@ -201,7 +201,7 @@ struct Kv8At {
 // The keys of four rows (4t .. 4t + 3 of each of four blocks) a lane as the first product wants them: 16 channels of row l % 16, run c of 64.
 // Rows of 128 codes are whole cache lines, and 16 lanes x 4 of 16 bytes take half of each of 16: both halves of eight rows in one
 // load instead (lanes 8.. of 16 take the other half of rows 0..7, and the first half of rows 8..15 in the second load), and the
-// halves back in place by a rotation in the registers.  (Bytes as they lie: the 1031 MB of 128 sequences 190 us, so 179.)
+// halves back in place by a rotation in the registers.  (The loads alone, 1031 MB of 128 sequences: bytes as they lie 190 us, so 179.)
 __device__ __forceinline__ uint32_t eight_away(uint32_t v) { return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x128, 0xF, 0xF, true); }
 __device__ __forceinline__ void halves_in_place(uint4 &x, uint4 &y, bool low) {
   const uint4 a = x, b = y;
@@ -212,7 +212,7 @@ __device__ __forceinline__ void halves_in_place(uint4 &x, uint4 &y, bool low) {
 // Runs of 16 channels of which a team's results go through LDS at once: all, or four where they would be more than 64 KB.
 __host__ __device__ constexpr int kv8_team_tiles(int rows, int nt) { return rows > 8 && nt > 4 ? 4 : nt; }
 
-// TEAM 1: every wave by itself, a run of plan.quota tiles.  TEAM 8: the waves of a workgroup take the tiles of one unit in turn and
+// TEAM 1: every wave by itself, a run of tiles or (a.whole) whole units.  TEAM 8: the waves of a workgroup take the tiles of one unit in turn and
 // put their results together in LDS.
 template <int DT, int CODE, int NT, int TEAM>
 __global__ __launch_bounds__(TEAM == 1 ? kBlock : TEAM * kWave, TEAM == 1 ? 1 : 2) void decode_attn_kv8_kernel(Kv8AttnArgs a) {
@@ -317,7 +317,7 @@ __global__ __launch_bounds__(TEAM == 1 ? kBlock : TEAM * kWave, TEAM == 1 ? 1 : 
   if (TEAM == 1 && at.tile >= at.tiles) next_unit(at);      // the run begins with a unit's end
   // Pages of a tile: of the block whose rows this lane loads as keys, and of the one whose positions it loads as values.  As the table has
   // them: what depends on them comes a tile later, and nothing waits here for the loads of keys and values in between (the ids
-  // looked at where they are loaded, every tile waited for all loads: 128 sequences' 1031 MB 186 us, so KKK).
+  // looked at where they are loaded, every tile waited for all loads: 1 sequence of 130000, 8 heads x 128 50 us, so 44; 16 of up to 8000, 40 x 64 75, so 69).
   const int last_page = max(a.c.max_pages - 1, 0);
   auto pages = [&](const Kv8At &x, int &kid, int &vid) {
     const int32_t *row = a.c.table + (int64_t)x.b * a.c.max_pages;
@@ -485,6 +485,8 @@ __global__ __launch_bounds__(TEAM == 1 ? kBlock : TEAM * kWave, TEAM == 1 ? 1 : 
     f32x4 s = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
+      // past the head: no channels, and an infinity of another one in their place would not vanish
+      if (D % 64 && 64 * c + 16 * g >= D) tail_k[c][0] = tail_k[c][1] = make_uint4(0, 0, 0, 0);
       s = M::k32(tail_k[c][0], q[c][0], s);
       s = M::k32(tail_k[c][1], q[c][1], s);
     }

@@ -226,7 +226,8 @@ __device__ __forceinline__ bool turn_key(const RotaryHow &how, const T *in, int 
 }
 
 // A wave takes a few rows of q, into q_out, or the row of a key or value head, into the tail and, where that completes the block, the block
-// into its page.
+// into its page.  (A few lanes a row, as for the 16-bit cache, and the blocks put one after another by the wave that completed them: 256
+// sequences, 64 / 8 heads x 128 22.9 us, so 9.9.)
 template <int DT, int CODE, int D>
 __global__ __launch_bounds__(kBlock) void kv8_append_kernel(Kv8AppendArgs a) {
   typedef typename Elem<DT>::T T;

@@ -3,7 +3,7 @@
 // A row of D channels is taken by LPR lanes, NP units each; a unit is two vectors of VEC channels, a and b, that hold both channels
 // of every pair they have a part in, so that the rotation needs no other lane: channels u VEC .. and R/2 + u VEC .. of the rotated part; where
 // pairs are neighbouring channels, and in the rest of the row, any two, and those are taken whose neighbours the neighbouring lanes take, so
-// that a load fills cache lines (4 prompts of 8000, 80 heads x 128, neighbouring pairs 357 -> KKK us).  Only the norm's sum crosses lanes.
+// that a load fills cache lines (4 prompts of 8000, 80 heads x 128, neighbouring pairs: 357 us where a unit's vectors are neighbours, so 212).  Only the norm's sum crosses lanes.
 // VEC is the largest of 8 (16-bit rows), 4, 2, 1 that divides R/2 and D (interleaved: R and D), a property of the head alone:
 // loads and stores take any element's address.
 #pragma once

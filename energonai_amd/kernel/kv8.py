@@ -187,7 +187,7 @@ def kv8_pages_read(cache, kv_len_list, max_seq_len: int, *, first: Optional[torc
 
 
 def decode_attn_kv8_workspace_bytes(batch_size: int, q_heads: int, head_num: int, capacity: int, size_per_head: int) -> int:
-    """Bytes of the buffer through which ``decode_attn_kv8`` passes its plan and partial results (0: caches of this capacity, in positions a
+    """Bytes of the buffer through which ``decode_attn_kv8`` passes its partial results (0: caches of this capacity, in positions a
     sequence, need none)."""
     return int(_lib.fn.en_decode_attn_kv8_workspace_bytes(int(batch_size), int(q_heads), int(head_num), int(capacity), int(size_per_head)))
 

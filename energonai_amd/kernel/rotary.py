@@ -42,19 +42,34 @@ def _span(t: torch.Tensor):
     return t.data_ptr(), t.data_ptr() + (1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride()))) * t.element_size() if t.numel() else t.data_ptr()
 
 
+def _apart(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether two sets of rows share no memory: one lies behind the other as a whole, in each token, or in each head's place."""
+    (a0, a1), (b0, b1) = _span(a), _span(b)
+    if a0 >= b1 or b0 >= a1:
+        return True
+    if b0 < a0:
+        a, b, a0, b0 = b, a, b0, a0
+    off, D, (token, head) = (b0 - a0) // a.element_size(), a.shape[2], a.stride()[:2]
+    if b.stride(0) == token and token > 0:
+        wide = [(t.shape[1] - 1) * t.stride(1) + D for t in (a, b)]
+        if wide[0] <= off % token and off % token + wide[1] <= token:
+            return True
+    single = a.shape[0] == 1 and b.shape[0] == 1
+    return head > 0 and b.stride(1) == head and (single or (b.stride(0) == token and token % head == 0)) and D <= off % head <= head - D
+
+
 def _not_over(who: str, inputs, outs) -> None:
     """Refuses results that would be written over rows still to be read: each may be its own input, or lie apart from all of them."""
     for o in outs:
-        if any(n > 1 and s < o.shape[2] for n, s in zip(o.shape[:2], o.stride()[:2])):
+        inner, outer = sorted((s, n) for n, s in zip(o.shape[:2], o.stride()[:2]))
+        if o.numel() and ((inner[1] > 1 and inner[0] < o.shape[2]) or (outer[1] > 1 and outer[0] < (inner[1] - 1) * inner[0] + o.shape[2])):
             raise RuntimeError(f"{who}: the rows of out must not overlap")
     for i, o in enumerate(outs):
-        if o.data_ptr() == inputs[i].data_ptr() and o.stride() == inputs[i].stride():
-            continue
-        for t in inputs:
-            (a0, a1), (b0, b1) = _span(o), _span(t)
-            if a0 < b1 and b0 < a1:
-                raise RuntimeError(f"{who}: out must be q and k themselves or lie apart from them")
-    if len(outs) == 2 and outs[0].data_ptr() == outs[1].data_ptr() and outs[0].numel() and outs[1].numel():
+        for j, t in enumerate(inputs):
+            own = i == j and o.data_ptr() == t.data_ptr() and o.stride() == t.stride()
+            if not own and not _apart(o, t):
+                raise RuntimeError(f"{who}: out must be q and k themselves, which share no memory then, or lie apart from them")
+    if len(outs) == 2 and not _apart(*outs):
         raise RuntimeError(f"{who}: the two results must not share memory")
 
 

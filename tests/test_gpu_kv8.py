@@ -322,6 +322,37 @@ def test_attention_without_pages():
         assert bool((got[1:] == 0).all())
 
 
+@pytest.mark.parametrize("D", [48, 64, 80, 112, 128])
+def test_an_infinite_key_in_the_tail(D):
+    """A key whose score is minus infinity is a masked one, as long as its block is in 16 bits; of any head size."""
+    K = _K()
+    announce("kv8 attention, infinite key", D)
+    g = torch.Generator().manual_seed(D)
+    H, n = 2, 21
+    cache = new_cache(1, H, D, 16, 3, 2, F16, I8, g, garbage=False)
+    deal_pages(cache, [n], 16, g)
+    k, v = (torch.randn(n, H, D, generator=g).to(F16) for _ in range(2))
+    q = torch.randn(1, H, 1, D, generator=g).to(F16)
+    q[0, :, 0, 0] = -1.0
+    k[18, :, 0] = float("inf")
+    gpu = to_gpu(cache)
+    from energonai_amd.seqinfo import build_seq_info
+    info = build_seq_info(torch.tensor([n], dtype=torch.int32, device="cuda"), 1)
+    K.kv8_pages_fill(k.cuda(), v.cuda(), gpu, 1, n, info)
+    got = K.decode_attn_kv8(q.cuda(), gpu, info)
+    kd, vd = (t.cpu().double() for t in K.kv8_pages_read(gpu, info, n))
+    kd[0, :, 18] = 0
+    s = (q[0, :, 0].double()[:, None] * kd[0]).sum(-1) * D ** -0.5
+    s[:, 18] = float("-inf")
+    want = (torch.softmax(s, -1)[..., None] * vd[0]).sum(1)
+    # half steps of 2^-11: of the keys as they are read here (a score is off by e, a probability by 2 e), of the values as they are read, of
+    # the probabilities, and of the result; sums in fp32 are off by less than 2^-16 of all that
+    p = torch.softmax(s, -1)
+    e = (2.0 ** -11 * (q[0, :, 0].double()[:, None] * kd[0]).abs().sum(-1) * D ** -0.5).amax(-1)[:, None]
+    room = (2 * e + 2.0 ** -10 + 2.0 ** -16) * (p[..., None] * vd[0].abs()).sum(1) + 2.0 ** -11 * want.abs() + 2.0 ** -20
+    assert bool(((got.cpu().double()[0, :, 0] - want).abs() <= room).all())
+
+
 def test_value_scales_far_apart():
     """Blocks of values from 2^-24 to 2^14 in fp16: a probability's product with its scale neither vanishes nor overflows, whichever block leads."""
     K = _K()

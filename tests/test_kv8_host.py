@@ -138,3 +138,43 @@ def test_restated_cache():
         assert torch.equal((y - c.float()).abs(), near) and s == x.float().abs().max() / ref.LARGEST[code]
         held = ref.Cache(1, 32, code).held(torch.cat((x, x[:3]))[None])
         assert torch.equal(held[0, 16:], x[:3].double()) and torch.equal(held[0, :16], c.float().double() * s.double())
+
+
+def test_results_over_rows_still_to_be_read():
+    """Which results of the norm and rotation are refused, against the elements that views really share: what shares any is refused; of the
+    layouts that projections have, what shares none is taken."""
+    import random
+    from energonai_amd.kernel.rotary import _apart, _not_over
+    rng = random.Random(3)
+
+    def elements(t):
+        return {int(i) for i in (t.storage_offset() + sum(torch.arange(n).view([-1 if j == d else 1 for j in range(3)]) * s
+                                                          for d, (n, s) in enumerate(zip(t.shape, t.stride())))).flatten()}
+    base = torch.zeros(4000)
+    shared = 0
+    for _ in range(3000):
+        D = rng.choice([1, 2, 4])
+        views = []
+        for _ in range(2):
+            T, H = rng.randint(1, 4), rng.randint(1, 4)
+            views.append(base.as_strided((T, H, D), (rng.choice([D, 2 * D, 3 * D, H * D, 4 * H * D, 50]), rng.choice([D, 2 * D, 3 * D, T * D, 50]), 1),
+                                         rng.randint(0, 60)))
+        if rng.random() < 0.5:                              # the same strides, as two parts of one projection have them
+            views[1] = base.as_strided((views[0].shape[0], views[1].shape[1], D), views[0].stride(), views[1].storage_offset())
+        a, b = views
+        share = bool(elements(a) & elements(b))
+        shared += share
+        assert not (share and _apart(a, b)) and _apart(a, b) == _apart(b, a), (a.shape, a.stride(), b.shape, b.stride())
+        if len(elements(a)) < a.numel():
+            with pytest.raises(RuntimeError, match="overlap"):
+                _not_over("t", [b], [a])
+    assert 300 < shared < 2700
+    x = torch.zeros(5, 3, 4, 8)
+    three = [x[:, i] for i in range(3)]                     # [T, 3, H, D]
+    of_heads = [x.view(5, 4, 3, 8)[:, :, i] for i in range(3)]
+    for q, k, _ in (three, of_heads, [x[:1, i] for i in range(3)], [x.view(5, 4, 3, 8)[:1, :, i] for i in range(3)]):
+        _not_over("t", [q, k], [q, k])
+    q = x.view(5, 12, 8)
+    for ins, outs in (([q[:, :8], q[:, 4:8]], [q[:, :8], q[:, 4:8]]), ([q, q], [q, torch.zeros(5, 12, 8)]), ([q[:4], q[1:]], [q[:4], torch.zeros(4, 12, 8)])):
+        with pytest.raises(RuntimeError):
+            _not_over("t", ins, outs)
