@@ -594,7 +594,7 @@ bool norm_rotary(PyObject *rotary, PyObject *q_weight, PyObject *k_weight, PyObj
     if (!PyTuple_CheckExact(rotary) || PyTuple_GET_SIZE(rotary) != 2) return false;
     const Tensor *c = plain_contiguous(PyTuple_GET_ITEM(rotary, 0)), *s = plain_contiguous(PyTuple_GET_ITEM(rotary, 1));
     if (!c || !s || c->dim() != 2 || c->sizes() != s->sizes() || c->scalar_type() != at::kFloat || s->scalar_type() != at::kFloat ||
-        c->device() != x.device() || s->device() != x.device() || 2 * c->size(1) > D || !fits_int({c->size(0)}))
+        c->device() != x.device() || s->device() != x.device() || c->size(0) < 1 || c->size(1) < 1 || 2 * c->size(1) > D || !fits_int({c->size(0)}))
       return false;
     out.cos = c->data_ptr<float>();
     out.sin = s->data_ptr<float>();

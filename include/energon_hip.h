@@ -500,7 +500,7 @@ typedef struct en_kv8_cache {
  * p < min(length, max_seq_len) of sequence b; rows from `tokens` on are not read.  overflow, if given, counts positions that had no page. */
 int en_kv8_fill(const void *k, const void *v, const en_kv8_cache *cache, const int32_t *cu_seqlens, int64_t tokens, int max_seq_len,
                 const int64_t *strides, int32_t *overflow, en_stream_t stream);
-/* A decode step: en_kv_append_paged_rotary into this cache.  q may be NULL with q_heads 0.  A sequence whose position kv_lens[b] has no
+/* A decode step: en_kv_append_paged_rotary into this cache, keys normed and turned in 64 bits.  q may be NULL with q_heads 0.  A sequence whose position kv_lens[b] has no
  * page keeps its cache, loses the new row and is counted in overflow. */
 int en_kv8_append(const void *q, const void *k_new, const void *v_new, void *q_out, const en_kv8_cache *cache,
                   const int32_t *kv_lens, int q_heads, const int64_t *strides, const en_norm_rotary *how, int32_t *overflow,

@@ -211,7 +211,7 @@ def test_refusals():
     rot = K.rotary_table(8, 64)
     ok = lambda **kw: K.qk_norm_rotary(*[kw.pop(n, d) for n, d in (("q", x), ("k", x), ("B", 1), ("lens", lens), ("rot", rot))], **kw)  # noqa: E731
     ok()
-    from energonai_amd.seqinfo import SeqInfo
+    from energonai_amd.seqinfo import SeqInfo, build_seq_info
     both = torch.zeros(4, 4, 64, device="cuda", dtype=F16)
     ok(q=both[:, :2], k=both[:, 2:], out=(both[:, :2], both[:, 2:]))          # two views of one projection, each over itself
     y = torch.zeros(4, 2, 64, device="cuda", dtype=F16)
@@ -222,7 +222,8 @@ def test_refusals():
         ok(q=both[:, :2], k=both[:, 2:], out=(both[:, 2:], both[:, :2]))       # each over the other
     for bad in (dict(q=x.cpu()), dict(q=x.float()), dict(q=x.to(torch.float64), k=None), dict(k=x[:3]), dict(k=x[..., :32]), dict(q=x.transpose(1, 2)),
                 dict(q=x[0]), dict(rot=(rot[0].half(), rot[1])), dict(rot=(rot[0], rot[1][:4])), dict(rot=K.rotary_table(8, 66)), dict(rot=(rot[0].cpu(), rot[1])),
-                dict(rot=(rot[0][:0], rot[1][:0])), dict(q_weight=torch.ones(64, device="cuda")), dict(k_weight=torch.ones(32, device="cuda", dtype=F16)),
+                dict(rot=(rot[0][:0], rot[1][:0])), dict(rot=(rot[0][:, :0].contiguous(), rot[1][:, :0].contiguous())),
+                dict(rot=(rot[0][:, :0].contiguous(), rot[1][:, :0].contiguous()), lens=build_seq_info(lens, 1)), dict(q_weight=torch.ones(64, device="cuda")), dict(k_weight=torch.ones(32, device="cuda", dtype=F16)),
                 dict(out=(x,)), dict(out=(x, x.float())), dict(positions=torch.zeros(3, dtype=torch.int32, device="cuda")),
                 dict(positions=torch.zeros(4, dtype=torch.int64, device="cuda")), dict(lens=SeqInfo(lens, None, 1, None, lens)),
                 dict(q=torch.zeros(4, 2, 257, device="cuda", dtype=F16), k=None, rot=None)):
