@@ -34,6 +34,10 @@ constexpr int kWaves = 1024;                  // of the launch: one a SIMD, whos
                                               // as many leave twice the partial results: 32 of up to 2000, 32 / 8 x 128 19.9 -> 25.5 us, 128 of up to 4000 104 -> 107
 constexpr int kQueries = 16;                  // columns of a tile: queries that share one pass
 constexpr float kRaise = 8.f;                 // log2
+// log2 that a value scale counts as at least: a block without values may have the highest scores by any margin, and what is a probability's
+// factor there (below: ratio) is then 2^64 and not one that takes the other blocks' scales past the fp32 numbers.
+constexpr float kLeastScale = -64.f;
+constexpr float kLargestFactor = 3.402823466e38f;
 constexpr int kTeam = 8;                      // waves of a workgroup that takes one unit
 constexpr int kTeamCapacity = 1024, kTeamUnits = 512;
 constexpr int kWholeCapacity = 256;
@@ -438,8 +442,10 @@ __global__ __launch_bounds__(TEAM == 1 ? kBlock : TEAM * kWave, TEAM == 1 ? 1 : 
         s[i][e] = in ? s[i][e] * by : -INFINITY;
         top = fmaxf(top, s[i][e]);
       }
-    st.raise(top, fmaxf(__builtin_amdgcn_logf(fabsf(vs)), -126.f));
-    const float base = st.base(), f = vs * st.ratio();
+    st.raise(top, fmaxf(__builtin_amdgcn_logf(fabsf(vs)), kLeastScale));
+    const float base = st.base();
+    float f = vs * st.ratio();
+    f = f > kLargestFactor ? kLargestFactor : f;             // scales of 2^57 and more; NaN stays what it is
     uint32_t p[8];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
