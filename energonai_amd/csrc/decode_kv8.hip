@@ -470,10 +470,12 @@ __global__ __launch_bounds__(TEAM == 1 ? kBlock : TEAM * kWave, TEAM == 1 ? 1 : 
     if constexpr (more.value) load_values(next, next_vid);
     __builtin_amdgcn_sched_barrier(0);
   };
-  // The positions behind the last full block, 16 bits as they are: row i of the one key tile is position i.
+  // The positions behind the last full block, 16 bits as they are: row i of the one key tile is position i.  Where their page is none, zeros.
   uint4 tail_k[NC][2];
   uint2 tail_v[NT];
+  int tail_id;
   auto load_tail = [&](const Kv8At &x) {
+    tail_id = a.c.table[(int64_t)x.b * a.c.max_pages + ((x.n / kBlk) >> a.c.lg_blocks)];
     const int64_t from = ((int64_t)x.b * a.c.H + x.h) * kBlk * D;
     const T *kt = reinterpret_cast<const T *>(a.c.kt) + from + col * D;
 #pragma unroll
@@ -488,6 +490,12 @@ __global__ __launch_bounds__(TEAM == 1 ? kBlock : TEAM * kWave, TEAM == 1 ? 1 : 
   };
   auto tail = [&](const Kv8At &x) {
     const int in_tail = x.n % kBlk;
+    if ((unsigned)tail_id >= (unsigned)a.c.num_pages) {
+#pragma unroll
+      for (int c = 0; c < NC; ++c) tail_k[c][0] = tail_k[c][1] = make_uint4(0, 0, 0, 0);
+#pragma unroll
+      for (int i = 0; i < NT; ++i) tail_v[i] = make_uint2(0, 0);
+    }
     f32x4 s = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int c = 0; c < NC; ++c) {

@@ -320,18 +320,19 @@ __global__ __launch_bounds__(kBlock) void kv8_read_kernel(Kv8ReadArgs a) {
   const int j = (int)min(j64, (int64_t)(INT32_MAX / kBlk));
   const bool is_v = unit >= H;
   const int h = is_v ? unit - H : unit;
-  const int id = there == kBlk ? kv8_page(a.c, b, j) : -1, blk = kv8_block_in_page(a.c, j);
+  const int id = there > 0 ? kv8_page(a.c, b, j) : -1, blk = kv8_block_in_page(a.c, j);
+  const bool codes_there = id >= 0 && there == kBlk, tail_there = id >= 0 && there < kBlk;
   const int64_t tail = ((int64_t)b * H + h) * kBlk * D;
   const int64_t to = (((int64_t)b * H + h) * a.seq_len + s0) * D;
   if (!is_v) {
     typedef KeyBlock<D> K;
     T *out = reinterpret_cast<T *>(a.k_out) + to;
-    const float scale = id >= 0 ? a.c.ks[kv8_k_scale(a.c, id, h, blk)] : 0.f;
+    const float scale = codes_there ? a.c.ks[kv8_k_scale(a.c, id, h, blk)] : 0.f;
 #pragma unroll
     for (int i = 0; i < K::kEach; ++i) {
       const int r = K::row(i, lane), c = K::channel(i, lane);
       uint4 w = make_uint4(0, 0, 0, 0);
-      if (id >= 0) {
+      if (codes_there) {
         const uint2 codes = *reinterpret_cast<const uint2 *>(kv8_k_block(a.c, id, h, blk, D) + r * D + c);
         Pack<T, 8> p;
         p.v[0] = E::from_float(Codes<CODE>::template value<0>(codes.x) * scale);
@@ -343,7 +344,7 @@ __global__ __launch_bounds__(kBlock) void kv8_read_kernel(Kv8ReadArgs a) {
         p.v[6] = E::from_float(Codes<CODE>::template value<2>(codes.y) * scale);
         p.v[7] = E::from_float(Codes<CODE>::template value<3>(codes.y) * scale);
         w = __builtin_bit_cast(uint4, p);
-      } else if (r < there && there < kBlk) {
+      } else if (r < there && tail_there) {
         w = *reinterpret_cast<const uint4 *>(reinterpret_cast<const T *>(a.c.kt) + tail + r * D + c);
       }
       if (K::has(i, lane) && r >= lo && r < hi) store16<NT>(out + (int64_t)r * D + c, w);
@@ -353,7 +354,7 @@ __global__ __launch_bounds__(kBlock) void kv8_read_kernel(Kv8ReadArgs a) {
     T *out = reinterpret_cast<T *>(a.v_out) + to;
     const int c = V::pair(lane), p0 = V::first(lane);
     uint32_t row[V::kEach];
-    if (id >= 0) {
+    if (codes_there) {
       const float scale = a.c.vs[kv8_v_scale(a.c, id, h, blk)];
       const uint8_t *from = kv8_v_block(a.c, id, h, blk, D) + 2 * c * kBlk + p0;
 #pragma unroll
@@ -368,7 +369,7 @@ __global__ __launch_bounds__(kBlock) void kv8_read_kernel(Kv8ReadArgs a) {
     } else {
 #pragma unroll
       for (int i = 0; i < V::kEach; ++i) row[i] = 0;
-      if (there > 0 && there < kBlk) {
+      if (tail_there) {
         value_rows<D>(reinterpret_cast<const uint16_t *>(a.c.vt) + tail, lane, row);
 #pragma unroll
         for (int i = 0; i < V::kEach; ++i) row[i] = p0 + i < there ? row[i] : 0u;

@@ -8,7 +8,8 @@ quantized once, from full values, and a cache filled by a prompt is the one that
 history in the projection's type (energonai/model/attention.py:61-71).
 
 Heads of 16, 32, .. 128 channels, fp16 and bf16, pages of a power of two of at least 16 positions.  A page id outside the pool reads as
-zeros and is not written.
+zeros and is not written, nor is the tail of positions that would lie there.  A new row that is lost for want of a page stays lost: named later,
+the page has whatever it (or, in an unfinished block, the tail) held in that position.
 
 A tail belongs to its sequence's place in the batch, as the row of ``page_table`` does, and holds the positions behind the last full block
 alone: a sequence that moves to another place takes both along, and a length may go back to no less than the last multiple of 16 it has

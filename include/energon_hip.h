@@ -482,7 +482,8 @@ int en_kv_append_paged_rotary(const void *q, const void *k_new, const void *v_ne
  * head of each.  The positions behind the last full block stay in 16 bits in k_tail [batch, head, EN_KV8_BLOCK, channel] and v_tail
  * [batch, head, channel, EN_KV8_BLOCK].  A block is quantized once, when it is full: with a its largest magnitude and M the
  * largest code (127; 448), scale = a / M and code = round(x * (M / a)) in fp32, to nearest even; scale and codes are 0 where
- * a < 2^-100, and the scale is NaN where a value is not finite.  A page id outside the pool reads as zeros and is not written. */
+ * a < 2^-100, and the scale is NaN where a value is not finite.  A page id outside the pool reads as zeros and is not written; so are
+ * the positions of a tail that would lie in it. */
 #define EN_KV8_BLOCK 16
 enum en_kv8_code { EN_KV8_INT8 = 0, EN_KV8_E4M3 = 1 };
 typedef struct en_kv8_cache {
