@@ -14,7 +14,8 @@
 //    in 16 bits as those below 1.
 // The probabilities are rounded to the cache's 16-bit type for the second product (half a step, 2^-12 or 2^-9, each; the first product's operands
 // are exact), relative to a reference m_o that follows score + log2(value scale), so that their products with the scale neither
-// vanish nor overflow in fp16; the sum of the softmax takes them in fp32 relative to the scores' own maximum m_s.
+// vanish nor overflow in fp16, and 2^7 below it there: a product of up to 2^(7 + 8) is an fp16 number, and the smallest one that is not
+// rounded to zero is 2^-32 of the largest.  The sum of the softmax takes them in fp32 relative to the scores' own maximum m_s.
 #include <type_traits>
 
 #include "kv8_common.hip.h"
@@ -38,6 +39,8 @@ constexpr float kRaise = 8.f;                 // log2
 // factor there (below: ratio) is then 2^64 and not one that takes the other blocks' scales past the fp32 numbers.
 constexpr float kLeastScale = -64.f;
 constexpr float kLargestFactor = 3.402823466e38f;
+// log2 that the largest probability stands above 1 for its product with the values (and up to kRaise more).
+template <int DT> constexpr float kStand = DT == EN_F16 ? 7.f : 0.f;
 constexpr int kTeam = 8;                      // waves of a workgroup that takes one unit
 constexpr int kTeamCapacity = 1024, kTeamUnits = 512;
 constexpr int kWholeCapacity = 256;
@@ -162,7 +165,7 @@ template <int NT> struct Kv8State {
 #pragma unroll
     for (int t = 0; t < NT; ++t) o[t] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
-  // Raises the references where a lane's largest score (log2) or score + log2 of its value scale passes them by kRaise.
+  // Raises the references where a lane's largest score (log2) or score + lv (log2 of its value scale, less kStand) passes them by kRaise.
   __device__ __forceinline__ void raise(float top, float lv) {
     const float top_o = top + lv;
     if (__ballot(top > m_s + kRaise || top_o > m_o + kRaise) == 0) return;
@@ -442,7 +445,7 @@ __global__ __launch_bounds__(TEAM == 1 ? kBlock : TEAM * kWave, TEAM == 1 ? 1 : 
         s[i][e] = in ? s[i][e] * by : -INFINITY;
         top = fmaxf(top, s[i][e]);
       }
-    st.raise(top, fmaxf(__builtin_amdgcn_logf(fabsf(vs)), kLeastScale));
+    st.raise(top, fmaxf(__builtin_amdgcn_logf(fabsf(vs)), kLeastScale) - kStand<DT>);
     const float base = st.base();
     float f = vs * st.ratio();
     f = f > kLargestFactor ? kLargestFactor : f;             // scales of 2^57 and more; NaN stays what it is
@@ -510,7 +513,7 @@ __global__ __launch_bounds__(TEAM == 1 ? kBlock : TEAM * kWave, TEAM == 1 ? 1 : 
       s[e] = 4 * g + e < in_tail ? s[e] * a.c_exp : -INFINITY;
       top = fmaxf(top, s[e]);
     }
-    st.raise(top, 0.f);
+    st.raise(top, -kStand<DT>);
     const float base = st.base(), f = st.ratio();
     float e4[4];
 #pragma unroll

@@ -1,5 +1,7 @@
 """Decode attention over the 8-bit cache where the value scales of a query's blocks lie as far apart as they can: blocks whose values are all
-zeros or next to nothing under the highest scores."""
+zeros or next to nothing under the highest scores, and many small weights beside a large one."""
+import math
+
 import pytest
 import torch
 
@@ -99,3 +101,41 @@ def _check(got, q, n, k, v, code, scale, holes, what):
         off = got[0, rows, 0] - want
         got[0, rows, 0] = want + torch.sign(off) * (off.abs() - room).clamp_min(0)
     check_attention(got, q, None, [n], [k], [v], code, scale, what, holes)
+
+
+@pytest.mark.parametrize("code", [I8, E4])
+@pytest.mark.parametrize("n,capacity,B", [
+    (1003, 1024, 1), (3000, 4096, 1), (60011, 65536, 1),      # the tiles of the sequence dealt to several waves
+    (4096, 4096, 1100), (240, 256, 600),                      # one wave has all of them: many sequences, on the same pages
+])
+def test_many_small_weights_beside_a_large_one(code, n, capacity, B):
+    """fp16: one position has a weight 2^26 times that of each of the others, whose values make up the result all the same where the one's
+    is zero.  A weight is rounded to fp16 for its product with the values; that leaves 2^-32 of the largest: numbers there go down to
+    2^-24, half of that is lost, and the largest stands at 2^7 or above."""
+    K = _K()
+    announce("kv8 small weights", code, n, capacity, B)
+    g = torch.Generator().manual_seed(n)
+    D, H, P, scale = 64, 1, 64, 0.125
+    u = torch.randint(0, 2, (D,), generator=g) * 2.0 - 1.0
+    k = torch.zeros(H, n, D)
+    k[:, 37] = 26 * math.log(2) / (8 * D * scale) * u
+    v = 50.0 * (1 + 0.2 * torch.randn(H, n, D, generator=g)) * (torch.arange(D) % 2 * 2 - 1)
+    v[:, 37, :32] = 0.0
+    ks, vs = [k.to(F16)], [v.to(F16)]
+    cache = new_cache(1, H, D, P, n // P + 2, capacity // P, F16, code, g)
+    deal_pages(cache, [n], P, g)
+    dev = _fill(cache, ks, vs, [n])
+    dev[4:] = [t.expand(B, *t.shape[1:]).contiguous() for t in dev[4:]]
+    q = (8 * u).expand(B, 2, 1, D).to(F16)
+    got = K.decode_attn_kv8(q.cuda(), dev, torch.full((B,), n, dtype=torch.int32).cuda(), scale=scale).double().cpu()[:, :, 0]
+    q = q[0, :, 0]
+    held = ref.Cache(H, D, code)
+    kd, vd = held.held(ks[0])[0], held.held(vs[0])[0]
+    want, size = ref.attention(q, kd, vd, scale)
+    m = scale * (q.double().abs() @ kd.abs().t()).max(-1, keepdim=True).values
+    # check_attention's bound with 2^-32 where that has 2^-25
+    tol = 2.0 ** -11 * (size + want.abs()) + 2.0 ** -24 + (2 * (D / 8 + 4) * 2.0 ** -24 * m + 2.0 ** -18) * size \
+        + 2.0 ** -32 * torch.softmax(q.double() @ kd.t() * scale, -1).max() * vd.abs().sum(0)
+    off = ((got - want).abs() - tol).amax((1, 2))
+    assert off.max() <= 0, (int(off.argmax()), float(off.max()))
+    assert bool((want[:, :32].abs() > 8 * tol[:, :32]).all())         # what the others come to is far more than the bound
