@@ -35,7 +35,7 @@ class MultiHeadAttention1D(nn.Module):
     (``torch.int8`` or ``torch.float8_e4m3fn``) keeps the cache in 8 bits, in pages."""
 
     # what is not there in a module saved before there was a choice
-    rotary_dim, rotary_base, rotary_interleaved, qk_norm, kv_cache_dtype, turned = 0, 10000.0, False, False, None, False
+    rotary_dim, rotary_base, rotary_interleaved, qk_norm, kv_cache_dtype = 0, 10000.0, False, False, None
 
     def __init__(self, hidden_size: int, num_heads: int, bias: bool = True, dtype: torch.dtype = torch.float16,
                  max_seq_len: int = 512, fused_qkv: bool = True, is_decoder: bool = True, disable_past_cache=False,
@@ -69,8 +69,7 @@ class MultiHeadAttention1D(nn.Module):
         if qk_norm:
             self.query_norm = nn.Parameter(torch.ones(self.attention_head_size, dtype=dtype))
             self.key_norm = nn.Parameter(torch.ones(self.attention_head_size, dtype=dtype))
-        self.turned = bool(rotary_dim or qk_norm)         # queries and keys are not used as they are projected
-        self._rotary_tables = {}                          # device -> (cos, sin)
+        self._rotary_tables = {}                          # (device, rows, rotary_dim, rotary_base) -> (cos, sin)
         if kv_cache_dtype is not None:
             if kv_cache_dtype not in (torch.int8, torch.float8_e4m3fn) or dtype not in (torch.float16, torch.bfloat16) \
                     or self.attention_head_size % 16 or self.attention_head_size > 128:
@@ -96,17 +95,34 @@ class MultiHeadAttention1D(nn.Module):
         v = project(self.value_, x).view(rows, H, D)
         return q, k, v, None
 
+    @property
+    def turned(self) -> bool:
+        """Whether queries and keys are used otherwise than as they are projected."""
+        return bool(self.rotary_dim or self.qk_norm)
+
+    # The tables follow from the module's numbers, and a loaded module may be on another device than the one they are kept for.
+    def __getstate__(self):
+        return {**super().__getstate__(), "_rotary_tables": {}}
+
+    def __setstate__(self, state):
+        super().__setstate__({**state, "_rotary_tables": {}})
+
     def _rotary(self, device, positions: int):
-        """The module's ``(cos, sin)`` on ``device``, for at least ``positions`` positions: as many as a cache can hold."""
-        if not self.rotary_dim:
-            return None
+        """The module's ``(cos, sin)`` on ``device`` for a prompt of up to ``positions`` positions: as many as a cache can hold."""
         page = self.kv_page_size or 1
         rows = (self.max_seq_len + page - 1) // page * page
-        if positions > rows:
+        if self.rotary_dim and positions > rows:
             raise RuntimeError(f"the batch is padded to {positions} positions but the rotation was planned for max_seq_len = {self.max_seq_len}")
-        tables = self._rotary_tables.get(device)
+        return self._tables(device, rows)
+
+    def _tables(self, device, rows: int):
+        """``(cos, sin)`` of ``rows`` positions.  Those of other numbers are kept too: a captured step goes on reading the ones it was captured with."""
+        if not self.rotary_dim:
+            return None
+        key = (device, rows, self.rotary_dim, self.rotary_base)
+        tables = self._rotary_tables.get(key)
         if tables is None:
-            tables = self._rotary_tables[device] = rotary_table(rows, self.rotary_dim, self.rotary_base, device)
+            tables = self._rotary_tables[key] = rotary_table(rows, self.rotary_dim, self.rotary_base, device)
         return tables
 
     def _turn_how(self) -> dict:
@@ -174,7 +190,7 @@ class MultiHeadAttention1D(nn.Module):
         cache = self.kv_cache
         q, k, v, _ = self._project(last)
         if self.turned:
-            q = cache.append_rotary(q, k, v, self._rotary(last.device, 0), **self._turn_how())
+            q = cache.append_rotary(q, k, v, self._tables(last.device, cache.max_seq_len), **self._turn_how())
         else:
             cache.append(k, v)
         ctx = cache.attend(q, self.scaling)      # [B,H,1,D], one pass over the caches
