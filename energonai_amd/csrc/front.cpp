@@ -715,11 +715,14 @@ bool kv8_cache(PyObject *o, en_kv8_cache &c, const Tensor *&home) {
   const int64_t v_shape[5] = {N, H, blocks, D, blk}, s_shape[3] = {N, H, blocks}, kt_shape[4] = {B, H, blk, D}, vt_shape[4] = {B, H, D, blk};
   if (P % blk || vp.sizes() != c10::IntArrayRef(v_shape) || ks.sizes() != c10::IntArrayRef(s_shape) || vs.sizes() != c10::IntArrayRef(s_shape) ||
       kt.sizes() != c10::IntArrayRef(kt_shape) || vt.sizes() != c10::IntArrayRef(vt_shape) || kp.stride(3) != 1 || kp.stride(2) != D ||
-      vp.stride(4) != 1 || vp.stride(3) != blk || vp.stride(2) != D * blk || (blocks > 1 && (ks.stride(2) != 1 || vs.stride(2) != 1)) ||
+      vp.stride(4) != 1 || vp.stride(3) != blk || (blocks > 1 && (vp.stride(2) != D * blk || ks.stride(2) != 1 || vs.stride(2) != 1)) ||
       !fits_int({N, H, P, D, B, table.size(1)}))
     return false;
+  // a dimension of one has whatever stride
+  auto page = [&](const Tensor &t) -> int64_t { return N > 1 ? t.stride(0) : 0; };
+  auto head = [&](const Tensor &t) -> int64_t { return H > 1 ? t.stride(1) : 0; };
   c = en_kv8_cache{kp.data_ptr(), vp.data_ptr(), ks.data_ptr<float>(), vs.data_ptr<float>(), kt.data_ptr(), vt.data_ptr(), i32(table),
-                   {kp.stride(0), kp.stride(1), vp.stride(0), vp.stride(1)}, {ks.stride(0), ks.stride(1), vs.stride(0), vs.stride(1)},
+                   {page(kp), head(kp), page(vp), head(vp)}, {page(ks), head(ks), page(vs), head(vs)},
                    (int32_t)N, (int32_t)P, (int32_t)table.size(1), (int32_t)B, (int32_t)H, (int32_t)D,
                    code == at::kChar ? EN_KV8_INT8 : EN_KV8_E4M3, type == at::kHalf ? EN_F16 : EN_BF16};
   home = t[4];

@@ -82,11 +82,11 @@ def _cache(cache, who: str) -> _lib.Kv8Cache:
     if vp.shape != (N, H, blocks, D, KV8_BLOCK) or ks.shape != (N, H, blocks) or vs.shape != ks.shape or kt.shape != (B, H, KV8_BLOCK, D) \
             or vt.shape != (B, H, D, KV8_BLOCK):
         raise RuntimeError(f"{who}: v_pages must be [pages, H, P / 16, D, 16], scales [pages, H, P / 16], tails [B, H, 16, D] and [B, H, D, 16]")
-    if kp.stride()[2:] != (D, 1) or vp.stride()[2:] != (D * KV8_BLOCK, KV8_BLOCK, 1) or (blocks > 1 and (ks.stride(2) != 1 or vs.stride(2) != 1)):
+    if kp.stride()[2:] != (D, 1) or vp.stride()[3:] != (KV8_BLOCK, 1) or (blocks > 1 and (vp.stride(2), ks.stride(2), vs.stride(2)) != (D * KV8_BLOCK, 1, 1)):
         raise RuntimeError(f"{who}: the positions of a page and head must be contiguous in pools and scales")
     c = _lib.Kv8Cache(kp.data_ptr(), vp.data_ptr(), ks.data_ptr(), vs.data_ptr(), kt.data_ptr(), vt.data_ptr(), table.data_ptr())
-    c.code_strides[:] = [kp.stride(0), kp.stride(1), vp.stride(0), vp.stride(1)]
-    c.scale_strides[:] = [ks.stride(0), ks.stride(1), vs.stride(0), vs.stride(1)]
+    strides = lambda t: [t.stride(0) if N > 1 else 0, t.stride(1) if H > 1 else 0]  # noqa: E731
+    c.code_strides[:], c.scale_strides[:] = strides(kp) + strides(vp), strides(ks) + strides(vs)
     c.num_pages, c.page_size, c.max_pages_per_seq, c.batch, c.head_num, c.size_per_head = N, P, table.shape[1], B, H, D
     c.code, c.dtype = _CODES[kp.dtype], _lib.dtype_tag(kt, who)
     return c
