@@ -92,6 +92,11 @@ def _cache(cache, who: str) -> _lib.Kv8Cache:
     return c
 
 
+def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether two contiguous tensors of a device share memory."""
+    return a.data_ptr() < b.data_ptr() + b.numel() * b.element_size() and b.data_ptr() < a.data_ptr() + a.numel() * a.element_size()
+
+
 def _lens(who: str, lens, B: int, device):
     info = seq_info(lens, B, device)
     if info.lens.device != device:
@@ -157,7 +162,7 @@ def kv8_pages_append(q, k_new, v_new, cache, kv_len_list, rotary=None, *, q_weig
 def kv8_pages_read(cache, kv_len_list, max_seq_len: int, *, first: Optional[torch.Tensor] = None, out=None):
     """The cached positions ``first[b] + s``, ``s < max_seq_len``, as ``(k, v)`` of ``[B,H,max_seq_len,D]`` in the tails' type, zeros from
     ``kv_len[b]`` on: what a prompt that goes on from a cached one attends to, or what a swapped-out sequence keeps.  ``first`` is int32 ``[B]``
-    (``None``: 0)."""
+    (``None``: 0, as which a negative one counts)."""
     who = "kv8_pages_read"
     if out is None and type(kv_len_list) is SeqInfo:
         pair = _lib.front.kv8_pages_read(cache, kv_len_list, max_seq_len, first)
@@ -179,8 +184,8 @@ def kv8_pages_read(cache, kv_len_list, max_seq_len: int, *, first: Optional[torc
     else:
         for t in out:
             _lib.require_gpu(t, "out")
-            if t.shape != shape or t.dtype != kt.dtype or t.device != device:
-                raise RuntimeError(f"{who}: out must be two contiguous [B,H,max_seq_len,D] tensors of the tails' dtype on the cache's device")
+        if len(out) != 2 or any(t.shape != shape or t.dtype != kt.dtype or t.device != device for t in out) or _overlap(*out):
+            raise RuntimeError(f"{who}: out must be two contiguous [B,H,max_seq_len,D] tensors of the tails' dtype on the cache's device, apart from one another")
     with _lib.device_guard(kt):
         _lib.check(_lib.fn.en_kv8_read(ctypes.byref(c), info.lens.data_ptr(), _lib.ptr(first) or None, S, out[0].data_ptr(), out[1].data_ptr(),
                                        _lib.stream_of(kt)), who)
@@ -219,8 +224,8 @@ def decode_attn_kv8(q, cache, kv_len_list, *, scale: Optional[float] = None, out
         out = torch.empty((B, Hq, 1, D), dtype=q.dtype, device=device)
     else:
         _lib.require_gpu(out, "out")
-        if out.numel() != B * Hq * D or out.dtype != q.dtype or out.device != device:
-            raise RuntimeError(f"{who}: out must be a contiguous [B,Hq,1,D] tensor of q's dtype on its device")
+        if out.numel() != B * Hq * D or out.dtype != q.dtype or out.device != device or (out.data_ptr() != q_.data_ptr() and _overlap(out, q_)):
+            raise RuntimeError(f"{who}: out must be a contiguous [B,Hq,1,D] tensor of q's dtype on its device, q itself or apart from it")
     need = decode_attn_kv8_workspace_bytes(B, Hq, c.head_num, c.max_pages_per_seq * c.page_size, D)
     if workspace is None:
         workspace = torch.empty(need, dtype=torch.uint8, device=device)

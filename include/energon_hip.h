@@ -511,7 +511,7 @@ int en_kv8_append(const void *q, const void *k_new, const void *v_new, void *q_o
 int en_kv8_read(const en_kv8_cache *cache, const int32_t *kv_lens, const int32_t *first, int seq_len, void *k_out, void *v_out,
                 en_stream_t stream);
 /* Decode attention: ctx[b, h] = softmax(scale * <q[b, h], K>) V over the kv_lens[b] cached positions of key head h / (q_heads /
- * head_num); zeros for an empty sequence.  q, ctx: contiguous [batch, q_heads, size_per_head].  With a capacity of max_pages_per_seq *
+ * head_num); zeros for an empty sequence.  q, ctx: contiguous [batch, q_heads, size_per_head], the same or apart.  With a capacity of max_pages_per_seq *
  * page_size, batch * head_num * ceil(q_heads / head_num / 16) * (capacity / 64 + 2) has to stay below 2^31.  workspace:
  * en_decode_attn_kv8_workspace_bytes (may be 0, then NULL), 16-byte aligned; its contents need not be kept or cleared, but calls that may
  * run at the same time need one each. */

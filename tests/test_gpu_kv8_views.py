@@ -51,3 +51,32 @@ def test_dimensions_of_one(native, N, H, P, odd):
         return (turned,) + K.kv8_pages_read(cache, now, n) + (K.decode_attn_kv8(q, cache, now),)
     for a, b in zip(run([]), run(odd)):
         assert torch.equal(a, b)
+
+
+def test_results_over_one_another():
+    """Two results of one read, or a context that lies partly over the queries, are refused; over the queries as a whole it may lie."""
+    import energonai_amd.kernel as K
+    announce("kv8 results over one another")
+    B, H, D, P = 3, 2, 64, 16
+    cache = K.kv8_pages(3, B, H, P, D, 1, F16, "cuda")
+    cache.page_table.copy_(torch.arange(3)[:, None])
+    x = torch.randn(27, 2 * H, D, device="cuda").half()
+    lens = torch.tensor([9, 9, 9], dtype=torch.int32).cuda()
+    K.kv8_pages_fill(x[:, :H], x[:, H:], cache, B, 9, lens)
+    k, v = K.kv8_pages_read(cache, lens, 12)
+    two = torch.empty(2, B, H, 12, D, device="cuda", dtype=F16)
+    got = K.kv8_pages_read(cache, lens, 12, out=(two[0], two[1]))
+    assert torch.equal(got[0], k) and torch.equal(got[1], v)
+    flat = torch.empty(two[0].numel() + 8, device="cuda", dtype=F16)
+    over = flat[:-8].view(k.shape), flat[8:].view(k.shape)
+    for out in ((two[0], two[0]), over, (over[1], over[0]), (two[0],), (two[0], two[1], two[1])):
+        with pytest.raises(RuntimeError):
+            K.kv8_pages_read(cache, lens, 12, out=out)
+    q = torch.randn(B, 4, 1, D, device="cuda").half()
+    want = K.decode_attn_kv8(q, cache, lens)
+    flat = torch.zeros(q.numel() + 64, device="cuda", dtype=F16)
+    qv = flat[:-64].view(q.shape)
+    qv.copy_(q)
+    with pytest.raises(RuntimeError):
+        K.decode_attn_kv8(qv, cache, lens, out=flat[64:].view(q.shape))
+    assert K.decode_attn_kv8(qv, cache, lens, out=qv) is qv and torch.equal(qv, want)
