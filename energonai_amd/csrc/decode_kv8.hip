@@ -2,8 +2,8 @@
 //
 // What bounds it is reading the codes, 2 D bytes a position and key head, and the split of very different lengths over the chip:
 //  - Work is dealt in tiles of 64 positions (four blocks).  The waves of the launch take equal, contiguous runs of all tiles of all (sequence,
-//    key head) units in a row, whatever the lengths are; the lengths are read here, so nothing depends on the caches' capacity.  A
-//    unit that one wave has whole is written by it; of others each wave leaves a partial result (at most two a wave: one at either end of its
+//    key head) units in a row, whatever the lengths are; the lengths are read here, and all that the caches' capacity decides is whether few or
+//    short units are dealt otherwise (kv8_deal).  A unit that one wave has whole is written by it; of others each wave leaves a partial result (at most two a wave: one at either end of its
 //    run), and a second, small launch combines those.
 //  - Scores are S^T = K Q^T on 16x16x32 matrix instructions: rows are positions, columns the up to 16 queries that share the key head.
 //    Row i of key tile t is position 4t + i%4 of block i/4 of the four.  A lane's 16 scores (column l%16) are then the 16 positions of block
@@ -12,10 +12,11 @@
 //  - Codes become 16-bit numbers exactly; the key scale multiplies the score, the value scale the probability.
 //  - The running maximum is raised only where a score passes it by 2^8: the sums are fp32, and probabilities of up to 2^8 are as exact
 //    in 16 bits as those below 1.
-// The probabilities are rounded to the cache's 16-bit type for the second product (half a step, 2^-12 or 2^-9, each; the first product's operands
-// are exact), relative to a reference m_o that follows score + log2(value scale), so that their products with the scale neither
-// vanish nor overflow in fp16, and 2^7 below it there: a product of up to 2^(7 + 8) is an fp16 number, and the smallest one that is not
-// rounded to zero is 2^-32 of the largest.  The sum of the softmax takes them in fp32 relative to the scores' own maximum m_s.
+// The probabilities, times their value scale, are rounded to the cache's 16-bit type for the second product (half a step, 2^-11 or 2^-8 of
+// each; the first product's operands are exact): the matrix instructions take both operands in one type, and in fp32 they are a sixteenth as
+// fast.  They are relative to a reference m_o that follows score + log2(value scale), so that they neither vanish nor overflow in fp16, and
+// 2^7 below it there: a product of up to 2^(7 + 8) is an fp16 number, and the smallest one that is not rounded to zero is 2^-32 of the
+// largest.  The sum of the softmax takes the probabilities in fp32, relative to the scores' own maximum m_s.
 #include <type_traits>
 
 #include "kv8_common.hip.h"
@@ -44,12 +45,13 @@ template <int DT> constexpr float kStand = DT == EN_F16 ? 7.f : 0.f;
 constexpr int kTeam = 8;                      // waves of a workgroup that takes one unit
 constexpr int kTeamCapacity = 1024, kTeamUnits = 512;
 constexpr int kWholeCapacity = 256;
-// How units are dealt: runs of tiles, equal whatever the lengths are, at the cost of a second launch; a workgroup a unit, where they are all
-// resident at once and a unit is at most two tiles a wave; or whole units to the waves in turn, where units are many and lengths cannot differ by
-// much.  us, pages of 64: runs / a workgroup a unit: 1 sequence of 100, 12 heads x 64 8.0 / 4.7; 32 of up to 500, 12 x 64 11.3 / 8.2;
-// 32 of up to 1000, 32 / 8 x 128 15.5 / 13.4, of up to 2000 19.5 / 20.2; 8 of up to 1000 11.7 / 12.2; 1 of 2000 10.3 / 18.1; 64 of up to 250,
-// 40 x 128 30.1 / 44.6.  Runs / whole units: 66 of 1, 128 / 8 x 80 9.3 / 6.6; 64 of up to 60, 40 x 128 19.7 / 17.0; 256 of up to 100, 8 x 128
-// 22.8 / 16.5; 64 of up to 250, 40 x 128 31.3 / 30.5, of up to 500 42.9 / 47.3; 20 of up to 500, 32 x 128 18.3 / 20.3; 40 of up to 2000 64 / 96.
+// How units are dealt: runs of tiles, equal whatever the lengths are, at the cost of a second launch; a workgroup a unit, where they are
+// all resident at once and a unit is at most two tiles a wave; or whole units to the waves in turn, where units are many and lengths cannot
+// differ by much.  us, pages of 64: runs / a workgroup a unit: 1 sequence of 100, 12 heads x 64 8.0 / 4.7; 32 of up to 500, 12 x 64 11.3 /
+// 8.2; 32 of up to 1000, 32 / 8 x 128 15.5 / 13.4, of up to 2000 19.5 / 20.2; 8 of up to 1000 11.7 / 12.2 (where the rule gives up 0.5); 1
+// of 2000 10.3 / 18.1; 64 of up to 250, 40 x 128 30.1 / 44.6.  Runs / whole units: 66 of 1, 128 / 8 x 80 9.3 / 6.6; 64 of up to 60, 40 x
+// 128 19.7 / 17.0; 256 of up to 100, 8 x 128 22.8 / 16.5; 64 of up to 250, 40 x 128 31.3 / 30.5, of up to 500 42.9 / 47.3; 20 of up to 500,
+// 32 x 128 18.3 / 20.3; 40 of up to 2000 64 / 96.
 enum class Deal { kTeam, kWhole, kRuns };
 inline Deal kv8_deal(int64_t units, int64_t capacity) {
   if (units <= kTeamUnits) return capacity <= kTeamCapacity ? Deal::kTeam : Deal::kRuns;
