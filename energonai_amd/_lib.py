@@ -34,6 +34,18 @@ class Kv8Cache(ctypes.Structure):
                 ("size_per_head", c_int), ("code", c_int), ("dtype", c_int)]
 
 
+class KvPages(ctypes.Structure):
+    """``en_kv_pages``"""
+    _fields_ = [("k_pool", c_void_p), ("v_pool", c_void_p), ("page_table", c_void_p), ("strides", c_int64 * 6), ("num_pages", c_int),
+                ("page_size", c_int), ("max_pages_per_seq", c_int), ("batch", c_int), ("head_num", c_int), ("size_per_head", c_int), ("dtype", c_int)]
+
+
+class W4(ctypes.Structure):
+    """``en_w4_weight``"""
+    _fields_ = [("codes", c_void_p), ("scales", c_void_p), ("zeros", c_void_p), ("out_features", c_int64), ("in_features", c_int64),
+                ("group", c_int), ("dtype", c_int)]
+
+
 # name -> (restype, argtypes); must list every symbol the header declares
 SIGNATURES = {
     "en_version": (c_int, []),
@@ -101,6 +113,15 @@ SIGNATURES = {
     "en_kv8_read": (c_int, [c_void_p] * 3 + [c_int] + [c_void_p] * 3),
     "en_decode_attn_kv8_workspace_bytes": (c_int64, [c_int] * 5),
     "en_decode_attn_kv8": (c_int, [c_void_p] * 4 + [c_int, c_float, c_void_p, c_int64, c_void_p]),
+    "en_draft_tree": (c_int, [c_void_p, c_void_p, c_int, c_int64] + [c_void_p] * 3),
+    "en_decode_attn_tree_workspace_bytes": (c_int64, [c_int] * 6),
+    "en_decode_attn_tree": (c_int, [c_void_p] * 9 + [c_int64, c_int, c_int, c_float, c_void_p, c_int64, c_void_p]),
+    "en_accept_drafts": (c_int, [c_void_p, c_int64, c_int, c_void_p, c_int, c_void_p, c_void_p, c_int, c_int64, c_int] + [c_void_p] * 3 + [c_int, c_void_p]),
+    "en_kv_extend_paged": (c_int, [c_void_p] * 6 + [c_int64, c_void_p, c_int] + [c_void_p] * 3),
+    "en_w4_codes_bytes": (c_int64, [c_int64] * 2),
+    "en_w4_groups": (c_int64, [c_int64, c_int64, c_int]),
+    "en_w4_pack": (c_int, [c_void_p] * 5),
+    "en_linear_w4": (c_int, [c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_int, c_void_p, c_void_p]),
     "en_copy_bytes": (c_int, [c_void_p, c_void_p, c_int64, c_void_p]),
     "en_stream_yardstick": (c_int, [c_void_p, c_void_p, c_int64, c_int, c_int, c_void_p]),
     "en_prefix_yardstick": (c_int, [c_void_p, c_void_p, c_void_p] + [c_int] * 7 + [c_void_p]),

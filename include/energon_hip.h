@@ -519,6 +519,80 @@ int64_t en_decode_attn_kv8_workspace_bytes(int batch, int q_heads, int head_num,
 int en_decode_attn_kv8(const void *q, void *ctx, const en_kv8_cache *cache, const int32_t *kv_lens, int q_heads, float scale,
                        void *workspace, int64_t workspace_bytes, en_stream_t stream);
 
+/* ---- drafted tokens: several nodes a sequence in one step -------------------- */
+
+/* A step may take several tokens of a sequence at once: the newest one, which is certain, and tokens drafted behind it, as a tree of up to
+ * EN_DRAFT_MAX_NODES nodes.  The nodes of a batch are packed rows, sequence b's from cu_seqlens[b] to cu_seqlens[b + 1] (what lies
+ * past EN_DRAFT_MAX_NODES, or past max_nodes where a call has it, does not exist); parents[row] is the node's parent in its sequence, -1 for none.  Node 0 is
+ * the root; a parent comes before its node (any other number counts as -1).  Their keys and values stay outside the cache until
+ * they are accepted. */
+#define EN_DRAFT_MAX_NODES 64
+
+/* masks[row]: bit i for node i on the way from the root to the node, itself among them; depths[row]: its steps from the root.  Rows of nodes that
+ * do not exist get 0 and 0. */
+int en_draft_tree(const int32_t *parents, const int32_t *cu_seqlens, int batch, int64_t nodes, int64_t *masks, int32_t *depths,
+                  en_stream_t stream);
+
+/* K and V in pages: position j of sequence b is row j % page_size of page page_table[b, j / page_size]. */
+typedef struct en_kv_pages {
+  void *k_pool, *v_pool;                 /* [pages, head_num, page_size, size_per_head] */
+  const int32_t *page_table;             /* [batch, max_pages_per_seq] */
+  int64_t strides[6];                    /* elements: page, head, row of k; of v.  Channels are contiguous */
+  int32_t num_pages, page_size, max_pages_per_seq, batch, head_num, size_per_head;   /* page_size a power of two, at least 16 */
+  int32_t dtype;
+} en_kv_pages;
+
+/* Attention of the nodes: row r of q (node i of sequence b, query head h) sees the kv_lens[b] cached positions of key head h / (q_heads /
+ * head_num) and those nodes of its sequence whose bit is set in masks[r] (bits of nodes that do not exist are ignored); zeros where it sees
+ * nothing.  A page id outside the pool reads as zeros, as in en_decode_attn_paged.  A value that is not a number reaches the nodes that see it and no
+ * others.  fp16 and bf16, heads of a multiple of 8 channels up to 128, scale positive.  strides: (token, head) in elements of q [nodes,
+ * q_heads, size_per_head], k_new, v_new [nodes, head_num, size_per_head], multiples of 8; ctx is contiguous [nodes, q_heads,
+ * size_per_head], its rows of nodes that do not exist are left as they are.  workspace: en_decode_attn_tree_workspace_bytes (may be 0, then NULL) for a capacity of
+ * max_pages_per_seq * page_size, 16-byte aligned; its contents need not be kept or cleared, but calls that may run at the same time need one each. */
+int64_t en_decode_attn_tree_workspace_bytes(int batch, int q_heads, int head_num, int capacity, int size_per_head, int max_nodes);
+int en_decode_attn_tree(const void *q, const void *k_new, const void *v_new, const int64_t *strides, void *ctx, const en_kv_pages *cache,
+                        const int32_t *kv_lens, const int32_t *cu_seqlens, const int64_t *masks, int64_t nodes, int max_nodes, int q_heads,
+                        float scale, void *workspace, int64_t workspace_bytes, en_stream_t stream);
+
+/* Greedy acceptance.  From node 0 on: t is the index of the largest of the node's logits (the lowest of equal ones; NaN counts as the
+ * largest); its lowest child whose token is t is accepted next, and where there is none, t is the token that follows.
+ * path[b, i], i < max_nodes: the i-th accepted node (node 0 first), -1 behind the last; counts[b]: how many; next_tokens[b]: t.  A sequence
+ * without nodes has 0 and -1.  logits: [nodes, vocab] rows, logits_stride elements apart; tokens int32 or int64 (tokens_are_i64). */
+int en_accept_drafts(const void *logits, int64_t logits_stride, int vocab, const void *tokens, int tokens_are_i64, const int32_t *parents,
+                     const int32_t *cu_seqlens, int batch, int64_t nodes, int max_nodes, int32_t *path, int32_t *counts, int64_t *next_tokens,
+                     int dtype, en_stream_t stream);
+
+/* The accepted nodes' keys and values into their pages: row cu_seqlens[b] + path[b, i] of k_new and v_new becomes position kv_lens[b] + i of
+ * sequence b, i < min(counts[b], path_width).  Entries of path that are no node of the sequence are passed over; a position without a page in the pool
+ * is not written and counted in overflow, if given.  strides: (token, head) in elements of k_new, v_new [nodes, head_num, size_per_head].
+ * The caller advances the lengths afterwards. */
+int en_kv_extend_paged(const void *k_new, const void *v_new, const int64_t *strides, const en_kv_pages *cache, const int32_t *kv_lens,
+                       const int32_t *cu_seqlens, int64_t nodes, const int32_t *path, int path_width, const int32_t *counts,
+                       int32_t *overflow, en_stream_t stream);
+
+/* ---- weights in 4 bits ------------------------------------------------------ */
+
+/* A weight [out_features, in_features] in 4 bits: W[n, k] = (code[n, k] - zero[n, k / group]) * scale[n, k / group], codes and zero points
+ * 0 .. 15 (without zero points 8), scales of the activations' dtype, groups of 32, 64 or 128 channels.  in_features is a multiple of 8.  It
+ * is laid out once, by en_w4_pack, in tiles of 16 rows and 128 channels as the kernels load them; rows and channels that fill up the last
+ * tiles have code 0 and scale 0. */
+typedef struct en_w4_weight {
+  const void *codes;                     /* en_w4_codes_bytes, 16-byte aligned */
+  const void *scales;                    /* en_w4_groups elements of dtype, 16-byte aligned */
+  const void *zeros;                     /* as many bytes, 16-byte aligned, or NULL */
+  int64_t out_features, in_features;
+  int32_t group, dtype;                  /* EN_F16 or EN_BF16 */
+} en_w4_weight;
+int64_t en_w4_codes_bytes(int64_t out_features, int64_t in_features);
+int64_t en_w4_groups(int64_t out_features, int64_t in_features, int group);
+/* codes [out_features, in_features / 2] bytes, channel 2i in the lower half of byte i; scales, zeros (or NULL) [out_features,
+ * ceil(in_features / group)]; contiguous.  The results' pointers in `weight` are written through. */
+int en_w4_pack(const uint8_t *codes, const void *scales, const uint8_t *zeros, const en_w4_weight *weight, en_stream_t stream);
+/* y = act(x W^T + bias): x [rows, in_features], x_stride elements apart (a multiple of 8), 16-byte aligned; y contiguous [rows,
+ * out_features]; bias [out_features] or NULL; activation an en_activation.  Sums are fp32. */
+int en_linear_w4(const void *x, int64_t rows, int64_t x_stride, const en_w4_weight *weight, const void *bias, int activation, void *y,
+                 en_stream_t stream);
+
 /* ---- measurement helper ------------------------------------------------- */
 
 /* The whole step in one call: depad, transpose_pad, QK^T, scale_mask_softmax, PV,
