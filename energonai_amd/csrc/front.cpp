@@ -455,6 +455,17 @@ void order_stream(PyObject *info, const Tensor &t) {
   Py_DECREF(done);
 }
 
+// Exactly a SeqInfo.
+bool seq_info(PyObject *o) {
+  static PyTypeObject *known = nullptr;
+  if (Py_TYPE(o) == known) return true;
+  PyObject *module = PyImport_ImportModule("energonai_amd.seqinfo"), *type = module ? PyObject_GetAttrString(module, "SeqInfo") : nullptr;
+  Py_XDECREF(module);
+  if (!type) fail("SeqInfo: no type");
+  known = reinterpret_cast<PyTypeObject *>(type);      // held on
+  return Py_TYPE(o) == known;
+}
+
 // Numbers and flags of a plain call.  False, with no Python error left, for what is none or does not fit: the Python call names it.
 bool whole(PyObject *o, int64_t &v) {
   if (!PyLong_Check(o)) return false;
@@ -822,6 +833,181 @@ PyObject *decode_attn_kv8(PyObject *const *a) {
   const hipStream_t stream = stream_of(*q);
   check(without_gil([&] { return en_decode_attn_kv8(q_p, out_p, &c, lens_p, (int)Hq, scale, ws_p, need, stream); }), "decode_attn_kv8");
   return THPVariable_Wrap(out);
+}
+
+// ---- drafted steps, weights in 4 bits ------------------------------------------------------------------------------------
+
+// A DraftTree (parents, masks, depths, info, max_nodes): the `field` of its tensors that a call reads, one for each of `nodes` rows, and
+// the offsets of `batch` sequences.
+bool draft_tree_of(PyObject *o, const Tensor &home, int64_t nodes, int64_t batch, int field, at::ScalarType type, const Tensor *&t, Lens &info, int64_t &most) {
+  if (!PyTuple_Check(o) || PyTuple_GET_SIZE(o) != 5 || !whole(PyTuple_GET_ITEM(o, 4), most) || most < 1 || most > EN_DRAFT_MAX_NODES) return false;
+  if (field >= 0) {
+    t = plain_contiguous(PyTuple_GET_ITEM(o, field));
+    if (!t || t->dim() != 1 || t->numel() != nodes || t->scalar_type() != type || t->device() != home.device()) return false;
+  }
+  return seq_info(PyTuple_GET_ITEM(o, 3)) && lens_of(PyTuple_GET_ITEM(o, 3), home, batch, true, info);
+}
+
+// en_kv_pages of two pools and a table for `batch` sequences.
+bool kv_pages(const Tensor *kp, const Tensor *vp, PyObject *table_o, int64_t &batch, en_kv_pages &c) {
+  if (!kp || !vp || vp->sizes() != kp->sizes() || vp->scalar_type() != kp->scalar_type() || vp->device() != kp->device()) return false;
+  const Tensor *table = plain_contiguous(table_o);
+  if (!table || table->dim() != 2 || table->scalar_type() != at::kInt || table->device() != kp->device()) return false;
+  const int64_t N = kp->size(0), H = kp->size(1), P = kp->size(2), D = kp->size(3);
+  const int tag = known_tag(*kp);
+  batch = table->size(0);
+  if (tag < 0 || !fits_int({N, H, P, D, batch, table->size(1), table->size(1) * P})) return false;
+  auto page = [&](const Tensor &t) -> int64_t { return N > 1 ? t.stride(0) : 0; };      // a dimension of one has whatever stride
+  auto head = [&](const Tensor &t) -> int64_t { return H > 1 ? t.stride(1) : 0; };
+  c = en_kv_pages{kp->data_ptr(), vp->data_ptr(), i32(*table), {page(*kp), head(*kp), kp->stride(2), page(*vp), head(*vp), vp->stride(2)},
+                  (int32_t)N, (int32_t)P, (int32_t)table->size(1), (int32_t)batch, (int32_t)H, (int32_t)D, tag};
+  return true;
+}
+
+// Strides (token, head) of [nodes, heads, D] rows; those of a dimension of one may be any.
+bool node_rows(const Tensor *t, const Tensor &pool, int64_t nodes, int64_t heads, int64_t D, int64_t *strides) {
+  if (!t || t->size(0) != nodes || (heads > 0 && t->size(1) != heads) || t->size(2) != D || t->scalar_type() != pool.scalar_type() || t->device() != pool.device())
+    return false;
+  strides[0] = t->size(0) > 1 ? t->stride(0) : 0;
+  strides[1] = t->size(1) > 1 ? t->stride(1) : 0;
+  return true;
+}
+bool vectors(const Tensor &t, const int64_t *strides, int n) {
+  if (reinterpret_cast<uintptr_t>(t.data_ptr()) % 16) return false;
+  for (int i = 0; i < n; ++i)
+    if (strides[i] % 8) return false;
+  return true;
+}
+
+// decode_attn_tree(q, k_new, v_new, k_pool, v_pool, SeqInfo, page_table, DraftTree, scale or None) -> ctx or None
+PyObject *decode_attn_tree(PyObject *const *a) {
+  const Tensor *q = plain_rows(a[0], 3), *kn = plain_rows(a[1], 3), *vn = plain_rows(a[2], 3), *kp = plain_rows(a[3], 4), *vp = plain_rows(a[4], 4), *masks;
+  en_kv_pages c;
+  int64_t B, most, st[6];
+  Lens info, tree;
+  if (!q || modes_on() || !kv_pages(kp, vp, a[6], B, c) || c.dtype == EN_F32) Py_RETURN_NONE;
+  const int64_t T = q->size(0), Hq = q->size(1), D = c.size_per_head;
+  float scale = (float)std::pow((double)D, -0.5);
+  if (!fits_int({T, Hq}) || Hq % c.head_num || D % 8 || D > 128 || !node_rows(q, *kp, T, 0, D, st) || !node_rows(kn, *kp, T, c.head_num, D, st + 2) ||
+      !node_rows(vn, *kp, T, c.head_num, D, st + 4) || !vectors(*q, st, 2) || !vectors(*kn, st + 2, 2) || !vectors(*vn, st + 4, 2) ||
+      !vectors(*kp, c.strides, 3) || !vectors(*vp, c.strides + 3, 3) || !seq_info(a[5]) || !lens_of(a[5], *kp, B, false, info) ||
+      !draft_tree_of(a[7], *kp, T, B, 1, at::kLong, masks, tree, most) || (a[8] != Py_None && !number(a[8], scale)))
+    Py_RETURN_NONE;
+  const c10::DeviceGuard guard(q->device());
+  order_stream(a[5], *q);
+  order_stream(PyTuple_GET_ITEM(a[7], 3), *q);
+  const int64_t need = en_decode_attn_tree_workspace_bytes((int)B, (int)Hq, c.head_num, c.max_pages_per_seq * c.page_size, (int)D, (int)most);
+  const Tensor out = at::empty({T, Hq, D}, q->options());
+  Tensor ws;
+  if (need > 0) ws = at::empty({need}, q->options().dtype(at::kByte));
+  const void *q_p = q->data_ptr(), *kn_p = kn->data_ptr(), *vn_p = vn->data_ptr();
+  void *out_p = out.data_ptr(), *ws_p = need > 0 ? ws.data_ptr() : nullptr;
+  const int32_t *lens_p = i32(*info.lens), *cu_p = i32(*tree.cu);
+  const int64_t *masks_p = masks->data_ptr<int64_t>();
+  const hipStream_t stream = stream_of(*q);
+  check(without_gil([&] {
+          return en_decode_attn_tree(q_p, kn_p, vn_p, st, out_p, &c, lens_p, cu_p, masks_p, T, (int)most, (int)Hq, scale, ws_p, need, stream);
+        }), "decode_attn_tree");
+  return THPVariable_Wrap(out);
+}
+
+// accept_drafts(logits, tokens, DraftTree) -> (path, counts, next tokens) or None
+PyObject *accept_drafts(PyObject *const *a) {
+  const Tensor *logits = plain_rows(a[0], 2), *tokens = plain_contiguous(a[1]), *parents;
+  if (!logits || !tokens || modes_on() || !PyTuple_Check(a[2]) || PyTuple_GET_SIZE(a[2]) != 5) Py_RETURN_NONE;
+  const int64_t T = logits->size(0), V = logits->size(1), stride = T > 1 ? logits->stride(0) : V;
+  const int tag = known_tag(*logits);
+  const bool wide = tokens->scalar_type() == at::kLong;
+  static PyObject *const size = PyUnicode_InternFromString("batch_size");
+  PyObject *info_o = PyTuple_GET_ITEM(a[2], 3);
+  if (!seq_info(info_o)) Py_RETURN_NONE;
+  const int64_t B = integer(held(info_o, size));
+  int64_t most;
+  Lens tree;
+  if (tag < 0 || tokens->dim() != 1 || tokens->numel() != T || (!wide && tokens->scalar_type() != at::kInt) || tokens->device() != logits->device() ||
+      !fits_int({T, V, B}) || !draft_tree_of(a[2], *logits, T, B, 0, at::kInt, parents, tree, most))
+    Py_RETURN_NONE;
+  const c10::DeviceGuard guard(logits->device());
+  order_stream(info_o, *logits);
+  const auto opt = logits->options();
+  const Tensor path = at::empty({B, most}, opt.dtype(at::kInt)), counts = at::empty({B}, opt.dtype(at::kInt)), next = at::empty({B}, opt.dtype(at::kLong));
+  const void *logits_p = logits->data_ptr(), *tokens_p = tokens->data_ptr();
+  const int32_t *parents_p = i32(*parents), *cu_p = i32(*tree.cu);
+  int32_t *path_p = path.data_ptr<int32_t>(), *counts_p = counts.data_ptr<int32_t>();
+  int64_t *next_p = next.data_ptr<int64_t>();
+  const hipStream_t stream = stream_of(*logits);
+  check(without_gil([&] {
+          return en_accept_drafts(logits_p, stride, (int)V, tokens_p, wide, parents_p, cu_p, (int)B, T, (int)most, path_p, counts_p, next_p, tag, stream);
+        }), "accept_drafts");
+  return tuple({path, counts, next});
+}
+
+// kv_pages_extend(k_new, v_new, k_pool, v_pool, SeqInfo, page_table, DraftTree, path, counts, overflow or None) -> True or None
+PyObject *kv_pages_extend(PyObject *const *a) {
+  const Tensor *kn = plain_rows(a[0], 3), *vn = plain_rows(a[1], 3), *kp = plain_rows(a[2], 4), *vp = plain_rows(a[3], 4), *path = plain_contiguous(a[7]),
+               *counts = plain_contiguous(a[8]), *none;
+  en_kv_pages c;
+  int64_t B, most, st[4];
+  int32_t *over;
+  Lens info, tree;
+  if (!kn || !path || !counts || modes_on() || !kv_pages(kp, vp, a[5], B, c)) Py_RETURN_NONE;
+  const int64_t T = kn->size(0), D = c.size_per_head;
+  if (!fits_int({T}) || !node_rows(kn, *kp, T, c.head_num, D, st) || !node_rows(vn, *kp, T, c.head_num, D, st + 2) || !seq_info(a[4]) ||
+      !lens_of(a[4], *kp, B, false, info) || !draft_tree_of(a[6], *kp, T, B, -1, at::kInt, none, tree, most) || path->dim() != 2 || path->size(0) != B ||
+      path->size(1) > EN_DRAFT_MAX_NODES || path->scalar_type() != at::kInt || path->device() != kp->device() || counts->dim() != 1 ||
+      counts->numel() != B || counts->scalar_type() != at::kInt || counts->device() != kp->device() || !counter(a[9], *kp, over))
+    Py_RETURN_NONE;
+  const c10::DeviceGuard guard(kp->device());
+  order_stream(a[4], *kp);
+  order_stream(PyTuple_GET_ITEM(a[6], 3), *kp);
+  const void *kn_p = kn->data_ptr(), *vn_p = vn->data_ptr();
+  const int32_t *lens_p = i32(*info.lens), *cu_p = i32(*tree.cu), *path_p = i32(*path), *counts_p = i32(*counts);
+  const int width = (int)path->size(1);
+  const hipStream_t stream = stream_of(*kp);
+  check(without_gil([&] { return en_kv_extend_paged(kn_p, vn_p, st, &c, lens_p, cu_p, T, path_p, width, counts_p, over, stream); }), "kv_pages_extend");
+  Py_RETURN_TRUE;
+}
+
+// linear_w4(inputs, W4Weight, bias or None, activation) -> y or None
+PyObject *linear_w4(PyObject *const *a) {
+  const Tensor *x = plain(a[0]);
+  if (!x || modes_on() || !PyTuple_Check(a[1]) || PyTuple_GET_SIZE(a[1]) != 6 || x->dim() < 1 || x->dim() > 8) Py_RETURN_NONE;
+  const Tensor *codes = plain_contiguous(PyTuple_GET_ITEM(a[1], 0)), *scales = plain_contiguous(PyTuple_GET_ITEM(a[1], 1)), *zeros = nullptr, *bias = nullptr;
+  int64_t N, K, G, act;
+  if (!codes || !scales || !whole(PyTuple_GET_ITEM(a[1], 3), N) || !whole(PyTuple_GET_ITEM(a[1], 4), K) || !whole(PyTuple_GET_ITEM(a[1], 5), G) ||
+      !whole(a[3], act) || !fits_int({N, K, G}))
+    Py_RETURN_NONE;
+  const int tag = known_tag(*x);
+  if ((tag != EN_F16 && tag != EN_BF16) || scales->scalar_type() != x->scalar_type() || codes->scalar_type() != at::kByte || codes->device() != x->device() ||
+      scales->device() != x->device() || codes->numel() != en_w4_codes_bytes(N, K) || scales->numel() != en_w4_groups(N, K, (int)G) || x->size(-1) != K)
+    Py_RETURN_NONE;
+  if (PyTuple_GET_ITEM(a[1], 2) != Py_None) {
+    zeros = plain_contiguous(PyTuple_GET_ITEM(a[1], 2));
+    if (!zeros || zeros->scalar_type() != at::kByte || zeros->device() != x->device() || zeros->numel() != scales->numel()) Py_RETURN_NONE;
+  }
+  if (a[2] != Py_None) {
+    bias = plain_contiguous(a[2]);
+    if (!bias || bias->dim() != 1 || bias->numel() != N || bias->scalar_type() != x->scalar_type() || bias->device() != x->device()) Py_RETURN_NONE;
+  }
+  // contiguous, or a matrix of rows some vectors apart
+  const int64_t rows = x->numel() / K;
+  int64_t stride = K;
+  if (!x->is_contiguous()) {
+    if (x->dim() != 2 || x->stride(1) != 1 || x->stride(0) < K || x->stride(0) % 8) Py_RETURN_NONE;
+    stride = x->stride(0);
+  }
+  if (reinterpret_cast<uintptr_t>(x->data_ptr()) % 16) Py_RETURN_NONE;
+  const c10::DeviceGuard guard(x->device());
+  int64_t shape[8];
+  for (int64_t i = 0; i < x->dim(); ++i) shape[i] = x->size(i);
+  shape[x->dim() - 1] = N;
+  const Tensor y = at::empty(c10::IntArrayRef(shape, x->dim()), x->options());
+  const en_w4_weight w{codes->data_ptr(), scales->data_ptr(), zeros ? zeros->data_ptr() : nullptr, N, K, (int32_t)G, tag};
+  const void *x_p = x->data_ptr(), *bias_p = bias ? bias->data_ptr() : nullptr;
+  void *y_p = y.data_ptr();
+  const hipStream_t stream = stream_of(*x);
+  check(without_gil([&] { return en_linear_w4(x_p, rows, stride, &w, bias_p, (int)act, y_p, stream); }), "linear_w4");
+  return THPVariable_Wrap(y);
 }
 
 // depad(src, SeqInfo, batch, left_padded, total) -> packed rows or None
@@ -1271,6 +1457,10 @@ PyMethodDef kMethods[] = {
     EN_FAST(kv8_pages_append, 11, "kv8_pages_append of plain operands, or None"),
     EN_FAST(kv8_pages_read, 4, "kv8_pages_read of plain operands, or None"),
     EN_FAST(decode_attn_kv8, 4, "decode_attn_kv8 of plain operands, or None"),
+    EN_FAST(decode_attn_tree, 9, "decode_attn_tree of plain operands, or None"),
+    EN_FAST(accept_drafts, 3, "accept_drafts of plain operands, or None"),
+    EN_FAST(kv_pages_extend, 10, "kv_pages_extend of plain operands, or None"),
+    EN_FAST(linear_w4, 4, "linear_w4 of plain operands, or None"),
     EN_FAST(depad, 5, "depad of plain operands, or None"),
     EN_FAST(transpose_pad, 6, "transpose_pad of plain operands, or None"),
     EN_FAST(transpose_depad, 7, "transpose_depad of plain operands, or None"),

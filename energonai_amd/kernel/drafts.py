@@ -131,6 +131,10 @@ def decode_attn_tree(q, k_new, v_new, k_pool, v_pool, kv_len_list, page_table, t
     that do not exist are left as they are.  fp16 and bf16, heads of a multiple of 8 channels up to 128.  ``scale`` defaults to ``D ** -0.5``;
     ``out`` may be ``q``; ``workspace``: any tensor of ``decode_attn_tree_workspace_bytes`` bytes (``None``: a temporary)."""
     who = "decode_attn_tree"
+    if out is None and workspace is None and type(tree) is DraftTree:
+        ctx = _lib.front.decode_attn_tree(q, k_new, v_new, k_pool, v_pool, kv_len_list, page_table, tree, scale)
+        if ctx is not None:
+            return ctx
     B = page_table.shape[0] if isinstance(page_table, torch.Tensor) and page_table.dim() == 2 else 0
     c = _kv_pages(who, k_pool, v_pool, page_table, B)
     if k_pool.dtype not in _TYPES:
@@ -186,6 +190,10 @@ def accept_drafts(logits, tokens, tree):
     with contiguous rows, ``tokens`` int32 or int64 ``[nodes]``.  Returns ``(path, counts, next_tokens)``: int32 ``[B, max_nodes]``, the
     accepted nodes and -1 behind them; int32 ``[B]``, how many (at least 1; 0 for a sequence without nodes); int64 ``[B]``, the token that follows (-1)."""
     who = "accept_drafts"
+    if type(tree) is DraftTree:
+        found = _lib.front.accept_drafts(logits, tokens, tree)
+        if found is not None:
+            return found
     _lib.require_gpu(logits, "logits", contiguous=False)
     if logits.dim() != 2 or (logits.shape[1] > 1 and logits.stride(1) != 1) or logits.shape[1] < 1:
         raise RuntimeError(f"{who}: logits must be a [nodes, vocab] tensor with contiguous rows")
@@ -213,6 +221,8 @@ def kv_pages_extend(k_new, v_new, k_pool, v_pool, kv_len_list, page_table, tree,
     (any token and head strides) become positions ``kv_len[b] + i`` of sequence ``b``.  The caller advances the lengths afterwards.  Entries of
     ``path`` that name no node are passed over; a position that has no page in the pool is not written and counted in ``overflow``."""
     who = "kv_pages_extend"
+    if type(tree) is DraftTree and _lib.front.kv_pages_extend(k_new, v_new, k_pool, v_pool, kv_len_list, page_table, tree, path, counts, overflow):
+        return
     B = page_table.shape[0] if isinstance(page_table, torch.Tensor) and page_table.dim() == 2 else 0
     c = _kv_pages(who, k_pool, v_pool, page_table, B)
     T = k_new.shape[0] if isinstance(k_new, torch.Tensor) and k_new.dim() == 3 else 0

@@ -120,6 +120,10 @@ def linear_w4(inputs, weight, bias=None, activation: Optional[str] = None):
     """``linear`` with a weight in 4 bits: ``act(inputs[..., din] @ W[dout, din]^T + bias)`` -> ``[..., dout]``, fp16 or bf16 as the weight's
     scales are.  Sums are fp32 and no weight is rounded to 16 bits.  ``activation``: ``"relu"``, ``"gelu_tanh"`` or ``"gelu"``."""
     who = "linear_w4"
+    if type(weight) is W4Weight and activation in _ACTIVATIONS:
+        y = _lib.front.linear_w4(inputs, weight, bias, _ACTIVATIONS[activation])
+        if y is not None:
+            return y
     w = _struct(who, weight)
     _lib.require_gpu(inputs, "inputs", contiguous=False)
     if inputs.dim() < 1 or inputs.shape[-1] != w.in_features or inputs.dtype != weight.scales.dtype or inputs.device != weight.codes.device:
