@@ -116,7 +116,9 @@ SIGNATURES = {
     "en_draft_tree": (c_int, [c_void_p, c_void_p, c_int, c_int64] + [c_void_p] * 3),
     "en_decode_attn_tree_workspace_bytes": (c_int64, [c_int] * 6),
     "en_decode_attn_tree": (c_int, [c_void_p] * 9 + [c_int64, c_int, c_int, c_float, c_void_p, c_int64, c_void_p]),
-    "en_accept_drafts": (c_int, [c_void_p, c_int64, c_int, c_void_p, c_int, c_void_p, c_void_p, c_int, c_int64, c_int] + [c_void_p] * 3 + [c_int, c_void_p]),
+    "en_accept_drafts": (c_int, [c_void_p, c_int64, c_int, c_void_p, c_int, c_void_p, c_void_p, c_int, c_int64, c_int] + [c_void_p] * 3 +
+                         [c_int, c_void_p, c_int64, c_void_p]),
+    "en_accept_drafts_workspace_bytes": (c_int64, [c_int64, c_int, c_int]),
     "en_kv_extend_paged": (c_int, [c_void_p] * 6 + [c_int64, c_void_p, c_int] + [c_void_p] * 3),
     "en_w4_codes_bytes": (c_int64, [c_int64] * 2),
     "en_w4_groups": (c_int64, [c_int64, c_int64, c_int]),

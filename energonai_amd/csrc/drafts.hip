@@ -1,5 +1,7 @@
 // Drafted tokens around their attention: the tree's masks, which of them a greedy decoding accepts, and the accepted rows' way into the
 // cache.
+#include <type_traits>
+
 #include "paged_common.hip.h"
 
 namespace en {
@@ -33,6 +35,116 @@ __global__ __launch_bounds__(kWave) void draft_tree_kernel(const int32_t *parent
 
 // ---- acceptance ------------------------------------------------------------------------------------------------------------------
 
+// What counts is how a row's largest logit is found: the rows on the way are read one after another, each by what the one before chose, and a
+// compute unit that reads one by itself is bound by its instructions as much as by its loads.  So a lane takes vectors of 16 bytes, 16-bit
+// logits two at a time in the order of signed integers (sign and magnitude turned into it), and remembers only which of its vectors holds the
+// best; the vector is read once more for the index.  That order is that of the numbers but for zeros of two signs and NaN, whose
+// largest magnitude is kept beside; a row that has NaN, or zero for its largest, is gone over once more element by element.
+typedef short s16x2 __attribute__((ext_vector_type(2)));
+typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+
+template <int DT> struct Logits {
+  static constexpr int kPer = 16 / Elem<DT>::kSize;
+  static constexpr uint32_t kInf = DT == EN_F16 ? 0x7c00u : DT == EN_BF16 ? 0x7f80u : 0x7f800000u;
+  // The vector's largest in the integers' order, and the largest magnitude's bits.
+  __device__ static __forceinline__ int largest(const uint4 &v, uint32_t &magnitude) {
+    if constexpr (DT == EN_F32) {
+      auto order = [](uint32_t x) { return (int)(x ^ ((uint32_t)((int)x >> 31) & 0x7fffffffu)); };
+      magnitude = max(max(v.x & 0x7fffffffu, v.y & 0x7fffffffu), max(v.z & 0x7fffffffu, v.w & 0x7fffffffu));
+      return max(max(order(v.x), order(v.y)), max(order(v.z), order(v.w)));
+    } else {
+      auto order = [](uint32_t x) {
+        const s16x2 sign = __builtin_bit_cast(s16x2, x) >> 15;
+        return __builtin_bit_cast(s16x2, x ^ (__builtin_bit_cast(uint32_t, sign) & 0x7fff7fffu));
+      };
+      auto size = [](uint32_t x) { return __builtin_bit_cast(u16x2, x & 0x7fff7fffu); };
+      const u16x2 m = __builtin_elementwise_max(__builtin_elementwise_max(size(v.x), size(v.y)), __builtin_elementwise_max(size(v.z), size(v.w)));
+      magnitude = max((uint32_t)m.x, (uint32_t)m.y);
+      const s16x2 o = __builtin_elementwise_max(__builtin_elementwise_max(order(v.x), order(v.y)), __builtin_elementwise_max(order(v.z), order(v.w)));
+      return max((int)o.x, (int)o.y);
+    }
+  }
+  // Index of the first element that is `order`.
+  __device__ static __forceinline__ int first(const uint4 &v, int order) {
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+    const uint32_t bits = order < 0 ? (uint32_t)order ^ 0x7fffffffu : (uint32_t)order;
+    int at = 0;
+#pragma unroll
+    for (int i = kPer - 1; i >= 0; --i) {
+      const bool same = DT == EN_F32 ? w[i % 4] == bits : (uint16_t)(w[i / 2 % 4] >> (16 * (i % 2))) == (uint16_t)((order < 0 ? order ^ 0x7fff : order));
+      at = same ? i : at;
+    }
+    return at;
+  }
+};
+
+// Logits in an order of whole numbers, NaN above all, zeros equal; 0 is below all of them.
+__device__ __forceinline__ uint32_t ordered(float x) {
+  const uint32_t u = __float_as_uint(x);
+  return x != x ? 0xffffffffu : x == 0.f ? 0x80000000u : u & 0x80000000u ? ~u : u | 0x80000000u;
+}
+__device__ __forceinline__ uint64_t wave_largest(uint64_t v) {
+#pragma unroll
+  for (int d = 1; d < kWave; d *= 2) {
+    const uint64_t w = (uint64_t)(uint32_t)__shfl_xor((int)(v >> 32), d, kWave) << 32 | (uint32_t)__shfl_xor((int)(uint32_t)v, d, kWave);
+    v = w > v ? w : v;
+  }
+  return v;
+}
+// Over a workgroup of W waves; every lane has the result.  Slots belong to one of two calls in turn.
+template <int W> __device__ __forceinline__ uint64_t block_largest(uint64_t v, uint64_t *slots) {
+  v = wave_largest(v);
+  if (threadIdx.x % kWave == 0) slots[threadIdx.x / kWave] = v;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < W; ++w) v = max(v, slots[w]);
+  return v;
+}
+
+// The largest of elements from .. to - 1 of a row, at least one: `ordered` above, the complement of its index below.
+template <int DT, int W>
+__device__ __forceinline__ uint64_t row_best(const typename Elem<DT>::T *row, int from, int to, uint64_t (*slots)[W]) {
+  typedef Logits<DT> L;
+  typedef typename Elem<DT>::T T;
+  constexpr int kThreads = W * kWave, kPer = L::kPer, kAhead = 4;
+  if (to - from >= kPer) {
+    const int vectors = (to - from + kPer - 1) / kPer;
+    auto start = [&](int v) { return min(from + v * kPer, to - kPer); };       // the last one overlaps the one before
+    int best = INT32_MIN, at = 0;
+    uint32_t magnitude = 0;
+    for (int v0 = threadIdx.x; v0 < vectors; v0 += kAhead * kThreads) {
+      uint4 x[kAhead];
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) x[i] = load16_at<false, sizeof(T)>(row + start(min(v0 + i * kThreads, vectors - 1)));
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) {
+        uint32_t m;
+        const int o = L::largest(x[i], m);
+        magnitude = max(magnitude, m);
+        if (o > best) {
+          best = o;
+          at = min(v0 + i * kThreads, vectors - 1);
+        }
+      }
+    }
+    const uint64_t mine = (uint64_t)((uint32_t)best ^ 0x80000000u) << 32 | (uint32_t)~at;
+    // (a lane without vectors has INT32_MIN, which is 0 here)
+    const uint64_t top = block_largest<W>(magnitude > L::kInf ? ~0ull : mine, slots[0]);
+    const int order = (int)((uint32_t)(top >> 32) ^ 0x80000000u);
+    if (top != ~0ull && order != 0 && order != -1) {
+      const int s = start((int)~(uint32_t)top);
+      const int i = s + L::first(load16_at<false, sizeof(T)>(row + s), order);
+      return (uint64_t)ordered(Elem<DT>::to_float(row[i])) << 32 | (uint32_t)~i;
+    }
+  }
+  uint64_t best = 0;
+  for (int i = from + threadIdx.x; i < to; i += kThreads) {
+    const uint64_t v = (uint64_t)ordered(Elem<DT>::to_float(row[i])) << 32 | (uint32_t)~i;
+    best = v > best ? v : best;
+  }
+  return block_largest<W>(best, slots[1]);
+}
+
 struct AcceptArgs {
   const void *logits;
   int64_t stride, total;
@@ -43,58 +155,65 @@ struct AcceptArgs {
   int max_nodes;
   int32_t *path, *counts;
   int64_t *next;
+  uint64_t *best;                // [rows][slices] where all rows are looked at first
+  int slices, slice;             // elements of a slice, a multiple of a vector
 };
 
-// Logits in an order of whole numbers, NaN above all; 0 is below all of them.
-template <int DT> __device__ __forceinline__ uint32_t ordered(float x) {
-  const uint32_t u = __float_as_uint(x);
-  return x != x ? 0xffffffffu : x == 0.f ? 0x80000000u : u & 0x80000000u ? ~u : u | 0x80000000u;
+// The largest logit of every row, in slices.
+constexpr int kBestWaves = 4;
+template <int DT>
+__global__ __launch_bounds__(kBestWaves *kWave) void accept_rows_kernel(AcceptArgs a) {
+  __shared__ uint64_t s_best[2][kBestWaves];
+  const int64_t row = blockIdx.x;
+  const int from = blockIdx.y * a.slice;
+  const uint64_t best = row_best<DT, kBestWaves>(reinterpret_cast<const typename Elem<DT>::T *>(a.logits) + row * a.stride, from, min(from + a.slice, a.vocab), s_best);
+  if (threadIdx.x == 0) a.best[row * a.slices + blockIdx.y] = best;
 }
 
-constexpr int kAcceptThreads = 1024;
-
-// A workgroup walks a sequence's tree, a node a round.
-template <int DT>
-__global__ __launch_bounds__(kAcceptThreads) void accept_kernel(AcceptArgs a) {
-  typedef Elem<DT> E;
-  typedef typename E::T T;
-  __shared__ uint64_t s_best[2][kAcceptThreads / kWave];
+// A workgroup walks a sequence's tree: W waves that read a row a round, or one wave where all rows have been looked at.
+template <int DT, int W>
+__global__ __launch_bounds__(W *kWave) void accept_walk_kernel(AcceptArgs a) {
+  __shared__ uint64_t s_best[2][2][W];
   const int b = blockIdx.x, first = a.cu[b], lane = threadIdx.x % kWave;
   const int nodes = (int)min((int64_t)draft_nodes(a.cu, b, a.max_nodes), a.total - first);
   int32_t *path = a.path + (int64_t)b * a.max_nodes;
   // every wave has the whole tree, a node a lane
-  const int parent = lane < nodes ? a.parents[first + lane] : -2;
-  const int64_t token = lane >= nodes ? -1 : a.tokens_i64 ? reinterpret_cast<const int64_t *>(a.tokens)[first + lane] : reinterpret_cast<const int32_t *>(a.tokens)[first + lane];
+  const bool there = lane < nodes;
+  const int parent = there ? a.parents[first + lane] : -2;
+  const int64_t token = !there ? -1 : a.tokens_i64 ? reinterpret_cast<const int64_t *>(a.tokens)[first + lane] : reinterpret_cast<const int32_t *>(a.tokens)[first + lane];
+  uint64_t mine = 0;
+  if constexpr (W == 1)
+    for (int i = 0; there && i < a.slices; ++i) mine = max(mine, a.best[(int64_t)(first + lane) * a.slices + i]);
   int cur = 0, count = 0;
   int64_t chosen = -1;
   while (cur < nodes) {
-    const T *row = reinterpret_cast<const T *>(a.logits) + (first + cur) * a.stride;
-    uint64_t best = 0;           // the value's order above, the complement of its index below
-    for (int i = threadIdx.x; i < a.vocab; i += kAcceptThreads) {
-      const uint64_t v = (uint64_t)ordered<DT>(E::to_float(row[i])) << 32 | ~(uint32_t)i;
-      best = v > best ? v : best;
+    uint32_t low;
+    if constexpr (W == 1) {
+      low = (uint32_t)__shfl((int)(uint32_t)mine, cur, kWave);
+    } else {
+      low = (uint32_t)row_best<DT, W>(reinterpret_cast<const typename Elem<DT>::T *>(a.logits) + (first + cur) * a.stride, 0, a.vocab, s_best[count & 1]);
     }
-#pragma unroll
-    for (int d = 1; d < kWave; d *= 2) {
-      const uint64_t v = (uint64_t)(uint32_t)__shfl_xor((int)(best >> 32), d, kWave) << 32 | (uint32_t)__shfl_xor((int)(uint32_t)best, d, kWave);
-      best = v > best ? v : best;
-    }
-    if (lane == 0) s_best[count & 1][threadIdx.x / kWave] = best;
-    __syncthreads();
-#pragma unroll
-    for (int w = 0; w < kAcceptThreads / kWave; ++w) best = max(best, s_best[count & 1][w]);
-    chosen = (int64_t)(~(uint32_t)best);
+    chosen = (int64_t)(uint32_t)~low;
     if (threadIdx.x == 0) path[count] = cur;
     ++count;
     const uint64_t fits = __ballot(lane > cur && parent == cur && token == chosen);
     if (!fits) break;
     cur = __builtin_ctzll(fits);
   }
-  for (int i = count + threadIdx.x; i < a.max_nodes; i += kAcceptThreads) path[i] = -1;
+  for (int i = count + threadIdx.x; i < a.max_nodes; i += W * kWave) path[i] = -1;
   if (threadIdx.x == 0) {
     a.counts[b] = count;
     a.next[b] = chosen;
   }
+}
+
+constexpr int kWalkWaves = 16;
+constexpr int64_t kAllBytes = 24ll << 20, kSliceBytes = 32 << 10;
+// Slices of a row where all rows are looked at first; 0: a row at a time, as the walk comes to it.
+inline int accept_slices(int64_t nodes, int64_t vocab, int es) {
+  if (nodes * vocab * es > kAllBytes) return 0;
+  const int64_t n = ceil_div(vocab * es, kSliceBytes);
+  return (int)(n < 1 ? 1 : n);
 }
 
 // ---- accepted rows into the pages --------------------------------------------------------------------------------------------------
@@ -148,22 +267,43 @@ int en_draft_tree(const int32_t *parents, const int32_t *cu_seqlens, int batch, 
   return EN_OK;
 }
 
+int64_t en_accept_drafts_workspace_bytes(int64_t nodes, int vocab, int dtype) {
+  const int es = dtype_size(dtype);
+  if (es == 0 || nodes < 1 || nodes > INT32_MAX || vocab < 1) return 0;
+  return nodes * accept_slices(nodes, vocab, es) * 8;
+}
+
 int en_accept_drafts(const void *logits, int64_t logits_stride, int vocab, const void *tokens, int tokens_are_i64, const int32_t *parents,
                      const int32_t *cu_seqlens, int batch, int64_t nodes, int max_nodes, int32_t *path, int32_t *counts, int64_t *next_tokens,
-                     int dtype, en_stream_t stream) {
+                     int dtype, void *workspace, int64_t workspace_bytes, en_stream_t stream) {
   const int es = dtype_size(dtype);
   if (es == 0) return EN_ERR_DTYPE;
-  if (batch < 0 || nodes < 0 || nodes > INT32_MAX || max_nodes < 1 || max_nodes > kNodes || vocab < 1 || logits_stride < 0) return EN_ERR_SHAPE;
+  if (batch < 0 || nodes < 0 || nodes > INT32_MAX || max_nodes < 1 || max_nodes > kNodes || vocab < 1 || vocab > INT32_MAX - (1 << 20) || logits_stride < 0) return EN_ERR_SHAPE;
   if (batch == 0) return EN_OK;
-  if (!cu_seqlens || !path || !counts || !next_tokens || (nodes > 0 && (!logits || !tokens || !parents))) return EN_ERR_NULL;
-  if (!aligned_to(logits, es) || !aligned_to(tokens, tokens_are_i64 ? 8 : 4) || !aligned_to(next_tokens, 8)) return EN_ERR_ALIGN;
+  const int64_t need = en_accept_drafts_workspace_bytes(nodes, vocab, dtype);
+  if (!cu_seqlens || !path || !counts || !next_tokens || (nodes > 0 && (!logits || !tokens || !parents)) || (need > 0 && !workspace)) return EN_ERR_NULL;
+  if (workspace_bytes < need) return EN_ERR_SHAPE;
+  if (!aligned_to(logits, es) || !aligned_to(tokens, tokens_are_i64 ? 8 : 4) || !aligned_to(next_tokens, 8) || !aligned_to(workspace, 8)) return EN_ERR_ALIGN;
   for (const void *p : {(const void *)parents, (const void *)cu_seqlens, (const void *)path, (const void *)counts})
     if (!aligned_to(p, 4)) return EN_ERR_ALIGN;
-  const AcceptArgs a{logits, logits_stride, nodes, vocab, tokens, tokens_are_i64, parents, cu_seqlens, max_nodes, path, counts, next_tokens};
+  AcceptArgs a{logits, logits_stride, nodes, vocab, tokens, tokens_are_i64, parents, cu_seqlens, max_nodes, path, counts, next_tokens, (uint64_t *)workspace,
+               nodes > 0 ? accept_slices(nodes, vocab, es) : 1, 0};
   const hipStream_t s = (hipStream_t)stream;
-  if (dtype == EN_F32) accept_kernel<EN_F32><<<(unsigned)batch, kAcceptThreads, 0, s>>>(a);
-  else if (dtype == EN_F16) accept_kernel<EN_F16><<<(unsigned)batch, kAcceptThreads, 0, s>>>(a);
-  else accept_kernel<EN_BF16><<<(unsigned)batch, kAcceptThreads, 0, s>>>(a);
+  auto launch = [&](auto dt) {
+    constexpr int DT = decltype(dt)::value;
+    if (a.slices == 0) {
+      accept_walk_kernel<DT, kWalkWaves><<<(unsigned)batch, kWalkWaves * kWave, 0, s>>>(a);
+      return;
+    }
+    const int per = 16 / es;
+    a.slice = (int)(ceil_div(ceil_div(vocab, a.slices), per) * per);
+    a.slices = (int)ceil_div(vocab, a.slice);
+    if (nodes > 0) accept_rows_kernel<DT><<<dim3((unsigned)nodes, (unsigned)a.slices), kBestWaves * kWave, 0, s>>>(a);
+    accept_walk_kernel<DT, 1><<<(unsigned)batch, kWave, 0, s>>>(a);
+  };
+  if (dtype == EN_F32) launch(std::integral_constant<int, EN_F32>{});
+  else if (dtype == EN_F16) launch(std::integral_constant<int, EN_F16>{});
+  else launch(std::integral_constant<int, EN_BF16>{});
   EN_RETURN_IF_LAUNCH_FAILED();
   return EN_OK;
 }

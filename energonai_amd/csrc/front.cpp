@@ -931,13 +931,17 @@ PyObject *accept_drafts(PyObject *const *a) {
   order_stream(info_o, *logits);
   const auto opt = logits->options();
   const Tensor path = at::empty({B, most}, opt.dtype(at::kInt)), counts = at::empty({B}, opt.dtype(at::kInt)), next = at::empty({B}, opt.dtype(at::kLong));
+  const int64_t need = en_accept_drafts_workspace_bytes(T, (int)V, tag);
+  Tensor ws;
+  if (need > 0) ws = at::empty({need}, opt.dtype(at::kByte));
+  void *ws_p = need > 0 ? ws.data_ptr() : nullptr;
   const void *logits_p = logits->data_ptr(), *tokens_p = tokens->data_ptr();
   const int32_t *parents_p = i32(*parents), *cu_p = i32(*tree.cu);
   int32_t *path_p = path.data_ptr<int32_t>(), *counts_p = counts.data_ptr<int32_t>();
   int64_t *next_p = next.data_ptr<int64_t>();
   const hipStream_t stream = stream_of(*logits);
   check(without_gil([&] {
-          return en_accept_drafts(logits_p, stride, (int)V, tokens_p, wide, parents_p, cu_p, (int)B, T, (int)most, path_p, counts_p, next_p, tag, stream);
+          return en_accept_drafts(logits_p, stride, (int)V, tokens_p, wide, parents_p, cu_p, (int)B, T, (int)most, path_p, counts_p, next_p, tag, ws_p, need, stream);
         }), "accept_drafts");
   return tuple({path, counts, next});
 }

@@ -209,10 +209,12 @@ def accept_drafts(logits, tokens, tree):
     path = torch.empty((B, tree.max_nodes), dtype=torch.int32, device=logits.device)
     counts = torch.empty(B, dtype=torch.int32, device=logits.device)
     following = torch.empty(B, dtype=torch.int64, device=logits.device)
+    need = int(_lib.fn.en_accept_drafts_workspace_bytes(T, V, dtype))
+    workspace = torch.empty(need, dtype=torch.uint8, device=logits.device)
     with _lib.device_guard(logits):
         _lib.check(_lib.fn.en_accept_drafts(logits.data_ptr(), logits.stride(0) if T > 1 else V, V, tokens.data_ptr(), int(tokens.dtype == torch.int64),
                                             tree.parents.data_ptr(), info.cu_seqlens.data_ptr(), B, T, tree.max_nodes, path.data_ptr(),
-                                            counts.data_ptr(), following.data_ptr(), dtype, _lib.stream_of(logits)), who)
+                                            counts.data_ptr(), following.data_ptr(), dtype, _lib.ptr(workspace) or None, need, _lib.stream_of(logits)), who)
     return path, counts, following
 
 

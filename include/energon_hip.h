@@ -557,10 +557,13 @@ int en_decode_attn_tree(const void *q, const void *k_new, const void *v_new, con
 /* Greedy acceptance.  From node 0 on: t is the index of the largest of the node's logits (the lowest of equal ones; NaN counts as the
  * largest); its lowest child whose token is t is accepted next, and where there is none, t is the token that follows.
  * path[b, i], i < max_nodes: the i-th accepted node (node 0 first), -1 behind the last; counts[b]: how many; next_tokens[b]: t.  A sequence
- * without nodes has 0 and -1.  logits: [nodes, vocab] rows, logits_stride elements apart; tokens int32 or int64 (tokens_are_i64). */
+ * without nodes has 0 and -1.  logits: [nodes, vocab] rows, logits_stride elements apart; tokens int32 or int64 (tokens_are_i64).
+ * workspace: en_accept_drafts_workspace_bytes (may be 0, then NULL), 8-byte aligned; its contents need not be kept or cleared, but calls that may
+ * run at the same time need one each. */
+int64_t en_accept_drafts_workspace_bytes(int64_t nodes, int vocab, int dtype);
 int en_accept_drafts(const void *logits, int64_t logits_stride, int vocab, const void *tokens, int tokens_are_i64, const int32_t *parents,
                      const int32_t *cu_seqlens, int batch, int64_t nodes, int max_nodes, int32_t *path, int32_t *counts, int64_t *next_tokens,
-                     int dtype, en_stream_t stream);
+                     int dtype, void *workspace, int64_t workspace_bytes, en_stream_t stream);
 
 /* The accepted nodes' keys and values into their pages: row cu_seqlens[b] + path[b, i] of k_new and v_new becomes position kv_lens[b] + i of
  * sequence b, i < min(counts[b], path_width).  Entries of path that are no node of the sequence are passed over; a position without a page in the pool

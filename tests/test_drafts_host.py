@@ -81,8 +81,8 @@ def test_attention_refuses():
 def test_acceptance_refuses():
     fn = _lib().fn.en_accept_drafts
 
-    def call(logits=PTR, stride=100, vocab=100, tokens=PTR, i64=1, parents=PTR, cu=PTR, batch=2, nodes=5, max_nodes=4, path=PTR, counts=PTR, nxt=PTR, dtype=1):
-        return fn(logits, stride, vocab, tokens, i64, parents, cu, batch, nodes, max_nodes, path, counts, nxt, dtype, None)
+    def call(logits=PTR, stride=100, vocab=100, tokens=PTR, i64=1, parents=PTR, cu=PTR, batch=2, nodes=5, max_nodes=4, path=PTR, counts=PTR, nxt=PTR, dtype=1, ws=PTR, ws_bytes=1 << 30):
+        return fn(logits, stride, vocab, tokens, i64, parents, cu, batch, nodes, max_nodes, path, counts, nxt, dtype, ws, ws_bytes, None)
     assert call(batch=0) == 0
     for kw in (dict(logits=None), dict(tokens=None), dict(parents=None), dict(cu=None), dict(path=None), dict(counts=None), dict(nxt=None)):
         assert call(**kw) == NULL, kw
@@ -91,6 +91,9 @@ def test_acceptance_refuses():
     for kw in (dict(logits=PTR + 1), dict(tokens=PTR + 4), dict(tokens=PTR + 2, i64=0), dict(nxt=PTR + 4), dict(path=PTR + 2)):
         assert call(**kw) == ALIGN, kw
     assert call(dtype=3) == DTYPE
+    need = _lib().fn.en_accept_drafts_workspace_bytes
+    assert need(5, 100, 1) > 0 and need(0, 100, 1) == 0 and need(4096, 130000, 1) == 0
+    assert call(ws=None) == NULL and call(ws_bytes=need(5, 100, 1) - 1) == SHAPE and call(ws=PTR + 4) == ALIGN
 
 
 def test_extension_refuses():
