@@ -19,7 +19,7 @@ typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 b16x8 __attribute__((ext_vector_type(8)));
 
 constexpr int kTileRows = 16, kTileCols = 128;
-constexpr int64_t kMostFeatures = 1 << 23;      // 64 rows of x stay within 2^30 bytes
+constexpr int64_t kMostFeatures = 1 << 21;      // 256 rows of x stay within 2^30 bytes
 
 template <int DT> __device__ __forceinline__ f32x4 mma(const uint4 &a, const uint4 &b, f32x4 c) {
   if constexpr (DT == EN_F16)
@@ -195,6 +195,160 @@ __global__ __launch_bounds__(NW *kWave) void w4_rows_kernel(W4Args a) {
   }
 }
 
+// ---- many rows ---------------------------------------------------------------------------------------------------------------------------
+
+// 256 rows of x times 256 rows of W a workgroup, 64 channels a stage; eight waves, 128 x 64 each.  Bound by the matrix instructions: x goes
+// from memory into LDS as operands lie (a wave's load of 16 rows x 32 channels is one operand, 1 KB in lane order), and so do the
+// weights, each turned into 16 bits once for the 256 rows: (code - zero) * scale in fp32, rounded as a weight kept in 16 bits would be
+// (half a step of the activations' type; scaling sums of codes instead takes four multiplications for each four matrix instructions of a
+// group of 32, as many cycles as those themselves).
+constexpr int kManyRows = 256, kManyCols = 256, kManyWaves = 8;
+
+template <int DT> __device__ __forceinline__ uint32_t pack_two(float lo, float hi);
+template <> __device__ __forceinline__ uint32_t pack_two<EN_F16>(float lo, float hi) {
+  typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+  return __builtin_bit_cast(uint32_t, f16x2{(_Float16)lo, (_Float16)hi});
+}
+template <> __device__ __forceinline__ uint32_t pack_two<EN_BF16>(float lo, float hi) {
+  typedef __bf16 b16x2 __attribute__((ext_vector_type(2)));
+  return __builtin_bit_cast(uint32_t, b16x2{(__bf16)lo, (__bf16)hi});
+}
+// Eight codes times scale plus off.
+template <int DT> __device__ __forceinline__ uint4 scaled(uint32_t w, float scale, float off) {
+  const uint32_t lo = w & 0x0f0f0f0fu, hi = w >> 4 & 0x0f0f0f0fu;
+  float f[8];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    f[i] = (float)(lo >> (8 * i) & 0xffu) * scale + off;
+    f[4 + i] = (float)(hi >> (8 * i) & 0xffu) * scale + off;
+  }
+  return make_uint4(pack_two<DT>(f[0], f[1]), pack_two<DT>(f[2], f[3]), pack_two<DT>(f[4], f[5]), pack_two<DT>(f[6], f[7]));
+}
+
+template <int DT, int GROUP>
+__global__ __launch_bounds__(kManyWaves *kWave, 2) void w4_many_kernel(W4Args a) {
+  typedef Elem<DT> E;
+  typedef typename E::T T;
+  constexpr int kGroups = kTileCols / GROUP, RT = 8, CT = 4;
+  constexpr int kXStage = kManyRows * 64 * 2, kWStage = kManyCols * 64 * 2, kStage = kXStage + kWStage;
+  __shared__ __align__(16) char s_mem[2 * kStage];      // two stages: x operands [row tile][half][lane], W operands [tile][half][lane]
+  const int lane = threadIdx.x % kWave, j = lane % 16, g = lane / 16;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), wr = wave % 2, wc = wave / 2;
+  // a column block's row blocks one after another: they read the same codes
+  const int row_blocks = (a.R + kManyRows - 1) / kManyRows;
+  const int rb = blockIdx.x % row_blocks, cb = blockIdx.x / row_blocks;
+  const int r0 = rb * kManyRows, t0 = cb * (kManyCols / kTileRows);
+
+  // x: this wave moves row tiles 2 wave, 2 wave + 1; channels past K and rows past R arrive as zeros
+  const T *x0 = reinterpret_cast<const T *>(a.x) + (int64_t)r0 * a.x_stride;
+  const int rows = min(kManyRows, a.R - r0);
+  const uint32_t x_bytes = (uint32_t)(((int64_t)(rows - 1) * a.x_stride + a.K) * 2);
+  const desc_t x_desc = make_desc(x0, x_bytes);
+  uint32_t xrow[2];
+#pragma unroll
+  for (int t = 0; t < 2; ++t) {
+    const int r = (2 * wave + t) * 16 + j;
+    xrow[t] = r < rows ? (uint32_t)((int64_t)r * a.x_stride * 2) : kOutOfRange;
+  }
+  const uint32_t lds0 = lds_address(s_mem);
+  auto load_x = [&](int stage, int buf) {
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        const int k = stage * 64 + half * 32 + g * 8;
+        buffer_load16_to_lds(x_desc, lds0 + buf * kStage + ((2 * wave + t) * 2 + half) * 1024,
+                             (xrow[t] + (uint32_t)k * 2u) | (xrow[t] & kOutOfRange) | (k < a.K ? 0u : kOutOfRange));
+      }
+  };
+  // W: this wave turns tiles 2 wave, 2 wave + 1 into 16 bits; a lane's row of W is l % 16
+  uint4 codes[2];
+  float sc[2][kGroups], ze[2][kGroups];
+  auto load_codes = [&](int step) {
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      const int64_t tile = (int64_t)min(t0 + 2 * wave + t, a.tiles - 1) * a.steps + step;
+      codes[t] = a.codes[tile * kWave + lane];
+#pragma unroll
+      for (int i = 0; i < kGroups; ++i) {
+        const int64_t at = (tile * kGroups + i) * 16 + j;
+        sc[t][i] = E::to_float(reinterpret_cast<const T *>(a.scales)[at]);
+        ze[t][i] = a.zeros ? (float)a.zeros[at] : 8.f;
+      }
+    }
+  };
+  auto put_w = [&](int part, int buf) {
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        const int word = 2 * part + half, i = word * 32 / GROUP;
+        const uint32_t w = word == 0 ? codes[t].x : word == 1 ? codes[t].y : word == 2 ? codes[t].z : codes[t].w;
+        *reinterpret_cast<uint4 *>(s_mem + buf * kStage + kXStage + ((2 * wave + t) * 2 + half) * 1024 + lane * 16) =
+            scaled<DT>(w, sc[t][i], -ze[t][i] * sc[t][i]);
+      }
+  };
+
+  f32x4 acc[RT][CT];
+#pragma unroll
+  for (int t = 0; t < RT; ++t)
+#pragma unroll
+    for (int c = 0; c < CT; ++c) acc[t][c] = f32x4{0.f, 0.f, 0.f, 0.f};
+  auto multiply = [&](int buf) {
+    const char *xs = s_mem + buf * kStage + wr * RT * 2048 + lane * 16, *ws = s_mem + buf * kStage + kXStage + wc * CT * 2048 + lane * 16;
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      uint4 w[CT];
+#pragma unroll
+      for (int c = 0; c < CT; ++c) w[c] = *reinterpret_cast<const uint4 *>(ws + c * 2048 + half * 1024);
+#pragma unroll
+      for (int t = 0; t < RT; ++t) {
+        const uint4 x = *reinterpret_cast<const uint4 *>(xs + t * 2048 + half * 1024);
+#pragma unroll
+        for (int c = 0; c < CT; ++c) acc[t][c] = mma<DT>(w[c], x, acc[t][c]);
+      }
+    }
+  };
+  auto arrived = [] { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); };      // the loads into LDS among them
+
+  load_codes(0);
+  load_x(0, 0);
+  put_w(0, 0);
+  arrived();
+  lds_barrier();
+  for (int step = 0; step < a.steps; ++step) {
+    load_x(2 * step + 1, 1);
+    put_w(1, 1);
+    if (step + 1 < a.steps) load_codes(step + 1);
+    multiply(0);
+    arrived();
+    lds_barrier();
+    if (step + 1 < a.steps) {
+      load_x(2 * step + 2, 0);
+      put_w(0, 0);
+    }
+    multiply(1);
+    arrived();
+    lds_barrier();
+  }
+#pragma unroll
+  for (int t = 0; t < RT; ++t) {
+    const int r = r0 + (wr * RT + t) * 16 + j;
+    if (r >= a.R) continue;
+#pragma unroll
+    for (int c = 0; c < CT; ++c) {
+      const int n = (t0 + wc * CT + c) * kTileRows + 4 * g;
+      T *y = reinterpret_cast<T *>(a.y) + (int64_t)r * a.N + n;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        if (n + e >= a.N) continue;
+        const float with = acc[t][c][e] + (a.bias ? E::to_float(reinterpret_cast<const T *>(a.bias)[n + e]) : 0.f);
+        y[e] = E::from_float(w4_activate(with, a.act));
+      }
+    }
+  }
+}
+
 static int check_w4(const en_w4_weight *w) {
   if (!w) return EN_ERR_NULL;
   if (w->dtype != EN_F16 && w->dtype != EN_BF16) return EN_ERR_DTYPE;
@@ -254,7 +408,12 @@ int en_linear_w4(const void *x, int64_t rows, int64_t x_stride, const en_w4_weig
     const dim3 grid((unsigned)ceil_div(a.tiles, CT), (unsigned)ceil_div(rows, 16 * RT));
     w4_rows_kernel<decltype(dt)::value, decltype(group)::value, RT, CT, NW><<<grid, NW * kWave, 0, s>>>(a);
   };
+  auto many = [&](auto dt, auto group) {
+    const int64_t blocks = ceil_div(rows, kManyRows) * ceil_div(N, kManyCols);
+    w4_many_kernel<decltype(dt)::value, decltype(group)::value><<<(unsigned)blocks, kManyWaves * kWave, 0, s>>>(a);
+  };
   auto shape = [&](auto dt, auto group) {
+    if (rows > 128) return many(dt, group);
     if (rows <= 16) launch(dt, group, std::integral_constant<int, 1>{});
     else if (rows <= 32) launch(dt, group, std::integral_constant<int, 2>{});
     else launch(dt, group, std::integral_constant<int, 4>{});

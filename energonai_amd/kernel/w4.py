@@ -118,7 +118,7 @@ def w4_quantize(weight, group_size: int = 128, zero_points: bool = False) -> W4W
 
 def linear_w4(inputs, weight, bias=None, activation: Optional[str] = None):
     """``linear`` with a weight in 4 bits: ``act(inputs[..., din] @ W[dout, din]^T + bias)`` -> ``[..., dout]``, fp16 or bf16 as the weight's
-    scales are.  Sums are fp32 and no weight is rounded to 16 bits.  ``activation``: ``"relu"``, ``"gelu_tanh"`` or ``"gelu"``."""
+    scales are.  Sums are fp32; up to 128 rows no weight is rounded, from there on each is, to the inputs' type.  ``activation``: ``"relu"``, ``"gelu_tanh"`` or ``"gelu"``."""
     who = "linear_w4"
     if type(weight) is W4Weight and activation in _ACTIVATIONS:
         y = _lib.front.linear_w4(inputs, weight, bias, _ACTIVATIONS[activation])

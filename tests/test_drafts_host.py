@@ -124,7 +124,7 @@ def test_w4_refuses():
     for kw in (dict(x=None), dict(y=None), dict(codes=None), dict(scales=None)):
         assert call(**kw) == NULL, kw
     assert lib.fn.en_linear_w4(PTR, 1, 200, None, None, 0, PTR, None) == NULL
-    for kw in (dict(rows=-1), dict(stride=192), dict(stride=-8), dict(out_features=0), dict(in_features=0), dict(in_features=204), dict(in_features=1 << 24), dict(rows=1 << 32)):
+    for kw in (dict(rows=-1), dict(stride=192), dict(stride=-8), dict(out_features=0), dict(in_features=0), dict(in_features=204), dict(in_features=1 << 22), dict(rows=1 << 32)):
         assert call(**kw) == SHAPE, kw
     for kw in (dict(group=48), dict(act=4), dict(act=-1)):
         assert call(**kw) == UNSUPPORTED, kw

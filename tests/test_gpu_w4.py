@@ -21,12 +21,23 @@ def weight(N, Kd, group, dtype, zeros, seed):
     return codes, scales, z
 
 
-def tolerance(want, size, dtype, Kd, act):
+MANY = 128            # rows up to which no weight is rounded
+
+
+def tolerance(want, size, dtype, Kd, act, rounded=None):
     """Half a step of the result, and fp32 sums: at most 128 products of a group and their sums of x, the groups' sums one after another, over
-    the waves and the bias, each half of 2^-23 of sum |scale| (code + zero) |x|.  GELU's slope is below 1.13, and its fp32 functions are good to 2^-19."""
+    the waves and the bias, each half of 2^-23 of sum |scale| (code + zero) |x|.  GELU's slope is below 1.13, and its fp32 functions are good to 2^-19.
+    ``rounded``: sum |weight| |x| of products with weights that are rounded to the activations' type, half a step of each (all
+    scales here are above 2^-10 and weights whole multiples of them, so that none is among fp16's subnormal numbers)."""
     off = size * (2 * 128 + Kd // 32 + 32) * 2 ** -24
+    if rounded is not None:
+        off = off + torch.finfo(dtype).eps / 2 * rounded
     slope, own = (1.13, want.abs() * 2 ** -19 + 2 ** -21) if act in ("gelu", "gelu_tanh") else (1.0, 0.0)
     return torch.finfo(dtype).eps / 2 * want.abs() + slope * off + own + (2 ** -25 if dtype == torch.float16 else 1e-40)
+
+
+def rounding(rows, x, codes, scales, z, group):
+    return x.double().abs() @ ref.w4_values(codes, scales, z, group)[0].abs().t() if rows > MANY else None
 
 
 CASES = [
@@ -48,7 +59,7 @@ def test_product(rows, Kd, N, group, zeros, dtype):
     want, size = ref.w4_linear(x, codes, scales, z, group)
     got = K().linear_w4(x.cuda(), w).cpu()
     assert got.shape == (rows, N)
-    off = (got.double() - want).abs() - tolerance(want, size, dtype, Kd, None)
+    off = (got.double() - want).abs() - tolerance(want, size, dtype, Kd, None, rounding(rows, x, codes, scales, z, group))
     assert float(off.max()) <= 0, float(off.max())
 
 
@@ -65,7 +76,7 @@ def test_bias_and_activation(rows, act, dtype):
     want, size = ref.w4_linear(x[0], codes, scales, z, group, bias, act)
     got = K().linear_w4(x.cuda(), w, bias=bias.cuda(), activation=act).cpu()
     assert got.shape == (1, rows, N)
-    off = (got[0].double() - want).abs() - tolerance(want, size, dtype, Kd, act)
+    off = (got[0].double() - want).abs() - tolerance(want, size, dtype, Kd, act, rounding(rows, x[0], codes, scales, z, group))
     assert float(off.max()) <= 0, float(off.max())
 
 
