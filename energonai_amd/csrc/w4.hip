@@ -9,6 +9,7 @@
 // The products are of codes as they are; a group's sum, in fp32, is then scale * (sum of code x - zero * sum of x), with the sums of x from a
 // matrix instruction whose other operand is ones.  No weight is rounded.
 #include <type_traits>
+#include <utility>
 
 #include "common.hip.h"
 
@@ -213,16 +214,13 @@ template <> __device__ __forceinline__ uint32_t pack_two<EN_BF16>(float lo, floa
   typedef __bf16 b16x2 __attribute__((ext_vector_type(2)));
   return __builtin_bit_cast(uint32_t, b16x2{(__bf16)lo, (__bf16)hi});
 }
-// Eight codes times scale plus off.
-template <int DT> __device__ __forceinline__ uint4 scaled(uint32_t w, float scale, float off) {
-  const uint32_t lo = w & 0x0f0f0f0fu, hi = w >> 4 & 0x0f0f0f0fu;
-  float f[8];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    f[i] = (float)(lo >> (8 * i) & 0xffu) * scale + off;
-    f[4 + i] = (float)(hi >> (8 * i) & 0xffu) * scale + off;
-  }
-  return make_uint4(pack_two<DT>(f[0], f[1]), pack_two<DT>(f[2], f[3]), pack_two<DT>(f[4], f[5]), pack_two<DT>(f[6], f[7]));
+template <typename F, int... I> __device__ __forceinline__ void each(F &&f, std::integer_sequence<int, I...>) { (f(std::integral_constant<int, I>{}), ...); }
+
+// Codes 2 I and 2 I + 1 of a word times scale plus off.
+template <int DT, int I> __device__ __forceinline__ uint32_t scaled_two(uint32_t w, float scale, float off) {
+  const uint32_t b = I < 2 ? w & 0x0f0f0f0fu : w >> 4 & 0x0f0f0f0fu;
+  constexpr int kShift = I % 2 * 16;
+  return pack_two<DT>((float)(b >> kShift & 0xffu) * scale + off, (float)(b >> (kShift + 8) & 0xffu) * scale + off);
 }
 
 template <int DT, int GROUP>
@@ -262,31 +260,47 @@ __global__ __launch_bounds__(kManyWaves *kWave, 2) void w4_many_kernel(W4Args a)
       }
   };
   // W: this wave turns tiles 2 wave, 2 wave + 1 into 16 bits; a lane's row of W is l % 16
-  uint4 codes[2];
-  float sc[2][kGroups], ze[2][kGroups];
+  uint4 codes[2], next_codes[2];
+  T sc[2][kGroups], next_sc[2][kGroups];
+  uint8_t ze[2][kGroups], next_ze[2][kGroups];
   auto load_codes = [&](int step) {
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
       const int64_t tile = (int64_t)min(t0 + 2 * wave + t, a.tiles - 1) * a.steps + step;
-      codes[t] = a.codes[tile * kWave + lane];
+      next_codes[t] = a.codes[tile * kWave + lane];
 #pragma unroll
       for (int i = 0; i < kGroups; ++i) {
         const int64_t at = (tile * kGroups + i) * 16 + j;
-        sc[t][i] = E::to_float(reinterpret_cast<const T *>(a.scales)[at]);
-        ze[t][i] = a.zeros ? (float)a.zeros[at] : 8.f;
+        next_sc[t][i] = reinterpret_cast<const T *>(a.scales)[at];
+        next_ze[t][i] = a.zeros ? a.zeros[at] : 8;
       }
     }
   };
-  auto put_w = [&](int part, int buf) {
+  auto take_codes = [&] {
 #pragma unroll
-    for (int t = 0; t < 2; ++t)
+    for (int t = 0; t < 2; ++t) {
+      codes[t] = next_codes[t];
 #pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        const int word = 2 * part + half, i = word * 32 / GROUP;
-        const uint32_t w = word == 0 ? codes[t].x : word == 1 ? codes[t].y : word == 2 ? codes[t].z : codes[t].w;
-        *reinterpret_cast<uint4 *>(s_mem + buf * kStage + kXStage + ((2 * wave + t) * 2 + half) * 1024 + lane * 16) =
-            scaled<DT>(w, sc[t][i], -ze[t][i] * sc[t][i]);
+      for (int i = 0; i < kGroups; ++i) {
+        sc[t][i] = next_sc[t][i];
+        ze[t][i] = next_ze[t][i];
       }
+    }
+  };
+  // Sixteen pieces of the weights of half a step: two codes a lane of operand piece / 4, which goes to LDS with its fourth.
+  uint32_t piece4[4];
+  auto put_w = [&](auto piece, int part, int buf) {
+    constexpr int P = decltype(piece)::value, t = P / 8, half = P / 4 % 2;
+    const int word = 2 * part + half, i = word * 32 / GROUP;
+    const uint32_t w = word == 0 ? codes[t].x : word == 1 ? codes[t].y : word == 2 ? codes[t].z : codes[t].w;
+    const float scale = E::to_float(sc[t][i]);
+    piece4[P % 4] = scaled_two<DT, P % 4>(w, scale, -(float)ze[t][i] * scale);
+    if constexpr (P % 4 == 3)
+      *reinterpret_cast<uint4 *>(s_mem + buf * kStage + kXStage + ((2 * wave + t) * 2 + half) * 1024 + lane * 16) =
+          make_uint4(piece4[0], piece4[1], piece4[2], piece4[3]);
+  };
+  auto put_all = [&](int part, int buf) {
+    each([&](auto piece) { put_w(piece, part, buf); }, std::make_integer_sequence<int, 16>{});
   };
 
   f32x4 acc[RT][CT];
@@ -294,43 +308,49 @@ __global__ __launch_bounds__(kManyWaves *kWave, 2) void w4_many_kernel(W4Args a)
   for (int t = 0; t < RT; ++t)
 #pragma unroll
     for (int c = 0; c < CT; ++c) acc[t][c] = f32x4{0.f, 0.f, 0.f, 0.f};
-  auto multiply = [&](int buf) {
+  // A stage's products, and between them, while the matrix instructions run, the pieces of the next stage's weights.
+  auto multiply = [&](int buf, auto more, int part) {
     const char *xs = s_mem + buf * kStage + wr * RT * 2048 + lane * 16, *ws = s_mem + buf * kStage + kXStage + wc * CT * 2048 + lane * 16;
+    uint4 w[2][CT], x[2];
 #pragma unroll
-    for (int half = 0; half < 2; ++half) {
-      uint4 w[CT];
+    for (int c = 0; c < CT; ++c) w[0][c] = *reinterpret_cast<const uint4 *>(ws + c * 2048);
+    x[0] = *reinterpret_cast<const uint4 *>(xs);
+    auto one = [&](auto index) {
+      constexpr int I = decltype(index)::value, t = I % RT, half = I / RT;
+      if constexpr (I + 1 < 2 * RT) x[(I + 1) % 2] = *reinterpret_cast<const uint4 *>(xs + (I + 1) % RT * 2048 + (I + 1) / RT * 1024);
+      if constexpr (half == 0 && t >= RT - CT) w[1][t - (RT - CT)] = *reinterpret_cast<const uint4 *>(ws + (t - (RT - CT)) * 2048 + 1024);
 #pragma unroll
-      for (int c = 0; c < CT; ++c) w[c] = *reinterpret_cast<const uint4 *>(ws + c * 2048 + half * 1024);
-#pragma unroll
-      for (int t = 0; t < RT; ++t) {
-        const uint4 x = *reinterpret_cast<const uint4 *>(xs + t * 2048 + half * 1024);
-#pragma unroll
-        for (int c = 0; c < CT; ++c) acc[t][c] = mma<DT>(w[c], x, acc[t][c]);
-      }
-    }
+      for (int c = 0; c < CT; ++c) acc[t][c] = mma<DT>(w[half][c], x[I % 2], acc[t][c]);
+      if constexpr (more.value) put_w(index, part, buf ^ 1);
+      __builtin_amdgcn_sched_barrier(0);
+    };
+    each(one, std::make_integer_sequence<int, 2 * RT>{});
   };
   auto arrived = [] { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); };      // the loads into LDS among them
 
   load_codes(0);
   load_x(0, 0);
-  put_w(0, 0);
+  take_codes();
+  put_all(0, 0);
   arrived();
   lds_barrier();
-  for (int step = 0; step < a.steps; ++step) {
+  for (int step = 0; step + 1 < a.steps; ++step) {
+    load_codes(step + 1);
     load_x(2 * step + 1, 1);
-    put_w(1, 1);
-    if (step + 1 < a.steps) load_codes(step + 1);
-    multiply(0);
+    multiply(0, std::true_type{}, 1);
     arrived();
     lds_barrier();
-    if (step + 1 < a.steps) {
-      load_x(2 * step + 2, 0);
-      put_w(0, 0);
-    }
-    multiply(1);
+    take_codes();
+    load_x(2 * step + 2, 0);
+    multiply(1, std::true_type{}, 0);
     arrived();
     lds_barrier();
   }
+  load_x(2 * a.steps - 1, 1);
+  multiply(0, std::true_type{}, 1);
+  arrived();
+  lds_barrier();
+  multiply(1, std::false_type{}, 0);
 #pragma unroll
   for (int t = 0; t < RT; ++t) {
     const int r = r0 + (wr * RT + t) * 16 + j;
