@@ -48,6 +48,19 @@ __device__ __forceinline__ float w4_activate(float v, int act) {
   }
 }
 
+// Four neighbours of a row, `left` of them inside it, at any element's address.
+template <typename T> __device__ __forceinline__ void w4_store(T *y, const Pack<T, 4> &v, int left) {
+  typedef uint32_t u32x2_by2 __attribute__((ext_vector_type(2), aligned(2)));
+  typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+  if (left >= 4) {
+    *reinterpret_cast<u32x2_by2 *>(y) = __builtin_bit_cast(u32x2, v);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 3; ++e)
+      if (e < left) y[e] = v.v[e];
+  }
+}
+
 // ---- layout ----------------------------------------------------------------------------------------------------------------------------
 
 struct PackArgs {
@@ -57,7 +70,7 @@ struct PackArgs {
   uint32_t *codes_out;
   uint16_t *scales_out;
   uint8_t *zeros_out;
-  int64_t N, K, groups, steps, per_row;     // per_row: groups of a row of tiles
+  int64_t N, K, groups, steps, per_step;    // per_step: groups of a tile
   int64_t words, scale_count;
 };
 
@@ -81,7 +94,8 @@ __global__ __launch_bounds__(kBlock) void w4_pack_kernel(PackArgs a) {
     a.codes_out[i] = w;
   }
   if (i < a.scale_count) {
-    const int64_t group = i / 16 % a.per_row, n = i / 16 / a.per_row * kTileRows + i % 16;
+    // of a tile: its groups, row by row
+    const int64_t tile = i / (16 * a.per_step), in = i % (16 * a.per_step), group = tile % a.steps * a.per_step + in % a.per_step, n = tile / a.steps * kTileRows + in / a.per_step;
     const bool there = n < a.N && group < a.groups;
     a.scales_out[i] = there ? a.scales[n * a.groups + group] : 0;
     if (a.zeros) a.zeros_out[i] = there ? a.zeros[n * a.groups + group] & 15 : 0;
@@ -128,18 +142,15 @@ __global__ __launch_bounds__(NW *kWave) void w4_rows_kernel(W4Args a) {
     for (int c = 0; c < CT; ++c) acc[t][c] = f32x4{0.f, 0.f, 0.f, 0.f};
   for (int step = wave; step < a.steps; step += NW) {
     uint4 w[CT], x[RT][4];
-    Pack<T, 4> sc[CT][kGroups];
-    uint32_t ze[CT][kGroups];
+    Pack<T, 4 * kGroups> sc[CT];
+    Pack<uint8_t, 4 * kGroups> ze[CT];
 #pragma unroll
     for (int c = 0; c < CT; ++c) {
       const int64_t tile = min(t0 + c, a.tiles - 1);
       w[c] = a.codes[(tile * a.steps + step) * kWave + lane];
-#pragma unroll
-      for (int i = 0; i < kGroups; ++i) {
-        const int64_t at = ((tile * a.steps + step) * kGroups + i) * 16 + 4 * g;
-        sc[c][i] = load_pack<T, 4>(reinterpret_cast<const T *>(a.scales) + at);
-        ze[c][i] = a.zeros ? *reinterpret_cast<const uint32_t *>(a.zeros + at) : 0x08080808u;
-      }
+      const int64_t at = ((tile * a.steps + step) * 16 + 4 * g) * kGroups;
+      sc[c] = load_pack<T, 4 * kGroups>(reinterpret_cast<const T *>(a.scales) + at);
+      if (a.zeros) ze[c] = load_pack<uint8_t, 4 * kGroups>(a.zeros + at);
     }
 #pragma unroll
     for (int t = 0; t < RT; ++t)
@@ -169,7 +180,7 @@ __global__ __launch_bounds__(NW *kWave) void w4_rows_kernel(W4Args a) {
           for (int k = 0; k < kPer; ++k) p = mma<DT>(wide[k], x[t][i * kPer + k], p);
 #pragma unroll
           for (int e = 0; e < 4; ++e)
-            acc[t][c][e] += E::to_float(sc[c][i].v[e]) * (p[e] - (float)(ze[c][i] >> (8 * e) & 0xffu) * sum[t][e]);
+            acc[t][c][e] += E::to_float(sc[c].v[e * kGroups + i]) * (p[e] - (a.zeros ? (float)ze[c].v[e * kGroups + i] : 8.f) * sum[t][e]);
         }
       }
     }
@@ -186,13 +197,13 @@ __global__ __launch_bounds__(NW *kWave) void w4_rows_kernel(W4Args a) {
     f32x4 v = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int k = 0; k < NW; ++k) v += *reinterpret_cast<const f32x4 *>(s_acc[k][tc][lane]);
-    T *y = reinterpret_cast<T *>(a.y) + (int64_t)r * a.N + n;
+    Pack<T, 4> y;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      if (n + e >= a.N) continue;
-      const float with = v[e] + (a.bias ? E::to_float(reinterpret_cast<const T *>(a.bias)[n + e]) : 0.f);
-      y[e] = E::from_float(w4_activate(with, a.act));
+      const float bias = a.bias && n + e < a.N ? E::to_float(reinterpret_cast<const T *>(a.bias)[n + e]) : 0.f;
+      y.v[e] = E::from_float(w4_activate(v[e] + bias, a.act));
     }
+    w4_store(reinterpret_cast<T *>(a.y) + (int64_t)r * a.N + n, y, a.N - n);
   }
 }
 
@@ -228,8 +239,8 @@ __global__ __launch_bounds__(kManyWaves *kWave, 2) void w4_many_kernel(W4Args a)
   typedef Elem<DT> E;
   typedef typename E::T T;
   constexpr int kGroups = kTileCols / GROUP, RT = 8, CT = 4;
-  constexpr int kXStage = kManyRows * 64 * 2, kWStage = kManyCols * 64 * 2, kStage = kXStage + kWStage;
-  __shared__ __align__(16) char s_mem[2 * kStage];      // two stages: x operands [row tile][half][lane], W operands [tile][half][lane]
+  constexpr int kXStage = kManyRows * 64 * 2, kWStage = kManyCols * 64 * 2, kW = 3 * kXStage;
+  __shared__ __align__(16) char s_mem[3 * kXStage + 2 * kWStage];      // x operands [row tile][half][lane] of three stages, W operands [tile][half][lane] of two
   const int lane = threadIdx.x % kWave, j = lane % 16, g = lane / 16;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), wr = wave % 2, wc = wave / 2;
   // a column block's row blocks one after another: they read the same codes
@@ -255,24 +266,38 @@ __global__ __launch_bounds__(kManyWaves *kWave, 2) void w4_many_kernel(W4Args a)
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
         const int k = stage * 64 + half * 32 + g * 8;
-        buffer_load16_to_lds(x_desc, lds0 + buf * kStage + ((2 * wave + t) * 2 + half) * 1024,
+        buffer_load16_to_lds(x_desc, lds0 + buf * kXStage + ((2 * wave + t) * 2 + half) * 1024,
                              (xrow[t] + (uint32_t)k * 2u) | (xrow[t] & kOutOfRange) | (k < a.K ? 0u : kOutOfRange));
       }
   };
   // W: this wave turns tiles 2 wave, 2 wave + 1 into 16 bits; a lane's row of W is l % 16
   uint4 codes[2], next_codes[2];
-  T sc[2][kGroups], next_sc[2][kGroups];
-  uint8_t ze[2][kGroups], next_ze[2][kGroups];
+  Pack<T, kGroups> sc[2], next_sc[2];
+  Pack<uint8_t, kGroups> ze[2], next_ze[2];
+  rsrc_t code_rsrc[2], scale_rsrc[2], zero_rsrc[2];      // of a row of tiles
+#pragma unroll
+  for (int t = 0; t < 2; ++t) {
+    const int64_t tile = (int64_t)min(t0 + 2 * wave + t, a.tiles - 1) * a.steps;
+    code_rsrc[t] = make_rsrc(a.codes + tile * kWave, a.steps * 1024);
+    scale_rsrc[t] = make_rsrc(reinterpret_cast<const T *>(a.scales) + tile * 16 * kGroups, a.steps * 32 * kGroups);
+    zero_rsrc[t] = make_rsrc(a.zeros + tile * 16 * kGroups, a.zeros ? a.steps * 16 * kGroups : 0);
+  }
   auto load_codes = [&](int step) {
 #pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      const int64_t tile = (int64_t)min(t0 + 2 * wave + t, a.tiles - 1) * a.steps + step;
-      next_codes[t] = a.codes[tile * kWave + lane];
+    for (int t = 0; t < 2; ++t) next_codes[t] = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(code_rsrc[t], lane * 16, step * 1024, 0));
+  };
+  auto load_scales = [&](int step) {
 #pragma unroll
-      for (int i = 0; i < kGroups; ++i) {
-        const int64_t at = (tile * kGroups + i) * 16 + j;
-        next_sc[t][i] = reinterpret_cast<const T *>(a.scales)[at];
-        next_ze[t][i] = a.zeros ? a.zeros[at] : 8;
+    for (int t = 0; t < 2; ++t) {
+      if constexpr (kGroups == 4) {
+        next_sc[t] = __builtin_bit_cast(Pack<T, 4>, __builtin_amdgcn_raw_buffer_load_b64(scale_rsrc[t], j * 8, step * 128, 0));
+        next_ze[t] = __builtin_bit_cast(Pack<uint8_t, 4>, __builtin_amdgcn_raw_buffer_load_b32(zero_rsrc[t], j * 4, step * 64, 0));
+      } else if constexpr (kGroups == 2) {
+        next_sc[t] = __builtin_bit_cast(Pack<T, 2>, __builtin_amdgcn_raw_buffer_load_b32(scale_rsrc[t], j * 4, step * 64, 0));
+        next_ze[t] = __builtin_bit_cast(Pack<uint8_t, 2>, __builtin_amdgcn_raw_buffer_load_b16(zero_rsrc[t], j * 2, step * 32, 0));
+      } else {
+        next_sc[t].v[0] = __builtin_bit_cast(T, __builtin_amdgcn_raw_buffer_load_b16(scale_rsrc[t], j * 2, step * 32, 0));
+        next_ze[t].v[0] = __builtin_amdgcn_raw_buffer_load_b8(zero_rsrc[t], j, step * 16, 0);
       }
     }
   };
@@ -280,11 +305,8 @@ __global__ __launch_bounds__(kManyWaves *kWave, 2) void w4_many_kernel(W4Args a)
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
       codes[t] = next_codes[t];
-#pragma unroll
-      for (int i = 0; i < kGroups; ++i) {
-        sc[t][i] = next_sc[t][i];
-        ze[t][i] = next_ze[t][i];
-      }
+      sc[t] = next_sc[t];
+      ze[t] = next_ze[t];
     }
   };
   // Sixteen pieces of the weights of half a step: two codes a lane of operand piece / 4, which goes to LDS with its fourth.
@@ -293,10 +315,24 @@ __global__ __launch_bounds__(kManyWaves *kWave, 2) void w4_many_kernel(W4Args a)
     constexpr int P = decltype(piece)::value, t = P / 8, half = P / 4 % 2;
     const int word = 2 * part + half, i = word * 32 / GROUP;
     const uint32_t w = word == 0 ? codes[t].x : word == 1 ? codes[t].y : word == 2 ? codes[t].z : codes[t].w;
-    const float scale = E::to_float(sc[t][i]);
-    piece4[P % 4] = scaled_two<DT, P % 4>(w, scale, -(float)ze[t][i] * scale);
+    // from the registers that hold them, every time: kept as fp32 numbers they would take sixteen more
+    uint32_t raw_scale = 0, raw_zero = 0;
+    if constexpr (kGroups == 4) {
+      const uint2 two = __builtin_bit_cast(uint2, sc[t]);
+      raw_scale = i < 2 ? two.x : two.y;
+      raw_zero = __builtin_bit_cast(uint32_t, ze[t]);
+    } else if constexpr (kGroups == 2) {
+      raw_scale = __builtin_bit_cast(uint32_t, sc[t]);
+      raw_zero = __builtin_bit_cast(uint16_t, ze[t]);
+    } else {
+      raw_scale = __builtin_bit_cast(uint16_t, sc[t]);
+      raw_zero = ze[t].v[0];
+    }
+    asm volatile("" : "+v"(raw_scale), "+v"(raw_zero));
+    const float scale = E::to_float(__builtin_bit_cast(T, (uint16_t)(raw_scale >> (i % 2 * 16)))), zero = a.zeros ? (float)(raw_zero >> (i * 8) & 0xffu) : 8.f;
+    piece4[P % 4] = scaled_two<DT, P % 4>(w, scale, -zero * scale);
     if constexpr (P % 4 == 3)
-      *reinterpret_cast<uint4 *>(s_mem + buf * kStage + kXStage + ((2 * wave + t) * 2 + half) * 1024 + lane * 16) =
+      *reinterpret_cast<uint4 *>(s_mem + kW + buf * kWStage + ((2 * wave + t) * 2 + half) * 1024 + lane * 16) =
           make_uint4(piece4[0], piece4[1], piece4[2], piece4[3]);
   };
   auto put_all = [&](int part, int buf) {
@@ -309,63 +345,84 @@ __global__ __launch_bounds__(kManyWaves *kWave, 2) void w4_many_kernel(W4Args a)
 #pragma unroll
     for (int c = 0; c < CT; ++c) acc[t][c] = f32x4{0.f, 0.f, 0.f, 0.f};
   // A stage's products, and between them, while the matrix instructions run, the pieces of the next stage's weights.
-  auto multiply = [&](int buf, auto more, int part) {
-    const char *xs = s_mem + buf * kStage + wr * RT * 2048 + lane * 16, *ws = s_mem + buf * kStage + kXStage + wc * CT * 2048 + lane * 16;
-    uint4 w[2][CT], x[2];
+  auto multiply = [&](int xbuf, int buf, auto more, int part) {
+    const char *xs = s_mem + xbuf * kXStage + wr * RT * 2048 + lane * 16, *ws = s_mem + kW + buf * kWStage + wc * CT * 2048 + lane * 16;
+    uint4 w[CT], x[2];
 #pragma unroll
-    for (int c = 0; c < CT; ++c) w[0][c] = *reinterpret_cast<const uint4 *>(ws + c * 2048);
+    for (int c = 0; c < CT; ++c) w[c] = *reinterpret_cast<const uint4 *>(ws + c * 2048);
     x[0] = *reinterpret_cast<const uint4 *>(xs);
     auto one = [&](auto index) {
       constexpr int I = decltype(index)::value, t = I % RT, half = I / RT;
       if constexpr (I + 1 < 2 * RT) x[(I + 1) % 2] = *reinterpret_cast<const uint4 *>(xs + (I + 1) % RT * 2048 + (I + 1) / RT * 1024);
-      if constexpr (half == 0 && t >= RT - CT) w[1][t - (RT - CT)] = *reinterpret_cast<const uint4 *>(ws + (t - (RT - CT)) * 2048 + 1024);
 #pragma unroll
-      for (int c = 0; c < CT; ++c) acc[t][c] = mma<DT>(w[half][c], x[I % 2], acc[t][c]);
+      for (int c = 0; c < CT; ++c) {
+        acc[t][c] = mma<DT>(w[c], x[I % 2], acc[t][c]);
+        if constexpr (half == 0 && t == RT - 1) w[c] = *reinterpret_cast<const uint4 *>(ws + c * 2048 + 1024);
+      }
       if constexpr (more.value) put_w(index, part, buf ^ 1);
       __builtin_amdgcn_sched_barrier(0);
     };
     each(one, std::make_integer_sequence<int, 2 * RT>{});
   };
-  auto arrived = [] { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); };      // the loads into LDS among them
+  // All loads have arrived, those into LDS among them (as an instruction that the compiler counts with: it adds no wait of its own).
+  auto arrived = [] {
+    __builtin_amdgcn_sched_barrier(0);
+    __builtin_amdgcn_s_waitcnt(0x0f70);
+    __builtin_amdgcn_sched_barrier(0);
+  };
 
+  // Stage s has the first half of step s / 2 or the second.  In its first stage a step sends for x two stages ahead and waits for what was
+  // sent before; in its second also for the codes of the step after next.  So x has one or two stages to arrive, codes have two.
   load_codes(0);
+  load_scales(0);
   load_x(0, 0);
-  take_codes();
-  put_all(0, 0);
+  load_x(1, 1);
   arrived();
+  take_codes();
+  load_codes(min(1, a.steps - 1));
+  put_all(0, 0);
   lds_barrier();
+  int xbuf = 0;                               // of the step's first stage
+  auto ring = [](int b) { return b >= 3 ? b - 3 : b; };
   for (int step = 0; step + 1 < a.steps; ++step) {
-    load_codes(step + 1);
-    load_x(2 * step + 1, 1);
-    multiply(0, std::true_type{}, 1);
+    load_scales(step + 1);
+    load_x(2 * step + 2, ring(xbuf + 2));
+    multiply(xbuf, 0, std::true_type{}, 1);
     arrived();
     lds_barrier();
     take_codes();
-    load_x(2 * step + 2, 0);
-    multiply(1, std::true_type{}, 0);
-    arrived();
+    load_codes(min(step + 2, a.steps - 1));
+    load_x(2 * step + 3, xbuf);
+    multiply(ring(xbuf + 1), 1, std::true_type{}, 0);
     lds_barrier();
+    xbuf = ring(xbuf + 2);
   }
-  load_x(2 * a.steps - 1, 1);
-  multiply(0, std::true_type{}, 1);
+  multiply(xbuf, 0, std::true_type{}, 1);
   arrived();
   lds_barrier();
-  multiply(1, std::false_type{}, 0);
-#pragma unroll
-  for (int t = 0; t < RT; ++t) {
-    const int r = r0 + (wr * RT + t) * 16 + j;
-    if (r >= a.R) continue;
+  multiply(ring(xbuf + 1), 1, std::false_type{}, 0);
+  auto finish = [&](auto act) {
 #pragma unroll
     for (int c = 0; c < CT; ++c) {
-      const int n = (t0 + wc * CT + c) * kTileRows + 4 * g;
-      T *y = reinterpret_cast<T *>(a.y) + (int64_t)r * a.N + n;
+      const int n = (t0 + wc * CT + c) * kTileRows + 4 * g, left = a.N - n;
+      float bias[4];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        if (n + e >= a.N) continue;
-        const float with = acc[t][c][e] + (a.bias ? E::to_float(reinterpret_cast<const T *>(a.bias)[n + e]) : 0.f);
-        y[e] = E::from_float(w4_activate(with, a.act));
+      for (int e = 0; e < 4; ++e) bias[e] = a.bias && e < left ? E::to_float(reinterpret_cast<const T *>(a.bias)[n + e]) : 0.f;
+#pragma unroll
+      for (int t = 0; t < RT; ++t) {
+        const int r = r0 + (wr * RT + t) * 16 + j;
+        Pack<T, 4> y;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) y.v[e] = E::from_float(w4_activate(acc[t][c][e] + bias[e], act.value));
+        if (r < a.R) w4_store(reinterpret_cast<T *>(a.y) + (int64_t)r * a.N + n, y, left);
       }
     }
+  };
+  switch (a.act) {
+    case EN_ACT_RELU: finish(std::integral_constant<int, EN_ACT_RELU>{}); break;
+    case EN_ACT_GELU_TANH: finish(std::integral_constant<int, EN_ACT_GELU_TANH>{}); break;
+    case EN_ACT_GELU: finish(std::integral_constant<int, EN_ACT_GELU>{}); break;
+    default: finish(std::integral_constant<int, EN_ACT_NONE>{});
   }
 }
 
@@ -401,7 +458,7 @@ int en_w4_pack(const uint8_t *codes, const void *scales, const uint8_t *zeros, c
   if (!aligned_to(scales, 2)) return EN_ERR_ALIGN;
   PackArgs a{codes, (const uint16_t *)scales, zeros, (uint32_t *)weight->codes, (uint16_t *)weight->scales, (uint8_t *)weight->zeros,
              weight->out_features, weight->in_features, ceil_div(weight->in_features, weight->group), ceil_div(weight->in_features, kTileCols), 0, 0, 0};
-  a.per_row = a.steps * (kTileCols / weight->group);
+  a.per_step = kTileCols / weight->group;
   a.words = en_w4_codes_bytes(a.N, a.K) / 4;
   a.scale_count = en_w4_groups(a.N, a.K, weight->group);
   const int64_t blocks = ceil_div(a.words > a.scale_count ? a.words : a.scale_count, kBlock);

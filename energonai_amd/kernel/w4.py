@@ -21,7 +21,7 @@ _ACTIVATIONS = {None: 0, "none": 0, "relu": 1, "gelu_tanh": 2, "gelu": 3}
 class W4Weight(NamedTuple):
     """A weight as ``linear_w4`` reads it (made by ``w4_weight`` or ``w4_quantize``)."""
     codes: torch.Tensor                 # uint8 [tiles of 16 rows, tiles of 128 channels, 1024]
-    scales: torch.Tensor                # fp16 or bf16 [tiles of 16 rows, groups, 16]
+    scales: torch.Tensor                # fp16 or bf16 [tiles of 16 rows, tiles of 128 channels, 16, groups of a tile]
     zeros: Optional[torch.Tensor]       # uint8, as many; None: 8
     out_features: int
     in_features: int
@@ -61,7 +61,7 @@ def w4_weight(codes, scales, zeros=None, group_size: int = 128) -> W4Weight:
     if scales.shape != shape or scales.dtype not in _TYPES or (zeros is not None and (zeros.shape != shape or zeros.dtype != torch.uint8)):
         raise RuntimeError(f"{who}: scales must be float16 or bfloat16 and zeros uint8, {list(shape)} each")
     tiles, steps = -(-N // 16), -(-K // 128)
-    per = (tiles, steps * (128 // group_size), 16)
+    per = (tiles, steps, 16, 128 // group_size)
     w = W4Weight(torch.empty((tiles, steps, 1024), dtype=torch.uint8, device=codes.device), torch.empty(per, dtype=scales.dtype, device=codes.device),
                  None if zeros is None else torch.empty(per, dtype=torch.uint8, device=codes.device), N, K, int(group_size))
     with _lib.device_guard(codes):
