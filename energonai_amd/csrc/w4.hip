@@ -311,26 +311,17 @@ __global__ __launch_bounds__(kManyWaves *kWave, 2) void w4_many_kernel(W4Args a)
   };
   // Sixteen pieces of the weights of half a step: two codes a lane of operand piece / 4, which goes to LDS with its fourth.
   uint32_t piece4[4];
+  float scale = 0.f, off = 0.f;
   auto put_w = [&](auto piece, int part, int buf) {
     constexpr int P = decltype(piece)::value, t = P / 8, half = P / 4 % 2;
     const int word = 2 * part + half, i = word * 32 / GROUP;
     const uint32_t w = word == 0 ? codes[t].x : word == 1 ? codes[t].y : word == 2 ? codes[t].z : codes[t].w;
-    // from the registers that hold them, every time: kept as fp32 numbers they would take sixteen more
-    uint32_t raw_scale = 0, raw_zero = 0;
-    if constexpr (kGroups == 4) {
-      const uint2 two = __builtin_bit_cast(uint2, sc[t]);
-      raw_scale = i < 2 ? two.x : two.y;
-      raw_zero = __builtin_bit_cast(uint32_t, ze[t]);
-    } else if constexpr (kGroups == 2) {
-      raw_scale = __builtin_bit_cast(uint32_t, sc[t]);
-      raw_zero = __builtin_bit_cast(uint16_t, ze[t]);
-    } else {
-      raw_scale = __builtin_bit_cast(uint16_t, sc[t]);
-      raw_zero = ze[t].v[0];
+    if constexpr (P % 4 == 0) {
+      scale = E::to_float(sc[t].v[i]);
+      off = -(a.zeros ? (float)ze[t].v[i] : 8.f) * scale;
+      asm volatile("" : "+v"(scale), "+v"(off));         // here, not all operands' at once: sixteen registers more
     }
-    asm volatile("" : "+v"(raw_scale), "+v"(raw_zero));
-    const float scale = E::to_float(__builtin_bit_cast(T, (uint16_t)(raw_scale >> (i % 2 * 16)))), zero = a.zeros ? (float)(raw_zero >> (i * 8) & 0xffu) : 8.f;
-    piece4[P % 4] = scaled_two<DT, P % 4>(w, scale, -zero * scale);
+    piece4[P % 4] = scaled_two<DT, P % 4>(w, scale, off);
     if constexpr (P % 4 == 3)
       *reinterpret_cast<uint4 *>(s_mem + kW + buf * kWStage + ((2 * wave + t) * 2 + half) * 1024 + lane * 16) =
           make_uint4(piece4[0], piece4[1], piece4[2], piece4[3]);
