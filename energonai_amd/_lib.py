@@ -123,7 +123,8 @@ SIGNATURES = {
     "en_w4_codes_bytes": (c_int64, [c_int64] * 2),
     "en_w4_groups": (c_int64, [c_int64, c_int64, c_int]),
     "en_w4_pack": (c_int, [c_void_p] * 5),
-    "en_linear_w4": (c_int, [c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_int, c_void_p, c_void_p]),
+    "en_linear_w4_workspace_bytes": (c_int64, [c_int64] * 3),
+    "en_linear_w4": (c_int, [c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_int64, c_void_p]),
     "en_copy_bytes": (c_int, [c_void_p, c_void_p, c_int64, c_void_p]),
     "en_stream_yardstick": (c_int, [c_void_p, c_void_p, c_int64, c_int, c_int, c_void_p]),
     "en_prefix_yardstick": (c_int, [c_void_p, c_void_p, c_void_p] + [c_int] * 7 + [c_void_p]),

@@ -1006,11 +1006,15 @@ PyObject *linear_w4(PyObject *const *a) {
   for (int64_t i = 0; i < x->dim(); ++i) shape[i] = x->size(i);
   shape[x->dim() - 1] = N;
   const Tensor y = at::empty(c10::IntArrayRef(shape, x->dim()), x->options());
+  const int64_t need = en_linear_w4_workspace_bytes(rows, N, K);
+  Tensor ws;
+  if (need > 0) ws = at::empty({need}, x->options().dtype(at::kByte));
+  void *ws_p = need > 0 ? ws.data_ptr() : nullptr;
   const en_w4_weight w{codes->data_ptr(), scales->data_ptr(), zeros ? zeros->data_ptr() : nullptr, N, K, (int32_t)G, tag};
   const void *x_p = x->data_ptr(), *bias_p = bias ? bias->data_ptr() : nullptr;
   void *y_p = y.data_ptr();
   const hipStream_t stream = stream_of(*x);
-  check(without_gil([&] { return en_linear_w4(x_p, rows, stride, &w, bias_p, (int)act, y_p, stream); }), "linear_w4");
+  check(without_gil([&] { return en_linear_w4(x_p, rows, stride, &w, bias_p, (int)act, y_p, ws_p, need, stream); }), "linear_w4");
   return THPVariable_Wrap(y);
 }
 

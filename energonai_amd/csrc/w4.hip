@@ -20,6 +20,7 @@ typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 b16x8 __attribute__((ext_vector_type(8)));
 
 constexpr int kTileRows = 16, kTileCols = 128;
+constexpr int kManyRows = 256, kManyCols = 256, kManyWaves = 8;
 constexpr int64_t kMostFeatures = 1 << 21;      // 256 rows of x stay within 2^30 bytes
 
 template <int DT> __device__ __forceinline__ f32x4 mma(const uint4 &a, const uint4 &b, f32x4 c) {
@@ -114,7 +115,35 @@ struct W4Args {
   const void *bias;
   int act;
   void *y;
+  int per;                        // steps of a run
+  float *part;                    // [runs][R][16 tiles] sums, or null
 };
+
+// Loads of a row of tiles: codes, scales and zero points of a lane for matrix operands (all groups of four rows of W), by step.  Steps past
+// the end arrive as zeros, whose products are zeros.
+template <typename T, int GROUPS> struct W4Tiles {
+  rsrc_t codes, scales, zeros;
+  __device__ __forceinline__ W4Tiles(const W4Args &a, int tile, int steps) {
+    const int64_t first = (int64_t)min(tile, a.tiles - 1) * a.steps;
+    codes = make_rsrc(a.codes + first * kWave, steps * 1024);
+    scales = make_rsrc(reinterpret_cast<const T *>(a.scales) + first * 16 * GROUPS, steps * 32 * GROUPS);
+    zeros = make_rsrc(a.zeros + first * 16 * GROUPS, a.zeros ? steps * 16 * GROUPS : 0);
+  }
+};
+template <int BYTES, int AUX> __device__ __forceinline__ Pack<uint8_t, BYTES> w4_load(rsrc_t r, uint32_t at) {
+  if constexpr (BYTES == 32) {
+    Pack<uint8_t, 32> both;
+    const uint4 lo = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(r, (int)at, 0, AUX)),
+                hi = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(r, (int)at + 16, 0, AUX));
+    __builtin_memcpy(&both, &lo, 16);
+    __builtin_memcpy(both.v + 16, &hi, 16);
+    return both;
+  } else if constexpr (BYTES == 16) return __builtin_bit_cast(Pack<uint8_t, 16>, __builtin_amdgcn_raw_buffer_load_b128(r, (int)at, 0, AUX));
+  else if constexpr (BYTES == 8) return __builtin_bit_cast(Pack<uint8_t, 8>, __builtin_amdgcn_raw_buffer_load_b64(r, (int)at, 0, AUX));
+  else if constexpr (BYTES == 4) return __builtin_bit_cast(Pack<uint8_t, 4>, __builtin_amdgcn_raw_buffer_load_b32(r, (int)at, 0, AUX));
+  else if constexpr (BYTES == 2) return __builtin_bit_cast(Pack<uint8_t, 2>, __builtin_amdgcn_raw_buffer_load_b16(r, (int)at, 0, AUX));
+  else return Pack<uint8_t, 1>{{__builtin_amdgcn_raw_buffer_load_b8(r, (int)at, 0, AUX)}};
+}
 
 // The NW waves of a workgroup share the channels of CT tiles of W and 16 RT rows of x.
 template <int DT, int GROUP, int RT, int CT, int NW>
@@ -122,8 +151,9 @@ __global__ __launch_bounds__(NW *kWave) void w4_rows_kernel(W4Args a) {
   typedef Elem<DT> E;
   typedef typename E::T T;
   constexpr int kGroups = kTileCols / GROUP, kPer = GROUP / 32;       // groups of a step, matrix instructions of a group
+  constexpr int kAtOnce = CT < 4 ? CT : GROUP > 32 && RT == 1 ? 4 : GROUP > 32 || RT < 3 ? 2 : 1;      // tiles of W whose sums are under way
   __shared__ __align__(16) float s_acc[NW][RT * CT][kWave][4];
-  const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave, j = lane % 16, g = lane / 16;
+  const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), j = lane % 16, g = lane / 16;
   const int t0 = blockIdx.x * CT, r0 = blockIdx.y * 16 * RT;
   // rows past R and channels past K arrive as zeros
   const T *x0 = reinterpret_cast<const T *>(a.x) + r0 * a.x_stride;
@@ -131,59 +161,78 @@ __global__ __launch_bounds__(NW *kWave) void w4_rows_kernel(W4Args a) {
   const rsrc_t x_rsrc = make_rsrc(x0, (uint32_t)(((rows - 1) * a.x_stride + a.K) * 2));
   uint32_t xrow[RT];
 #pragma unroll
-  for (int t = 0; t < RT; ++t) xrow[t] = t * 16 + j < rows ? (uint32_t)((t * 16 + j) * a.x_stride * 2) : kOutOfRange;
+  for (int t = 0; t < RT; ++t) xrow[t] = t * 16 + j < rows ? (uint32_t)((t * 16 + j) * a.x_stride * 2) + g * 16 : kOutOfRange;
   const uint32_t one = DT == EN_F16 ? 0x3c003c00u : 0x3f803f80u;
   const uint4 ones = make_uint4(one, one, one, one);
+  typedef W4Tiles<T, kGroups> Tiles;
+  const int begin = blockIdx.z * a.per, end = min(begin + a.per, a.steps), channels = min(a.K, end * kTileCols);
+  auto tiles = [&](int c) { return Tiles(a, t0 + c, end); };
+  const Tiles tile0 = tiles(0), tile1 = tiles(CT > 1 ? 1 : 0), tile2 = tiles(CT > 2 ? 2 : 0), tile3 = tiles(CT > 3 ? 3 : 0);
+
+  uint4 w[CT], x[RT][4];
+  Pack<T, 4 * kGroups> sc[CT];
+  Pack<uint8_t, 4 * kGroups> ze[CT];
+  auto fetch = [&](int step) {
+#pragma unroll
+    for (int c = 0; c < CT; ++c) {
+      const Tiles &t = c == 0 ? tile0 : c == 1 ? tile1 : c == 2 ? tile2 : tile3;
+      w[c] = __builtin_bit_cast(uint4, w4_load<16, 2>(t.codes, (step * kWave + lane) * 16));
+      sc[c] = __builtin_bit_cast(Pack<T, 4 * kGroups>, w4_load<8 * kGroups, 0>(t.scales, (step * 4 + g) * 8 * kGroups));
+      ze[c] = w4_load<4 * kGroups, 0>(t.zeros, (step * 4 + g) * 4 * kGroups);
+    }
+    const int left = channels - step * kTileCols - g * 8;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int t = 0; t < RT; ++t)
+        x[t][i] = buffer_load16(x_rsrc, (xrow[t] + (uint32_t)(step * 256 + i * 64)) | (xrow[t] & kOutOfRange) | (i * 32 < left ? 0u : kOutOfRange));
+  };
 
   f32x4 acc[RT][CT];
 #pragma unroll
   for (int t = 0; t < RT; ++t)
 #pragma unroll
     for (int c = 0; c < CT; ++c) acc[t][c] = f32x4{0.f, 0.f, 0.f, 0.f};
-  for (int step = wave; step < a.steps; step += NW) {
-    uint4 w[CT], x[RT][4];
-    Pack<T, 4 * kGroups> sc[CT];
-    Pack<uint8_t, 4 * kGroups> ze[CT];
+  fetch(begin + wave);
+  for (int step = begin + wave; step < end; step += NW) {
 #pragma unroll
-    for (int c = 0; c < CT; ++c) {
-      const int64_t tile = min(t0 + c, a.tiles - 1);
-      w[c] = a.codes[(tile * a.steps + step) * kWave + lane];
-      const int64_t at = ((tile * a.steps + step) * 16 + 4 * g) * kGroups;
-      sc[c] = load_pack<T, 4 * kGroups>(reinterpret_cast<const T *>(a.scales) + at);
-      if (a.zeros) ze[c] = load_pack<uint8_t, 4 * kGroups>(a.zeros + at);
-    }
+      for (int i = 0; i < kGroups; ++i) {
+        // products of independent sums follow one another: each waits for the one before it of its own
+        f32x4 sum[RT];
 #pragma unroll
-    for (int t = 0; t < RT; ++t)
+        for (int t = 0; t < RT; ++t) sum[t] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int k = step * kTileCols + i * 32 + g * 8;
-        x[t][i] = buffer_load16(x_rsrc, xrow[t] + (uint32_t)k * 2u | xrow[t] & kOutOfRange | (k < a.K ? 0u : kOutOfRange));
-      }
+        for (int c0 = 0; c0 < CT; c0 += kAtOnce) {
+          f32x4 p[kAtOnce][RT];
 #pragma unroll
-    for (int i = 0; i < kGroups; ++i) {
-      f32x4 sum[RT];
+          for (int c = 0; c < kAtOnce; ++c)
 #pragma unroll
-      for (int t = 0; t < RT; ++t) {
-        sum[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+            for (int t = 0; t < RT; ++t) p[c][t] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int k = 0; k < kPer; ++k) sum[t] = mma<DT>(ones, x[t][i * kPer + k], sum[t]);
-      }
+          for (int k = 0; k < kPer; ++k) {
+            const int word = i * kPer + k;
+            if (c0 == 0)
 #pragma unroll
-      for (int c = 0; c < CT; ++c) {
-        uint4 wide[kPer];
+              for (int t = 0; t < RT; ++t) sum[t] = mma<DT>(ones, x[t][word], sum[t]);
 #pragma unroll
-        for (int k = 0; k < kPer; ++k) wide[k] = widen<DT>((&w[c].x)[i * kPer + k]);
+            for (int c = 0; c < kAtOnce; ++c) {
+              const uint4 all = w[c0 + c], wide = widen<DT>(word == 0 ? all.x : word == 1 ? all.y : word == 2 ? all.z : all.w);
 #pragma unroll
-        for (int t = 0; t < RT; ++t) {
-          f32x4 p = {0.f, 0.f, 0.f, 0.f};
+              for (int t = 0; t < RT; ++t) p[c][t] = mma<DT>(wide, x[t][word], p[c][t]);
+            }
+          }
 #pragma unroll
-          for (int k = 0; k < kPer; ++k) p = mma<DT>(wide[k], x[t][i * kPer + k], p);
+          for (int c = 0; c < kAtOnce; ++c)
 #pragma unroll
-          for (int e = 0; e < 4; ++e)
-            acc[t][c][e] += E::to_float(sc[c].v[e * kGroups + i]) * (p[e] - (a.zeros ? (float)ze[c].v[e * kGroups + i] : 8.f) * sum[t][e]);
+            for (int e = 0; e < 4; ++e) {
+              const float scale = E::to_float(sc[c0 + c].v[e * kGroups + i]), zero = a.zeros ? (float)ze[c0 + c].v[e * kGroups + i] : 8.f;
+#pragma unroll
+              for (int t = 0; t < RT; ++t) acc[t][c0 + c][e] += scale * (p[c][t][e] - zero * sum[t][e]);
+            }
+          if constexpr (GROUP == 32) __builtin_amdgcn_sched_barrier(0);      // a group's scales at a time in fp32
         }
       }
-    }
+    fetch(step + NW);
   }
 #pragma unroll
   for (int t = 0; t < RT; ++t)
@@ -197,6 +246,10 @@ __global__ __launch_bounds__(NW *kWave) void w4_rows_kernel(W4Args a) {
     f32x4 v = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int k = 0; k < NW; ++k) v += *reinterpret_cast<const f32x4 *>(s_acc[k][tc][lane]);
+    if (a.part) {
+      *reinterpret_cast<f32x4 *>(a.part + ((int64_t)blockIdx.z * a.R + r) * (a.tiles * kTileRows) + n) = v;
+      continue;
+    }
     Pack<T, 4> y;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
@@ -207,14 +260,26 @@ __global__ __launch_bounds__(NW *kWave) void w4_rows_kernel(W4Args a) {
   }
 }
 
-// ---- many rows ---------------------------------------------------------------------------------------------------------------------------
+// The sums of the runs of steps, four neighbours of a row a lane.
+template <int DT> __global__ __launch_bounds__(kBlock) void w4_join_kernel(W4Args a, int splits) {
+  typedef Elem<DT> E;
+  typedef typename E::T T;
+  const int n = (blockIdx.x * kBlock + threadIdx.x) * 4, r = blockIdx.y, pitch = a.tiles * kTileRows;
+  if (n >= a.N) return;
+  const float *p = a.part + (int64_t)r * pitch + n;
+  f32x4 v = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+  for (int s = 0; s < splits; ++s) v += *reinterpret_cast<const f32x4 *>(p + (int64_t)s * a.R * pitch);
+  Pack<T, 4> y;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const float bias = a.bias && n + e < a.N ? E::to_float(reinterpret_cast<const T *>(a.bias)[n + e]) : 0.f;
+    y.v[e] = E::from_float(w4_activate(v[e] + bias, a.act));
+  }
+  w4_store(reinterpret_cast<T *>(a.y) + (int64_t)r * a.N + n, y, a.N - n);
+}
 
-// 256 rows of x times 256 rows of W a workgroup, 64 channels a stage; eight waves, 128 x 64 each.  Bound by the matrix instructions: x goes
-// from memory into LDS as operands lie (a wave's load of 16 rows x 32 channels is one operand, 1 KB in lane order), and so do the
-// weights, each turned into 16 bits once for the 256 rows: (code - zero) * scale in fp32, rounded as a weight kept in 16 bits would be
-// (half a step of the activations' type; scaling sums of codes instead takes four multiplications for each four matrix instructions of a
-// group of 32, as many cycles as those themselves).
-constexpr int kManyRows = 256, kManyCols = 256, kManyWaves = 8;
+// ---- more rows ---------------------------------------------------------------------------------------------------------------------------
 
 template <int DT> __device__ __forceinline__ uint32_t pack_two(float lo, float hi);
 template <> __device__ __forceinline__ uint32_t pack_two<EN_F16>(float lo, float hi) {
@@ -229,10 +294,195 @@ template <typename F, int... I> __device__ __forceinline__ void each(F &&f, std:
 
 // Codes 2 I and 2 I + 1 of a word times scale plus off.
 template <int DT, int I> __device__ __forceinline__ uint32_t scaled_two(uint32_t w, float scale, float off) {
-  const uint32_t b = I < 2 ? w & 0x0f0f0f0fu : w >> 4 & 0x0f0f0f0fu;
+  uint32_t b = I < 2 ? w & 0x0f0f0f0fu : w >> 4 & 0x0f0f0f0fu;
+  asm("" : "+v"(b));             // bytes of a word, which a conversion takes by itself
   constexpr int kShift = I % 2 * 16;
   return pack_two<DT>((float)(b >> kShift & 0xffu) * scale + off, (float)(b >> (kShift + 8) & 0xffu) * scale + off);
 }
+
+// Bias, activation and the store of a wave's tiles.
+template <int DT, int RT, int CT> __device__ __forceinline__ void w4_finish(const W4Args &a, const f32x4 (&acc)[RT][CT], int r0, int t0) {
+  typedef Elem<DT> E;
+  typedef typename E::T T;
+  const int lane = threadIdx.x % kWave, j = lane % 16, g = lane / 16;
+  auto with = [&](auto act) {
+#pragma unroll
+    for (int c = 0; c < CT; ++c) {
+      const int n = (t0 + c) * kTileRows + 4 * g, left = a.N - n;
+      float bias[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) bias[e] = a.bias && e < left ? E::to_float(reinterpret_cast<const T *>(a.bias)[n + e]) : 0.f;
+#pragma unroll
+      for (int t = 0; t < RT; ++t) {
+        const int r = r0 + t * 16 + j;
+        Pack<T, 4> y;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) y.v[e] = E::from_float(w4_activate(acc[t][c][e] + bias[e], act.value));
+        if (r < a.R) w4_store(reinterpret_cast<T *>(a.y) + (int64_t)r * a.N + n, y, left);
+      }
+    }
+  };
+  switch (a.act) {
+    case EN_ACT_RELU: with(std::integral_constant<int, EN_ACT_RELU>{}); break;
+    case EN_ACT_GELU_TANH: with(std::integral_constant<int, EN_ACT_GELU_TANH>{}); break;
+    case EN_ACT_GELU: with(std::integral_constant<int, EN_ACT_GELU>{}); break;
+    default: with(std::integral_constant<int, EN_ACT_NONE>{});
+  }
+}
+
+// ROWS rows of x times COLS rows of W a workgroup, 64 channels a stage.  x and the codes come through registers, U steps of 128 channels ahead,
+// into LDS, x as matrix operands lie (1 KB in lane order) and the weights too, each turned into 16 bits once for all rows: (code - zero) *
+// scale in fp32, rounded as a weight kept in 16 bits would be (half a step of the activations' type; scaling sums of codes instead takes four
+// multiplications for each four matrix instructions of a group of 32, as many cycles as those themselves).  Where the workgroups of all rows
+// and columns are few, runs of steps are shared out too, and a second launch adds up.
+template <int ROWS_, int COLS_, int WR_, int WC_, int U_> struct W4Shape {
+  static constexpr int ROWS = ROWS_, COLS = COLS_, WR = WR_, WC = WC_, NW = WR * WC, U = U_;
+  static constexpr int RT = ROWS / 16 / WR, CT = COLS / 16 / WC;       // row tiles and tiles of W that a wave multiplies
+  static constexpr int XT = ROWS / 16 / NW, WT = COLS / 16 / NW;       // ... that it brings into LDS
+  static constexpr int kXStage = ROWS * 128, kWStage = COLS * 128;
+  static_assert(XT * NW * 16 == ROWS && WT * NW * 16 == COLS && 8 * WT % (2 * RT) == 0, "whole tiles, pieces a row tile");
+};
+
+template <int DT, int GROUP, typename S>
+__global__ __launch_bounds__(S::NW *kWave, 2) void w4_tile_kernel(W4Args a) {
+  typedef Elem<DT> E;
+  typedef typename E::T T;
+  constexpr int kGroups = kTileCols / GROUP, RT = S::RT, CT = S::CT, XT = S::XT, WT = S::WT, U = S::U, kPieces = 8 * WT / (2 * RT);
+  constexpr int kXStage = S::kXStage, kWStage = S::kWStage, kW = 2 * kXStage;
+  __shared__ __align__(16) char s_mem[2 * kXStage + 2 * kWStage];      // x operands [row tile][half][lane] of two stages, W operands [tile][half][lane]
+  const int lane = threadIdx.x % kWave, j = lane % 16, g = lane / 16;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), wr = wave % S::WR, wc = wave / S::WR;
+  // a column block's row blocks one after another: they read the same codes
+  const int row_blocks = (a.R + S::ROWS - 1) / S::ROWS;
+  const int rb = blockIdx.x % row_blocks, cb = blockIdx.x / row_blocks;
+  const int r0 = rb * S::ROWS, t0 = cb * (S::COLS / kTileRows);
+  const int begin = blockIdx.y * a.per, end = min(begin + a.per, a.steps);      // one step at least
+
+  // x: this wave moves row tiles XT wave ..; channels past K and rows past R arrive as zeros
+  const T *x0 = reinterpret_cast<const T *>(a.x) + (int64_t)r0 * a.x_stride;
+  const int rows = min(S::ROWS, a.R - r0);
+  const rsrc_t x_rsrc = make_rsrc(x0, (uint32_t)(((int64_t)(rows - 1) * a.x_stride + a.K) * 2));
+  uint32_t xrow[XT];
+#pragma unroll
+  for (int t = 0; t < XT; ++t) {
+    const int r = (XT * wave + t) * 16 + j;
+    xrow[t] = r < rows ? (uint32_t)((int64_t)r * a.x_stride * 2) + g * 16 : kOutOfRange;
+  }
+  // W: this wave turns tiles WT wave .. into 16 bits; a lane's row of W is l % 16
+  rsrc_t code_rsrc[WT], scale_rsrc[WT], zero_rsrc[WT];
+#pragma unroll
+  for (int t = 0; t < WT; ++t) {
+    const W4Tiles<T, kGroups> tiles(a, t0 + WT * wave + t, a.steps);
+    code_rsrc[t] = tiles.codes;
+    scale_rsrc[t] = tiles.scales;
+    zero_rsrc[t] = tiles.zeros;
+  }
+  uint4 xr[U][XT][4], codes[U][WT];
+  Pack<T, kGroups> sc[U][WT];
+  Pack<uint8_t, kGroups> ze[U][WT];
+  auto fetch = [&](int u, int step) {
+    const uint32_t none = step < end ? 0u : kOutOfRange;      // nothing is read past the run
+#pragma unroll
+    for (int t = 0; t < WT; ++t) {
+      codes[u][t] = __builtin_bit_cast(uint4, w4_load<16, 0>(code_rsrc[t], (step * kWave + lane) * 16 | none));
+      sc[u][t] = __builtin_bit_cast(Pack<T, kGroups>, w4_load<2 * kGroups, 0>(scale_rsrc[t], (step * 16 + j) * 2 * kGroups | none));
+      ze[u][t] = w4_load<kGroups, 0>(zero_rsrc[t], (step * 16 + j) * kGroups | none);
+    }
+    const int left = a.K - step * kTileCols - g * 8;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int t = 0; t < XT; ++t)
+        xr[u][t][i] = buffer_load16(x_rsrc, (xrow[t] + (uint32_t)(step * 256 + i * 64)) | (xrow[t] & kOutOfRange) | none | (i * 32 < left ? 0u : kOutOfRange));
+  };
+  // The pieces of the weights of half a step: two codes a lane of operand piece / 4, which goes to LDS with its fourth.
+  uint32_t piece4[4];
+  float scale = 0.f, off = 0.f;
+  auto put_w = [&](auto piece, int u, int part, int buf) {
+    constexpr int P = decltype(piece)::value, t = P / 8, half = P / 4 % 2;
+    const int word = 2 * part + half, i = word * 32 / GROUP;
+    const uint32_t w = word == 0 ? codes[u][t].x : word == 1 ? codes[u][t].y : word == 2 ? codes[u][t].z : codes[u][t].w;
+    if constexpr (P % 4 == 0) {
+      scale = E::to_float(sc[u][t].v[i]);
+      off = -(a.zeros ? (float)ze[u][t].v[i] : 8.f) * scale;
+      asm volatile("" : "+v"(scale), "+v"(off));         // here, not all operands' at once
+    }
+    piece4[P % 4] = scaled_two<DT, P % 4>(w, scale, off);
+    if constexpr (P % 4 == 3)
+      *reinterpret_cast<uint4 *>(s_mem + kW + buf * kWStage + ((WT * wave + t) * 2 + half) * 1024 + lane * 16) = make_uint4(piece4[0], piece4[1], piece4[2], piece4[3]);
+  };
+  auto put_x = [&](int u, int part, int buf) {
+#pragma unroll
+    for (int t = 0; t < XT; ++t)
+#pragma unroll
+      for (int half = 0; half < 2; ++half)
+        *reinterpret_cast<uint4 *>(s_mem + buf * kXStage + ((XT * wave + t) * 2 + half) * 1024 + lane * 16) = xr[u][t][2 * part + half];
+  };
+
+  f32x4 acc[RT][CT];
+#pragma unroll
+  for (int t = 0; t < RT; ++t)
+#pragma unroll
+    for (int c = 0; c < CT; ++c) acc[t][c] = f32x4{0.f, 0.f, 0.f, 0.f};
+  // A stage's products from buffer `buf`, and between them the next stage's operands into the other one.
+  auto multiply = [&](int buf, int u, int part) {
+    const char *xs = s_mem + buf * kXStage + wr * RT * 2048 + lane * 16, *ws = s_mem + kW + buf * kWStage + wc * CT * 2048 + lane * 16;
+    uint4 w[CT], x[2];
+#pragma unroll
+    for (int c = 0; c < CT; ++c) w[c] = *reinterpret_cast<const uint4 *>(ws + c * 2048);
+    x[0] = *reinterpret_cast<const uint4 *>(xs);
+    put_x(u, part, buf ^ 1);
+    auto one = [&](auto index) {
+      constexpr int I = decltype(index)::value, t = I % RT, half = I / RT;
+      if constexpr (I + 1 < 2 * RT) x[(I + 1) % 2] = *reinterpret_cast<const uint4 *>(xs + (I + 1) % RT * 2048 + (I + 1) / RT * 1024);
+#pragma unroll
+      for (int c = 0; c < CT; ++c) {
+        acc[t][c] = mma<DT>(w[c], x[I % 2], acc[t][c]);
+        if constexpr (half == 0 && t == RT - 1) w[c] = *reinterpret_cast<const uint4 *>(ws + c * 2048 + 1024);
+      }
+      each([&](auto p) { put_w(std::integral_constant<int, I * kPieces + decltype(p)::value>{}, u, part, buf ^ 1); }, std::make_integer_sequence<int, kPieces>{});
+      __builtin_amdgcn_sched_barrier(0);
+    };
+    each(one, std::make_integer_sequence<int, 2 * RT>{});
+  };
+#pragma unroll
+  for (int u = 0; u < U; ++u) fetch(u, begin + u);
+  put_x(0, 0, 0);
+  each([&](auto piece) { put_w(piece, 0, 0, 0); }, std::make_integer_sequence<int, 8 * WT>{});
+  lds_barrier();
+  // (steps past the run are zeros times zeros; their products are left out, and the barriers are the workgroup's)
+  for (int step = begin; step < end; step += U) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (step + u < end) {
+        multiply(0, u, 1);
+        lds_barrier();
+        fetch(u, step + u + U);
+        multiply(1, (u + 1) % U, 0);
+        lds_barrier();
+      }
+    }
+  }
+  if (a.part) {
+#pragma unroll
+    for (int t = 0; t < RT; ++t) {
+      const int r = r0 + (wr * RT + t) * 16 + j;
+#pragma unroll
+      for (int c = 0; c < CT; ++c) {
+        const int n = (t0 + wc * CT + c) * kTileRows + 4 * g;
+        if (r < a.R && n < a.N) *reinterpret_cast<f32x4 *>(a.part + ((int64_t)blockIdx.y * a.R + r) * (a.tiles * kTileRows) + n) = acc[t][c];
+      }
+    }
+    return;
+  }
+  w4_finish<DT, RT, CT>(a, acc, r0 + wr * RT * 16, t0 + wc * CT);
+}
+
+// 256 rows of x times 256 rows of W a workgroup, 64 channels a stage; eight waves, 128 x 64 each.  Bound by the matrix instructions: x goes
+// from memory into LDS as operands lie (a wave's load of 16 rows x 32 channels is one operand, 1 KB in lane order), and so do the
+// weights, each turned into 16 bits once for the 256 rows: (code - zero) * scale in fp32, rounded as a weight kept in 16 bits would be
+// (half a step of the activations' type; scaling sums of codes instead takes four multiplications for each four matrix instructions of a
+// group of 32, as many cycles as those themselves).
 
 template <int DT, int GROUP>
 __global__ __launch_bounds__(kManyWaves *kWave, 2) void w4_many_kernel(W4Args a) {
@@ -392,29 +642,7 @@ __global__ __launch_bounds__(kManyWaves *kWave, 2) void w4_many_kernel(W4Args a)
   arrived();
   lds_barrier();
   multiply(ring(xbuf + 1), 1, std::false_type{}, 0);
-  auto finish = [&](auto act) {
-#pragma unroll
-    for (int c = 0; c < CT; ++c) {
-      const int n = (t0 + wc * CT + c) * kTileRows + 4 * g, left = a.N - n;
-      float bias[4];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) bias[e] = a.bias && e < left ? E::to_float(reinterpret_cast<const T *>(a.bias)[n + e]) : 0.f;
-#pragma unroll
-      for (int t = 0; t < RT; ++t) {
-        const int r = r0 + (wr * RT + t) * 16 + j;
-        Pack<T, 4> y;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) y.v[e] = E::from_float(w4_activate(acc[t][c][e] + bias[e], act.value));
-        if (r < a.R) w4_store(reinterpret_cast<T *>(a.y) + (int64_t)r * a.N + n, y, left);
-      }
-    }
-  };
-  switch (a.act) {
-    case EN_ACT_RELU: finish(std::integral_constant<int, EN_ACT_RELU>{}); break;
-    case EN_ACT_GELU_TANH: finish(std::integral_constant<int, EN_ACT_GELU_TANH>{}); break;
-    case EN_ACT_GELU: finish(std::integral_constant<int, EN_ACT_GELU>{}); break;
-    default: finish(std::integral_constant<int, EN_ACT_NONE>{});
-  }
+  w4_finish<DT, RT, CT>(a, acc, r0 + wr * RT * 16, t0 + wc * CT);
 }
 
 static int check_w4(const en_w4_weight *w) {
@@ -425,6 +653,34 @@ static int check_w4(const en_w4_weight *w) {
   if (!w->codes || !w->scales) return EN_ERR_NULL;
   if (!aligned_to(w->codes, 16) || !aligned_to(w->scales, 16) || !aligned_to(w->zeros, 16)) return EN_ERR_ALIGN;
   return EN_OK;
+}
+
+// Which kernel, and in how many runs the channels are shared out (a launch more, and the sums through memory).  us, groups of 128, bf16:
+//  - narrow / wide (one tile of W a workgroup, or four, which share the loads of x): 1 x 768 -> 2304 5.3 / 5.9, 64 x 768 -> 2304 6.5 / 9.1, 1 x 4096
+//    -> 4096 5.3 / 8.2, 16 x 4096 -> 4096 6.8 / 9.0; 1 x 9216 -> 9216 18.2 / 16.4, 16 x 9216 -> 9216 30.4 / 17.0, 16 x 7168 -> 28672 54 / 27.5;
+//  - wide, runs 1 / 3 or 4: 16 x 9216 -> 9216 17.0 / 17.7; 40 x 9216 -> 9216 33 / 28, 64 x 9216 -> 9216 44.5 / 41.9, 40 x 4096 -> 4096 17 / 11.6,
+//    64 x 4096 -> 4096 23 / 14.2;
+//  - wide / tiles of 128 x 128: 64 x 9216 -> 9216 42 / 41, 128 x 9216 -> 9216 86 / 56;
+//  - tiles of 128 x 128 / of 256 x 256: 512 x 9216 -> 9216 148 / 217, 200 x 7168 -> 28672 146 / 171, 1000 x 9216 -> 9216 257 / 218, 2000 x 5120 -> 13841 374 / 281.
+enum class W4Form { kNarrow, kWide, kTile, kMany };
+struct W4Plan {
+  W4Form form;
+  int64_t runs;
+};
+inline W4Plan w4_plan(int64_t rows, int64_t tiles, int64_t steps) {
+  auto share = [&](int64_t workgroups, int64_t enough, int64_t most) {
+    int64_t runs = enough / workgroups;
+    runs = runs > most ? most : runs;
+    runs = runs > steps / 4 ? steps / 4 : runs;
+    return runs < 1 ? 1 : runs;
+  };
+  if (rows > 64) {
+    if (ceil_div(rows, kManyRows) * ceil_div(tiles, kManyCols / kTileRows) >= 128) return {W4Form::kMany, 1};
+    return {W4Form::kTile, share(ceil_div(rows, 128) * ceil_div(tiles, 8), 512, 8)};
+  }
+  if (rows <= 16) return {tiles < 512 ? W4Form::kNarrow : W4Form::kWide, 1};
+  if (tiles * steps < 2048) return {W4Form::kNarrow, 1};
+  return {W4Form::kWide, share(ceil_div(tiles, 4), 448, 4)};
 }
 
 }  // namespace en
@@ -459,32 +715,60 @@ int en_w4_pack(const uint8_t *codes, const void *scales, const uint8_t *zeros, c
   return EN_OK;
 }
 
+int64_t en_linear_w4_workspace_bytes(int64_t rows, int64_t out_features, int64_t in_features) {
+  if (rows < 1 || out_features < 1 || in_features < 1) return 0;
+  const W4Plan p = w4_plan(rows, ceil_div(out_features, kTileRows), ceil_div(in_features, kTileCols));
+  return p.runs > 1 ? p.runs * rows * ceil_div(out_features, kTileRows) * kTileRows * 4 : 0;
+}
+
 int en_linear_w4(const void *x, int64_t rows, int64_t x_stride, const en_w4_weight *weight, const void *bias, int activation, void *y,
-                 en_stream_t stream) {
+                 void *workspace, int64_t workspace_bytes, en_stream_t stream) {
   if (const int bad = check_w4(weight)) return bad;
   const int64_t N = weight->out_features, K = weight->in_features;
   if (activation < EN_ACT_NONE || activation > EN_ACT_GELU) return EN_ERR_UNSUPPORTED;
   if (rows < 0 || rows > (1 << 20) || x_stride < 0 || (rows > 1 && x_stride < K) || x_stride > kMostFeatures) return EN_ERR_SHAPE;
   if (rows == 0) return EN_OK;
-  if (!x || !y) return EN_ERR_NULL;
-  if (!aligned_to(x, 16) || x_stride % 8 || !aligned_to(y, 2) || !aligned_to(bias, 2)) return EN_ERR_ALIGN;
+  const int64_t need = en_linear_w4_workspace_bytes(rows, N, K);
+  if (!x || !y || (need > 0 && !workspace)) return EN_ERR_NULL;
+  if (workspace_bytes < need) return EN_ERR_SHAPE;
+  if (!aligned_to(x, 16) || x_stride % 8 || !aligned_to(y, 2) || !aligned_to(bias, 2) || !aligned_to(workspace, 16)) return EN_ERR_ALIGN;
   W4Args a{x, x_stride, (int)rows, (int)N, (int)K, (int)ceil_div(K, kTileCols), (int)ceil_div(N, kTileRows), (const uint4 *)weight->codes,
-           weight->scales, (const uint8_t *)weight->zeros, bias, activation, y};
+           weight->scales, (const uint8_t *)weight->zeros, bias, activation, y, 0, nullptr};
+  const W4Plan plan = w4_plan(rows, a.tiles, a.steps);
+  a.per = (int)ceil_div(a.steps, plan.runs);
+  if (plan.runs > 1) a.part = reinterpret_cast<float *>(workspace);
+  const unsigned runs = (unsigned)ceil_div(a.steps, a.per);
   const hipStream_t s = (hipStream_t)stream;
-  auto launch = [&](auto dt, auto group, auto rt) {
-    constexpr int RT = decltype(rt)::value, CT = 1, NW = 8;
-    const dim3 grid((unsigned)ceil_div(a.tiles, CT), (unsigned)ceil_div(rows, 16 * RT));
+  auto few = [&](auto dt, auto group, auto rt, auto ct, auto nw) {
+    constexpr int RT = decltype(rt)::value, CT = decltype(ct)::value, NW = decltype(nw)::value;
+    const dim3 grid((unsigned)ceil_div(a.tiles, CT), (unsigned)ceil_div(rows, 16 * RT), runs);
     w4_rows_kernel<decltype(dt)::value, decltype(group)::value, RT, CT, NW><<<grid, NW * kWave, 0, s>>>(a);
   };
-  auto many = [&](auto dt, auto group) {
-    const int64_t blocks = ceil_div(rows, kManyRows) * ceil_div(N, kManyCols);
-    w4_many_kernel<decltype(dt)::value, decltype(group)::value><<<(unsigned)blocks, kManyWaves * kWave, 0, s>>>(a);
-  };
   auto shape = [&](auto dt, auto group) {
-    if (rows > 128) return many(dt, group);
-    if (rows <= 16) launch(dt, group, std::integral_constant<int, 1>{});
-    else if (rows <= 32) launch(dt, group, std::integral_constant<int, 2>{});
-    else launch(dt, group, std::integral_constant<int, 4>{});
+    constexpr int DT = decltype(dt)::value, GROUP = decltype(group)::value;
+    typedef std::integral_constant<int, 1> i1;
+    typedef std::integral_constant<int, 2> i2;
+    typedef std::integral_constant<int, 3> i3;
+    typedef std::integral_constant<int, 4> i4;
+    typedef std::integral_constant<int, 8> i8;
+    const int row_tiles = (int)ceil_div(rows, 16);
+    if (plan.form == W4Form::kMany) {
+      w4_many_kernel<DT, GROUP><<<(unsigned)(ceil_div(rows, kManyRows) * ceil_div(N, kManyCols)), kManyWaves * kWave, 0, s>>>(a);
+    } else if (plan.form == W4Form::kTile) {
+      typedef W4Shape<128, 128, 2, 2, 2> S;
+      w4_tile_kernel<DT, GROUP, S><<<dim3((unsigned)(ceil_div(rows, S::ROWS) * ceil_div(N, S::COLS)), runs), S::NW * kWave, 0, s>>>(a);
+    } else if (plan.form == W4Form::kNarrow) {
+      if (row_tiles == 1) few(dt, group, i1{}, i1{}, i8{});
+      else if (row_tiles == 2) few(dt, group, i2{}, i1{}, i8{});
+      else if (row_tiles == 3) few(dt, group, i3{}, i1{}, i8{});
+      else few(dt, group, i4{}, i1{}, i8{});
+    } else {
+      if (row_tiles == 1) few(dt, group, i1{}, i4{}, i8{});
+      else if (row_tiles == 2) few(dt, group, i2{}, i4{}, i4{});
+      else if (row_tiles == 3) few(dt, group, i3{}, i4{}, i4{});
+      else few(dt, group, i4{}, i4{}, i4{});
+    }
+    if (a.part) w4_join_kernel<DT><<<dim3((unsigned)ceil_div(N, 4 * kBlock), (unsigned)rows), kBlock, 0, s>>>(a, (int)runs);
   };
   auto groups = [&](auto dt) {
     if (weight->group == 32) shape(dt, std::integral_constant<int, 32>{});

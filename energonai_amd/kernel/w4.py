@@ -118,7 +118,7 @@ def w4_quantize(weight, group_size: int = 128, zero_points: bool = False) -> W4W
 
 def linear_w4(inputs, weight, bias=None, activation: Optional[str] = None):
     """``linear`` with a weight in 4 bits: ``act(inputs[..., din] @ W[dout, din]^T + bias)`` -> ``[..., dout]``, fp16 or bf16 as the weight's
-    scales are.  Sums are fp32; up to 128 rows no weight is rounded, from there on each is, to the inputs' type.  ``activation``: ``"relu"``, ``"gelu_tanh"`` or ``"gelu"``."""
+    scales are.  Sums are fp32; up to 64 rows no weight is rounded, from there on each is, to the inputs' type.  ``activation``: ``"relu"``, ``"gelu_tanh"`` or ``"gelu"``."""
     who = "linear_w4"
     if type(weight) is W4Weight and activation in _ACTIVATIONS:
         y = _lib.front.linear_w4(inputs, weight, bias, _ACTIVATIONS[activation])
@@ -141,7 +141,9 @@ def linear_w4(inputs, weight, bias=None, activation: Optional[str] = None):
         x = x.clone(memory_format=torch.contiguous_format)
     rows = x.shape[0]
     out = torch.empty((*inputs.shape[:-1], w.out_features), dtype=inputs.dtype, device=inputs.device)
+    need = int(_lib.fn.en_linear_w4_workspace_bytes(rows, w.out_features, w.in_features))
+    workspace = torch.empty(need, dtype=torch.uint8, device=inputs.device)
     with _lib.device_guard(inputs):
         _lib.check(_lib.fn.en_linear_w4(x.data_ptr(), rows, x.stride(0) if rows > 1 else w.in_features, ctypes.byref(w), _lib.ptr(bias) or None,
-                                        _ACTIVATIONS[activation], out.data_ptr(), _lib.stream_of(inputs)), who)
+                                        _ACTIVATIONS[activation], out.data_ptr(), _lib.ptr(workspace) or None, need, _lib.stream_of(inputs)), who)
     return out

@@ -592,10 +592,12 @@ int64_t en_w4_groups(int64_t out_features, int64_t in_features, int group);
  * ceil(in_features / group)]; contiguous.  The results' pointers in `weight` are written through. */
 int en_w4_pack(const uint8_t *codes, const void *scales, const uint8_t *zeros, const en_w4_weight *weight, en_stream_t stream);
 /* y = act(x W^T + bias): x [rows, in_features], x_stride elements apart (a multiple of 8), 16-byte aligned; y contiguous [rows,
- * out_features]; bias [out_features] or NULL; activation an en_activation.  Sums are fp32; up to 128
- * rows no weight is rounded, from there on each is, to dtype, as a 16-bit weight would be. */
+ * out_features]; bias [out_features] or NULL; activation an en_activation.  Sums are fp32; up to 64
+ * rows no weight is rounded, from there on each is, to dtype, as a 16-bit weight would be.  workspace: en_linear_w4_workspace_bytes (may be
+ * 0, then NULL), 16-byte aligned; its contents need not be kept or cleared, but calls that may run at the same time need one each. */
+int64_t en_linear_w4_workspace_bytes(int64_t rows, int64_t out_features, int64_t in_features);
 int en_linear_w4(const void *x, int64_t rows, int64_t x_stride, const en_w4_weight *weight, const void *bias, int activation, void *y,
-                 en_stream_t stream);
+                 void *workspace, int64_t workspace_bytes, en_stream_t stream);
 
 /* ---- measurement helper ------------------------------------------------- */
 

@@ -118,12 +118,12 @@ def test_w4_refuses():
     assert lib.fn.en_w4_codes_bytes(40, 200) == 3 * 2 * 1024 and lib.fn.en_w4_groups(40, 200, 64) == 3 * 2 * 2 * 16
     assert lib.fn.en_w4_codes_bytes(0, 8) == 0 and lib.fn.en_w4_groups(16, 128, 48) == 0
 
-    def call(x=PTR, rows=4, stride=200, bias=None, act=0, y=PTR, **kw):
-        return lib.fn.en_linear_w4(x, rows, stride, ctypes.byref(_w4(**kw)), bias, act, y, None)
+    def call(x=PTR, rows=4, stride=200, bias=None, act=0, y=PTR, ws=PTR, ws_bytes=1 << 40, **kw):
+        return lib.fn.en_linear_w4(x, rows, stride, ctypes.byref(_w4(**kw)), bias, act, y, ws, ws_bytes, None)
     assert call(rows=0) == 0
     for kw in (dict(x=None), dict(y=None), dict(codes=None), dict(scales=None)):
         assert call(**kw) == NULL, kw
-    assert lib.fn.en_linear_w4(PTR, 1, 200, None, None, 0, PTR, None) == NULL
+    assert lib.fn.en_linear_w4(PTR, 1, 200, None, None, 0, PTR, None, 0, None) == NULL
     for kw in (dict(rows=-1), dict(stride=192), dict(stride=-8), dict(out_features=0), dict(in_features=0), dict(in_features=204), dict(in_features=1 << 22), dict(rows=1 << 32)):
         assert call(**kw) == SHAPE, kw
     for kw in (dict(group=48), dict(act=4), dict(act=-1)):
@@ -132,6 +132,10 @@ def test_w4_refuses():
         assert call(**kw) == ALIGN, kw
     for dtype in (0, 3):
         assert call(dtype=dtype) == DTYPE
+    need = lib.fn.en_linear_w4_workspace_bytes
+    assert need(1, 4096, 4096) == 0 and need(0, 4096, 4096) == 0 and need(40, 4096, 4096) > 0
+    wide = dict(rows=40, stride=4096, out_features=4096, in_features=4096)
+    assert call(ws=None, **wide) == NULL and call(ws_bytes=need(40, 4096, 4096) - 1, **wide) == SHAPE and call(ws=PTR + 8, **wide) == ALIGN
     pack = lib.fn.en_w4_pack
     assert pack(None, PTR, None, ctypes.byref(_w4()), None) == NULL and pack(PTR, PTR, PTR, ctypes.byref(_w4()), None) == NULL
     assert pack(PTR, PTR + 1, None, ctypes.byref(_w4()), None) == ALIGN and pack(PTR, PTR, None, ctypes.byref(_w4(group=16)), None) == UNSUPPORTED

@@ -21,7 +21,7 @@ def weight(N, Kd, group, dtype, zeros, seed):
     return codes, scales, z
 
 
-MANY = 128            # rows up to which no weight is rounded
+MANY = 64            # rows up to which no weight is rounded
 
 
 def tolerance(want, size, dtype, Kd, act, rounded=None):
@@ -44,7 +44,8 @@ CASES = [
     # rows, din, dout, group
     (1, 8, 1, 32), (1, 768, 2304, 64), (1, 136, 17, 128), (2, 32, 16, 32), (7, 200, 33, 64), (16, 128, 48, 128), (17, 1000, 65, 32), (31, 2048, 64, 64),
     (33, 512, 100, 128), (48, 384, 31, 64), (64, 1024, 272, 128), (65, 264, 128, 32), (100, 640, 50, 64), (130, 1536, 144, 128), (257, 520, 300, 32),
-    (400, 256, 96, 64), (1, 8192, 32, 128), (5, 16384, 16, 128), (3, 64, 5000, 64),
+    (400, 256, 96, 64), (1, 8192, 32, 128), (5, 16384, 16, 128), (3, 64, 5000, 64), (2, 200, 9001, 32), (16, 264, 8200, 128), (20, 2304, 2000, 64),
+    (48, 2200, 1111, 32), (64, 3200, 1500, 128), (90, 4096, 700, 64), (300, 1160, 1000, 128), (1100, 136, 8230, 64), (520, 264, 16500, 32), (257, 1000, 16400, 128),
 ]
 
 
@@ -85,7 +86,7 @@ def test_rows_keep_to_themselves():
     N, Kd, group, dtype = 40, 200, 64, torch.float16
     codes, scales, z = weight(N, Kd, group, dtype, True, 8)
     w = K().w4_weight(codes.cuda(), scales.cuda(), z.cuda(), group_size=group)
-    for rows in (3, 40, 150):
+    for rows in (3, 40, 150, 300):
         wide = torch.full((rows, Kd + 16), float("nan"), dtype=dtype, device="cuda")
         x = wide[:, 8:8 + Kd]
         x.copy_(torch.randn(rows, Kd, generator=torch.Generator().manual_seed(9)))
