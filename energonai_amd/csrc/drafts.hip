@@ -37,43 +37,40 @@ __global__ __launch_bounds__(kWave) void draft_tree_kernel(const int32_t *parent
 
 // What counts is how a row's largest logit is found: the rows on the way are read one after another, each by what the one before chose, and a
 // compute unit that reads one by itself is bound by its instructions as much as by its loads.  So a lane takes vectors of 16 bytes, 16-bit
-// logits two at a time in the order of signed integers (sign and magnitude turned into it), and remembers only which of its vectors holds the
-// best; the vector is read once more for the index.  That order is that of the numbers but for zeros of two signs and NaN, whose
-// largest magnitude is kept beside; a row that has NaN, or zero for its largest, is gone over once more element by element.
+// logits two at a time as the integers that they are stored as, and remembers only which of its vectors holds the largest; the vector is read
+// once more for the index.  As signed integers numbers from 0 up are in their order and above the negative ones, and NaN is above
+// infinity; as unsigned ones a negative NaN is above all.  A row with NaN, or whose largest logit is 0 or negative, is gone over once more
+// element by element.  (64 trees, 12 rows of 128000 on the longest way, bf16: 71 us in the numbers' own order, sign and magnitude turned
+// into it, 35 instructions a vector.)
 typedef short s16x2 __attribute__((ext_vector_type(2)));
 typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
 
 template <int DT> struct Logits {
   static constexpr int kPer = 16 / Elem<DT>::kSize;
-  static constexpr uint32_t kInf = DT == EN_F16 ? 0x7c00u : DT == EN_BF16 ? 0x7f80u : 0x7f800000u;
-  // The vector's largest in the integers' order, and the largest magnitude's bits.
-  __device__ static __forceinline__ int largest(const uint4 &v, uint32_t &magnitude) {
+  static constexpr int kInf = DT == EN_F16 ? 0x7c00 : DT == EN_BF16 ? 0x7f80 : 0x7f800000;
+  // The vector's largest as signed integers; `top` is raised to its largest as unsigned ones, half by half.
+  __device__ static __forceinline__ int largest(const uint4 &v, uint32_t &top) {
     if constexpr (DT == EN_F32) {
-      auto order = [](uint32_t x) { return (int)(x ^ ((uint32_t)((int)x >> 31) & 0x7fffffffu)); };
-      magnitude = max(max(v.x & 0x7fffffffu, v.y & 0x7fffffffu), max(v.z & 0x7fffffffu, v.w & 0x7fffffffu));
-      return max(max(order(v.x), order(v.y)), max(order(v.z), order(v.w)));
+      top = max(max(top, v.x), max(max(v.y, v.z), v.w));
+      return max(max((int)v.x, (int)v.y), max((int)v.z, (int)v.w));
     } else {
-      auto order = [](uint32_t x) {
-        const s16x2 sign = __builtin_bit_cast(s16x2, x) >> 15;
-        return __builtin_bit_cast(s16x2, x ^ (__builtin_bit_cast(uint32_t, sign) & 0x7fff7fffu));
-      };
-      auto size = [](uint32_t x) { return __builtin_bit_cast(u16x2, x & 0x7fff7fffu); };
-      const u16x2 m = __builtin_elementwise_max(__builtin_elementwise_max(size(v.x), size(v.y)), __builtin_elementwise_max(size(v.z), size(v.w)));
-      magnitude = max((uint32_t)m.x, (uint32_t)m.y);
-      const s16x2 o = __builtin_elementwise_max(__builtin_elementwise_max(order(v.x), order(v.y)), __builtin_elementwise_max(order(v.z), order(v.w)));
+      auto s = [](uint32_t x) { return __builtin_bit_cast(s16x2, x); };
+      auto u = [](uint32_t x) { return __builtin_bit_cast(u16x2, x); };
+      top = __builtin_bit_cast(uint32_t, __builtin_elementwise_max(u(top), __builtin_elementwise_max(__builtin_elementwise_max(u(v.x), u(v.y)), __builtin_elementwise_max(u(v.z), u(v.w)))));
+      const s16x2 o = __builtin_elementwise_max(__builtin_elementwise_max(s(v.x), s(v.y)), __builtin_elementwise_max(s(v.z), s(v.w)));
       return max((int)o.x, (int)o.y);
     }
   }
-  // Index of the first element that is `order`.
-  __device__ static __forceinline__ int first(const uint4 &v, int order) {
+  __device__ static __forceinline__ bool negative_nan(uint32_t top) {
+    if constexpr (DT == EN_F32) return top > 0xff800000u;
+    else return max(top & 0xffffu, top >> 16) > (0x8000u | (uint32_t)kInf);
+  }
+  // Index of the first element that is stored as `bits`.
+  __device__ static __forceinline__ int first(const uint4 &v, uint32_t bits) {
     const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-    const uint32_t bits = order < 0 ? (uint32_t)order ^ 0x7fffffffu : (uint32_t)order;
     int at = 0;
 #pragma unroll
-    for (int i = kPer - 1; i >= 0; --i) {
-      const bool same = DT == EN_F32 ? w[i % 4] == bits : (uint16_t)(w[i / 2 % 4] >> (16 * (i % 2))) == (uint16_t)((order < 0 ? order ^ 0x7fff : order));
-      at = same ? i : at;
-    }
+    for (int i = kPer - 1; i >= 0; --i) at = (DT == EN_F32 ? w[i % 4] : w[i / 2 % 4] >> (16 * (i % 2)) & 0xffffu) == bits ? i : at;
     return at;
   }
 };
@@ -111,29 +108,27 @@ __device__ __forceinline__ uint64_t row_best(const typename Elem<DT>::T *row, in
     const int vectors = (to - from + kPer - 1) / kPer;
     auto start = [&](int v) { return min(from + v * kPer, to - kPer); };       // the last one overlaps the one before
     int best = INT32_MIN, at = 0;
-    uint32_t magnitude = 0;
+    uint32_t above = 0;
     for (int v0 = threadIdx.x; v0 < vectors; v0 += kAhead * kThreads) {
       uint4 x[kAhead];
 #pragma unroll
       for (int i = 0; i < kAhead; ++i) x[i] = load16_at<false, sizeof(T)>(row + start(min(v0 + i * kThreads, vectors - 1)));
 #pragma unroll
       for (int i = 0; i < kAhead; ++i) {
-        uint32_t m;
-        const int o = L::largest(x[i], m);
-        magnitude = max(magnitude, m);
+        const int o = L::largest(x[i], above);
         if (o > best) {
           best = o;
           at = min(v0 + i * kThreads, vectors - 1);
         }
       }
     }
-    const uint64_t mine = (uint64_t)((uint32_t)best ^ 0x80000000u) << 32 | (uint32_t)~at;
     // (a lane without vectors has INT32_MIN, which is 0 here)
-    const uint64_t top = block_largest<W>(magnitude > L::kInf ? ~0ull : mine, slots[0]);
-    const int order = (int)((uint32_t)(top >> 32) ^ 0x80000000u);
-    if (top != ~0ull && order != 0 && order != -1) {
-      const int s = start((int)~(uint32_t)top);
-      const int i = s + L::first(load16_at<false, sizeof(T)>(row + s), order);
+    const uint64_t mine = (uint64_t)((uint32_t)best ^ 0x80000000u) << 32 | (uint32_t)~at;
+    const uint64_t all = block_largest<W>(L::negative_nan(above) ? ~0ull : mine, slots[0]);
+    const int largest = (int)((uint32_t)(all >> 32) ^ 0x80000000u);
+    if (largest > 0 && largest <= L::kInf) {
+      const int s = start((int)~(uint32_t)all);
+      const int i = s + L::first(load16_at<false, sizeof(T)>(row + s), (uint32_t)largest);
       return (uint64_t)ordered(Elem<DT>::to_float(row[i])) << 32 | (uint32_t)~i;
     }
   }
