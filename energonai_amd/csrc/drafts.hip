@@ -103,7 +103,7 @@ template <int DT, int W>
 __device__ __forceinline__ uint64_t row_best(const typename Elem<DT>::T *row, int from, int to, uint64_t (*slots)[W]) {
   typedef Logits<DT> L;
   typedef typename Elem<DT>::T T;
-  constexpr int kThreads = W * kWave, kPer = L::kPer, kAhead = 4;
+  constexpr int kThreads = W * kWave, kPer = L::kPer, kAhead = 8;
   if (to - from >= kPer) {
     const int vectors = (to - from + kPer - 1) / kPer;
     auto start = [&](int v) { return min(from + v * kPer, to - kPer); };       // the last one overlaps the one before

@@ -339,7 +339,6 @@ __global__ __launch_bounds__(S::kThreads, 2) void tree_attn_kernel(TreeArgs a) {
         for (int u = 0; u < kSub; ++u)
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            sc[t][u][e] *= a.c_exp;
             if (!whole) {
               const int pos = (wk * kSub + u) * 16 + 4 * g + e;
               const bool seen = own ? pos < kNodes && (mask[t] >> (pos & 63) & 1) : pos < left;
@@ -347,6 +346,7 @@ __global__ __launch_bounds__(S::kThreads, 2) void tree_attn_kernel(TreeArgs a) {
             }
             top = fmaxf(top, sc[t][u][e]);
           }
+        top *= a.c_exp;
         if (__ballot(top > m[t] + kRaise)) {
           const float to = fmaxf(m[t], over_groups_max(top));
           const float keep = to > -INFINITY ? __builtin_amdgcn_exp2f(m[t] - to) : 1.f;
@@ -361,7 +361,7 @@ __global__ __launch_bounds__(S::kThreads, 2) void tree_attn_kernel(TreeArgs a) {
           float e4[4];
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            e4[e] = __builtin_amdgcn_exp2f(sc[t][u][e] - base);
+            e4[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[t][u][e], a.c_exp, -base));
             l[t] += e4[e];
           }
           p[t][u][0] = M::two(e4[0], e4[1]);
@@ -630,7 +630,7 @@ extern "C" int en_decode_attn_tree(const void *q, const void *k_new, const void 
     tree_attn_kernel<DT, S><<<a.runs ? kGroups : (unsigned)units, S::kThreads, 0, s>>>(a);
     if (!a.runs) return;
     // rows of a unit in workgroups of their own where units are few; where units are many, each has few shares
-    const dim3 shares((unsigned)units, (unsigned)(units >= 512 ? ceil_div(at_once, kCombineGroups) : at_once));
+    const dim3 shares((unsigned)units, (unsigned)(units >= 64 ? ceil_div(at_once, kCombineGroups) : at_once));
     tree_combine_kernel<DT, S::kTile, S::kRows><<<shares, kBlock, 0, s>>>(a);
   };
   auto rows_of = [&](auto dt, auto nt) {
