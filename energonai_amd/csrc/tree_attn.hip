@@ -331,6 +331,27 @@ __global__ __launch_bounds__(S::kThreads, 2) void tree_attn_kernel(TreeArgs a) {
       }
       const int left = s.len - tile * kTile;       // of the context, from this tile on
       const bool whole = !own && left >= kTile;
+      if (!whole) {
+#pragma unroll
+        for (int t = 0; t < QT; ++t) {
+          // bit i: whether the lane's i-th position of this wave's tiles is seen
+          uint32_t seen = 0;
+          if (own) {
+#pragma unroll
+            for (int u = 0; u < kSub; ++u) {
+              const int from = (wk * kSub + u) * 16 + 4 * g;
+              seen |= (uint32_t)(from < kNodes ? mask[t] >> from & 15 : 0) << (4 * u);
+            }
+          } else {
+#pragma unroll
+            for (int u = 0; u < kSub; ++u) seen |= ((1u << min(max(left - (wk * kSub + u) * 16 - 4 * g, 0), 4)) - 1) << (4 * u);
+          }
+#pragma unroll
+          for (int u = 0; u < kSub; ++u)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) sc[t][u][e] = seen >> (4 * u + e) & 1 ? sc[t][u][e] : -INFINITY;
+        }
+      }
       uint32_t p[QT][kSub][2];
 #pragma unroll
       for (int t = 0; t < QT; ++t) {
@@ -338,14 +359,7 @@ __global__ __launch_bounds__(S::kThreads, 2) void tree_attn_kernel(TreeArgs a) {
 #pragma unroll
         for (int u = 0; u < kSub; ++u)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            if (!whole) {
-              const int pos = (wk * kSub + u) * 16 + 4 * g + e;
-              const bool seen = own ? pos < kNodes && (mask[t] >> (pos & 63) & 1) : pos < left;
-              sc[t][u][e] = seen ? sc[t][u][e] : -INFINITY;
-            }
-            top = fmaxf(top, sc[t][u][e]);
-          }
+          for (int e = 0; e < 4; ++e) top = fmaxf(top, sc[t][u][e]);
         top *= a.c_exp;
         if (__ballot(top > m[t] + kRaise)) {
           const float to = fmaxf(m[t], over_groups_max(top));
