@@ -127,6 +127,7 @@ template <int NT_, int QT_, int QW_, int KW_> struct TreeShape {
   static constexpr int kStep = kThreads / kSlots, kEach = kTile / kStep, kWaveRows = kWave / kSlots;
   static constexpr int kKeyPitch = NT * 32 + 16, kValuePitch = NT * 32 + 32;      // bytes: rows shifted by 4 and 8 banks
   static constexpr int kValues = kTile * kKeyPitch, kBytes = kValues + kTile * kValuePitch;
+  static constexpr int kBuffers = KW == 1 ? 2 : 1;                        // of tiles in LDS, so that two workgroups fit a CU
   static constexpr int kMerge = (KW - 1) * QT * NT * 1024, kMergeBytes = kMerge + KW * QT * 128;
   static_assert(NT % 2 == 0 && kSub % 2 == 0 && kTile % kStep == 0 && kWaveRows <= 16 && kMergeBytes <= kBytes, "whole vectors, pairs of key tiles, rows of one page");
 };
@@ -137,9 +138,8 @@ __global__ __launch_bounds__(S::kThreads, 2) void tree_attn_kernel(TreeArgs a) {
   typedef typename E::T T;
   typedef Mma<DT> M;
   constexpr int NT = S::NT, QT = S::QT, QW = S::QW, KW = S::KW, NC = S::NC, kSub = S::kSub, kTile = S::kTile, kEach = S::kEach;
-  __shared__ __align__(16) char s_mem[S::kBytes];
+  __shared__ __align__(16) char s_mem[S::kBuffers * S::kBytes];
   __shared__ uint32_t s_odd[kNodes / 32];      // nodes with a value that is not a number, or infinite
-  char *const s_k = s_mem, *const s_v = s_mem + S::kValues;
   const int lane = threadIdx.x % kWave, col = lane % 16, g = lane / 16;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), wq = wave % QW, wk = wave / QW;
 
@@ -254,7 +254,8 @@ __global__ __launch_bounds__(S::kThreads, 2) void tree_attn_kernel(TreeArgs a) {
   };
   // A node's value that is not a number, or infinite, may not meet the zeros of rows that do not see it: it is a zero here and
   // added where it is seen (below).
-  auto put = [&](bool own) {
+  auto put = [&](bool own, int buf) {
+    char *const s_k = s_mem + buf * S::kBytes, *const s_v = s_k + S::kValues;
     const bool whole = __ballot(valid != (1u << kEach) - 1) == 0;
 #pragma unroll
     for (int i = 0; i < kEach; ++i) {
@@ -276,6 +277,7 @@ __global__ __launch_bounds__(S::kThreads, 2) void tree_attn_kernel(TreeArgs a) {
   bool first_segment = true;
   while (true) {
     // a unit, or this run's part of it
+    lds_barrier();                             // the one before has been read
     const int begin = tile, stop = (int)min((uint32_t)s.tiles, tile + (end - x));
     if (a.runs && tile == 0 && h == 0 && chunk == 0 && threadIdx.x == 0) a.first_tile[b] = x;
     if (begin < s.context) pages(begin);
@@ -306,16 +308,15 @@ __global__ __launch_bounds__(S::kThreads, 2) void tree_attn_kernel(TreeArgs a) {
 #pragma unroll
       for (int n = 0; n < NT; ++n) o[t][n] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
+    if (threadIdx.x < kNodes / 32) s_odd[threadIdx.x] = 0;
+    lds_barrier();
+    put(tile >= s.context, 0);
+    if (tile + 1 < stop) load(tile + 1);
+    lds_barrier();
+    int buf = 0;
     for (; tile < stop; ++tile) {
       const bool own = tile >= s.context;
-      lds_barrier();
-      if (own) {
-        if (threadIdx.x < kNodes / 32) s_odd[threadIdx.x] = 0;
-        lds_barrier();
-      }
-      put(own);
-      if (tile + 1 < stop) load(tile + 1);
-      lds_barrier();
+      const char *const s_k = s_mem + buf * S::kBytes, *const s_v = s_k + S::kValues;
       f32x4 sc[QT][kSub];
 #pragma unroll
       for (int u = 0; u < kSub; ++u) {
@@ -328,6 +329,10 @@ __global__ __launch_bounds__(S::kThreads, 2) void tree_attn_kernel(TreeArgs a) {
 #pragma unroll
           for (int t = 0; t < QT; ++t) sc[t][u] = M::k32(k, q[t][c], sc[t][u]);
         }
+      }
+      if (S::kBuffers == 2 && tile + 1 < stop) {
+        put(tile + 1 >= s.context, buf ^ 1);
+        if (tile + 2 < stop) load(tile + 2);
       }
       const int left = s.len - tile * kTile;       // of the context, from this tile on
       const bool whole = !own && left >= kTile;
@@ -392,6 +397,16 @@ __global__ __launch_bounds__(S::kThreads, 2) void tree_attn_kernel(TreeArgs a) {
 #pragma unroll
           for (int t = 0; t < QT; ++t) o[t][n] = M::k32(v, make_uint4(p[t][u][0], p[t][u][1], p[t][u + 1][0], p[t][u + 1][1]), o[t][n]);
         }
+      if (tile + 1 < stop) {
+        lds_barrier();
+        if constexpr (S::kBuffers == 1) {
+          put(tile + 1 >= s.context, 0);
+          if (tile + 2 < stop) load(tile + 2);
+          lds_barrier();
+        } else {
+          buf ^= 1;
+        }
+      }
       if (!own || (s_odd[0] | s_odd[1]) == 0) continue;
       const uint64_t odd = (uint64_t)s_odd[1] << 32 | s_odd[0];
       for (int k = 0; k < kSub * 16; ++k) {
