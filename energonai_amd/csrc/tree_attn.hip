@@ -123,7 +123,7 @@ template <int TILE, int ROWS> __device__ __forceinline__ TreeSeq tree_seq(const 
 template <int NT_, int QT_, int QW_, int KW_> struct TreeShape {
   static constexpr int NT = NT_, QT = QT_, QW = QW_, KW = KW_;
   static constexpr int kThreads = QW * KW * kWave, kTile = KW == 4 ? 128 : 64, kRows = 16 * QT * QW, kSub = kTile / 16 / KW, NC = NT / 2;
-  static constexpr int kSlots = NT > 4 ? 16 : 2 * NT;                     // lanes a row of a tile is moved by: whole rows a wave, and no more than 16
+  static constexpr int kSlots = NT > 4 ? 16 : NT == 2 && QW == 8 ? 8 : 2 * NT;                     // lanes a row of a tile is moved by: whole rows a wave, and no more than 16
   static constexpr int kStep = kThreads / kSlots, kEach = kTile / kStep, kWaveRows = kWave / kSlots;
   static constexpr int kKeyPitch = NT * 32 + 16, kValuePitch = NT * 32 + 32;      // bytes: rows shifted by 4 and 8 banks
   static constexpr int kValues = kTile * kKeyPitch, kBytes = kValues + kTile * kValuePitch;
@@ -598,8 +598,9 @@ __global__ __launch_bounds__(kBlock) void tree_combine_kernel(TreeArgs a) {
 }
 
 // Rows a workgroup takes at a time, by the rows a unit may have.
-inline int tree_rows(int64_t rows) { return rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 ? 64 : 128; }
-constexpr int kGroups = 512;                  // workgroups that share all tiles: two a CU
+inline int tree_rows(int64_t rows) { return rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 ? 64 : rows <= 128 ? 128 : 256; }
+// Workgroups that share all tiles: two of four waves a CU, or one of eight.
+inline int tree_groups(int at_once) { return at_once == 256 ? 256 : 512; }
 inline bool tree_runs(int64_t units, int64_t capacity) { return capacity > 1024 || units > 512; }
 
 }  // namespace en
@@ -610,7 +611,7 @@ extern "C" int64_t en_decode_attn_tree_workspace_bytes(int batch, int q_heads, i
   if (batch < 1 || head_num < 1 || q_heads < head_num || q_heads % head_num || capacity < 0 || size_per_head < 1 || max_nodes < 1) return 0;
   const int64_t rows = (int64_t)max_nodes * (q_heads / head_num), at_once = tree_rows(rows);
   if (!tree_runs((int64_t)batch * head_num * ceil_div(rows, at_once), capacity)) return 0;
-  return 2 * kGroups * at_once * (4 * (int64_t)size_per_head + 8) + 4 * ((int64_t)batch + 1);
+  return 2 * tree_groups((int)at_once) * at_once * (4 * (int64_t)size_per_head + 8) + 4 * ((int64_t)batch + 1);
 }
 
 extern "C" int en_decode_attn_tree(const void *q, const void *k_new, const void *v_new, const int64_t *strides, void *ctx,
@@ -650,13 +651,13 @@ extern "C" int en_decode_attn_tree(const void *q, const void *k_new, const void 
   a.max_nodes = max_nodes; a.total = (int)nodes;
   a.c_exp = scale * 1.4426950408889634f;
   a.part_o = reinterpret_cast<float *>(workspace);
-  a.part_ml = reinterpret_cast<float2 *>(a.part_o + 2 * kGroups * at_once * c.size_per_head);
-  a.first_tile = reinterpret_cast<uint32_t *>(a.part_ml + 2 * kGroups * at_once);
+  a.part_ml = reinterpret_cast<float2 *>(a.part_o + (int64_t)2 * tree_groups((int)at_once) * at_once * c.size_per_head);
+  a.first_tile = reinterpret_cast<uint32_t *>(a.part_ml + (int64_t)2 * tree_groups((int)at_once) * at_once);
   const hipStream_t s = (hipStream_t)stream;
   auto launch = [&](auto dt, auto shape) {
     constexpr int DT = decltype(dt)::value;
     typedef decltype(shape) S;
-    tree_attn_kernel<DT, S><<<a.runs ? kGroups : (unsigned)units, S::kThreads, 0, s>>>(a);
+    tree_attn_kernel<DT, S><<<a.runs ? tree_groups((int)at_once) : (unsigned)units, S::kThreads, 0, s>>>(a);
     if (!a.runs) return;
     // rows of a unit in workgroups of their own where units are few; where units are many, each has few shares
     const dim3 shares((unsigned)units, (unsigned)(units >= 64 ? ceil_div(at_once, kCombineGroups) : at_once));
@@ -667,7 +668,8 @@ extern "C" int en_decode_attn_tree(const void *q, const void *k_new, const void 
     if (at_once == 16) launch(dt, TreeShape<NT, 1, 1, 4>{});
     else if (at_once == 32) launch(dt, TreeShape<NT, 2, 1, 4>{});
     else if (at_once == 64) launch(dt, TreeShape<NT, 1, 4, 1>{});
-    else launch(dt, TreeShape<NT, 2, 4, 1>{});
+    else if (at_once == 128) launch(dt, TreeShape<NT, 2, 4, 1>{});
+    else launch(dt, TreeShape<NT, 2, 8, 1>{});
   };
   auto heads = [&](auto dt) {
     if (a.D <= 32) rows_of(dt, std::integral_constant<int, 2>{});
