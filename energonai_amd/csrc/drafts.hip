@@ -203,7 +203,9 @@ __global__ __launch_bounds__(W *kWave) void accept_walk_kernel(AcceptArgs a) {
 }
 
 constexpr int kWalkWaves = 16;
-constexpr int64_t kAllBytes = 24ll << 20, kSliceBytes = 32 << 10;
+// us, a row at a time as the walk comes to it / all rows first: 4 trees of up to 32 nodes, vocabulary 128000 (23 MB) 17.0 / 11.0; 32 of 16, 50257 (49
+// MB) 26.5 / 14.7; 8 of 32, 128000 (62 MB) 17.2 / 14.7; 64 of 16, 50257 (98 MB) 26.6 / 23.4; 16 of 32, 128000 (125 MB) 17.4 / 23.5.
+constexpr int64_t kAllBytes = 96ll << 20, kSliceBytes = 32 << 10;
 // Slices of a row where all rows are looked at first; 0: a row at a time, as the walk comes to it.
 inline int accept_slices(int64_t nodes, int64_t vocab, int es) {
   if (nodes * vocab * es > kAllBytes) return 0;

@@ -597,11 +597,16 @@ __global__ __launch_bounds__(kBlock) void tree_combine_kernel(TreeArgs a) {
   }
 }
 
-// Rows a workgroup takes at a time, by the rows a unit may have.
-inline int tree_rows(int64_t rows) { return rows <= 16 ? 16 : rows <= 32 ? 32 : rows <= 64 ? 64 : rows <= 128 ? 128 : 256; }
+// Rows a workgroup takes at a time, by the rows a unit may have: sixteen in four waves that share a tile's positions; else sixteen or
+// thirty-two a wave.  us, 24 sequences of up to 4000, 32 / 8 x 128, rows 16 / 64 / 128 / 256 at a time: 16 rows a unit 43 / 47 / 59 / 88; 32 73 / 49 / 64 / 93;
+// 64 130 / 53 / 68 / 97; 128 242 / 93 / 81 / 110; 8 sequences of up to 8000, 64 / 8 heads, 512 rows - / 280 / 186 / 178.
+inline int tree_rows(int64_t rows) { return rows <= 16 ? 16 : rows <= 64 ? 64 : rows <= 128 ? 128 : 256; }
 // Workgroups that share all tiles: two of four waves a CU, or one of eight.
 inline int tree_groups(int at_once) { return at_once == 256 ? 256 : 512; }
-inline bool tree_runs(int64_t units, int64_t capacity) { return capacity > 1024 || units > 512; }
+// Equal runs of tiles, whatever the lengths are, at the cost of a second launch, or a workgroup a unit where caches are short.  us, a
+// workgroup a unit / runs: 1 sequence of 100, 12 x 64 8.2 / 13.6, of 1000 16.4 / 13.3; 4 of up to 1000, 32 / 8 x 128 40 / 22; 32 of up to 500, 12 x 64
+// 13.5 / 18.8; 32 of up to 1000, 32 / 8 x 128 39.9 / 42.3; 64 of up to 250, 40 x 128 69 / 76; 128 of up to 200, 64 / 8 x 128 55 / 63; 8 of up to 2000 54 / 31.
+inline bool tree_runs(int64_t units, int64_t capacity) { return capacity > (units >= 256 ? 1152 : 512); }
 
 }  // namespace en
 
@@ -666,7 +671,6 @@ extern "C" int en_decode_attn_tree(const void *q, const void *k_new, const void 
   auto rows_of = [&](auto dt, auto nt) {
     constexpr int NT = decltype(nt)::value;
     if (at_once == 16) launch(dt, TreeShape<NT, 1, 1, 4>{});
-    else if (at_once == 32) launch(dt, TreeShape<NT, 2, 1, 4>{});
     else if (at_once == 64) launch(dt, TreeShape<NT, 1, 4, 1>{});
     else if (at_once == 128) launch(dt, TreeShape<NT, 2, 4, 1>{});
     else launch(dt, TreeShape<NT, 2, 8, 1>{});
