@@ -1,12 +1,12 @@
 // Attention of drafted tokens: the nodes of a tree behind each sequence's cached positions, over a paged cache and over one another.
 //
 // A sequence's up to 64 nodes times the G query heads that share a key head are the rows of one unit, and one pass over the unit's keys
-// and values serves them all.  A workgroup takes a unit's rows, 16 QT QW of them at a time, and goes over its tiles of keys: those of the
-// context in pages, and behind them one tile that holds the nodes' own keys, where a row sees what its mask says.
+// and values serves them all.  A workgroup takes a unit's rows, 16 QT QW of them at a time, and goes over its tiles of keys: the
+// context's, in pages, and right behind its last position the nodes' own, of which a row sees what its mask says.
 //  - Scores are S^T = K Q^T on 16x16x32 matrix instructions: rows are positions, columns queries.  A lane's scores of two neighbouring
 //    key tiles (positions 4g .. 4g + 3 of each) are, packed to 16 bits, in place as the operand of O^T = V^T P^T when V^T is read from
 //    LDS with the same order of positions, by its transposing read.
-//  - Keys and values go through registers into LDS, a tile ahead: what lies behind a sequence's end or in no page arrives there as zeros,
+//  - Keys and values go through registers into LDS, a tile ahead: what lies behind a sequence's nodes or in no page arrives there as zeros,
 //    so that nothing of another sequence, and no NaN of a page never written, meets a probability of zero.
 //  - The running maximum is raised only where a score passes it by 2^8: the sums are fp32, and probabilities of up to 2^8 are as exact in
 //    16 bits as those below 1.
@@ -104,7 +104,8 @@ __device__ __forceinline__ float share_weight(float m, float l, float top) {
 // A sequence's part in the row of all tiles: per key head, per run of rows, its tiles and the unit's end.
 constexpr int kUnitCost = 1;
 struct TreeSeq {
-  int first, nodes, rows, len, context, tiles, chunks;
+  int first, nodes, rows, len, chunks;
+  int context, tiles;            // tiles of the context alone; all, the nodes following the context's last position
   __device__ __forceinline__ uint32_t per_unit() const { return tiles + kUnitCost; }
 };
 template <int TILE, int ROWS> __device__ __forceinline__ TreeSeq tree_seq(const TreeArgs &a, int first, int next, int len) {
@@ -113,8 +114,8 @@ template <int TILE, int ROWS> __device__ __forceinline__ TreeSeq tree_seq(const 
   s.nodes = min(max(min(next, a.total) - first, 0), a.max_nodes);
   s.rows = s.nodes * a.G;
   s.len = min(max(len, 0), a.max_pages << a.lg_page);
-  s.context = (s.len + TILE - 1) / TILE;
-  s.tiles = s.context + 1;
+  s.context = s.len / TILE;
+  s.tiles = (s.len + s.nodes + TILE - 1) / TILE;
   s.chunks = (s.rows + ROWS - 1) / ROWS;
   return s;
 }
@@ -215,14 +216,14 @@ __global__ __launch_bounds__(S::kThreads, 2) void tree_attn_kernel(TreeArgs a) {
   uint32_t valid = 0;
   const int slot = lane % S::kSlots, lane_row = lane / S::kSlots, ch = slot * 8;
   const uint32_t ch_bytes = ch < a.D ? ch * 2 : 0;
-  // Pages of a context tile: of the rows that this wave moves, which are in one page a step.
+  // Pages of a tile: of the rows that this wave moves, which are in one page a step.
   auto pages = [&](int t) {
     const int32_t *names = a.table + (int64_t)b * a.max_pages;
 #pragma unroll
     for (int i = 0; i < kEach; ++i)
-      id[i] = scalar_word(names + min((t * kTile + i * S::kStep + wave * S::kWaveRows) >> a.lg_page, max(a.max_pages - 1, 0)));
+      id[i] = scalar_word(names + min((t * kTile + i * S::kStep + wave * S::kWaveRows) >> a.lg_page, a.max_pages - 1));
   };
-  // Rows past the context, and of pages that are none, are loaded from wherever there is memory, and taken for zeros.
+  // Rows of pages that are none are loaded from wherever there is memory, and taken for zeros.
   auto load_context = [&](int t) {
     valid = 0;
 #pragma unroll
@@ -234,38 +235,44 @@ __global__ __launch_bounds__(S::kThreads, 2) void tree_attn_kernel(TreeArgs a) {
       const uint32_t row = (pos0 & ((1 << a.lg_page) - 1)) + lane_row;
       kr[i] = *reinterpret_cast<const uint4 *>(kp + (row * a.k_row + ch_bytes));
       vr[i] = *reinterpret_cast<const uint4 *>(vp + (row * a.v_row + ch_bytes));
-      if (named && pos0 + lane_row < s.len && ch < a.D) valid |= 1u << i;
+      if (named && ch < a.D) valid |= 1u << i;
     }
   };
-  auto load_nodes = [&] {
+  // A tile in which the context ends or that is behind it: the nodes follow its last position.
+  auto load_end = [&](int t) {
     valid = 0;
 #pragma unroll
     for (int i = 0; i < kEach; ++i) {
-      const int r = i * S::kStep + wave * S::kWaveRows + lane_row, row = s.first + min(r, s.nodes - 1);
-      kr[i] = *reinterpret_cast<const uint4 *>(a.k_new + row * a.kn_token + h * a.kn_head + ch_bytes);
-      vr[i] = *reinterpret_cast<const uint4 *>(a.v_new + row * a.vn_token + h * a.vn_head + ch_bytes);
-      if (r < s.nodes && ch < a.D) valid |= 1u << i;
+      const int pos0 = t * kTile + i * S::kStep + wave * S::kWaveRows, node = pos0 + lane_row - s.len;
+      const bool named = pos0 < s.len && (unsigned)id[i] < (unsigned)a.num_pages;
+      const int64_t page = named ? id[i] : 0, row = (pos0 & ((1 << a.lg_page) - 1)) + lane_row, from = s.first + min(max(node, 0), s.nodes - 1);
+      const char *kp = node < 0 ? a.k_pool + page * a.k_page + h * a.k_head + row * a.k_row : a.k_new + from * a.kn_token + h * a.kn_head;
+      const char *vp = node < 0 ? a.v_pool + page * a.v_page + h * a.v_head + row * a.v_row : a.v_new + from * a.vn_token + h * a.vn_head;
+      kr[i] = *reinterpret_cast<const uint4 *>(kp + ch_bytes);
+      vr[i] = *reinterpret_cast<const uint4 *>(vp + ch_bytes);
+      if ((node < 0 ? named : node < s.nodes) && ch < a.D) valid |= 1u << i;
     }
   };
   auto load = [&](int t) {
     if (t < s.context) load_context(t);
-    else load_nodes();
-    if (t + 1 < s.context) pages(t + 1);
+    else load_end(t);
+    if ((t + 1) * kTile < s.len) pages(t + 1);
   };
   // A node's value that is not a number, or infinite, may not meet the zeros of rows that do not see it: it is a zero here and
   // added where it is seen (below).
-  auto put = [&](bool own, int buf) {
+  auto put = [&](int t, int buf) {
     char *const s_k = s_mem + buf * S::kBytes, *const s_v = s_k + S::kValues;
     const bool whole = __ballot(valid != (1u << kEach) - 1) == 0;
 #pragma unroll
     for (int i = 0; i < kEach; ++i) {
       const int r = i * S::kStep + wave * S::kWaveRows + lane_row;
       if (!whole && !(valid >> i & 1)) kr[i] = vr[i] = make_uint4(0, 0, 0, 0);
-      if (own) {
+      const int node = t * kTile + r - s.len;
+      if (t >= s.context && node >= 0) {
         const uint4 odd = make_uint4(odd_halves<DT>(vr[i].x), odd_halves<DT>(vr[i].y), odd_halves<DT>(vr[i].z), odd_halves<DT>(vr[i].w));
         if (odd.x | odd.y | odd.z | odd.w) {
           vr[i] = make_uint4(vr[i].x & ~odd.x, vr[i].y & ~odd.y, vr[i].z & ~odd.z, vr[i].w & ~odd.w);
-          atomicOr(&s_odd[r / 32], 1u << (r % 32));
+          atomicOr(&s_odd[node / 32], 1u << (node % 32));
         }
       }
       if (S::kSlots > 2 * NT && slot >= 2 * NT) continue;
@@ -280,7 +287,7 @@ __global__ __launch_bounds__(S::kThreads, 2) void tree_attn_kernel(TreeArgs a) {
     lds_barrier();                             // the one before has been read
     const int begin = tile, stop = (int)min((uint32_t)s.tiles, tile + (end - x));
     if (a.runs && tile == 0 && h == 0 && chunk == 0 && threadIdx.x == 0) a.first_tile[b] = x;
-    if (begin < s.context) pages(begin);
+    if (begin * kTile < s.len) pages(begin);
     load(begin);
     // queries: column l % 16 of tile t, channels 32 c + 8 g ..
     uint4 q[QT][NC];
@@ -310,7 +317,7 @@ __global__ __launch_bounds__(S::kThreads, 2) void tree_attn_kernel(TreeArgs a) {
     }
     if (threadIdx.x < kNodes / 32) s_odd[threadIdx.x] = 0;
     lds_barrier();
-    put(tile >= s.context, 0);
+    put(tile, 0);
     if (tile + 1 < stop) load(tile + 1);
     lds_barrier();
     int buf = 0;
@@ -331,25 +338,20 @@ __global__ __launch_bounds__(S::kThreads, 2) void tree_attn_kernel(TreeArgs a) {
         }
       }
       if (S::kBuffers == 2 && tile + 1 < stop) {
-        put(tile + 1 >= s.context, buf ^ 1);
+        put(tile + 1, buf ^ 1);
         if (tile + 2 < stop) load(tile + 2);
       }
-      const int left = s.len - tile * kTile;       // of the context, from this tile on
-      const bool whole = !own && left >= kTile;
-      if (!whole) {
+      if (own) {
 #pragma unroll
         for (int t = 0; t < QT; ++t) {
           // bit i: whether the lane's i-th position of this wave's tiles is seen
           uint32_t seen = 0;
-          if (own) {
 #pragma unroll
-            for (int u = 0; u < kSub; ++u) {
-              const int from = (wk * kSub + u) * 16 + 4 * g;
-              seen |= (uint32_t)(from < kNodes ? mask[t] >> from & 15 : 0) << (4 * u);
-            }
-          } else {
-#pragma unroll
-            for (int u = 0; u < kSub; ++u) seen |= ((1u << min(max(left - (wk * kSub + u) * 16 - 4 * g, 0), 4)) - 1) << (4 * u);
+          for (int u = 0; u < kSub; ++u) {
+            const int node = tile * kTile + (wk * kSub + u) * 16 + 4 * g - s.len;      // of the first of four
+            const uint32_t before = (1u << min(max(-node, 0), 4)) - 1;
+            const uint32_t nodes = node >= kNodes || node <= -4 ? 0u : (uint32_t)(node >= 0 ? mask[t] >> node : mask[t] << -node) & 15u;
+            seen |= (before | nodes) << (4 * u);
           }
 #pragma unroll
           for (int u = 0; u < kSub; ++u)
@@ -400,7 +402,7 @@ __global__ __launch_bounds__(S::kThreads, 2) void tree_attn_kernel(TreeArgs a) {
       if (tile + 1 < stop) {
         lds_barrier();
         if constexpr (S::kBuffers == 1) {
-          put(tile + 1 >= s.context, 0);
+          put(tile + 1, 0);
           if (tile + 2 < stop) load(tile + 2);
           lds_barrier();
         } else {
@@ -410,8 +412,8 @@ __global__ __launch_bounds__(S::kThreads, 2) void tree_attn_kernel(TreeArgs a) {
       if (!own || (s_odd[0] | s_odd[1]) == 0) continue;
       const uint64_t odd = (uint64_t)s_odd[1] << 32 | s_odd[0];
       for (int k = 0; k < kSub * 16; ++k) {
-        const int node = wk * kSub * 16 + k;
-        if (node >= s.nodes || !(odd >> node & 1)) continue;
+        const int node = tile * kTile + wk * kSub * 16 + k - s.len;
+        if (node < 0 || node >= s.nodes || !(odd >> node & 1)) continue;
         const T *value = reinterpret_cast<const T *>(a.v_new + (int64_t)(s.first + node) * a.vn_token + h * a.vn_head) + 4 * g;
 #pragma unroll
         for (int t = 0; t < QT; ++t) {
