@@ -11,6 +11,7 @@ from .kv_cache import KVCache, PagedKVCache, PagedKVCache8
 from .attention import MultiHeadAttention1D
 from .mlp import MLP1D
 from .endecoder import Block1D
+from .linear4 import Linear4, quantize_linears
 from .stack import PackedStack
 
-__all__ = ["KVCache", "PagedKVCache", "PagedKVCache8", "MultiHeadAttention1D", "MLP1D", "Block1D", "PackedStack", "set_gemm_tuning", "gemm_tuning"]
+__all__ = ["Linear4", "quantize_linears", "KVCache", "PagedKVCache", "PagedKVCache8", "MultiHeadAttention1D", "MLP1D", "Block1D", "PackedStack", "set_gemm_tuning", "gemm_tuning"]

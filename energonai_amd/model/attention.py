@@ -36,6 +36,7 @@ class MultiHeadAttention1D(nn.Module):
 
     # what is not there in a module saved before there was a choice
     rotary_dim, rotary_base, rotary_interleaved, qk_norm, kv_cache_dtype = 0, 10000.0, False, False, None
+    _nodes = None               # keys, values and tree of a step of drafted nodes, until they are accepted
 
     def __init__(self, hidden_size: int, num_heads: int, bias: bool = True, dtype: torch.dtype = torch.float16,
                  max_seq_len: int = 512, fused_qkv: bool = True, is_decoder: bool = True, disable_past_cache=False,
@@ -102,7 +103,7 @@ class MultiHeadAttention1D(nn.Module):
 
     # The tables follow from the module's numbers, and a loaded module may be on another device than the one they are kept for.
     def __getstate__(self):
-        return {**super().__getstate__(), "_rotary_tables": {}}
+        return {**super().__getstate__(), "_rotary_tables": {}, "_nodes": None}
 
     def __setstate__(self, state):
         super().__setstate__({**state, "_rotary_tables": {}})
@@ -195,6 +196,32 @@ class MultiHeadAttention1D(nn.Module):
             cache.append(k, v)
         ctx = cache.attend(q, self.scaling)      # [B,H,1,D], one pass over the caches
         return project(self.dense, ctx.view(B, 1, self.hidden_size))
+
+    # ---- one step of drafted nodes ------------------------------------------------------------
+    def forward_nodes(self, x: torch.Tensor, tree) -> torch.Tensor:
+        """``x`` is ``[1,nodes,hid]``: the nodes of a ``kernel.DraftTree``, each sequence's newest token first.  They see the cached positions and
+        the nodes that their masks name.  The cache stays as it is until ``accept_nodes``."""
+        cache = self.kv_cache
+        if cache is None:
+            raise RuntimeError("decode step before a first_cache=True call")
+        if not isinstance(cache, PagedKVCache):
+            raise RuntimeError("drafted nodes need a cache in pages (kv_page_size)")
+        H, D = self.num_heads, self.attention_head_size
+        T = x.numel() // self.hidden_size
+        q, k, v, _ = self._project(x)
+        if self.turned:
+            positions = torch.repeat_interleave(cache.lens, tree.info.lens, output_size=T) + tree.depths
+            q, k = qk_norm_rotary(q, k, cache.batch_size, None, self._tables(x.device, cache.max_seq_len), positions=positions, **self._turn_how())
+        ctx = cache.attend_nodes(q, k, v, tree, self.scaling)
+        self._nodes = (k, v, tree)
+        return project(self.dense, ctx.view(1, T, self.hidden_size))
+
+    def accept_nodes(self, path: torch.Tensor, counts: torch.Tensor, counts_host=None) -> None:
+        """The accepted nodes of the last ``forward_nodes`` (``kernel.accept_drafts``) go into the cache (see ``PagedKVCache.extend``)."""
+        if self._nodes is None:
+            raise RuntimeError("accept_nodes before a forward_nodes call")
+        self.kv_cache.extend(*self._nodes, path, counts, counts_host)
+        self._nodes = None
 
     def forward(self, hidden_states, attention_mask=None, first_cache=False, seq_lens=None):
         B, S, hid = hidden_states.shape

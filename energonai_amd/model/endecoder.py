@@ -159,6 +159,15 @@ class Block1D(nn.Module):
             return y
         return self._rows(x, lambda h: self.attn.forward_packed(h, info, batch_size, max_seq_len, fill_cache))
 
+    def forward_nodes(self, x: torch.Tensor, tree) -> torch.Tensor:
+        """One step of drafted nodes, packed ``[1,nodes,hid]`` rows (see ``MultiHeadAttention1D.forward_nodes``); the block's output for
+        each of them.  The padded history of outputs that other calls return has no part in it."""
+        return self._rows(x, lambda h: self.attn.forward_nodes(h, tree))
+
+    def accept_nodes(self, path: torch.Tensor, counts: torch.Tensor, counts_host=None) -> None:
+        """The nodes that were accepted go into the cache (see ``PagedKVCache.extend``)."""
+        self.attn.accept_nodes(path, counts, counts_host)
+
     def forward(self, hidden_states, attention_mask=None, first_cache=False, seq_lens=None):
         step = not self.disable_past_cache and not first_cache
         if step:

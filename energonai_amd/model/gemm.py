@@ -32,7 +32,7 @@ def gemm_algo():
 
 def project(layer: nn.Linear, x: torch.Tensor) -> torch.Tensor:
     """``layer(x)``; with tuning on, 16-bit ``[batch, rows, din]`` inputs take the tuned hipBLASLt GEMM."""
-    if _tuning and x.is_cuda and x.dim() == 3 and x.is_contiguous() and x.dtype in (torch.float16, torch.bfloat16) \
+    if _tuning and isinstance(layer, nn.Linear) and x.is_cuda and x.dim() == 3 and x.is_contiguous() and x.dtype in (torch.float16, torch.bfloat16) \
             and layer.weight.dtype == x.dtype:
         bias = None if layer.bias is None else layer.bias.detach()
         return linear(x, layer.weight.detach(), "auto", bias=bias)

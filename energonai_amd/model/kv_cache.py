@@ -14,8 +14,8 @@ from typing import Optional
 
 import torch
 
-from ..kernel import (decode_attn, decode_attn_kv8, decode_attn_paged, kv8_pages, kv8_pages_append, kv8_pages_fill, kv_cache_append,
-                      kv_cache_fill, kv_pages_append, kv_pages_append_rotary, kv_pages_fill, qk_norm_rotary, repad)
+from ..kernel import (decode_attn, decode_attn_kv8, decode_attn_paged, decode_attn_tree, kv8_pages, kv8_pages_append, kv8_pages_fill, kv_cache_append,
+                      kv_cache_fill, kv_pages_append, kv_pages_append_rotary, kv_pages_extend, kv_pages_fill, qk_norm_rotary, repad)
 from ..kernel.attention import kv_cache_start
 from ..seqinfo import SeqInfo
 
@@ -209,6 +209,24 @@ class PagedKVCache:
     def attend(self, q: torch.Tensor, scale: float) -> torch.Tensor:
         return decode_attn_paged(q, self.k, self.v, self.info, self.table, scale=scale)
 
+    def attend_nodes(self, q: torch.Tensor, k_new: torch.Tensor, v_new: torch.Tensor, tree, scale: float) -> torch.Tensor:
+        """Attention of drafted nodes, packed ``[nodes, H, D]`` rows, over the cached positions and over one another
+        (``kernel.decode_attn_tree``)."""
+        return decode_attn_tree(q, k_new, v_new, self.k, self.v, self.info, self.table, tree, scale=scale)
+
+    def extend(self, k_new: torch.Tensor, v_new: torch.Tensor, tree, path: torch.Tensor, counts: torch.Tensor, counts_host=None) -> None:
+        """The rows of the accepted nodes (``kernel.accept_drafts``) become the sequences' next positions; lengths advance by ``counts``.
+        The pages are assigned on the host, which needs the counts there: ``counts_host`` if the caller has them (the layers of a model share
+        them), else one copy from the device."""
+        counts_host = [int(n) for n in (counts.tolist() if counts_host is None else counts_host)]
+        if len(counts_host) != self.batch_size or min(counts_host, default=0) < 0:
+            raise RuntimeError(f"PagedKVCache.extend: counts must be one for each of the {self.batch_size} sequences")
+        P = self.page_size
+        self._assign([(b, (n + m + P - 1) // P) for b, (n, m) in enumerate(zip(self._host_lens, counts_host))])
+        kv_pages_extend(k_new, v_new, self.k, self.v, self.info, self.table, tree, path, counts)
+        self.lens.add_(counts)
+        self._host_lens = [n + m for n, m in zip(self._host_lens, counts_host)]
+
 
 class PagedKVCache8(PagedKVCache):
     """``PagedKVCache`` in 8 bits (int8 or float8_e4m3fn), with a scale for each block of 16 positions and head and each sequence's
@@ -243,6 +261,11 @@ class PagedKVCache8(PagedKVCache):
 
     def attend(self, q: torch.Tensor, scale: float) -> torch.Tensor:
         return decode_attn_kv8(q, self.pages, self.info, scale=scale)
+
+    def attend_nodes(self, *args, **kw):
+        raise RuntimeError("PagedKVCache8: drafted nodes need a cache in 16-bit pages (PagedKVCache)")
+
+    extend = attend_nodes
 
 
 class OutputHistory:

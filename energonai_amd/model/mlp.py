@@ -8,6 +8,7 @@ from torch import nn
 
 from ..kernel.cuda_native.linear_func import linear
 from .gemm import gemm_algo
+from .linear4 import Linear4
 
 
 def _epilogue_of(activation) -> Optional[str]:
@@ -50,9 +51,14 @@ class MLP1D(nn.Module):
         """The MLP on any ``[..., hid]`` rows (packed tokens or the last position of a batch).
 
         ReLU (the OPT models) and tanh-GELU are applied, with the bias, in the epilogue of the first GEMM;
-        any other activation runs as its own op between two library GEMMs, as in mlp.py:31-33.
+        any other activation runs as its own op between two library GEMMs, as in mlp.py:31-33.  With weights in 4 bits so is exact GELU.
         """
-        if self._epilogue is not None and x.is_cuda and x.dim() == 3 and x.is_contiguous():
+        if type(self.dense_1) is Linear4:
+            code = activation_code(self.activation, self._epilogue)
+            if code is not None:
+                return self.dense_2(self.dense_1(x, {1: "relu", 2: "gelu_tanh", 3: "gelu"}[code]))
+            return self.dense_2(self.activation(self.dense_1(x)))
+        if self._epilogue is not None and x.is_cuda and x.dim() == 3 and x.is_contiguous() and not isinstance(self.dense_2, Linear4):
             h = linear(x, self.dense_1.weight.detach(), gemm_algo(), bias=_detached(self.dense_1.bias),
                        activation=self._epilogue)
             return linear(h, self.dense_2.weight.detach(), gemm_algo(), bias=_detached(self.dense_2.bias))

@@ -47,3 +47,15 @@ class PackedStack(nn.Module):
         if self.norm is not None:
             x = self.norm(x)
         return repad(x, B, S, info, left_padded=left)
+
+    def forward_nodes(self, x: torch.Tensor, tree) -> torch.Tensor:
+        """One step of drafted nodes through every block (``Block1D.forward_nodes``): packed ``[1,nodes,hid]`` rows in and out."""
+        for blk in self.blocks:
+            x = blk.forward_nodes(x, tree)
+        return x if self.norm is None else self.norm(x)
+
+    def accept_nodes(self, path: torch.Tensor, counts: torch.Tensor, counts_host=None) -> None:
+        """The accepted nodes go into every block's cache; the counts are copied to the host once for all of them."""
+        counts_host = counts.tolist() if counts_host is None else counts_host
+        for blk in self.blocks:
+            blk.accept_nodes(path, counts, counts_host)

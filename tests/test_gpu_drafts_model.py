@@ -1,0 +1,123 @@
+"""Steps of drafted nodes and weights in 4 bits through the model layers."""
+import copy
+
+import pytest
+import torch
+
+from gpu_util import announce
+
+pytestmark = pytest.mark.gpu
+
+HID, HEADS = 256, 4
+
+
+def _block(dtype, **kw):
+    from energonai_amd.model import Block1D
+    torch.manual_seed(3)
+    return Block1D(HID, HEADS, 2, activation=kw.pop("activation", torch.nn.functional.relu), dtype=dtype, max_seq_len=128, kv_page_size=16, **kw).cuda().eval()
+
+
+def _prompt(lens, dtype, seed=1):
+    g = torch.Generator().manual_seed(seed)
+    x = torch.zeros(len(lens), max(lens), HID, dtype=dtype)
+    for b, n in enumerate(lens):
+        x[b, max(lens) - n:] = torch.randn(n, HID, generator=g).to(dtype)
+    return x.cuda()
+
+
+@pytest.mark.parametrize("turn", [{}, dict(rotary_dim=32, qk_norm=True)])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@torch.no_grad()
+def test_nodes_are_the_steps_they_stand_for(dtype, turn):
+    """A chain of nodes gives what steps of one token give; so does each way of a tree; and the accepted rows continue the cache."""
+    from energonai_amd import kernel as K
+    from energonai_amd.model import PackedStack
+    lens, B = [17, 30, 5], 3
+    blocks = [_block(dtype, **turn) for _ in range(2)]
+    stack, other = PackedStack(blocks), PackedStack([copy.deepcopy(b) for b in blocks])
+    x, lens_d = _prompt(lens, dtype), torch.tensor(lens, dtype=torch.int32, device="cuda")
+    for s in (stack, other):
+        s(x, first_cache=True, seq_lens=lens_d)
+    g = torch.Generator(device="cuda").manual_seed(5)
+    parents = [-1, 0, 1, 1] * B                              # two ways: 0 1 2 and 0 1 3
+    rows = torch.randn(B, 4, HID, generator=g, device="cuda", dtype=dtype)
+    tree = K.draft_tree(torch.tensor(parents, dtype=torch.int32, device="cuda"), [4] * B, B, 4)
+    announce("nodes of a stack", dtype, turn)
+    got = stack.forward_nodes(rows.view(1, -1, HID), tree).view(B, 4, HID)
+    want = [other(rows[:, i:i + 1], first_cache=False)[:, -1] for i in (0, 1, 3)]
+    # both round activations to 16 bits, in other orders of the same sums, through two blocks: a few steps of each
+    tol = 2 ** -8 if dtype == torch.float16 else 2 ** -5
+    for i, w in zip((0, 1, 3), want):
+        assert ((got[:, i] - w).abs() <= tol * (1 + w.abs())).all(), i
+    path = torch.tensor([[0, 1, 3, -1]] * B, dtype=torch.int32, device="cuda")
+    stack.accept_nodes(path, torch.full((B,), 3, dtype=torch.int32, device="cuda"))
+    for a, b in zip(stack.blocks, other.blocks):
+        assert a.attn.kv_cache.lens.tolist() == b.attn.kv_cache.lens.tolist() == [n + 3 for n in lens]
+        assert a.attn.kv_cache._host_lens == b.attn.kv_cache._host_lens
+    after = torch.randn(B, 1, HID, generator=g, device="cuda", dtype=dtype)
+    one = K.draft_tree(torch.full((B,), -1, dtype=torch.int32, device="cuda"), [1] * B, B, 1)
+    got, w = stack.forward_nodes(after.view(1, B, HID), one).view(B, HID), other(after, first_cache=False)[:, -1]
+    assert ((got - w).abs() <= tol * (1 + w.abs())).all()
+    # sequences of different counts, one of them with nothing
+    stack.accept_nodes(torch.zeros(B, 1, dtype=torch.int32, device="cuda"), torch.tensor([1, 0, 1], dtype=torch.int32, device="cuda"))
+    assert stack.blocks[0].attn.kv_cache.lens.tolist() == [n + 3 + m for n, m in zip(lens, (1, 0, 1))]
+
+
+@torch.no_grad()
+def test_refusals():
+    from energonai_amd import kernel as K
+    from energonai_amd.model import Block1D, PagedKVCache8
+    tree = K.draft_tree(torch.full((1,), -1, dtype=torch.int32, device="cuda"), [1], 1, 1)
+    x = torch.zeros(1, 1, HID, dtype=torch.float16, device="cuda")
+    b = _block(torch.float16)
+    with pytest.raises(RuntimeError, match="first_cache"):
+        b.forward_nodes(x, tree)
+    b(_prompt([5], torch.float16), first_cache=True)
+    with pytest.raises(RuntimeError, match="forward_nodes"):
+        b.accept_nodes(torch.zeros(1, 1, dtype=torch.int32, device="cuda"), torch.ones(1, dtype=torch.int32, device="cuda"))
+    whole = Block1D(HID, HEADS, 2, dtype=torch.float16, max_seq_len=64).cuda()
+    whole(_prompt([5], torch.float16), first_cache=True)
+    with pytest.raises(RuntimeError, match="kv_page_size"):
+        whole.forward_nodes(x, tree)
+    eight = Block1D(HID, HEADS, 2, dtype=torch.float16, max_seq_len=64, kv_cache_dtype=torch.int8).cuda()
+    eight(_prompt([5], torch.float16), first_cache=True)
+    assert type(eight.attn.kv_cache) is PagedKVCache8
+    with pytest.raises(RuntimeError, match="16-bit"):
+        eight.forward_nodes(x, tree)
+    # a pool that is used up keeps its lengths
+    b.forward_nodes(x, tree)
+    cache = b.attn.kv_cache
+    cache._free.clear()
+    cache._host_lens = [16]
+    with pytest.raises(RuntimeError, match="used up"):
+        b.accept_nodes(torch.zeros(1, 1, dtype=torch.int32, device="cuda"), torch.ones(1, dtype=torch.int32, device="cuda"))
+    assert cache.lens.tolist() == [5]
+
+
+@pytest.mark.parametrize("activation", [torch.nn.functional.relu, torch.nn.GELU(), torch.nn.GELU(approximate="tanh"), torch.nn.functional.silu])
+@pytest.mark.parametrize("zero_points", [False, True])
+@torch.no_grad()
+def test_block_with_weights_in_4_bits(activation, zero_points):
+    """A block whose projections are replaced gives, for prompts and steps, what a block gives whose weights are the rounded ones."""
+    from energonai_amd.model import Linear4, quantize_linears
+    dtype, lens = torch.float16, [9, 33]
+    plain = _block(dtype, activation=activation)
+    small = quantize_linears(copy.deepcopy(plain), 64, zero_points)
+    layers = [(n, m) for n, m in small.named_modules() if isinstance(m, Linear4)]
+    assert sorted(n for n, _ in layers) == ["attn.dense", "attn.query_key_value", "mlp.dense_1", "mlp.dense_2"]
+    announce("4-bit block", activation, zero_points)
+    for n, m in layers:
+        eye = torch.eye(m.in_features, dtype=dtype, device="cuda")
+        bias = m.bias
+        m.bias = None
+        plain.get_submodule(n).weight.copy_(m(eye).t())       # rounded to 16 bits
+        m.bias = bias
+    x, lens_d = _prompt(lens, dtype), torch.tensor(lens, dtype=torch.int32, device="cuda")
+    step = torch.randn(2, 1, HID, device="cuda", dtype=dtype)
+    for got, want in ((small(x, first_cache=True, seq_lens=lens_d), plain(x, first_cache=True, seq_lens=lens_d)), (small(step), plain(step))):
+        # both round activations and (the plain one) weights to fp16, in other orders of the same sums
+        assert ((got - want).abs() <= 2 ** -7 * (1 + want.abs())).all()
+    state = small.state_dict()
+    again = quantize_linears(copy.deepcopy(plain), 64, zero_points)
+    again.load_state_dict(state)
+    assert torch.equal(again(x, first_cache=True, seq_lens=lens_d), small(x, first_cache=True, seq_lens=lens_d))
