@@ -23,7 +23,7 @@ from . import _lib
 from .seqinfo import SeqInfo, seq_info
 
 
-# attn_pv reads a row of probabilities only as far as the row's own query sees, so the softmax writes no tail
+# attn_pv reads a row of probabilities only as far as the row's own query sees, so a softmax whose result stays inside a step writes no tail
 SOFTMAX_TAIL_ROWS = 1
 
 
@@ -119,8 +119,8 @@ def padding_removal_layer(hidden_padded: torch.Tensor, qkv_packed: torch.Tensor,
             if pk:
                 probs = scale_mask_softmax_packed(B, S, H, scores, info, scale=scale)
             else:
-                probs = scale_mask_softmax(B, S, H, scores, info, scale=scale, causal=causal,
-                                           tail_rows=SOFTMAX_TAIL_ROWS)
+                # probabilities that are handed out are the reference's: zeros behind what a row sees, not what the memory held
+                probs = scale_mask_softmax(B, S, H, scores, info, scale=scale, causal=causal, tail_rows=0)
             ctx_packed = attn_pv_varlen(probs, v, B, S, info, causal=causal, packed_scores=pk)
         attn_out = ctx_packed.view(1, T, H * D) if dense_out is None else dense_out
         y = layer_norm_forward(attn_out, gamma, beta, (hid,), eps, residual=x)
@@ -132,7 +132,7 @@ def padding_removal_layer(hidden_padded: torch.Tensor, qkv_packed: torch.Tensor,
         ctx = attn_fused(q, k, v, info, scale=scale, causal=causal)
     else:
         scores = attn_qk(q, k, info, causal=causal)
-        probs = scale_mask_softmax(B, S, H, scores, info, scale=scale, causal=causal, tail_rows=SOFTMAX_TAIL_ROWS)
+        probs = scale_mask_softmax(B, S, H, scores, info, scale=scale, causal=causal, tail_rows=0)
         ctx = attn_pv(probs, v, info, causal=causal)
     ctx_packed = transpose_depad(ctx, B, T, S, info, H, D)
     attn_out = ctx_packed.view(1, T, H * D) if dense_out is None else dense_out
