@@ -208,7 +208,7 @@ constexpr int kWalkWaves = 16;
 constexpr int64_t kAllBytes = 96ll << 20, kSliceBytes = 32 << 10;
 // Slices of a row where all rows are looked at first; 0: a row at a time, as the walk comes to it.
 inline int accept_slices(int64_t nodes, int64_t vocab, int es) {
-  if (nodes * vocab * es > kAllBytes) return 0;
+  if (nodes > kAllBytes / (vocab * es)) return 0;
   const int64_t n = ceil_div(vocab * es, kSliceBytes);
   return (int)(n < 1 ? 1 : n);
 }

@@ -997,7 +997,7 @@ PyObject *linear_w4(PyObject *const *a) {
   const int64_t rows = x->numel() / K;
   int64_t stride = K;
   if (!x->is_contiguous()) {
-    if (x->dim() != 2 || x->stride(1) != 1 || x->stride(0) < K || x->stride(0) % 8) Py_RETURN_NONE;
+    if (x->dim() != 2 || x->stride(1) != 1 || x->stride(0) < K || x->stride(0) % 8 || x->stride(0) > 1 << 21) Py_RETURN_NONE;
     stride = x->stride(0);
   }
   if (reinterpret_cast<uintptr_t>(x->data_ptr()) % 16) Py_RETURN_NONE;

@@ -636,7 +636,7 @@ extern "C" int en_decode_attn_tree(const void *q, const void *k_new, const void 
     if (!aligned_to(p, 16)) return EN_ERR_ALIGN;
   for (int i = 0; i < 6; ++i)
     if (strides[i] % 8 || c.strides[i] % 8) return EN_ERR_ALIGN;
-  if (c.page_size * c.strides[2] > (1 << 30) || c.page_size * c.strides[5] > (1 << 30)) return EN_ERR_SHAPE;      // 32-bit offsets in a page
+  if (c.strides[2] > (1 << 30) / c.page_size || c.strides[5] > (1 << 30) / c.page_size) return EN_ERR_SHAPE;      // 32-bit offsets in a page
   const int64_t capacity = (int64_t)c.max_pages_per_seq * c.page_size, rows = (int64_t)max_nodes * (q_heads / c.head_num), at_once = tree_rows(rows);
   TreeArgs a{};
   a.chunks = (int)ceil_div(rows, at_once);

@@ -141,7 +141,7 @@ def decode_attn_tree(q, k_new, v_new, k_pool, v_pool, kv_len_list, page_table, t
         raise RuntimeError(f"{who}: Datatype not implemented ({k_pool.dtype}); expected float16 or bfloat16")
     H, D, device = c.head_num, c.size_per_head, k_pool.device
     T, Hq = _node_rows(who, q, "q", None, None, D, k_pool).shape[:2]
-    if Hq < H or Hq % H:
+    if H < 1 or Hq < H or Hq % H:
         raise RuntimeError(f"{who}: q must have a multiple of the pools' {H} heads")
     for t, n in ((k_new, "k_new"), (v_new, "v_new")):
         _node_rows(who, t, n, T, H, D, k_pool)
@@ -221,7 +221,8 @@ def accept_drafts(logits, tokens, tree):
 def kv_pages_extend(k_new, v_new, k_pool, v_pool, kv_len_list, page_table, tree, path, counts, *, overflow: Optional[torch.Tensor] = None) -> None:
     """``kv_pages_append`` of the accepted nodes: the rows of nodes ``path[b, i]``, ``i < counts[b]``, of ``k_new`` and ``v_new`` ``[nodes, H, D]``
     (any token and head strides) become positions ``kv_len[b] + i`` of sequence ``b``.  The caller advances the lengths afterwards.  Entries of
-    ``path`` that name no node are passed over; a position that has no page in the pool is not written and counted in ``overflow``."""
+    ``path`` that name no node are passed over; a position that has no page in the pool is not written and counted in ``overflow``.  Up to 65535
+    sequences."""
     who = "kv_pages_extend"
     if type(tree) is DraftTree and _lib.front.kv_pages_extend(k_new, v_new, k_pool, v_pool, kv_len_list, page_table, tree, path, counts, overflow):
         return

@@ -15,6 +15,7 @@ from .. import _lib
 
 _TYPES = (torch.float16, torch.bfloat16)
 _GROUPS = (32, 64, 128)
+_FARTHEST = 1 << 21          # elements from row to row that en_linear_w4 takes
 _ACTIVATIONS = {None: 0, "none": 0, "relu": 1, "gelu_tanh": 2, "gelu": 3}
 
 
@@ -118,7 +119,8 @@ def w4_quantize(weight, group_size: int = 128, zero_points: bool = False) -> W4W
 
 def linear_w4(inputs, weight, bias=None, activation: Optional[str] = None):
     """``linear`` with a weight in 4 bits: ``act(inputs[..., din] @ W[dout, din]^T + bias)`` -> ``[..., dout]``, fp16 or bf16 as the weight's
-    scales are.  Sums are fp32; up to 64 rows no weight is rounded, from there on each is, to the inputs' type.  ``activation``: ``"relu"``, ``"gelu_tanh"`` or ``"gelu"``."""
+    scales are.  Sums are fp32; up to 64 rows no weight is rounded, from there on each is, to the inputs' type.  ``activation``: ``"relu"``, ``"gelu_tanh"`` or ``"gelu"``.  Up to
+    2^20 rows and 2^21 features.  Like the other operators of this package it is for inference: no gradient flows through it."""
     who = "linear_w4"
     if type(weight) is W4Weight and activation in _ACTIVATIONS:
         y = _lib.front.linear_w4(inputs, weight, bias, _ACTIVATIONS[activation])
@@ -135,7 +137,7 @@ def linear_w4(inputs, weight, bias=None, activation: Optional[str] = None):
         if bias.shape != (w.out_features,) or bias.dtype != inputs.dtype or bias.device != inputs.device:
             raise RuntimeError(f"{who}: bias must be [{w.out_features}] of the inputs' dtype on their device")
     x = inputs if inputs.dim() == 2 else inputs.reshape(-1, w.in_features)
-    if x.shape[0] > 1 and (x.stride(0) % 8 or x.stride(0) < w.in_features) or x.stride(1) != 1:
+    if x.shape[0] > 1 and (x.stride(0) % 8 or not w.in_features <= x.stride(0) <= _FARTHEST) or x.stride(1) != 1:
         x = x.contiguous()
     if x.data_ptr() % 16:
         x = x.clone(memory_format=torch.contiguous_format)

@@ -36,7 +36,7 @@ class MultiHeadAttention1D(nn.Module):
 
     # what is not there in a module saved before there was a choice
     rotary_dim, rotary_base, rotary_interleaved, qk_norm, kv_cache_dtype = 0, 10000.0, False, False, None
-    _nodes = None               # keys, values and tree of a step of drafted nodes, until they are accepted
+    _nodes = None               # a step of drafted nodes until they are accepted: keys, values, tree, the cache and its steps
 
     def __init__(self, hidden_size: int, num_heads: int, bias: bool = True, dtype: torch.dtype = torch.float16,
                  max_seq_len: int = 512, fused_qkv: bool = True, is_decoder: bool = True, disable_past_cache=False,
@@ -210,17 +210,23 @@ class MultiHeadAttention1D(nn.Module):
         T = x.numel() // self.hidden_size
         q, k, v, _ = self._project(x)
         if self.turned:
-            positions = torch.repeat_interleave(cache.lens, tree.info.lens, output_size=T) + tree.depths
+            # of a row's sequence, found in bounds whatever the offsets are
+            seq = torch.searchsorted(seq_info(tree.info, cache.batch_size, x.device).cu_seqlens[1:], torch.arange(T, dtype=torch.int32, device=x.device), right=True)
+            positions = cache.lens[seq.clamp(max=cache.batch_size - 1)] + tree.depths
             q, k = qk_norm_rotary(q, k, cache.batch_size, None, self._tables(x.device, cache.max_seq_len), positions=positions, **self._turn_how())
         ctx = cache.attend_nodes(q, k, v, tree, self.scaling)
-        self._nodes = (k, v, tree)
+        self._nodes = (k, v, tree, cache, cache.steps)
         return project(self.dense, ctx.view(1, T, self.hidden_size))
 
     def accept_nodes(self, path: torch.Tensor, counts: torch.Tensor, counts_host=None) -> None:
         """The accepted nodes of the last ``forward_nodes`` (``kernel.accept_drafts``) go into the cache (see ``PagedKVCache.extend``)."""
         if self._nodes is None:
             raise RuntimeError("accept_nodes before a forward_nodes call")
-        self.kv_cache.extend(*self._nodes, path, counts, counts_host)
+        *rows, cache, at = self._nodes
+        if cache is not self.kv_cache or cache.steps != at:
+            self._nodes = None
+            raise RuntimeError("accept_nodes: the cache has gone on since the forward_nodes call")
+        cache.extend(*rows, path, counts, counts_host)
         self._nodes = None
 
     def forward(self, hidden_states, attention_mask=None, first_cache=False, seq_lens=None):

@@ -98,6 +98,8 @@ class PagedKVCache:
     device: a sequence gets its next page when its host-side length reaches a page boundary (one small copy to the
     device, every ``page_size`` steps)."""
 
+    steps = 0               # fills, appends and extensions so far
+
     def __init__(self, batch_size: int, head_num: int, max_seq_len: int, size_per_head: int, dtype, device,
                  page_size: int = 64, pool_pages: Optional[int] = None):
         if page_size < 16 or page_size & (page_size - 1):
@@ -171,6 +173,7 @@ class PagedKVCache:
         self._fill_pages(k_src, v_src, bound, info, k_head_first, v_head_first)
         self.lens.copy_(info.lens)
         self._host_lens = lens_host
+        self.steps += 1
 
     def _fill_pages(self, k_src, v_src, bound: int, info: SeqInfo, k_head_first: int, v_head_first: int) -> None:
         kv_pages_fill(k_src, self.k, self.batch_size, bound, info, self.table, k_head_first)
@@ -190,6 +193,7 @@ class PagedKVCache:
 
     def appended(self) -> None:
         self._host_lens = [n + 1 for n in self._host_lens]
+        self.steps += 1
 
     def append(self, k_new: torch.Tensor, v_new: torch.Tensor) -> None:
         """One new ``[B,H,D]`` row per sequence; lengths advance by one (see ``prepare_append``)."""
@@ -226,6 +230,7 @@ class PagedKVCache:
         kv_pages_extend(k_new, v_new, self.k, self.v, self.info, self.table, tree, path, counts)
         self.lens.add_(counts)
         self._host_lens = [n + m for n, m in zip(self._host_lens, counts_host)]
+        self.steps += 1
 
 
 class PagedKVCache8(PagedKVCache):

@@ -568,7 +568,7 @@ int en_accept_drafts(const void *logits, int64_t logits_stride, int vocab, const
 /* The accepted nodes' keys and values into their pages: row cu_seqlens[b] + path[b, i] of k_new and v_new becomes position kv_lens[b] + i of
  * sequence b, i < min(counts[b], path_width).  Entries of path that are no node of the sequence are passed over; a position without a page in the pool
  * is not written and counted in overflow, if given.  strides: (token, head) in elements of k_new, v_new [nodes, head_num, size_per_head].
- * The caller advances the lengths afterwards. */
+ * Up to 65535 sequences.  The caller advances the lengths afterwards. */
 int en_kv_extend_paged(const void *k_new, const void *v_new, const int64_t *strides, const en_kv_pages *cache, const int32_t *kv_lens,
                        const int32_t *cu_seqlens, int64_t nodes, const int32_t *path, int path_width, const int32_t *counts,
                        int32_t *overflow, en_stream_t stream);
@@ -592,9 +592,10 @@ int64_t en_w4_groups(int64_t out_features, int64_t in_features, int group);
  * ceil(in_features / group)]; contiguous.  The results' pointers in `weight` are written through. */
 int en_w4_pack(const uint8_t *codes, const void *scales, const uint8_t *zeros, const en_w4_weight *weight, en_stream_t stream);
 /* y = act(x W^T + bias): x [rows, in_features], x_stride elements apart (a multiple of 8), 16-byte aligned; y contiguous [rows,
- * out_features]; bias [out_features] or NULL; activation an en_activation.  Sums are fp32; up to 64
- * rows no weight is rounded, from there on each is, to dtype, as a 16-bit weight would be.  workspace: en_linear_w4_workspace_bytes (may be
- * 0, then NULL), 16-byte aligned; its contents need not be kept or cleared, but calls that may run at the same time need one each. */
+ * out_features]; bias [out_features] or NULL; activation an en_activation.  Up to 2^20 rows, and 2^21 features or elements from row to row.  Sums
+ * are fp32; up to 64 rows no weight is rounded, from there on each is, to dtype, as a 16-bit weight would be.  A row of x that holds an infinity
+ * may give NaN where the formula has an infinity (zero points are taken off the sums).  workspace: en_linear_w4_workspace_bytes (may be 0, then
+ * NULL), 16-byte aligned; its contents need not be kept or cleared, but calls that may run at the same time need one each. */
 int64_t en_linear_w4_workspace_bytes(int64_t rows, int64_t out_features, int64_t in_features);
 int en_linear_w4(const void *x, int64_t rows, int64_t x_stride, const en_w4_weight *weight, const void *bias, int activation, void *y,
                  void *workspace, int64_t workspace_bytes, en_stream_t stream);

@@ -176,3 +176,15 @@ def test_codes_are_the_nearest():
 def test_restatement_of_masks():
     m, d = ref.masks([-1, 0, 0, 1, 5, -1, 0], [5, 2])
     assert m == [1, 3, 5, 11, 16, 1, 3] and d == [0, 1, 1, 2, 0, 0, 1]
+
+
+def test_sizes_past_64_bits_are_refused():
+    """Products of sizes that pass 64 bits: no workspace for them, and strides that would come round to a small offset."""
+    fn = _lib().fn
+    assert fn.en_accept_drafts_workspace_bytes((1 << 31) - 1, (1 << 31) - 1, 0) == 0
+    st = (ctypes.c_int64 * 6)(*(256, 64) * 3)
+    far = (1 << 18, 1 << 14, 1 << 61, 1 << 18, 1 << 14, 64)
+    c = _pages()
+    for strides in (far, far[3:] + far[:3]):
+        c.strides[:] = strides
+        assert fn.en_decode_attn_tree(PTR, PTR, PTR, st, PTR, ctypes.byref(c), PTR, PTR, PTR, 5, 4, 4 * c.head_num, 0.1, PTR, 1 << 40, None) == SHAPE

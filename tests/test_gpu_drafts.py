@@ -91,6 +91,107 @@ def test_attention(lens, counts, Hq, H, D, P, dtype):
     assert float(off.max()) <= 0, float(off.max())
 
 
+@pytest.mark.parametrize("B,H,Hq,longest,most", [(70, 2, 4, 700, 5), (150, 3, 3, 1300, 2), (130, 1, 17, 600, 9)])
+def test_batches_of_more_than_a_wave_of_sequences(B, H, Hq, longest, most):
+    """Runs of tiles over many sequences, among them ones without nodes, without positions, without either."""
+    r = random.Random(B)
+    counts = [r.choice([0, 1, most]) for _ in range(B - 1)] + [most]
+    lens = [r.choice([0, 1, 63, 64, r.randrange(200)]) for _ in range(B - 1)] + [longest - most]
+    counts[:2] = counts[66:68] = [0, 0]
+    D, P, dtype = 32, 64, torch.float16
+    announce("many sequences", B, H, Hq, longest, most)
+    q, k, v, kp, vp, table = step(lens, counts, Hq, H, D, P, dtype, B, table_pages=21)
+    assert K().decode_attn_tree_workspace_bytes(B, Hq, H, 21 * P, D, most) > 0
+    parents = trees(counts, B)
+    tree = K().draft_tree(torch.tensor(parents, dtype=torch.int32, device="cuda"), counts, B, most)
+    masks, _ = ref.masks(parents, counts)
+    want, size, top = ref.attend(q, k, v, kp, vp, lens, table, masks, counts)
+    got = run(q, k, v, kp, vp, lens, table, tree)
+    assert float(((got.double() - want).abs() - tolerance(want, size, top, dtype, D, longest + 64)).max()) <= 0
+
+
+def test_tables_without_pages():
+    """Sequences that hold nothing, in a table of no columns: the nodes see one another, and nothing has room."""
+    counts, H, D, P, dtype = [3, 1], 2, 64, 16, torch.bfloat16
+    q, k, v, kp, vp, _ = step([0, 0], counts, H, H, D, P, dtype, 3)
+    table = torch.empty(2, 0, dtype=torch.int32)
+    tree = K().draft_tree(torch.tensor([-1, 0, 0, -1], dtype=torch.int32, device="cuda"), counts, 2, 3)
+    announce("tables without pages")
+    for lens in ([0, 0], [5, 0]):                        # a length without pages counts as none
+        want, size, most = ref.attend(q, k, v, kp, vp, [0, 0], table, ref.masks([-1, 0, 0, -1], counts)[0], counts)
+        got = run(q, k, v, kp, vp, lens, table, tree)
+        assert float(((got.double() - want).abs() - tolerance(want, size, most, dtype, D, 64)).max()) <= 0
+    lost = torch.zeros(1, dtype=torch.int32, device="cuda")
+    kp_d, vp_d = torch.ones_like(kp).cuda(), torch.ones_like(vp).cuda()
+    path, taken = torch.tensor([[0, 1], [0, -1]], dtype=torch.int32, device="cuda"), torch.tensor([2, 1], dtype=torch.int32, device="cuda")
+    K().kv_pages_extend(k.cuda(), v.cuda(), kp_d, vp_d, torch.zeros(2, dtype=torch.int32, device="cuda"), table.cuda(), tree, path, taken, overflow=lost)
+    assert int(lost) == 3 and (kp_d == 1).all() and (vp_d == 1).all()
+
+
+@pytest.mark.parametrize("counts,most", [([20, 64, 5], 6), ([70, 3], 64), ([1, 2], 64)])
+def test_nodes_past_the_largest_do_not_exist(counts, most):
+    """Rows behind ``max_nodes`` nodes of a sequence keep what is in them, and no other node sees them."""
+    lens, Hq, H, D, P, dtype = [30, 7, 100][:len(counts)], 4, 2, 64, 16, torch.float16
+    q, k, v, kp, vp, table = step(lens, counts, Hq, H, D, P, dtype, most)
+    parents = trees(counts, most)
+    tree = K().draft_tree(torch.tensor(parents, dtype=torch.int32, device="cuda"), counts, len(counts), most)
+    masks, first, there = ref.masks(parents, counts)[0], 0, []
+    for n in counts:
+        there += [i < most for i in range(n)]
+        first += n
+    masks = [m & ((1 << most) - 1) if most < 64 else m for m in masks]
+    want, size, top = ref.attend(q, k, v, kp, vp, lens, table, masks, counts)
+    announce("nodes past the largest", counts, most)
+    out = torch.full((len(parents), Hq, D), 9.0, dtype=dtype, device="cuda")
+    got = run(q, k, v, kp, vp, lens, table, tree, out=out)
+    there = torch.tensor(there)
+    off = ((got.double() - want).abs() - tolerance(want, size, top, dtype, D, 164))[there]
+    assert float(off.max()) <= 0 and (got[~there] == 9).all()
+
+
+def test_pools_past_4_gib():
+    """Pages whose offsets pass 32 bits, read and written."""
+    H, D, P, dtype, counts, lens = 8, 128, 128, torch.float16, [3, 2], [300, 90]
+    N = (5 << 30) // (H * P * D * 2)
+    q, k, v, kp, vp, table = step(lens, counts, H, H, D, P, dtype, 4)
+    n = kp.shape[0]
+    parents = trees(counts, 1)
+    tree = K().draft_tree(torch.tensor(parents, dtype=torch.int32, device="cuda"), counts, 2, 3)
+    announce("pools past 4 GiB")
+    want = run(q, k, v, kp, vp, lens, table, tree)
+    pools = [torch.empty((N, H, P, D), dtype=dtype, device="cuda") for _ in range(2)]
+    for pool, small in zip(pools, (kp, vp)):
+        pool[N - n:].copy_(small)
+    far = torch.where(table >= 0, table + (N - n), table)
+    lens_d = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    assert torch.equal(K().decode_attn_tree(q.cuda(), k.cuda(), v.cuda(), *pools, lens_d, far.cuda(), tree).cpu(), want)
+    path, taken = torch.tensor([[0, 1, 2], [0, 1, -1]], dtype=torch.int32, device="cuda"), torch.tensor([3, 2], dtype=torch.int32, device="cuda")
+    K().kv_pages_extend(k.cuda(), v.cuda(), *pools, lens_d, far.cuda(), tree, path, taken)
+    for pool, small, new in zip(pools, (kp, vp), (k, v)):
+        assert torch.equal(pool[N - n:].cpu().nan_to_num(), ref.extend(small, new, lens, table, counts, path.cpu(), taken.cpu())[0].nan_to_num())
+
+
+def test_logits_past_4_gib():
+    """Rows of logits whose offsets pass 32 bits: the way of the last trees."""
+    B, n, V = 270, 64, 130000
+    logits = torch.zeros(B * n, V, dtype=torch.bfloat16, device="cuda")
+    assert logits.numel() * 2 > 1 << 32
+    parents = ([-1] + list(range(n - 1))) * B
+    tokens = torch.zeros(B * n, dtype=torch.int64)
+    for b in (0, B - 1):
+        for i in range(4):
+            logits[b * n + i, V - 1 - i] = 1
+            tokens[b * n + i + 1] = V - 1 - i
+    tokens[[n * b + 1 for b in range(1, B - 1)]] = 5           # not what their roots choose, the first of equal ones
+    tokens[[5, (B - 1) * n + 5]] = 1
+    announce("logits past 4 GiB")
+    tree = K().draft_tree(torch.tensor(parents, dtype=torch.int32, device="cuda"), [n] * B, B, n)
+    path, taken, following = (t.tolist() for t in K().accept_drafts(logits, tokens.cuda(), tree))
+    for b in range(B):
+        m = 5 if b in (0, B - 1) else 1
+        assert path[b] == list(range(m)) + [-1] * (n - m) and taken[b] == m and following[b] == 0
+
+
 @pytest.mark.parametrize("counts,reach", [([64], 64), ([64, 1, 0, 5], 1), ([70, 3], 3), ([1] * 40, 1)])
 def test_trees(counts, reach):
     announce("trees", counts)

@@ -94,6 +94,49 @@ def test_refusals():
     assert cache.lens.tolist() == [5]
 
 
+@torch.no_grad()
+def test_nodes_of_a_cache_that_has_gone_on_are_refused():
+    """Once the cache has taken in anything else, the rows of an earlier step of nodes do not belong behind it."""
+    from energonai_amd import kernel as K
+    tree = K.draft_tree(torch.tensor([-1, 0], dtype=torch.int32, device="cuda"), [2], 1, 2)
+    x, one = torch.randn(1, 2, HID, dtype=torch.float16, device="cuda"), torch.ones(1, dtype=torch.int32, device="cuda")
+    path = torch.tensor([[0, -1]], dtype=torch.int32, device="cuda")
+    announce("nodes of a cache that has gone on")
+    b = _block(torch.float16)
+    for between in (lambda: b(x[:, :1], first_cache=False), lambda: b(_prompt([9], torch.float16), first_cache=True),
+                    lambda: b.attn.kv_cache.extend(*b.attn._nodes[:3], path, one)):
+        b(_prompt([5], torch.float16), first_cache=True)
+        b.forward_nodes(x, tree)
+        between()
+        lens = b.attn.kv_cache.lens.tolist()
+        with pytest.raises(RuntimeError, match="gone on"):
+            b.accept_nodes(path, one)
+        assert b.attn.kv_cache.lens.tolist() == lens
+        with pytest.raises(RuntimeError, match="forward_nodes"):
+            b.accept_nodes(path, one)
+    # the nodes may be gone over again, and finished sequences released
+    b.forward_nodes(x, tree)
+    b.forward_nodes(x, tree)
+    b.attn.kv_cache.release(0)
+    b.accept_nodes(path, torch.zeros_like(one))
+    assert b.attn.kv_cache.lens.tolist() == [0]
+
+
+@torch.no_grad()
+def test_rotated_nodes_whose_counts_say_more_than_there_is():
+    """Offsets past the rows of a call: every row of it has its own sequence's position, and nothing past them is written."""
+    from energonai_amd import kernel as K
+    from energonai_amd.seqinfo import build_seq_info
+    b = _block(torch.float16, rotary_dim=32)
+    b(_prompt([5, 9], torch.float16), first_cache=True, seq_lens=torch.tensor([5, 9], dtype=torch.int32, device="cuda"))
+    x = torch.randn(1, 3, HID, dtype=torch.float16, device="cuda")
+    parents = torch.tensor([-1, 0, -1], dtype=torch.int32, device="cuda")
+    announce("counts past the rows")
+    got = b.forward_nodes(x, K.draft_tree(parents, build_seq_info([2, 60], 2), 2, 64))
+    want = b.forward_nodes(x, K.draft_tree(parents, [2, 1], 2, 64))
+    assert torch.equal(got, want)
+
+
 @pytest.mark.parametrize("activation", [torch.nn.functional.relu, torch.nn.GELU(), torch.nn.GELU(approximate="tanh"), torch.nn.functional.silu])
 @pytest.mark.parametrize("zero_points", [False, True])
 @torch.no_grad()

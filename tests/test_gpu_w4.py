@@ -118,6 +118,35 @@ def test_results_do_not_change_from_call_to_call():
             assert torch.equal(K().linear_w4(x, w), first)
 
 
+def test_codes_past_4_gib():
+    """Codes whose offsets pass 32 bits: a weight of equal rows, whose products are equal too.  (Scales are above 2^-14 here, and so is what is
+    rounded.)"""
+    N, Kd, dtype = 4112, 1 << 21, torch.float16
+    codes, scales, z = weight(16, Kd, 128, dtype, False, 4)
+    w = K().w4_weight(codes.cuda().repeat(N // 16, 1), scales.cuda().repeat(N // 16, 1), group_size=128)
+    assert w.codes.numel() > 1 << 32
+    x = torch.randn(130, Kd, generator=torch.Generator().manual_seed(2)).to(dtype)
+    want, size = ref.w4_linear(x[:1], codes, scales, z, 128)
+    for rows in (1, 20, 130):
+        announce("codes past 4 GiB", rows)
+        got = K().linear_w4(x[:rows].cuda(), w).cpu()
+        assert torch.equal(got.view(rows, -1, 16), got[:, :16].view(rows, 1, 16).expand(-1, N // 16, -1))
+        rounded = x[:1].double().abs() @ ref.w4_values(codes, scales, z, 128)[0].abs().t() if rows > MANY else None
+        assert ((got[:1, :16].double() - want).abs() <= tolerance(want, size, dtype, Kd, None, rounded)).all()
+
+
+def test_rows_far_apart():
+    """Rows of a view of any stride, among them those farther apart than the kernels take."""
+    N, Kd, dtype = 40, 64, torch.bfloat16
+    codes, scales, z = weight(N, Kd, 32, dtype, True, 8)
+    w = K().w4_weight(codes.cuda(), scales.cuda(), z.cuda(), group_size=32)
+    for rows, apart in ((3, 1 << 21), (3, (1 << 21) + 8), (300, 1 << 21), (2, 1 << 24), (5, 0)):
+        x = torch.zeros(rows * apart + Kd, dtype=dtype, device="cuda").as_strided((rows, Kd), (apart, 1))
+        x.copy_(torch.randn(1 if apart == 0 else rows, Kd, generator=torch.Generator().manual_seed(9)).to(dtype)) if apart else x[0].copy_(torch.randn(Kd).to(dtype))
+        announce("w4 rows far apart", rows, apart)
+        assert torch.equal(K().linear_w4(x, w), K().linear_w4(x.contiguous(), w))
+
+
 @pytest.mark.parametrize("zero_points", [False, True])
 def test_quantized_weight(zero_points):
     announce("w4 quantize", zero_points)
