@@ -119,30 +119,32 @@ struct W4Args {
   float *part;                    // [runs][R][16 tiles] sums, or null
 };
 
-// Loads of a row of tiles: codes, scales and zero points of a lane for matrix operands (all groups of four rows of W), by step.  Steps past
-// the end arrive as zeros, whose products are zeros.
+// Loads of `count` tiles of W that follow `tile`: codes, scales and zero points of a lane for matrix operands (all groups of four rows of W), by
+// step.
 template <typename T, int GROUPS> struct W4Tiles {
   rsrc_t codes, scales, zeros;
-  __device__ __forceinline__ W4Tiles(const W4Args &a, int tile, int steps) {
-    const int64_t first = (int64_t)min(tile, a.tiles - 1) * a.steps;
+  __device__ __forceinline__ W4Tiles(const W4Args &a, int tile, int count) {
+    const int64_t first = (int64_t)tile * a.steps;
+    const uint32_t steps = count * a.steps;
     codes = make_rsrc(a.codes + first * kWave, steps * 1024);
     scales = make_rsrc(reinterpret_cast<const T *>(a.scales) + first * 16 * GROUPS, steps * 32 * GROUPS);
     zeros = make_rsrc(a.zeros + first * 16 * GROUPS, a.zeros ? steps * 16 * GROUPS : 0);
   }
 };
-template <int BYTES, int AUX> __device__ __forceinline__ Pack<uint8_t, BYTES> w4_load(rsrc_t r, uint32_t at) {
+// `base` is the same for the whole wave.
+template <int BYTES, int AUX> __device__ __forceinline__ Pack<uint8_t, BYTES> w4_load(rsrc_t r, uint32_t at, uint32_t base = 0) {
   if constexpr (BYTES == 32) {
     Pack<uint8_t, 32> both;
-    const uint4 lo = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(r, (int)at, 0, AUX)),
-                hi = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(r, (int)at + 16, 0, AUX));
+    const uint4 lo = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(r, (int)at, (int)base, AUX)),
+                hi = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(r, (int)at + 16, (int)base, AUX));
     __builtin_memcpy(&both, &lo, 16);
     __builtin_memcpy(both.v + 16, &hi, 16);
     return both;
-  } else if constexpr (BYTES == 16) return __builtin_bit_cast(Pack<uint8_t, 16>, __builtin_amdgcn_raw_buffer_load_b128(r, (int)at, 0, AUX));
-  else if constexpr (BYTES == 8) return __builtin_bit_cast(Pack<uint8_t, 8>, __builtin_amdgcn_raw_buffer_load_b64(r, (int)at, 0, AUX));
-  else if constexpr (BYTES == 4) return __builtin_bit_cast(Pack<uint8_t, 4>, __builtin_amdgcn_raw_buffer_load_b32(r, (int)at, 0, AUX));
-  else if constexpr (BYTES == 2) return __builtin_bit_cast(Pack<uint8_t, 2>, __builtin_amdgcn_raw_buffer_load_b16(r, (int)at, 0, AUX));
-  else return Pack<uint8_t, 1>{{__builtin_amdgcn_raw_buffer_load_b8(r, (int)at, 0, AUX)}};
+  } else if constexpr (BYTES == 16) return __builtin_bit_cast(Pack<uint8_t, 16>, __builtin_amdgcn_raw_buffer_load_b128(r, (int)at, (int)base, AUX));
+  else if constexpr (BYTES == 8) return __builtin_bit_cast(Pack<uint8_t, 8>, __builtin_amdgcn_raw_buffer_load_b64(r, (int)at, (int)base, AUX));
+  else if constexpr (BYTES == 4) return __builtin_bit_cast(Pack<uint8_t, 4>, __builtin_amdgcn_raw_buffer_load_b32(r, (int)at, (int)base, AUX));
+  else if constexpr (BYTES == 2) return __builtin_bit_cast(Pack<uint8_t, 2>, __builtin_amdgcn_raw_buffer_load_b16(r, (int)at, (int)base, AUX));
+  else return Pack<uint8_t, 1>{{__builtin_amdgcn_raw_buffer_load_b8(r, (int)at, (int)base, AUX)}};
 }
 
 // The NW waves of a workgroup share the channels of CT tiles of W and 16 RT rows of x.
@@ -152,7 +154,8 @@ __global__ __launch_bounds__(NW *kWave) void w4_rows_kernel(W4Args a) {
   typedef typename E::T T;
   constexpr int kGroups = kTileCols / GROUP, kPer = GROUP / 32;       // groups of a step, matrix instructions of a group
   constexpr int kAtOnce = CT < 4 ? CT : GROUP > 32 && RT == 1 ? 4 : GROUP > 32 || RT < 3 ? 2 : 1;      // tiles of W whose sums are under way
-  __shared__ __align__(16) float s_acc[NW][RT * CT][kWave][4];
+  constexpr int kMeet = CT < 4 ? CT : 4;                              // tiles of W whose sums meet in LDS at once
+  __shared__ __align__(16) float s_acc[NW][RT * kMeet][kWave][4];
   const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), j = lane % 16, g = lane / 16;
   const int t0 = blockIdx.x * CT, r0 = blockIdx.y * 16 * RT;
   // rows past R and channels past K arrive as zeros
@@ -166,19 +169,20 @@ __global__ __launch_bounds__(NW *kWave) void w4_rows_kernel(W4Args a) {
   const uint4 ones = make_uint4(one, one, one, one);
   typedef W4Tiles<T, kGroups> Tiles;
   const int begin = blockIdx.z * a.per, end = min(begin + a.per, a.steps), channels = min(a.K, end * kTileCols);
-  auto tiles = [&](int c) { return Tiles(a, t0 + c, end); };
-  const Tiles tile0 = tiles(0), tile1 = tiles(CT > 1 ? 1 : 0), tile2 = tiles(CT > 2 ? 2 : 0), tile3 = tiles(CT > 3 ? 3 : 0);
+  const int last = min(CT, a.tiles - t0) - 1;  // tiles past the last one are the last one, and not stored
+  const Tiles tile(a, t0, last + 1);
 
   uint4 w[CT], x[RT][4];
   Pack<T, 4 * kGroups> sc[CT];
   Pack<uint8_t, 4 * kGroups> ze[CT];
   auto fetch = [&](int step) {
+    const uint32_t none = step < end ? 0u : kOutOfRange;      // nothing is read past the run
 #pragma unroll
     for (int c = 0; c < CT; ++c) {
-      const Tiles &t = c == 0 ? tile0 : c == 1 ? tile1 : c == 2 ? tile2 : tile3;
-      w[c] = __builtin_bit_cast(uint4, w4_load<16, 2>(t.codes, (step * kWave + lane) * 16));
-      sc[c] = __builtin_bit_cast(Pack<T, 4 * kGroups>, w4_load<8 * kGroups, 0>(t.scales, (step * 4 + g) * 8 * kGroups));
-      ze[c] = w4_load<4 * kGroups, 0>(t.zeros, (step * 4 + g) * 4 * kGroups);
+      const uint32_t from = min(c, last) * a.steps;
+      w[c] = __builtin_bit_cast(uint4, w4_load<16, 2>(tile.codes, (step * kWave + lane) * 16 | none, from * 1024));
+      sc[c] = __builtin_bit_cast(Pack<T, 4 * kGroups>, w4_load<8 * kGroups, 0>(tile.scales, (step * 4 + g) * 8 * kGroups | none, from * 32 * kGroups));
+      ze[c] = w4_load<4 * kGroups, 0>(tile.zeros, (step * 4 + g) * 4 * kGroups | none, from * 16 * kGroups);
     }
     const int left = channels - step * kTileCols - g * 8;
 #pragma unroll
@@ -235,28 +239,32 @@ __global__ __launch_bounds__(NW *kWave) void w4_rows_kernel(W4Args a) {
     fetch(step + NW);
   }
 #pragma unroll
-  for (int t = 0; t < RT; ++t)
+  for (int c0 = 0; c0 < CT; c0 += kMeet) {
+    if (c0 > 0) __syncthreads();               // those before have been read
 #pragma unroll
-    for (int c = 0; c < CT; ++c) *reinterpret_cast<f32x4 *>(s_acc[wave][t * CT + c][lane]) = acc[t][c];
-  __syncthreads();
-  // lane (j, g) has rows 4g .. 4g + 3 of W, which are neighbours in y, of row j of x
-  for (int tc = wave; tc < RT * CT; tc += NW) {
-    const int t = tc / CT, c = tc % CT, r = r0 + t * 16 + j, n = (t0 + c) * kTileRows + 4 * g;
-    if (r >= a.R || n >= a.N) continue;
-    f32x4 v = {0.f, 0.f, 0.f, 0.f};
+    for (int t = 0; t < RT; ++t)
 #pragma unroll
-    for (int k = 0; k < NW; ++k) v += *reinterpret_cast<const f32x4 *>(s_acc[k][tc][lane]);
-    if (a.part) {
-      *reinterpret_cast<f32x4 *>(a.part + ((int64_t)blockIdx.z * a.R + r) * (a.tiles * kTileRows) + n) = v;
-      continue;
+      for (int c = 0; c < kMeet; ++c) *reinterpret_cast<f32x4 *>(s_acc[wave][t * kMeet + c][lane]) = acc[t][c0 + c];
+    __syncthreads();
+    // lane (j, g) has rows 4g .. 4g + 3 of W, which are neighbours in y, of row j of x
+    for (int tc = wave; tc < RT * kMeet; tc += NW) {
+      const int t = tc / kMeet, c = c0 + tc % kMeet, r = r0 + t * 16 + j, n = (t0 + c) * kTileRows + 4 * g;
+      if (r >= a.R || n >= a.N) continue;
+      f32x4 v = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int k = 0; k < NW; ++k) v += *reinterpret_cast<const f32x4 *>(s_acc[k][tc][lane]);
+      if (a.part) {
+        *reinterpret_cast<f32x4 *>(a.part + ((int64_t)blockIdx.z * a.R + r) * (a.tiles * kTileRows) + n) = v;
+        continue;
+      }
+      Pack<T, 4> y;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float bias = a.bias && n + e < a.N ? E::to_float(reinterpret_cast<const T *>(a.bias)[n + e]) : 0.f;
+        y.v[e] = E::from_float(w4_activate(v[e] + bias, a.act));
+      }
+      w4_store(reinterpret_cast<T *>(a.y) + (int64_t)r * a.N + n, y, a.N - n);
     }
-    Pack<T, 4> y;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const float bias = a.bias && n + e < a.N ? E::to_float(reinterpret_cast<const T *>(a.bias)[n + e]) : 0.f;
-      y.v[e] = E::from_float(w4_activate(v[e] + bias, a.act));
-    }
-    w4_store(reinterpret_cast<T *>(a.y) + (int64_t)r * a.N + n, y, a.N - n);
   }
 }
 
@@ -278,6 +286,13 @@ template <int DT> __global__ __launch_bounds__(kBlock) void w4_join_kernel(W4Arg
   }
   w4_store(reinterpret_cast<T *>(a.y) + (int64_t)r * a.N + n, y, a.N - n);
 }
+
+// Sixteen rows of x by 32 channels, one matrix operand: lane l loads vector `operand_vector` of row l / 4, so that four neighbours read 64
+// bytes of a row (a lane its own operand's 16 bytes, rows in turn, takes four times the accesses of the first-level cache), and the vectors
+// lie in LDS in the lanes' order; a lane's operand, row l % 16 and vector l / 16, is at `operand_slot`.  Vectors go round by one every four
+// rows, so that 16 lanes that read one vector of 16 rows meet all banks.
+__device__ __forceinline__ int operand_vector(int lane) { return (lane + lane / 16) % 4; }
+__device__ __forceinline__ int operand_slot(int lane) { return lane % 16 * 4 + (lane / 16 + 4 - lane % 16 / 4) % 4; }
 
 // ---- more rows ---------------------------------------------------------------------------------------------------------------------------
 
@@ -372,7 +387,7 @@ __global__ __launch_bounds__(S::NW *kWave, 2) void w4_tile_kernel(W4Args a) {
   rsrc_t code_rsrc[WT], scale_rsrc[WT], zero_rsrc[WT];
 #pragma unroll
   for (int t = 0; t < WT; ++t) {
-    const W4Tiles<T, kGroups> tiles(a, t0 + WT * wave + t, a.steps);
+    const W4Tiles<T, kGroups> tiles(a, min(t0 + WT * wave + t, a.tiles - 1), 1);
     code_rsrc[t] = tiles.codes;
     scale_rsrc[t] = tiles.scales;
     zero_rsrc[t] = tiles.zeros;
@@ -506,7 +521,7 @@ __global__ __launch_bounds__(kManyWaves *kWave, 2) void w4_many_kernel(W4Args a)
   uint32_t xrow[2];
 #pragma unroll
   for (int t = 0; t < 2; ++t) {
-    const int r = (2 * wave + t) * 16 + j;
+    const int r = (2 * wave + t) * 16 + lane / 4;
     xrow[t] = r < rows ? (uint32_t)((int64_t)r * a.x_stride * 2) : kOutOfRange;
   }
   const uint32_t lds0 = lds_address(s_mem);
@@ -515,7 +530,7 @@ __global__ __launch_bounds__(kManyWaves *kWave, 2) void w4_many_kernel(W4Args a)
     for (int t = 0; t < 2; ++t)
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
-        const int k = stage * 64 + half * 32 + g * 8;
+        const int k = stage * 64 + half * 32 + operand_vector(lane) * 8;
         buffer_load16_to_lds(x_desc, lds0 + buf * kXStage + ((2 * wave + t) * 2 + half) * 1024,
                              (xrow[t] + (uint32_t)k * 2u) | (xrow[t] & kOutOfRange) | (k < a.K ? 0u : kOutOfRange));
       }
@@ -587,7 +602,7 @@ __global__ __launch_bounds__(kManyWaves *kWave, 2) void w4_many_kernel(W4Args a)
     for (int c = 0; c < CT; ++c) acc[t][c] = f32x4{0.f, 0.f, 0.f, 0.f};
   // A stage's products, and between them, while the matrix instructions run, the pieces of the next stage's weights.
   auto multiply = [&](int xbuf, int buf, auto more, int part) {
-    const char *xs = s_mem + xbuf * kXStage + wr * RT * 2048 + lane * 16, *ws = s_mem + kW + buf * kWStage + wc * CT * 2048 + lane * 16;
+    const char *xs = s_mem + xbuf * kXStage + wr * RT * 2048 + operand_slot(lane) * 16, *ws = s_mem + kW + buf * kWStage + wc * CT * 2048 + lane * 16;
     uint4 w[CT], x[2];
 #pragma unroll
     for (int c = 0; c < CT; ++c) w[c] = *reinterpret_cast<const uint4 *>(ws + c * 2048);
