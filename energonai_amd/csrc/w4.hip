@@ -6,8 +6,12 @@
 // A byte of 0 .. 15 is, read as e4m3, that number times 2^-9 (the subnormal numbers and the first binade go in equal steps), so two
 // masks and four conversions with a scale of 2^9 make eight 16-bit numbers, exactly.
 //
-// The products are of codes as they are; a group's sum, in fp32, is then scale * (sum of code x - zero * sum of x), with the sums of x from a
-// matrix instruction whose other operand is ones.  No weight is rounded.
+// Up to 64 rows the products are of codes as they are; a group's sum, in fp32, is then scale * (sum of code x - zero * sum of x), with the
+// sums of x from a matrix instruction whose other operand is ones, and no weight is rounded.  For more rows, whose products are bound by the
+// matrix instructions, weights are turned into 16 bits once for all rows of a workgroup (below).
+//
+// us, groups of 128, bf16: 1 x 9216 -> 9216 16.2 (44 MB, 2.7 TB/s), 1 x 7168 -> 28672 25 (106 MB, 4.3 TB/s), 40 x 9216 -> 9216 26;
+// 1000 x 9216 -> 9216 218 (0.78 PFLOP/s), 512 rows of the same 172 (0.51 PFLOP/s: 288 tiles on 256 compute units).
 #include <type_traits>
 #include <utility>
 
@@ -147,15 +151,28 @@ template <int BYTES, int AUX> __device__ __forceinline__ Pack<uint8_t, BYTES> w4
   else return Pack<uint8_t, 1>{{__builtin_amdgcn_raw_buffer_load_b8(r, (int)at, (int)base, AUX)}};
 }
 
-// The NW waves of a workgroup share the channels of CT tiles of W and 16 RT rows of x.
-template <int DT, int GROUP, int RT, int CT, int NW>
-__global__ __launch_bounds__(NW *kWave) void w4_rows_kernel(W4Args a) {
+// Sixteen rows of x by 32 channels, one matrix operand: lane l loads vector `operand_vector` of row l / 4, so that four neighbours read 64
+// bytes of a row (a lane its own operand's 16 bytes, rows in turn, takes four times the accesses of the first-level cache: 40 x 9216 -> 9216 30 us, so 26), and the vectors
+// lie in LDS in the lanes' order; a lane's operand, row l % 16 and vector l / 16, is at `operand_slot`.  Vectors go round by one every four
+// rows, so that 16 lanes that read one vector of 16 rows meet all banks.
+__device__ __forceinline__ int operand_vector(int lane) { return (lane + lane / 16) % 4; }
+__device__ __forceinline__ int operand_slot(int lane) { return lane % 16 * 4 + (lane / 16 + 4 - lane % 16 / 4) % 4; }
+
+// The NW waves of a workgroup share the channels of CT tiles of W and 16 RT rows of x, a step of 128 channels each in turn, and their sums
+// meet in LDS in the end.  x goes through a wave's own part of LDS (see operand_vector); DIRECT: into registers as operands lie, for
+// rows that are so few that most lanes of an operand load nothing.  The next step's x is on its way while this one is multiplied; its codes
+// are asked for after that, which leaves the registers to a second wave a SIMD (codes ahead as well: 40 x 9216 -> 9216 26 -> 34 us).  With
+// 64 rows two waves a SIMD are worth 20 registers in scratch (64 x 9216 -> 9216 42.1 -> 36.7 us; groups of 64 spill twice as many, 47 -> 56).
+template <int DT, int GROUP, int RT, int CT, int NW, bool DIRECT>
+__global__ __launch_bounds__(NW *kWave, RT == 4 && GROUP == 128 ? 2 : 1) void w4_rows_kernel(W4Args a) {
   typedef Elem<DT> E;
   typedef typename E::T T;
   constexpr int kGroups = kTileCols / GROUP, kPer = GROUP / 32;       // groups of a step, matrix instructions of a group
   constexpr int kAtOnce = CT < 4 ? CT : GROUP > 32 && RT == 1 ? 4 : GROUP > 32 || RT < 3 ? 2 : 1;      // tiles of W whose sums are under way
   constexpr int kMeet = CT < 4 ? CT : 4;                              // tiles of W whose sums meet in LDS at once
-  __shared__ __align__(16) float s_acc[NW][RT * kMeet][kWave][4];
+  constexpr int kWords = CT < 4 && RT > 1 ? 2 : 4;                    // operands of a step that are in LDS at once
+  constexpr int kSlots = RT * (kMeet > kWords || DIRECT ? kMeet : kWords);
+  __shared__ __align__(16) float s_mem[NW][kSlots][kWave][4];         // a wave's own: operands of x, in the end its sums
   const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), j = lane % 16, g = lane / 16;
   const int t0 = blockIdx.x * CT, r0 = blockIdx.y * 16 * RT;
   // rows past R and channels past K arrive as zeros
@@ -163,8 +180,9 @@ __global__ __launch_bounds__(NW *kWave) void w4_rows_kernel(W4Args a) {
   const int rows = min(16 * RT, a.R - r0);
   const rsrc_t x_rsrc = make_rsrc(x0, (uint32_t)(((rows - 1) * a.x_stride + a.K) * 2));
   uint32_t xrow[RT];
+  const int x_row = DIRECT ? j : lane / 4, x_vector = DIRECT ? g : operand_vector(lane);
 #pragma unroll
-  for (int t = 0; t < RT; ++t) xrow[t] = t * 16 + j < rows ? (uint32_t)((t * 16 + j) * a.x_stride * 2) + g * 16 : kOutOfRange;
+  for (int t = 0; t < RT; ++t) xrow[t] = t * 16 + x_row < rows ? (uint32_t)((t * 16 + x_row) * a.x_stride * 2) + x_vector * 16 : kOutOfRange;
   const uint32_t one = DT == EN_F16 ? 0x3c003c00u : 0x3f803f80u;
   const uint4 ones = make_uint4(one, one, one, one);
   typedef W4Tiles<T, kGroups> Tiles;
@@ -175,7 +193,7 @@ __global__ __launch_bounds__(NW *kWave) void w4_rows_kernel(W4Args a) {
   uint4 w[CT], x[RT][4];
   Pack<T, 4 * kGroups> sc[CT];
   Pack<uint8_t, 4 * kGroups> ze[CT];
-  auto fetch = [&](int step) {
+  auto fetch_w = [&](int step) {
     const uint32_t none = step < end ? 0u : kOutOfRange;      // nothing is read past the run
 #pragma unroll
     for (int c = 0; c < CT; ++c) {
@@ -184,12 +202,27 @@ __global__ __launch_bounds__(NW *kWave) void w4_rows_kernel(W4Args a) {
       sc[c] = __builtin_bit_cast(Pack<T, 4 * kGroups>, w4_load<8 * kGroups, 0>(tile.scales, (step * 4 + g) * 8 * kGroups | none, from * 32 * kGroups));
       ze[c] = w4_load<4 * kGroups, 0>(tile.zeros, (step * 4 + g) * 4 * kGroups | none, from * 16 * kGroups);
     }
-    const int left = channels - step * kTileCols - g * 8;
+  };
+  auto fetch_x = [&](int step) {
+    const int left = channels - step * kTileCols - x_vector * 8;
 #pragma unroll
     for (int i = 0; i < 4; ++i)
 #pragma unroll
       for (int t = 0; t < RT; ++t)
         x[t][i] = buffer_load16(x_rsrc, (xrow[t] + (uint32_t)(step * 256 + i * 64)) | (xrow[t] & kOutOfRange) | (i * 32 < left ? 0u : kOutOfRange));
+  };
+  auto own_lds = [] {                          // one wave: its LDS accesses are in order
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+  };
+  auto put_x = [&](int from) {
+    own_lds();
+#pragma unroll
+    for (int i = 0; i < kWords; ++i)
+#pragma unroll
+      for (int t = 0; t < RT; ++t) *reinterpret_cast<uint4 *>(s_mem[wave][t * kWords + i][lane]) = x[t][from + i];
+    own_lds();
   };
 
   f32x4 acc[RT][CT];
@@ -197,46 +230,62 @@ __global__ __launch_bounds__(NW *kWave) void w4_rows_kernel(W4Args a) {
   for (int t = 0; t < RT; ++t)
 #pragma unroll
     for (int c = 0; c < CT; ++c) acc[t][c] = f32x4{0.f, 0.f, 0.f, 0.f};
-  fetch(begin + wave);
+  fetch_x(begin + wave);
+  fetch_w(begin + wave);
+  const int slot = operand_slot(lane);
   for (int step = begin + wave; step < end; step += NW) {
+    if constexpr (!DIRECT) {
+      put_x(0);
+      if (kWords == 4) fetch_x(step + NW);
+    }
 #pragma unroll
-      for (int i = 0; i < kGroups; ++i) {
-        // products of independent sums follow one another: each waits for the one before it of its own
-        f32x4 sum[RT];
+    for (int i = 0; i < kGroups; ++i) {
+      // products of independent sums follow one another: each waits for the one before it of its own
+      uint4 operand[RT][kPer];
+      f32x4 sum[RT];
 #pragma unroll
-        for (int t = 0; t < RT; ++t) sum[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+      for (int t = 0; t < RT; ++t) sum[t] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int c0 = 0; c0 < CT; c0 += kAtOnce) {
-          f32x4 p[kAtOnce][RT];
+      for (int c0 = 0; c0 < CT; c0 += kAtOnce) {
+        f32x4 p[kAtOnce][RT];
 #pragma unroll
-          for (int c = 0; c < kAtOnce; ++c)
+        for (int c = 0; c < kAtOnce; ++c)
 #pragma unroll
-            for (int t = 0; t < RT; ++t) p[c][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+          for (int t = 0; t < RT; ++t) p[c][t] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-          for (int k = 0; k < kPer; ++k) {
-            const int word = i * kPer + k;
-            if (c0 == 0)
+        for (int k = 0; k < kPer; ++k) {
+          const int word = i * kPer + k;
+          if (c0 == 0) {
+            if (!DIRECT && kWords < 4 && word == kWords) {
+              put_x(kWords);
+              fetch_x(step + NW);
+            }
 #pragma unroll
-              for (int t = 0; t < RT; ++t) sum[t] = mma<DT>(ones, x[t][word], sum[t]);
-#pragma unroll
-            for (int c = 0; c < kAtOnce; ++c) {
-              const uint4 all = w[c0 + c], wide = widen<DT>(word == 0 ? all.x : word == 1 ? all.y : word == 2 ? all.z : all.w);
-#pragma unroll
-              for (int t = 0; t < RT; ++t) p[c][t] = mma<DT>(wide, x[t][word], p[c][t]);
+            for (int t = 0; t < RT; ++t) {
+              operand[t][k] = DIRECT ? x[t][word] : *reinterpret_cast<const uint4 *>(s_mem[wave][t * kWords + word % kWords][slot]);
+              sum[t] = mma<DT>(ones, operand[t][k], sum[t]);
             }
           }
 #pragma unroll
-          for (int c = 0; c < kAtOnce; ++c)
+          for (int c = 0; c < kAtOnce; ++c) {
+            const uint4 all = w[c0 + c], wide = widen<DT>(word == 0 ? all.x : word == 1 ? all.y : word == 2 ? all.z : all.w);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const float scale = E::to_float(sc[c0 + c].v[e * kGroups + i]), zero = a.zeros ? (float)ze[c0 + c].v[e * kGroups + i] : 8.f;
-#pragma unroll
-              for (int t = 0; t < RT; ++t) acc[t][c0 + c][e] += scale * (p[c][t][e] - zero * sum[t][e]);
-            }
-          if constexpr (GROUP == 32) __builtin_amdgcn_sched_barrier(0);      // a group's scales at a time in fp32
+            for (int t = 0; t < RT; ++t) p[c][t] = mma<DT>(wide, operand[t][k], p[c][t]);
+          }
         }
+#pragma unroll
+        for (int c = 0; c < kAtOnce; ++c)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float scale = E::to_float(sc[c0 + c].v[e * kGroups + i]), zero = a.zeros ? (float)ze[c0 + c].v[e * kGroups + i] : 8.f;
+#pragma unroll
+            for (int t = 0; t < RT; ++t) acc[t][c0 + c][e] += scale * (p[c][t][e] - zero * sum[t][e]);
+          }
+        if constexpr (GROUP == 32) __builtin_amdgcn_sched_barrier(0);      // a group's scales at a time in fp32
       }
-    fetch(step + NW);
+    }
+    if constexpr (DIRECT) fetch_x(step + NW);
+    fetch_w(step + NW);
   }
 #pragma unroll
   for (int c0 = 0; c0 < CT; c0 += kMeet) {
@@ -244,7 +293,7 @@ __global__ __launch_bounds__(NW *kWave) void w4_rows_kernel(W4Args a) {
 #pragma unroll
     for (int t = 0; t < RT; ++t)
 #pragma unroll
-      for (int c = 0; c < kMeet; ++c) *reinterpret_cast<f32x4 *>(s_acc[wave][t * kMeet + c][lane]) = acc[t][c0 + c];
+      for (int c = 0; c < kMeet; ++c) *reinterpret_cast<f32x4 *>(s_mem[wave][t * kMeet + c][lane]) = acc[t][c0 + c];
     __syncthreads();
     // lane (j, g) has rows 4g .. 4g + 3 of W, which are neighbours in y, of row j of x
     for (int tc = wave; tc < RT * kMeet; tc += NW) {
@@ -252,7 +301,7 @@ __global__ __launch_bounds__(NW *kWave) void w4_rows_kernel(W4Args a) {
       if (r >= a.R || n >= a.N) continue;
       f32x4 v = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int k = 0; k < NW; ++k) v += *reinterpret_cast<const f32x4 *>(s_acc[k][tc][lane]);
+      for (int k = 0; k < NW; ++k) v += *reinterpret_cast<const f32x4 *>(s_mem[k][tc][lane]);
       if (a.part) {
         *reinterpret_cast<f32x4 *>(a.part + ((int64_t)blockIdx.z * a.R + r) * (a.tiles * kTileRows) + n) = v;
         continue;
@@ -286,13 +335,6 @@ template <int DT> __global__ __launch_bounds__(kBlock) void w4_join_kernel(W4Arg
   }
   w4_store(reinterpret_cast<T *>(a.y) + (int64_t)r * a.N + n, y, a.N - n);
 }
-
-// Sixteen rows of x by 32 channels, one matrix operand: lane l loads vector `operand_vector` of row l / 4, so that four neighbours read 64
-// bytes of a row (a lane its own operand's 16 bytes, rows in turn, takes four times the accesses of the first-level cache), and the vectors
-// lie in LDS in the lanes' order; a lane's operand, row l % 16 and vector l / 16, is at `operand_slot`.  Vectors go round by one every four
-// rows, so that 16 lanes that read one vector of 16 rows meet all banks.
-__device__ __forceinline__ int operand_vector(int lane) { return (lane + lane / 16) % 4; }
-__device__ __forceinline__ int operand_slot(int lane) { return lane % 16 * 4 + (lane / 16 + 4 - lane % 16 / 4) % 4; }
 
 // ---- more rows ---------------------------------------------------------------------------------------------------------------------------
 
@@ -346,7 +388,7 @@ template <int DT, int RT, int CT> __device__ __forceinline__ void w4_finish(cons
 }
 
 // ROWS rows of x times COLS rows of W a workgroup, 64 channels a stage.  x and the codes come through registers, U steps of 128 channels ahead,
-// into LDS, x as matrix operands lie (1 KB in lane order) and the weights too, each turned into 16 bits once for all rows: (code - zero) *
+// into LDS, x as matrix operands (see operand_vector) and the weights too, each turned into 16 bits once for all rows: (code - zero) *
 // scale in fp32, rounded as a weight kept in 16 bits would be (half a step of the activations' type; scaling sums of codes instead takes four
 // multiplications for each four matrix instructions of a group of 32, as many cycles as those themselves).  Where the workgroups of all rows
 // and columns are few, runs of steps are shared out too, and a second launch adds up.
@@ -380,8 +422,8 @@ __global__ __launch_bounds__(S::NW *kWave, 2) void w4_tile_kernel(W4Args a) {
   uint32_t xrow[XT];
 #pragma unroll
   for (int t = 0; t < XT; ++t) {
-    const int r = (XT * wave + t) * 16 + j;
-    xrow[t] = r < rows ? (uint32_t)((int64_t)r * a.x_stride * 2) + g * 16 : kOutOfRange;
+    const int r = (XT * wave + t) * 16 + lane / 4;
+    xrow[t] = r < rows ? (uint32_t)((int64_t)r * a.x_stride * 2) + operand_vector(lane) * 16 : kOutOfRange;
   }
   // W: this wave turns tiles WT wave .. into 16 bits; a lane's row of W is l % 16
   rsrc_t code_rsrc[WT], scale_rsrc[WT], zero_rsrc[WT];
@@ -403,7 +445,7 @@ __global__ __launch_bounds__(S::NW *kWave, 2) void w4_tile_kernel(W4Args a) {
       sc[u][t] = __builtin_bit_cast(Pack<T, kGroups>, w4_load<2 * kGroups, 0>(scale_rsrc[t], (step * 16 + j) * 2 * kGroups | none));
       ze[u][t] = w4_load<kGroups, 0>(zero_rsrc[t], (step * 16 + j) * kGroups | none);
     }
-    const int left = a.K - step * kTileCols - g * 8;
+    const int left = a.K - step * kTileCols - operand_vector(lane) * 8;
 #pragma unroll
     for (int i = 0; i < 4; ++i)
 #pragma unroll
@@ -441,7 +483,7 @@ __global__ __launch_bounds__(S::NW *kWave, 2) void w4_tile_kernel(W4Args a) {
     for (int c = 0; c < CT; ++c) acc[t][c] = f32x4{0.f, 0.f, 0.f, 0.f};
   // A stage's products from buffer `buf`, and between them the next stage's operands into the other one.
   auto multiply = [&](int buf, int u, int part) {
-    const char *xs = s_mem + buf * kXStage + wr * RT * 2048 + lane * 16, *ws = s_mem + kW + buf * kWStage + wc * CT * 2048 + lane * 16;
+    const char *xs = s_mem + buf * kXStage + wr * RT * 2048 + operand_slot(lane) * 16, *ws = s_mem + kW + buf * kWStage + wc * CT * 2048 + lane * 16;
     uint4 w[CT], x[2];
 #pragma unroll
     for (int c = 0; c < CT; ++c) w[c] = *reinterpret_cast<const uint4 *>(ws + c * 2048);
@@ -494,11 +536,11 @@ __global__ __launch_bounds__(S::NW *kWave, 2) void w4_tile_kernel(W4Args a) {
 }
 
 // 256 rows of x times 256 rows of W a workgroup, 64 channels a stage; eight waves, 128 x 64 each.  Bound by the matrix instructions: x goes
-// from memory into LDS as operands lie (a wave's load of 16 rows x 32 channels is one operand, 1 KB in lane order), and so do the
+// from memory into LDS as operands lie (a wave's load of 16 rows x 32 channels is one operand, 1 KB), and so do the
 // weights, each turned into 16 bits once for the 256 rows: (code - zero) * scale in fp32, rounded as a weight kept in 16 bits would be
 // (half a step of the activations' type; scaling sums of codes instead takes four multiplications for each four matrix instructions of a
-// group of 32, as many cycles as those themselves).
-
+// group of 32, as many cycles as those themselves).  2000 x 5120 -> 13841, bf16: 0.98 PFLOP/s, of 1.4 that a large product of 16-bit matrices
+// reaches; the rest is the last round of tiles, 440 of them on 256 compute units.
 template <int DT, int GROUP>
 __global__ __launch_bounds__(kManyWaves *kWave, 2) void w4_many_kernel(W4Args a) {
   typedef Elem<DT> E;
@@ -673,9 +715,9 @@ static int check_w4(const en_w4_weight *w) {
 // Which kernel, and in how many runs the channels are shared out (a launch more, and the sums through memory).  us, groups of 128, bf16:
 //  - narrow / wide (one tile of W a workgroup, or four, which share the loads of x): 1 x 768 -> 2304 5.3 / 5.9, 64 x 768 -> 2304 6.5 / 9.1, 1 x 4096
 //    -> 4096 5.3 / 8.2, 16 x 4096 -> 4096 6.8 / 9.0; 1 x 9216 -> 9216 18.2 / 16.4, 16 x 9216 -> 9216 30.4 / 17.0, 16 x 7168 -> 28672 54 / 27.5;
-//  - wide, runs 1 / 3 or 4: 16 x 9216 -> 9216 17.0 / 17.7; 40 x 9216 -> 9216 33 / 28, 64 x 9216 -> 9216 44.5 / 41.9, 40 x 4096 -> 4096 17 / 11.6,
-//    64 x 4096 -> 4096 23 / 14.2;
-//  - wide / tiles of 128 x 128: 64 x 9216 -> 9216 42 / 41, 128 x 9216 -> 9216 86 / 56;
+//  - wide, runs 1 / 3 or 4: 16 x 9216 -> 9216 17.0 / 17.7; 40 x 9216 -> 9216 46 / 27, 64 x 9216 -> 9216 48 / 41, 40 x 4096 -> 4096 20.5 / 11.6;
+//    in more they are slower again: 40 x 9216 -> 9216 in 4, 5, 6 33.5, 31.1, 32.2;
+//  - wide / tiles of 128 x 128: 64 x 9216 -> 9216 37 / 41, 128 x 9216 -> 9216 86 / 46;
 //  - tiles of 128 x 128 / of 256 x 256: 512 x 9216 -> 9216 148 / 217, 200 x 7168 -> 28672 146 / 171, 1000 x 9216 -> 9216 257 / 218, 2000 x 5120 -> 13841 374 / 281.
 enum class W4Form { kNarrow, kWide, kTile, kMany };
 struct W4Plan {
@@ -754,10 +796,10 @@ int en_linear_w4(const void *x, int64_t rows, int64_t x_stride, const en_w4_weig
   if (plan.runs > 1) a.part = reinterpret_cast<float *>(workspace);
   const unsigned runs = (unsigned)ceil_div(a.steps, a.per);
   const hipStream_t s = (hipStream_t)stream;
-  auto few = [&](auto dt, auto group, auto rt, auto ct, auto nw) {
+  auto few = [&](auto dt, auto group, auto rt, auto ct, auto nw, auto direct) {
     constexpr int RT = decltype(rt)::value, CT = decltype(ct)::value, NW = decltype(nw)::value;
     const dim3 grid((unsigned)ceil_div(a.tiles, CT), (unsigned)ceil_div(rows, 16 * RT), runs);
-    w4_rows_kernel<decltype(dt)::value, decltype(group)::value, RT, CT, NW><<<grid, NW * kWave, 0, s>>>(a);
+    w4_rows_kernel<decltype(dt)::value, decltype(group)::value, RT, CT, NW, decltype(direct)::value><<<grid, NW * kWave, 0, s>>>(a);
   };
   auto shape = [&](auto dt, auto group) {
     constexpr int DT = decltype(dt)::value, GROUP = decltype(group)::value;
@@ -767,21 +809,27 @@ int en_linear_w4(const void *x, int64_t rows, int64_t x_stride, const en_w4_weig
     typedef std::integral_constant<int, 4> i4;
     typedef std::integral_constant<int, 8> i8;
     const int row_tiles = (int)ceil_div(rows, 16);
+    const std::true_type yes;
+    const std::false_type no;
+    // us through LDS / direct: 1 x 9216 -> 9216 16.6 / 16.2, 8 16.4 / 16.0, 16 16.6 / 16.9; 8 x 7168 -> 28672 25.4 / 25.7, 16 27.3 / 28.3
+    const bool few_rows = rows <= 8;
     if (plan.form == W4Form::kMany) {
       w4_many_kernel<DT, GROUP><<<(unsigned)(ceil_div(rows, kManyRows) * ceil_div(N, kManyCols)), kManyWaves * kWave, 0, s>>>(a);
     } else if (plan.form == W4Form::kTile) {
       typedef W4Shape<128, 128, 2, 2, 2> S;
       w4_tile_kernel<DT, GROUP, S><<<dim3((unsigned)(ceil_div(rows, S::ROWS) * ceil_div(N, S::COLS)), runs), S::NW * kWave, 0, s>>>(a);
     } else if (plan.form == W4Form::kNarrow) {
-      if (row_tiles == 1) few(dt, group, i1{}, i1{}, i8{});
-      else if (row_tiles == 2) few(dt, group, i2{}, i1{}, i8{});
-      else if (row_tiles == 3) few(dt, group, i3{}, i1{}, i8{});
-      else few(dt, group, i4{}, i1{}, i8{});
+      if (few_rows) few(dt, group, i1{}, i1{}, i8{}, yes);
+      else if (row_tiles == 1) few(dt, group, i1{}, i1{}, i8{}, no);
+      else if (row_tiles == 2) few(dt, group, i2{}, i1{}, i8{}, no);
+      else if (row_tiles == 3) few(dt, group, i3{}, i1{}, i8{}, no);
+      else few(dt, group, i4{}, i1{}, i8{}, no);
     } else {
-      if (row_tiles == 1) few(dt, group, i1{}, i4{}, i8{});
-      else if (row_tiles == 2) few(dt, group, i2{}, i4{}, i4{});
-      else if (row_tiles == 3) few(dt, group, i3{}, i4{}, i4{});
-      else few(dt, group, i4{}, i4{}, i4{});
+      if (few_rows) few(dt, group, i1{}, i4{}, i8{}, yes);
+      else if (row_tiles == 1) few(dt, group, i1{}, i4{}, i8{}, no);
+      else if (row_tiles == 2) few(dt, group, i2{}, i4{}, i4{}, no);
+      else if (row_tiles == 3) few(dt, group, i3{}, i4{}, i4{}, no);
+      else few(dt, group, i4{}, i4{}, i4{}, no);
     }
     if (a.part) w4_join_kernel<DT><<<dim3((unsigned)ceil_div(N, 4 * kBlock), (unsigned)rows), kBlock, 0, s>>>(a, (int)runs);
   };
