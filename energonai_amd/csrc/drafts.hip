@@ -14,7 +14,7 @@ __device__ __forceinline__ int draft_nodes(const int32_t *cu, int b, int max_nod
 // on from where that one has.
 __global__ __launch_bounds__(kWave) void draft_tree_kernel(const int32_t *parents, const int32_t *cu, int64_t total, int64_t *masks, int32_t *depths) {
   const int b = blockIdx.x, lane = threadIdx.x, first = cu[b], nodes = draft_nodes(cu, b, INT32_MAX);
-  int up = lane < min(nodes, kNodes) && first + lane < total ? parents[first + lane] : -1;
+  int up = lane < min(nodes, kNodes) && (int64_t)first + lane < total ? parents[first + lane] : -1;
   if (up >= lane || up < 0) up = -1;
   uint64_t mask = 1ull << lane;
 #pragma unroll
@@ -30,6 +30,12 @@ __global__ __launch_bounds__(kWave) void draft_tree_kernel(const int32_t *parent
   for (int i = lane; i < nodes && first + (int64_t)i < total; i += kWave) {
     masks[first + i] = i < kNodes ? (int64_t)mask : 0;
     depths[first + i] = i < kNodes ? __popcll(mask) - 1 : 0;
+  }
+  // the rows behind the last sequence are no nodes either
+  if (b + 1 < (int)gridDim.x) return;
+  for (int64_t i = max(first + (int64_t)nodes, (int64_t)0) + lane; i < total; i += kWave) {
+    masks[i] = 0;
+    depths[i] = 0;
   }
 }
 

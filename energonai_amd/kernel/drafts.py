@@ -35,7 +35,8 @@ class DraftTree(NamedTuple):
 def draft_tree(parents, node_counts, batch_size: int, max_nodes: int = DRAFT_MAX_NODES) -> DraftTree:
     """Masks and depths of the nodes of ``batch_size`` trees.  ``parents`` is int32 ``[nodes]``, sequence by sequence; a number that is not
     that of an earlier node of the sequence counts as -1.  ``node_counts``: int32 or int64 numbers, a list, or a ``SeqInfo`` of them.
-    Nodes past the 64th of a sequence do not exist for any call, nor do those past ``max_nodes`` for the calls that take the tree."""
+    Nodes past the 64th of a sequence do not exist for any call, nor do those past ``max_nodes`` for the calls that take the tree; their rows, and
+    rows behind the last sequence, have mask and depth 0."""
     who = "draft_tree"
     _lib.require_gpu(parents, "parents")
     if parents.dim() != 1 or parents.dtype != torch.int32:
@@ -43,8 +44,8 @@ def draft_tree(parents, node_counts, batch_size: int, max_nodes: int = DRAFT_MAX
     if not 1 <= int(max_nodes) <= DRAFT_MAX_NODES:
         raise RuntimeError(f"{who}: max_nodes must be 1 .. {DRAFT_MAX_NODES}")
     info = _offsets(who, node_counts, int(batch_size), parents.device)
-    masks = torch.empty(parents.shape, dtype=torch.int64, device=parents.device)
-    depths = torch.empty_like(parents)
+    new = torch.empty if int(batch_size) > 0 else torch.zeros            # no sequence, no launch
+    masks, depths = (new(parents.shape, dtype=t, device=parents.device) for t in (torch.int64, torch.int32))
     with _lib.device_guard(parents):
         _lib.check(_lib.fn.en_draft_tree(parents.data_ptr(), info.cu_seqlens.data_ptr(), int(batch_size), parents.numel(), masks.data_ptr(),
                                          depths.data_ptr(), _lib.stream_of(parents)), who)

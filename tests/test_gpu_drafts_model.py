@@ -164,3 +164,23 @@ def test_block_with_weights_in_4_bits(activation, zero_points):
     again = quantize_linears(copy.deepcopy(plain), 64, zero_points)
     again.load_state_dict(state)
     assert torch.equal(again(x, first_cache=True, seq_lens=lens_d), small(x, first_cache=True, seq_lens=lens_d))
+
+
+@torch.no_grad()
+def test_padding_rows_of_rotated_nodes_do_not_change_from_call_to_call():
+    """Rows behind the last sequence are rotated by that sequence's length, not by what memory held."""
+    from energonai_amd import kernel as K
+    b = _block(torch.float16, rotary_dim=32)
+    b(_prompt([5, 9], torch.float16), first_cache=True, seq_lens=torch.tensor([5, 9], dtype=torch.int32, device="cuda"))
+    x = torch.randn(1, 40, HID, dtype=torch.float16, device="cuda")
+    parents = torch.full((40,), -1, dtype=torch.int32, device="cuda")
+    announce("padding rows of rotated nodes")
+    first = None
+    for fill in (0, 1 << 20, -5):
+        poison = [torch.full((40,), fill, dtype=t, device="cuda") for t in (torch.int64, torch.int32) for _ in range(8)]
+        torch.cuda.synchronize()
+        del poison
+        b.forward_nodes(x, K.draft_tree(parents, [2, 1], 2, 2))
+        keys = b.attn._nodes[0].clone()
+        first = keys if first is None else first
+        assert torch.equal(keys, first)
