@@ -36,7 +36,7 @@ class MultiHeadAttention1D(nn.Module):
 
     # what is not there in a module saved before there was a choice
     rotary_dim, rotary_base, rotary_interleaved, qk_norm, kv_cache_dtype = 0, 10000.0, False, False, None
-    _nodes = None               # a step of drafted nodes until they are accepted: keys, values, tree, the cache and its steps
+    _nodes = None               # a step of drafted nodes until they are accepted: keys, values, tree, the cache, its steps and who held its pages
 
     def __init__(self, hidden_size: int, num_heads: int, bias: bool = True, dtype: torch.dtype = torch.float16,
                  max_seq_len: int = 512, fused_qkv: bool = True, is_decoder: bool = True, disable_past_cache=False,
@@ -215,19 +215,29 @@ class MultiHeadAttention1D(nn.Module):
             positions = cache.lens[seq.clamp(max=cache.batch_size - 1)] + tree.depths
             q, k = qk_norm_rotary(q, k, cache.batch_size, None, self._tables(x.device, cache.max_seq_len), positions=positions, **self._turn_how())
         ctx = cache.attend_nodes(q, k, v, tree, self.scaling)
-        self._nodes = (k, v, tree, cache, cache.steps)
+        self._nodes = (k, v, tree, cache, cache.steps, cache.holders())
         return project(self.dense, ctx.view(1, T, self.hidden_size))
 
     def accept_nodes(self, path: torch.Tensor, counts: torch.Tensor, counts_host=None) -> None:
-        """The accepted nodes of the last ``forward_nodes`` (``kernel.accept_drafts``) go into the cache (see ``PagedKVCache.extend``)."""
+        """The accepted nodes of the last ``forward_nodes`` (``kernel.accept_drafts``) go into the cache (see ``PagedKVCache.extend``).  Sequences
+        released since then accept nothing: a count of theirs other than 0 is refused, and the nodes may be accepted again without it."""
+        counts_host = [int(n) for n in (counts.tolist() if counts_host is None else counts_host)]
+        self.check_accepted(counts_host)
+        k, v, tree, cache = self._nodes[:4]
+        cache.extend(k, v, tree, path, counts, counts_host)
+        self._nodes = None
+
+    def check_accepted(self, counts_host) -> None:
+        """Raises where ``accept_nodes`` of these counts has no place for the nodes."""
         if self._nodes is None:
             raise RuntimeError("accept_nodes before a forward_nodes call")
-        *rows, cache, at = self._nodes
+        cache, at, holders = self._nodes[3:]
         if cache is not self.kv_cache or cache.steps != at:
             self._nodes = None
             raise RuntimeError("accept_nodes: the cache has gone on since the forward_nodes call")
-        cache.extend(*rows, path, counts, counts_host)
-        self._nodes = None
+        gone = [b for b, n in enumerate(counts_host[:cache.batch_size]) if n > 0 and cache.released_since(holders, b)]
+        if gone:
+            raise RuntimeError(f"accept_nodes: sequences {gone} were released since the forward_nodes call, their counts have to be 0")
 
     def forward(self, hidden_states, attention_mask=None, first_cache=False, seq_lens=None):
         B, S, hid = hidden_states.shape

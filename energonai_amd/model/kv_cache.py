@@ -156,6 +156,14 @@ class PagedKVCache:
         self.table[b].fill_(-1)
         self.lens[b] = 0
 
+    def holders(self) -> list:
+        """Who holds the pages now (see ``released_since``)."""
+        return list(self._pages)
+
+    def released_since(self, holders: list, b: int) -> bool:
+        """Whether sequence ``b`` was released after ``holders()`` was asked: a released one begins a list of pages anew."""
+        return self._pages[b] is not holders[b]
+
     def fill(self, k_src: torch.Tensor, v_src: torch.Tensor, info: SeqInfo, k_head_first: int = 0,
              v_head_first: int = 0, longest: Optional[int] = None, lens_host=None) -> None:
         """Prefill from packed projections seen as ``[T,Hs,D]``.  The pages are assigned on the host, which needs

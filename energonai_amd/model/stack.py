@@ -55,7 +55,10 @@ class PackedStack(nn.Module):
         return x if self.norm is None else self.norm(x)
 
     def accept_nodes(self, path: torch.Tensor, counts: torch.Tensor, counts_host=None) -> None:
-        """The accepted nodes go into every block's cache; the counts are copied to the host once for all of them."""
-        counts_host = counts.tolist() if counts_host is None else counts_host
+        """The accepted nodes go into every block's cache, or, where one of them has no place for them, into none; the counts are copied to the host
+        once for all of them."""
+        counts_host = [int(n) for n in (counts.tolist() if counts_host is None else counts_host)]
+        for blk in self.blocks:
+            blk.attn.check_accepted(counts_host)
         for blk in self.blocks:
             blk.accept_nodes(path, counts, counts_host)

@@ -184,3 +184,48 @@ def test_padding_rows_of_rotated_nodes_do_not_change_from_call_to_call():
         keys = b.attn._nodes[0].clone()
         first = keys if first is None else first
         assert torch.equal(keys, first)
+
+
+@torch.no_grad()
+def test_released_sequences_accept_nothing():
+    """A sequence that was released after its nodes were gone over has no place for them; the others' nodes, and none of its own, may be accepted still."""
+    from energonai_amd import kernel as K
+    b = _block(torch.float16)
+    lens = torch.tensor([5, 9], dtype=torch.int32, device="cuda")
+    tree = K.draft_tree(torch.tensor([-1, 0] * 2, dtype=torch.int32, device="cuda"), [2, 2], 2, 2)
+    x = torch.randn(1, 4, HID, dtype=torch.float16, device="cuda")
+    path = torch.tensor([[0, 1], [0, 1]], dtype=torch.int32, device="cuda")
+    announce("released sequences")
+    for host in (False, True):
+        b(_prompt([5, 9], torch.float16), first_cache=True, seq_lens=lens)
+        b.forward_nodes(x, tree)
+        cache = b.attn.kv_cache
+        cache.release(0)
+        both = torch.tensor([2, 2], dtype=torch.int32, device="cuda")
+        with pytest.raises(RuntimeError, match="released"):
+            b.accept_nodes(path, both, [2, 2] if host else None)
+        assert cache.lens.tolist() == [0, 9] and cache._host_lens == [0, 9] and cache.pages_in_use() == 1
+        b.accept_nodes(path, torch.tensor([0, 2], dtype=torch.int32, device="cuda"), [0, 2] if host else None)
+        assert cache.lens.tolist() == [0, 11] and cache._host_lens == [0, 11]
+
+
+@torch.no_grad()
+def test_stacks_accept_in_all_blocks_or_in_none():
+    """One block whose cache has no place for the nodes keeps them out of the others' too."""
+    from energonai_amd import kernel as K
+    from energonai_amd.model import PackedStack
+    stack = PackedStack([_block(torch.float16) for _ in range(2)])
+    tree = K.draft_tree(torch.tensor([-1, 0], dtype=torch.int32, device="cuda"), [2], 1, 2)
+    x, one = torch.randn(1, 2, HID, dtype=torch.float16, device="cuda"), torch.ones(1, dtype=torch.int32, device="cuda")
+    path = torch.zeros(1, 1, dtype=torch.int32, device="cuda")
+    announce("stacks accept in all blocks or in none")
+    stack(_prompt([5], torch.float16), first_cache=True)
+    stack.forward_nodes(x, tree)
+    stack.blocks[1].attn.kv_cache.release(0)
+    with pytest.raises(RuntimeError, match="released"):
+        stack.accept_nodes(path, one)
+    assert stack.blocks[0].attn.kv_cache.lens.tolist() == [5]
+    stack(_prompt([5], torch.float16), first_cache=True)
+    stack.forward_nodes(x, tree)
+    stack.accept_nodes(path, one)
+    assert [b.attn.kv_cache.lens.tolist() for b in stack.blocks] == [[6], [6]]
