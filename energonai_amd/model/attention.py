@@ -9,6 +9,7 @@ reference concatenates and recomputes every position (attention.py:61-71).
 """
 from __future__ import annotations
 
+import weakref
 from typing import Optional
 
 import torch
@@ -36,7 +37,9 @@ class MultiHeadAttention1D(nn.Module):
 
     # what is not there in a module saved before there was a choice
     rotary_dim, rotary_base, rotary_interleaved, qk_norm, kv_cache_dtype = 0, 10000.0, False, False, None
-    _nodes = None               # a step of drafted nodes until they are accepted: keys, values, tree, the cache, its steps and who held its pages
+    # a step of drafted nodes until they are accepted: keys, values, tree, a weak reference to the cache, its steps and who held its pages; () once
+    # the cache has gone on
+    _nodes = None
 
     def __init__(self, hidden_size: int, num_heads: int, bias: bool = True, dtype: torch.dtype = torch.float16,
                  max_seq_len: int = 512, fused_qkv: bool = True, is_decoder: bool = True, disable_past_cache=False,
@@ -179,6 +182,7 @@ class MultiHeadAttention1D(nn.Module):
             cache.fill(k, v, info, longest=max_seq_len)
         else:
             cache.fill(k.contiguous(), v.contiguous(), info, longest=max_seq_len)
+        self.drop_nodes()
         self.kv_cache = cache       # only now: rows and lengths of a cache that was not filled are whatever the memory held
 
     # ---- one decode step: newest position only ----------------------------------------------
@@ -194,6 +198,7 @@ class MultiHeadAttention1D(nn.Module):
             q = cache.append_rotary(q, k, v, self._tables(last.device, cache.max_seq_len), **self._turn_how())
         else:
             cache.append(k, v)
+        self.drop_nodes()
         ctx = cache.attend(q, self.scaling)      # [B,H,1,D], one pass over the caches
         return project(self.dense, ctx.view(B, 1, self.hidden_size))
 
@@ -215,7 +220,7 @@ class MultiHeadAttention1D(nn.Module):
             positions = cache.lens[seq.clamp(max=cache.batch_size - 1)] + tree.depths
             q, k = qk_norm_rotary(q, k, cache.batch_size, None, self._tables(x.device, cache.max_seq_len), positions=positions, **self._turn_how())
         ctx = cache.attend_nodes(q, k, v, tree, self.scaling)
-        self._nodes = (k, v, tree, cache, cache.steps, cache.holders())
+        self._nodes = (k, v, tree, weakref.ref(cache), cache.steps, cache.holders())
         return project(self.dense, ctx.view(1, T, self.hidden_size))
 
     def accept_nodes(self, path: torch.Tensor, counts: torch.Tensor, counts_host=None) -> None:
@@ -223,19 +228,23 @@ class MultiHeadAttention1D(nn.Module):
         released since then accept nothing: a count of theirs other than 0 is refused, and the nodes may be accepted again without it."""
         counts_host = [int(n) for n in (counts.tolist() if counts_host is None else counts_host)]
         self.check_accepted(counts_host)
-        k, v, tree, cache = self._nodes[:4]
-        cache.extend(k, v, tree, path, counts, counts_host)
+        self.kv_cache.extend(*self._nodes[:3], path, counts, counts_host)
         self._nodes = None
+
+    def drop_nodes(self) -> None:
+        """The cache goes on without the nodes of the last ``forward_nodes``, if any are left: their rows are held no longer."""
+        if self._nodes:
+            self._nodes = ()
 
     def check_accepted(self, counts_host) -> None:
         """Raises where ``accept_nodes`` of these counts has no place for the nodes."""
         if self._nodes is None:
             raise RuntimeError("accept_nodes before a forward_nodes call")
-        cache, at, holders = self._nodes[3:]
-        if cache is not self.kv_cache or cache.steps != at:
+        cache = self.kv_cache
+        if not self._nodes or cache is None or self._nodes[3]() is not cache or cache.steps != self._nodes[4]:
             self._nodes = None
             raise RuntimeError("accept_nodes: the cache has gone on since the forward_nodes call")
-        gone = [b for b, n in enumerate(counts_host[:cache.batch_size]) if n > 0 and cache.released_since(holders, b)]
+        gone = [b for b, n in enumerate(counts_host[:cache.batch_size]) if n > 0 and cache.released_since(self._nodes[5], b)]
         if gone:
             raise RuntimeError(f"accept_nodes: sequences {gone} were released since the forward_nodes call, their counts have to be 0")
 

@@ -148,6 +148,8 @@ class Block1D(nn.Module):
         if out is not None:
             cache.appended()
             history.cur += 1
+            if attn._nodes:
+                attn.drop_nodes()
         return out
 
     def forward_packed(self, x: torch.Tensor, info: SeqInfo, batch_size: int, max_seq_len: int,

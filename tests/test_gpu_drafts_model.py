@@ -229,3 +229,35 @@ def test_stacks_accept_in_all_blocks_or_in_none():
     stack.forward_nodes(x, tree)
     stack.accept_nodes(path, one)
     assert [b.attn.kv_cache.lens.tolist() for b in stack.blocks] == [[6], [6]]
+
+
+@pytest.mark.parametrize("turn", [{}, dict(rotary_dim=32)])
+@torch.no_grad()
+def test_nodes_do_not_keep_what_they_belong_to(turn):
+    """A step of nodes that is never accepted holds no cache that was replaced or taken away, and no rows once the cache has gone on."""
+    import gc
+    import weakref
+
+    from energonai_amd import kernel as K
+    b = _block(torch.float16, **turn)
+    tree = K.draft_tree(torch.tensor([-1, 0], dtype=torch.int32, device="cuda"), [2], 1, 2)
+    x, one = torch.randn(1, 2, HID, dtype=torch.float16, device="cuda"), torch.ones(1, dtype=torch.int32, device="cuda")
+    path = torch.zeros(1, 1, dtype=torch.int32, device="cuda")
+    announce("nodes that are not accepted", turn)
+
+    def gone():
+        gc.collect()
+        return cache() is None
+    for between, takes_cache in ((lambda: b(_prompt([9], torch.float16), first_cache=True), True), (lambda: b(x[:, :1], first_cache=False), False),
+                                 (lambda: setattr(b.attn, "kv_cache", None), True)):
+        b(_prompt([5], torch.float16), first_cache=True)
+        b.forward_nodes(x, tree)
+        cache, rows = weakref.ref(b.attn.kv_cache), weakref.ref(b.attn._nodes[0])
+        between()
+        assert gone() == takes_cache
+        assert not takes_cache or b.attn.kv_cache is None or rows() is None
+        if not takes_cache:
+            assert rows() is None
+        with pytest.raises(RuntimeError, match="gone on"):
+            b.accept_nodes(path, one)
+        assert rows() is None
