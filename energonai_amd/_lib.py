@@ -120,6 +120,7 @@ SIGNATURES = {
                          [c_int, c_void_p, c_int64, c_void_p]),
     "en_accept_drafts_workspace_bytes": (c_int64, [c_int64, c_int, c_int]),
     "en_kv_extend_paged": (c_int, [c_void_p] * 6 + [c_int64, c_void_p, c_int] + [c_void_p] * 3),
+    "en_kv_extend_paged_nodes": (c_int, [c_void_p] * 6 + [c_int64, c_int, c_void_p, c_int] + [c_void_p] * 3),
     "en_w4_codes_bytes": (c_int64, [c_int64] * 2),
     "en_w4_groups": (c_int64, [c_int64, c_int64, c_int]),
     "en_w4_pack": (c_int, [c_void_p] * 5),

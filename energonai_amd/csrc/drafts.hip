@@ -227,7 +227,7 @@ struct ExtendArgs {
   int64_t kn_token, kn_head, vn_token, vn_head, k_page, k_head, k_row, v_page, v_head, v_row;      // bytes
   const int32_t *table, *lens, *cu, *path, *counts;
   int64_t total;
-  int width, num_pages, lg_page, max_pages, H;
+  int width, max_nodes, num_pages, lg_page, max_pages, H;
   int row_bytes;
   int32_t *overflow;
 };
@@ -238,7 +238,7 @@ struct ExtendArgs {
 template <int W>
 __global__ __launch_bounds__(kBlock) void extend_kernel(ExtendArgs a) {
   typedef Pack<uint8_t, W> P;
-  const int b = blockIdx.y, first = a.cu[b], count = min(a.counts[b], a.width), nodes = min(a.cu[b + 1] - first, kNodes), len = a.lens[b];
+  const int b = blockIdx.y, first = a.cu[b], count = min(a.counts[b], a.width), nodes = draft_nodes(a.cu, b, a.max_nodes), len = a.lens[b];
   const bool value = blockIdx.z;
   const char *from = value ? a.v_new : a.k_new;
   char *to = value ? a.v_pool : a.k_pool;
@@ -318,13 +318,13 @@ int en_accept_drafts(const void *logits, int64_t logits_stride, int vocab, const
   return EN_OK;
 }
 
-int en_kv_extend_paged(const void *k_new, const void *v_new, const int64_t *strides, const en_kv_pages *cache, const int32_t *kv_lens,
-                       const int32_t *cu_seqlens, int64_t nodes, const int32_t *path, int path_width, const int32_t *counts,
-                       int32_t *overflow, en_stream_t stream) {
+int en_kv_extend_paged_nodes(const void *k_new, const void *v_new, const int64_t *strides, const en_kv_pages *cache, const int32_t *kv_lens,
+                             const int32_t *cu_seqlens, int64_t nodes, int max_nodes, const int32_t *path, int path_width, const int32_t *counts,
+                             int32_t *overflow, en_stream_t stream) {
   if (!cache || !strides) return EN_ERR_NULL;
   const en_kv_pages &c = *cache;
   if (const int bad = check_kv_pages(c)) return bad;
-  if (nodes < 0 || nodes > INT32_MAX || path_width < 0 || path_width > kNodes || c.batch > 65535) return EN_ERR_SHAPE;
+  if (nodes < 0 || nodes > INT32_MAX || max_nodes < 0 || max_nodes > kNodes || path_width < 0 || path_width > kNodes || c.batch > 65535) return EN_ERR_SHAPE;
   for (int i = 0; i < 4; ++i)
     if (strides[i] < 0) return EN_ERR_SHAPE;
   if (c.batch == 0 || nodes == 0 || path_width == 0) return EN_OK;
@@ -337,7 +337,7 @@ int en_kv_extend_paged(const void *k_new, const void *v_new, const int64_t *stri
   a.k_page = es * c.strides[0]; a.k_head = es * c.strides[1]; a.k_row = es * c.strides[2];
   a.v_page = es * c.strides[3]; a.v_head = es * c.strides[4]; a.v_row = es * c.strides[5];
   a.table = c.page_table; a.lens = kv_lens; a.cu = cu_seqlens; a.path = path; a.counts = counts;
-  a.total = nodes; a.width = path_width; a.num_pages = c.num_pages; a.lg_page = page_log2(c.page_size); a.max_pages = c.max_pages_per_seq; a.H = c.head_num;
+  a.total = nodes; a.width = path_width; a.max_nodes = max_nodes; a.num_pages = c.num_pages; a.lg_page = page_log2(c.page_size); a.max_pages = c.max_pages_per_seq; a.H = c.head_num;
   a.row_bytes = (int)(es * c.size_per_head);
   a.overflow = overflow;
   // the widest access that every row's address and length allow
@@ -356,6 +356,12 @@ int en_kv_extend_paged(const void *k_new, const void *v_new, const int64_t *stri
   else extend_kernel<2><<<grid, kBlock, 0, s>>>(a);
   EN_RETURN_IF_LAUNCH_FAILED();
   return EN_OK;
+}
+
+int en_kv_extend_paged(const void *k_new, const void *v_new, const int64_t *strides, const en_kv_pages *cache, const int32_t *kv_lens,
+                       const int32_t *cu_seqlens, int64_t nodes, const int32_t *path, int path_width, const int32_t *counts,
+                       int32_t *overflow, en_stream_t stream) {
+  return en_kv_extend_paged_nodes(k_new, v_new, strides, cache, kv_lens, cu_seqlens, nodes, kNodes, path, path_width, counts, overflow, stream);
 }
 
 }  // extern "C"

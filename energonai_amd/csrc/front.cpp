@@ -968,7 +968,7 @@ PyObject *kv_pages_extend(PyObject *const *a) {
   const int32_t *lens_p = i32(*info.lens), *cu_p = i32(*tree.cu), *path_p = i32(*path), *counts_p = i32(*counts);
   const int width = (int)path->size(1);
   const hipStream_t stream = stream_of(*kp);
-  check(without_gil([&] { return en_kv_extend_paged(kn_p, vn_p, st, &c, lens_p, cu_p, T, path_p, width, counts_p, over, stream); }), "kv_pages_extend");
+  check(without_gil([&] { return en_kv_extend_paged_nodes(kn_p, vn_p, st, &c, lens_p, cu_p, T, (int)most, path_p, width, counts_p, over, stream); }), "kv_pages_extend");
   Py_RETURN_TRUE;
 }
 

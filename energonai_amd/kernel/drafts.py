@@ -222,7 +222,7 @@ def accept_drafts(logits, tokens, tree):
 def kv_pages_extend(k_new, v_new, k_pool, v_pool, kv_len_list, page_table, tree, path, counts, *, overflow: Optional[torch.Tensor] = None) -> None:
     """``kv_pages_append`` of the accepted nodes: the rows of nodes ``path[b, i]``, ``i < counts[b]``, of ``k_new`` and ``v_new`` ``[nodes, H, D]``
     (any token and head strides) become positions ``kv_len[b] + i`` of sequence ``b``.  The caller advances the lengths afterwards.  Entries of
-    ``path`` that name no node are passed over; a position that has no page in the pool is not written and counted in ``overflow``.  Up to 65535
+    ``path`` that name no node of the tree are passed over; a position that has no page in the pool is not written and counted in ``overflow``.  Up to 65535
     sequences."""
     who = "kv_pages_extend"
     if type(tree) is DraftTree and _lib.front.kv_pages_extend(k_new, v_new, k_pool, v_pool, kv_len_list, page_table, tree, path, counts, overflow):
@@ -245,6 +245,6 @@ def kv_pages_extend(k_new, v_new, k_pool, v_pool, kv_len_list, page_table, tree,
         raise RuntimeError(f"{who}: overflow must be on the pools' device")
     lens = _lens(who, kv_len_list, B, k_pool.device)
     with _lib.device_guard(k_pool):
-        _lib.check(_lib.fn.en_kv_extend_paged(k_new.data_ptr(), v_new.data_ptr(), _token_head(k_new, v_new), ctypes.byref(c), lens.lens.data_ptr(),
-                                              info.cu_seqlens.data_ptr(), T, path.data_ptr(), path.shape[1], counts.data_ptr(),
-                                              _lib.ptr(overflow) or None, _lib.stream_of(k_pool)), who)
+        _lib.check(_lib.fn.en_kv_extend_paged_nodes(k_new.data_ptr(), v_new.data_ptr(), _token_head(k_new, v_new), ctypes.byref(c), lens.lens.data_ptr(),
+                                                    info.cu_seqlens.data_ptr(), T, tree.max_nodes, path.data_ptr(), path.shape[1], counts.data_ptr(),
+                                                    _lib.ptr(overflow) or None, _lib.stream_of(k_pool)), who)

@@ -568,10 +568,13 @@ int en_accept_drafts(const void *logits, int64_t logits_stride, int vocab, const
 /* The accepted nodes' keys and values into their pages: row cu_seqlens[b] + path[b, i] of k_new and v_new becomes position kv_lens[b] + i of
  * sequence b, i < min(counts[b], path_width).  Entries of path that are no node of the sequence are passed over; a position without a page in the pool
  * is not written and counted in overflow, if given.  strides: (token, head) in elements of k_new, v_new [nodes, head_num, size_per_head].
- * Up to 65535 sequences.  The caller advances the lengths afterwards. */
+ * Up to 65535 sequences.  The caller advances the lengths afterwards.  en_kv_extend_paged_nodes: nodes past max_nodes of a sequence do not exist. */
 int en_kv_extend_paged(const void *k_new, const void *v_new, const int64_t *strides, const en_kv_pages *cache, const int32_t *kv_lens,
                        const int32_t *cu_seqlens, int64_t nodes, const int32_t *path, int path_width, const int32_t *counts,
                        int32_t *overflow, en_stream_t stream);
+int en_kv_extend_paged_nodes(const void *k_new, const void *v_new, const int64_t *strides, const en_kv_pages *cache, const int32_t *kv_lens,
+                             const int32_t *cu_seqlens, int64_t nodes, int max_nodes, const int32_t *path, int path_width, const int32_t *counts,
+                             int32_t *overflow, en_stream_t stream);
 
 /* ---- weights in 4 bits ------------------------------------------------------ */
 

@@ -188,3 +188,13 @@ def test_sizes_past_64_bits_are_refused():
     for strides in (far, far[3:] + far[:3]):
         c.strides[:] = strides
         assert fn.en_decode_attn_tree(PTR, PTR, PTR, st, PTR, ctypes.byref(c), PTR, PTR, PTR, 5, 4, 4 * c.head_num, 0.1, PTR, 1 << 40, None) == SHAPE
+
+
+def test_extension_with_a_largest_number_of_nodes_refuses():
+    fn = _lib().fn.en_kv_extend_paged_nodes
+
+    def call(nodes=5, most=4, path=PTR, width=4):
+        return fn(PTR, PTR, (ctypes.c_int64 * 4)(*(128, 64) * 2), ctypes.byref(_pages()), PTR, PTR, nodes, most, path, width, PTR, None, None)
+    assert call(nodes=0) == 0 and call(width=0) == 0 and call(path=None) == NULL
+    for most in (-1, 65):
+        assert call(most=most) == SHAPE

@@ -32,3 +32,27 @@ def test_rows_behind_the_last_sequence_have_no_node(counts, rows):
         nodes += [at + i for i in range(min(n, 64)) if at + i < rows]
         at += n
     assert (masks[nodes] != 0).all() and (depths[nodes] < 64).all()
+
+
+def test_extension_knows_the_largest_number_of_nodes():
+    """Entries of a path that name nodes past the tree's ``max_nodes`` are passed over, by the native call and by the checked one."""
+    from energonai_amd.seqinfo import build_seq_info
+    counts, H, D, P, dtype = [6, 3], 2, 64, 16, torch.float16
+    g = torch.Generator().manual_seed(5)
+    k, v = (torch.randn(9, H, D, generator=g).to(dtype).cuda() for _ in range(2))
+    lens = torch.tensor([3, 20], dtype=torch.int32, device="cuda")
+    table = torch.tensor([[0, 1], [2, 3]], dtype=torch.int32, device="cuda")
+    tree = K().draft_tree(torch.full((9,), -1, dtype=torch.int32, device="cuda"), counts, 2, 4)
+    path = torch.tensor([[0, 3, 4, 5], [2, 1, 3, 0]], dtype=torch.int32, device="cuda")
+    taken = torch.full((2,), 4, dtype=torch.int32, device="cuda")
+    announce("extension and the largest number of nodes")
+    for at in (build_seq_info([3, 20], 2), lens):
+        pools = [torch.zeros(4, H, P, D, dtype=dtype, device="cuda") for _ in range(2)]
+        lost = torch.zeros(1, dtype=torch.int32, device="cuda")
+        K().kv_pages_extend(k, v, *pools, at, table, tree, path, taken, overflow=lost)
+        for pool, new in zip(pools, (k, v)):
+            want = torch.zeros_like(pool)
+            want[0, :, 3], want[0, :, 4] = new[0], new[3]                      # nodes 4 and 5 are past the largest
+            want[3, :, 4], want[3, :, 5], want[3, :, 7] = new[8], new[7], new[6]    # ... and 3 is none of the sequence's
+            assert torch.equal(pool, want)
+        assert int(lost) == 0
