@@ -103,7 +103,7 @@ __global__ __launch_bounds__(kBlock) void w4_pack_kernel(PackArgs a) {
     const int64_t tile = i / (16 * a.per_step), in = i % (16 * a.per_step), group = tile % a.steps * a.per_step + in % a.per_step, n = tile / a.steps * kTileRows + in / a.per_step;
     const bool there = n < a.N && group < a.groups;
     a.scales_out[i] = there ? a.scales[n * a.groups + group] : 0;
-    if (a.zeros) a.zeros_out[i] = there ? a.zeros[n * a.groups + group] & 15 : 0;
+    if (a.zeros) a.zeros_out[i] = there ? a.zeros[n * a.groups + group] : 0;
   }
 }
 

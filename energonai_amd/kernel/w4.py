@@ -1,6 +1,6 @@
 """Weights in 4 bits with a scale for each group of neighbouring input channels, and the products with them.
 
-``W[n, k] = (code[n, k] - zero[n, g]) * scale[n, g]`` with codes 0 .. 15, ``g = k // group_size`` and zero points 0 .. 15 (without them 8).  A
+``W[n, k] = (code[n, k] - zero[n, g]) * scale[n, g]`` with codes 0 .. 15, ``g = k // group_size`` and zero points 0 .. 255 (without them 8).  A
 decode step of few rows is bound by the bytes of its weights, and these are a quarter of what 16 bits are.  The reference has weights in 16 bits
 alone (energonai/kernel/cuda_native/linear_func.py:11-32).
 """

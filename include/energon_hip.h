@@ -578,8 +578,8 @@ int en_kv_extend_paged_nodes(const void *k_new, const void *v_new, const int64_t
 
 /* ---- weights in 4 bits ------------------------------------------------------ */
 
-/* A weight [out_features, in_features] in 4 bits: W[n, k] = (code[n, k] - zero[n, k / group]) * scale[n, k / group], codes and zero points
- * 0 .. 15 (without zero points 8), scales of the activations' dtype, groups of 32, 64 or 128 channels.  in_features is a multiple of 8.  It
+/* A weight [out_features, in_features] in 4 bits: W[n, k] = (code[n, k] - zero[n, k / group]) * scale[n, k / group], codes 0 .. 15, zero
+ * points 0 .. 255 (without zero points 8), scales of the activations' dtype, groups of 32, 64 or 128 channels.  in_features is a multiple of 8.  It
  * is laid out once, by en_w4_pack, in tiles of 16 rows and 128 channels as the kernels load them; rows and channels that fill up the last
  * tiles have code 0 and scale 0. */
 typedef struct en_w4_weight {

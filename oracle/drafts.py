@@ -104,7 +104,7 @@ def w4_values(codes, scales, zeros, group):
     N, K = codes.shape[0], 2 * codes.shape[1]
     c = torch.stack((codes & 15, codes >> 4), -1).view(N, K).double()
     s = scales.double().repeat_interleave(group, 1)[:, :K]
-    z = torch.full_like(c, 8.0) if zeros is None else (zeros & 15).double().repeat_interleave(group, 1)[:, :K]
+    z = torch.full_like(c, 8.0) if zeros is None else zeros.double().repeat_interleave(group, 1)[:, :K]
     return (c - z) * s, s.abs() * (c + z)
 
 
