@@ -9,7 +9,8 @@
 //  - Keys and values go through registers into LDS, a tile ahead: what lies behind a sequence's nodes or in no page arrives there as zeros,
 //    so that nothing of another sequence, and no NaN of a page never written, meets a probability of zero.
 //  - The running maximum is raised only where a score passes it by 2^8: the sums are fp32, and probabilities of up to 2^8 are as exact in
-//    16 bits as those below 1.
+//    16 bits as those below 1.  In fp16 the maximum's own probability stands at 2^7, so that others count down to 2^-32 of it: from 1 on
+//    they would end at 2^-25, and over the 10^5 positions of a long cache what is left out would pass half a step of the result.
 // The probabilities are rounded to the cache's 16-bit type for the second product (half a step, 2^-11 or 2^-8 of each; the first product's
 // operands are exact): the matrix instructions take both operands in one type, and in fp32 they are a sixteenth as fast.  The sum of the
 // softmax takes them in fp32.
@@ -31,6 +32,7 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int kNodes = EN_DRAFT_MAX_NODES;
 constexpr float kRaise = 8.f;                 // log2
+template <int DT> constexpr float kTop = DT == EN_F16 ? 7.f : 0.f;      // log2 of the running maximum's probability: 2^(7 + 8) fits fp16
 
 template <int DT> struct Mma;
 template <> struct Mma<EN_F16> {
@@ -380,7 +382,7 @@ __global__ __launch_bounds__(S::kThreads, 2) void tree_attn_kernel(TreeArgs a) {
           for (int n = 0; n < NT; ++n) o[t][n] *= keep;
           m[t] = to;
         }
-        const float base = m[t] > -INFINITY ? m[t] : 0.f;
+        const float base = m[t] > -INFINITY ? m[t] - kTop<DT> : 0.f;
 #pragma unroll
         for (int u = 0; u < kSub; ++u) {
           float e4[4];

@@ -1,4 +1,6 @@
 """Steps of drafted tokens at their edges: rows that are no node's, nodes that no call of the tree has, weights far below the largest."""
+import math
+
 import pytest
 import torch
 
@@ -56,3 +58,29 @@ def test_extension_knows_the_largest_number_of_nodes():
             want[3, :, 4], want[3, :, 5], want[3, :, 7] = new[8], new[7], new[6]    # ... and 3 is none of the sequence's
             assert torch.equal(pool, want)
         assert int(lost) == 0
+
+
+@pytest.mark.parametrize("G", [4, 12, 32])
+def test_weights_far_below_the_largest(G):
+    """fp16: one position whose weight is 2^27 times that of each of 60000 others.  Together they are 4.5e-4 of the result.
+
+    Weights are kept down to 2^-32 of the largest, so each of n others is off by at most that much of it; beside it, half a step of the result, and in
+    the fp32 sums n additions of 2^-24 each of what they add up to."""
+    B, H, D, P, n, dtype = 64, 8, 64, 64, 60000, torch.float16
+    pages = -(-n // P)
+    kp, vp = torch.zeros(pages, H, P, D, dtype=dtype, device="cuda"), torch.ones(pages, H, P, D, dtype=dtype, device="cuda")
+    kp[0, :, 5, 0] = 18.71875
+    vp[0, :, 5] = 0
+    table = torch.arange(pages, dtype=torch.int32, device="cuda").repeat(B, 1)             # all sequences read the same pages: a workgroup has a whole one
+    nodes = 8
+    q = torch.zeros(B * nodes, H * G, D, dtype=dtype, device="cuda")
+    q[:, :, 0] = 1
+    new_k, new_v = torch.zeros(B * nodes, H, D, dtype=dtype, device="cuda"), torch.ones(B * nodes, H, D, dtype=dtype, device="cuda")
+    tree = K().draft_tree(torch.full((B * nodes,), -1, dtype=torch.int32, device="cuda"), [nodes] * B, B, nodes)
+    announce("weights far below the largest", G)
+    got = K().decode_attn_tree(q, new_k, new_v, kp, vp, torch.full((B,), n, dtype=torch.int32, device="cuda"), table, tree, scale=1.0).double()
+    w = n * math.exp(-18.71875)                              # n - 1 positions and the node itself
+    want = w / (1 + w)
+    tolerance = n * 2.0 ** -32 + 2.0 ** -11 * want + 2 * n * 2.0 ** -24 * want
+    assert tolerance < want / 8
+    assert float((got - want).abs().max()) <= tolerance, (float(got.min()), float(got.max()), want)
