@@ -70,16 +70,21 @@ def w4_weight(codes, scales, zeros=None, group_size: int = 128) -> W4Weight:
     return w
 
 
+def check_w4_codes(who: str, weight, group_size: int) -> None:
+    """Raises where ``w4_codes`` has no codes for a weight."""
+    if not isinstance(weight, torch.Tensor) or weight.dim() != 2 or weight.dtype not in _TYPES or weight.shape[1] % 8 or weight.numel() == 0:
+        raise RuntimeError(f"{who}: weight must be a float16 or bfloat16 [dout, din] tensor with din a multiple of 8")
+    if group_size not in _GROUPS:
+        raise RuntimeError(f"{who}: group_size must be one of {_GROUPS}")
+
+
 @torch.no_grad()
 def w4_codes(weight, group_size: int = 128, zero_points: bool = False):
     """``(codes, scales, zeros)`` of a ``[dout, din]`` weight, as ``w4_weight`` takes them, rounded to the nearest.  Without zero points a
     group's largest magnitude is code 0 (-8) or, where it is positive, 15 (7) or nearer to 0, whichever scale leaves the smaller squares; with them
     the group's range, and 0, are its codes 0 and 15.  A group without values has scale 0."""
     who = "w4_codes"
-    if not isinstance(weight, torch.Tensor) or weight.dim() != 2 or weight.dtype not in _TYPES or weight.shape[1] % 8 or weight.numel() == 0:
-        raise RuntimeError(f"{who}: weight must be a float16 or bfloat16 [dout, din] tensor with din a multiple of 8")
-    if group_size not in _GROUPS:
-        raise RuntimeError(f"{who}: group_size must be one of {_GROUPS}")
+    check_w4_codes(who, weight, group_size)
     N, K = weight.shape
     groups = -(-K // group_size)
     w = torch.nn.functional.pad(weight.float(), (0, groups * group_size - K)).view(N, groups, group_size)

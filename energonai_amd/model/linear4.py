@@ -9,7 +9,8 @@ from typing import Optional
 import torch
 from torch import nn
 
-from ..kernel.w4 import W4Weight, linear_w4, w4_codes, w4_weight
+from .. import _lib
+from ..kernel.w4 import W4Weight, check_w4_codes, linear_w4, w4_codes, w4_weight
 
 
 class Linear4(nn.Module):
@@ -39,10 +40,20 @@ class Linear4(nn.Module):
 
 
 def quantize_linears(module: nn.Module, group_size: int = 128, zero_points: bool = False) -> nn.Module:
-    """Replaces every ``torch.nn.Linear`` below ``module`` (fp16 or bf16, on a GPU) by a ``Linear4`` of it, in place; returns ``module``."""
-    for name, child in list(module.named_children()):
-        if type(child) is nn.Linear:
-            setattr(module, name, Linear4.from_linear(child, group_size, zero_points))
-        else:
-            quantize_linears(child, group_size, zero_points)
+    """Replaces every ``torch.nn.Linear`` below ``module`` (fp16 or bf16, on a GPU) by a ``Linear4`` of it, in place; returns ``module``.  One that
+    several modules share, or that has several names, becomes one that they share.  Where one cannot be replaced, none is."""
+    places = {}                 # the layer -> (module, name) of all its places
+    for parent in module.modules():
+        for name, child in parent._modules.items():
+            if type(child) is nn.Linear:
+                places.setdefault(child, []).append((parent, name))
+    for layer in places:
+        check_w4_codes("quantize_linears", layer.weight.detach(), group_size)
+        _lib.require_gpu(layer.weight, "weight", contiguous=False)
+    while places:               # the last one that holds a layer's 16-bit weight lets it go before the next is turned
+        layer, at = places.popitem()
+        small = Linear4.from_linear(layer, group_size, zero_points)
+        for parent, name in at:
+            setattr(parent, name, small)
+        del layer
     return module

@@ -261,3 +261,30 @@ def test_nodes_do_not_keep_what_they_belong_to(turn):
         with pytest.raises(RuntimeError, match="gone on"):
             b.accept_nodes(path, one)
         assert rows() is None
+
+
+@torch.no_grad()
+def test_layers_of_several_names_are_one_layer():
+    """A layer that is there twice is replaced at both places by one; a layer that cannot be replaced leaves all as they were."""
+    from energonai_amd.model import Linear4, quantize_linears
+    shared = torch.nn.Linear(64, 32, dtype=torch.float16, device="cuda")
+    m = torch.nn.Module()
+    m.a, m.b, m.inner = shared, shared, torch.nn.Sequential(shared, torch.nn.ReLU())
+    announce("layers of several names")
+    quantize_linears(m, 32)
+    assert type(m.a) is Linear4 and m.a is m.b is m.inner[0]
+    bad = torch.nn.Sequential(torch.nn.Linear(64, 32, dtype=torch.float16, device="cuda"), torch.nn.Linear(32, 8, dtype=torch.float32, device="cuda"))
+    with pytest.raises(RuntimeError):
+        quantize_linears(bad, 32)
+    assert all(type(layer) is torch.nn.Linear for layer in bad)
+    # a layer's 16-bit weight goes before the next is turned: the most that many layers take is what one takes
+    most = []
+    for n in (1, 24):
+        many = torch.nn.Sequential(*[torch.nn.Linear(2048, 2048, dtype=torch.float16, device="cuda") for _ in range(n)])
+        torch.cuda.synchronize()
+        before = torch.cuda.memory_allocated()
+        torch.cuda.reset_peak_memory_stats()
+        quantize_linears(many, 128)
+        most.append(torch.cuda.max_memory_allocated() - before)
+        assert torch.cuda.memory_allocated() < before
+    assert most[1] <= most[0]
