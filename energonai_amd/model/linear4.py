@@ -50,10 +50,10 @@ def quantize_linears(module: nn.Module, group_size: int = 128, zero_points: bool
     for layer in places:
         check_w4_codes("quantize_linears", layer.weight.detach(), group_size)
         _lib.require_gpu(layer.weight, "weight", contiguous=False)
+    child = None
     while places:               # the last one that holds a layer's 16-bit weight lets it go before the next is turned
         layer, at = places.popitem()
         small = Linear4.from_linear(layer, group_size, zero_points)
         for parent, name in at:
             setattr(parent, name, small)
-        del layer
     return module
