@@ -231,8 +231,9 @@ class PagedKVCache:
         The pages are assigned on the host, which needs the counts there: ``counts_host`` if the caller has them (the layers of a model share
         them), else one copy from the device."""
         counts_host = [int(n) for n in (counts.tolist() if counts_host is None else counts_host)]
-        if len(counts_host) != self.batch_size or min(counts_host, default=0) < 0:
-            raise RuntimeError(f"PagedKVCache.extend: counts must be one for each of the {self.batch_size} sequences")
+        steps = path.shape[1] if isinstance(path, torch.Tensor) and path.dim() == 2 else 0
+        if len(counts_host) != self.batch_size or min(counts_host, default=0) < 0 or max(counts_host, default=0) > steps:
+            raise RuntimeError(f"PagedKVCache.extend: counts must be one for each of the {self.batch_size} sequences, 0 .. {steps}, the path's steps")
         P = self.page_size
         self._assign([(b, (n + m + P - 1) // P) for b, (n, m) in enumerate(zip(self._host_lens, counts_host))])
         kv_pages_extend(k_new, v_new, self.k, self.v, self.info, self.table, tree, path, counts)

@@ -288,3 +288,22 @@ def test_layers_of_several_names_are_one_layer():
         most.append(torch.cuda.max_memory_allocated() - before)
         assert torch.cuda.memory_allocated() < before
     assert most[1] <= most[0]
+
+
+@torch.no_grad()
+def test_counts_past_the_path_are_refused():
+    """Lengths do not go on past the rows that a path has: the positions behind them would hold what the pages held."""
+    from energonai_amd import kernel as K
+    b = _block(torch.float16)
+    b(_prompt([5, 9], torch.float16), first_cache=True, seq_lens=torch.tensor([5, 9], dtype=torch.int32, device="cuda"))
+    tree = K.draft_tree(torch.tensor([-1, 0] * 2, dtype=torch.int32, device="cuda"), [2, 2], 2, 2)
+    announce("counts past the path")
+    b.forward_nodes(torch.randn(1, 4, HID, dtype=torch.float16, device="cuda"), tree)
+    path = torch.tensor([[0, 1], [0, 1]], dtype=torch.int32, device="cuda")
+    cache, pages = b.attn.kv_cache, b.attn.kv_cache.pages_in_use()
+    for counts in ([3, 1], [1, -1], [1]):
+        with pytest.raises(RuntimeError, match="counts"):
+            b.accept_nodes(path, torch.tensor(counts, dtype=torch.int32, device="cuda"))
+    assert cache.lens.tolist() == [5, 9] and cache._host_lens == [5, 9] and cache.pages_in_use() == pages
+    b.accept_nodes(path, torch.tensor([2, 1], dtype=torch.int32, device="cuda"))
+    assert cache.lens.tolist() == [7, 10]
