@@ -17,7 +17,7 @@
 //
 // Few rows a unit are bound by the stream of keys and values, many by exponents and matrix instructions in turn: 24 sequences of up to 4000, 32 / 8
 // heads x 128, up to 64 rows (bf16) 46 us + 6 for the joining launch, 4.8 TB/s; 16 of 500 to 2000, 56 heads x 128, up to 64 rows (fp16) 150 + 15 us, 4.6
-// TB/s; one of 130001, 64 / 8 heads x 128, 504 rows (bf16) 370 + 15 us, 0.72 PFLOP/s.
+// TB/s; one of 130001, 64 / 8 heads x 128, 504 rows (bf16) 370 in all, 15 of them the joining launch, 0.72 PFLOP/s.
 #include <type_traits>
 
 #include "paged_common.hip.h"

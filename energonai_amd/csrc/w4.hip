@@ -10,8 +10,8 @@
 // sums of x from a matrix instruction whose other operand is ones, and no weight is rounded.  For more rows, whose products are bound by the
 // matrix instructions, weights are turned into 16 bits once for all rows of a workgroup (below).
 //
-// us, groups of 128, bf16: 1 x 9216 -> 9216 16.2 (44 MB, 2.7 TB/s), 1 x 7168 -> 28672 25 (106 MB, 4.3 TB/s), 40 x 9216 -> 9216 26;
-// 1000 x 9216 -> 9216 218 (0.78 PFLOP/s), 512 rows of the same 172 (0.51 PFLOP/s: 288 tiles on 256 compute units).
+// us, groups of 128, bf16, weights that no cache holds: 1 x 9216 -> 9216 16 (44 MB, 2.7 TB/s), 1 x 7168 -> 28672 25 (106 MB, 4.3 TB/s), 40 x 9216 ->
+// 9216 26; 1000 x 9216 -> 9216 218 (0.78 PFLOP/s), 512 rows of the same 171 (0.51 PFLOP/s: 288 tiles on 256 compute units).
 #include <type_traits>
 #include <utility>
 
@@ -536,11 +536,11 @@ __global__ __launch_bounds__(S::NW *kWave, 2) void w4_tile_kernel(W4Args a) {
 }
 
 // 256 rows of x times 256 rows of W a workgroup, 64 channels a stage; eight waves, 128 x 64 each.  Bound by the matrix instructions: x goes
-// from memory into LDS as operands lie (a wave's load of 16 rows x 32 channels is one operand, 1 KB), and so do the
-// weights, each turned into 16 bits once for the 256 rows: (code - zero) * scale in fp32, rounded as a weight kept in 16 bits would be
+// straight from memory into LDS (a wave's load of 16 rows x 32 channels is one operand, 1 KB, its vectors in the order of operand_vector), and
+// the weights through registers as operands lie, each turned into 16 bits once for the 256 rows: (code - zero) * scale in fp32, rounded as a weight kept in 16 bits would be
 // (half a step of the activations' type; scaling sums of codes instead takes four multiplications for each four matrix instructions of a
-// group of 32, as many cycles as those themselves).  2000 x 5120 -> 13841, bf16: 0.98 PFLOP/s, of 1.4 that a large product of 16-bit matrices
-// reaches; the rest is the last round of tiles, 440 of them on 256 compute units.
+// group of 32, as many cycles as those themselves).  2000 x 5120 -> 13841, bf16: groups of 128 267 us, 1.06 PFLOP/s, of 32 290, of 32 with zero
+// points, bias and ReLU 298, 0.95 PFLOP/s, of 1.4 that a large product of 16-bit matrices reaches; the rest is the last round of tiles, 440 of them on 256 compute units.
 template <int DT, int GROUP>
 __global__ __launch_bounds__(kManyWaves *kWave, 2) void w4_many_kernel(W4Args a) {
   typedef Elem<DT> E;
@@ -712,13 +712,15 @@ static int check_w4(const en_w4_weight *w) {
   return EN_OK;
 }
 
-// Which kernel, and in how many runs the channels are shared out (a launch more, and the sums through memory).  us, groups of 128, bf16:
-//  - narrow / wide (one tile of W a workgroup, or four, which share the loads of x): 1 x 768 -> 2304 5.3 / 5.9, 64 x 768 -> 2304 6.5 / 9.1, 1 x 4096
-//    -> 4096 5.3 / 8.2, 16 x 4096 -> 4096 6.8 / 9.0; 1 x 9216 -> 9216 18.2 / 16.4, 16 x 9216 -> 9216 30.4 / 17.0, 16 x 7168 -> 28672 54 / 27.5;
-//  - wide, runs 1 / 3 or 4: 16 x 9216 -> 9216 17.0 / 17.7; 40 x 9216 -> 9216 46 / 27, 64 x 9216 -> 9216 48 / 41, 40 x 4096 -> 4096 20.5 / 11.6;
-//    in more they are slower again: 40 x 9216 -> 9216 in 4, 5, 6 33.5, 31.1, 32.2;
-//  - wide / tiles of 128 x 128: 64 x 9216 -> 9216 37 / 41, 128 x 9216 -> 9216 86 / 46;
-//  - tiles of 128 x 128 / of 256 x 256: 512 x 9216 -> 9216 148 / 217, 200 x 7168 -> 28672 146 / 171, 1000 x 9216 -> 9216 257 / 218, 2000 x 5120 -> 13841 374 / 281.
+// Which kernel, and in how many runs the channels are shared out (a launch more, and the sums through memory).  us, groups of 128, bf16, weights that no
+// cache holds, calls in a graph:
+//  - narrow / wide (one tile of W a workgroup, or four, which share the loads of x): 1 x 768 -> 2304 3.1 / 4.2, 64 x 768 -> 2304 5.2 / 9.7, 1 x 4096
+//    -> 4096 5.7 / 8.8, 16 x 4096 -> 4096 6.6 / 9.2; 1 x 9216 -> 9216 19.5 / 16.2, 16 x 9216 -> 9216 24.2 / 17.0, 16 x 7168 -> 28672 42 / 28;
+//  - wide, runs 1 / 3 or 4: 16 x 9216 -> 9216 17.0 / 17.8; 40 x 9216 -> 9216 45 / 26, 64 x 9216 -> 9216 55 / 36, 40 x 4096 -> 4096 21 / 11.7;
+//    in more they are slower again: 40 x 9216 -> 9216 in 4, 5, 6 32.5, 29.8, 31.2;
+//  - wide / tiles of 128 x 128, in the runs of each: 64 x 9216 -> 9216 36 / 38, 128 x 9216 -> 9216 63 / 46;
+//  - tiles of 128 x 128 / of 256 x 256: 512 x 9216 -> 9216 171 / 218, 717 171 / 218, 200 x 7168 -> 28672 137 / 174; 1000 x 9216 -> 9216 256 / 218,
+//    2000 x 5120 -> 13841 334 / 267, in groups of 32 344 / 290.
 enum class W4Form { kNarrow, kWide, kTile, kMany };
 struct W4Plan {
   W4Form form;
