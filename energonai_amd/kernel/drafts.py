@@ -189,7 +189,11 @@ def accept_drafts(logits, tokens, tree):
     """Which nodes a greedy decoding would have chosen: from node 0, which is certain, on, the lowest child whose token has the largest of
     the node's logits (the lowest index of equal ones; NaN counts as the largest), until there is none.  ``logits`` ``[nodes, vocab]``
     with contiguous rows, ``tokens`` int32 or int64 ``[nodes]``.  Returns ``(path, counts, next_tokens)``: int32 ``[B, max_nodes]``, the
-    accepted nodes and -1 behind them; int32 ``[B]``, how many (at least 1; 0 for a sequence without nodes); int64 ``[B]``, the token that follows (-1)."""
+    accepted nodes and -1 behind them; int32 ``[B]``, how many (at least 1; 0 for a sequence without nodes); int64 ``[B]``, the token that follows (-1).
+
+    It is exact for the logits that it is given.  A model's logits of a node differ, within its operators' roundings, from those that a step of single tokens gives:
+    sums go in another order and, with weights in 4 bits, more than 64 rows are multiplied by rounded weights.  Where a row's two largest logits are nearer than
+    that, the two ways of decoding may choose differently."""
     who = "accept_drafts"
     if type(tree) is DraftTree:
         found = _lib.front.accept_drafts(logits, tokens, tree)

@@ -124,8 +124,9 @@ def w4_quantize(weight, group_size: int = 128, zero_points: bool = False) -> W4W
 
 def linear_w4(inputs, weight, bias=None, activation: Optional[str] = None):
     """``linear`` with a weight in 4 bits: ``act(inputs[..., din] @ W[dout, din]^T + bias)`` -> ``[..., dout]``, fp16 or bf16 as the weight's
-    scales are.  Sums are fp32; up to 64 rows no weight is rounded, from there on each is, to the inputs' type.  ``activation``: ``"relu"``, ``"gelu_tanh"`` or ``"gelu"``.  Up to
-    2^20 rows and 2^21 features.  Like the other operators of this package it is for inference: no gradient flows through it."""
+    scales are.  Sums are fp32; up to 64 rows no weight is rounded, from there on each is, to the inputs' type: a row's result differs, within those roundings, with
+    how many rows it comes among, and so may what is chosen from near ties.  Up to 64 rows a row that holds an infinity may give NaN where the formula has an infinity
+    (zero points are taken off the sums).  ``activation``: ``"relu"``, ``"gelu_tanh"`` or ``"gelu"``.  Up to 2^20 rows and 2^21 features.  Like the other operators of this package it is for inference: no gradient flows through it."""
     who = "linear_w4"
     if type(weight) is W4Weight and activation in _ACTIVATIONS:
         y = _lib.front.linear_w4(inputs, weight, bias, _ACTIVATIONS[activation])

@@ -205,7 +205,8 @@ class MultiHeadAttention1D(nn.Module):
     # ---- one step of drafted nodes ------------------------------------------------------------
     def forward_nodes(self, x: torch.Tensor, tree) -> torch.Tensor:
         """``x`` is ``[1,nodes,hid]``: the nodes of a ``kernel.DraftTree``, each sequence's newest token first.  They see the cached positions and
-        the nodes that their masks name.  The cache stays as it is until ``accept_nodes``."""
+        the nodes that their masks name.  The cache stays as it is until ``accept_nodes``, which takes the nodes of one call once: a captured step that is
+        replayed uses the calls of ``kernel`` instead."""
         cache = self.kv_cache
         if cache is None:
             raise RuntimeError("decode step before a first_cache=True call")

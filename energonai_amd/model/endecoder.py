@@ -163,7 +163,8 @@ class Block1D(nn.Module):
 
     def forward_nodes(self, x: torch.Tensor, tree) -> torch.Tensor:
         """One step of drafted nodes, packed ``[1,nodes,hid]`` rows (see ``MultiHeadAttention1D.forward_nodes``); the block's output for
-        each of them.  The padded history of outputs that other calls return has no part in it."""
+        each of them.  The padded history of outputs that ``forward`` returns has no part in it: sequences accept different numbers of nodes.  A ``forward``
+        step afterwards goes on behind the accepted nodes; its last position is the newest, and those before it are the ones that ``forward`` itself computed."""
         return self._rows(x, lambda h: self.attn.forward_nodes(h, tree))
 
     def accept_nodes(self, path: torch.Tensor, counts: torch.Tensor, counts_host=None) -> None:

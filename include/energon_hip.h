@@ -529,7 +529,7 @@ int en_decode_attn_kv8(const void *q, void *ctx, const en_kv8_cache *cache, cons
 #define EN_DRAFT_MAX_NODES 64
 
 /* masks[row]: bit i for node i on the way from the root to the node, itself among them; depths[row]: its steps from the root.  Rows of nodes that
- * do not exist get 0 and 0. */
+ * do not exist, those behind the last sequence among them, get 0 and 0. */
 int en_draft_tree(const int32_t *parents, const int32_t *cu_seqlens, int batch, int64_t nodes, int64_t *masks, int32_t *depths,
                   en_stream_t stream);
 

@@ -307,3 +307,29 @@ def test_counts_past_the_path_are_refused():
     assert cache.lens.tolist() == [5, 9] and cache._host_lens == [5, 9] and cache.pages_in_use() == pages
     b.accept_nodes(path, torch.tensor([2, 1], dtype=torch.int32, device="cuda"))
     assert cache.lens.tolist() == [7, 10]
+
+
+@torch.no_grad()
+def test_single_steps_after_accepted_nodes():
+    """An ordinary step goes on behind the accepted nodes: its newest position is the one that single steps give.  The positions before it are those of
+    the calls that return them: accepted nodes are not among them."""
+    from energonai_amd import kernel as K
+    lens, B, dtype = [17, 5], 2, torch.float16
+    b = _block(dtype)
+    other = copy.deepcopy(b)
+    g = torch.Generator(device="cuda").manual_seed(15)
+    rows, after = (torch.randn(B, n, HID, generator=g, device="cuda", dtype=dtype) for n in (2, 1))
+    lens_d = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    for m in (b, other):
+        m(_prompt(lens, dtype), first_cache=True, seq_lens=lens_d)
+    tree = K.draft_tree(torch.tensor([-1, 0] * B, dtype=torch.int32, device="cuda"), [2] * B, B, 2)
+    announce("single steps after accepted nodes")
+    b.forward_nodes(rows.view(1, -1, HID), tree)
+    b.accept_nodes(torch.tensor([[0, 1]] * B, dtype=torch.int32, device="cuda"), torch.full((B,), 2, dtype=torch.int32, device="cuda"))
+    for i in range(2):
+        other(rows[:, i:i + 1], first_cache=False)
+    got, want = b(after, first_cache=False), other(after, first_cache=False)
+    # both round activations to 16 bits, in other orders of the same sums: a few steps of each
+    assert ((got[:, -1] - want[:, -1]).abs() <= 2 ** -8 * (1 + want[:, -1].abs())).all()
+    assert got.shape[1] == max(lens) + 1 and want.shape[1] == max(lens) + 3
+    assert b.attn.kv_cache.lens.tolist() == other.attn.kv_cache.lens.tolist() == [n + 3 for n in lens]
