@@ -31,9 +31,8 @@ __global__ __launch_bounds__(kWave) void draft_tree_kernel(const int32_t *parent
     masks[first + i] = i < kNodes ? (int64_t)mask : 0;
     depths[first + i] = i < kNodes ? __popcll(mask) - 1 : 0;
   }
-  // the rows behind the last sequence are no nodes either
-  if (b + 1 < (int)gridDim.x) return;
-  for (int64_t i = max(first + (int64_t)nodes, (int64_t)0) + lane; i < total; i += kWave) {
+  // the rows behind the last sequence are no nodes either: all waves' work
+  for (int64_t i = max(cu[gridDim.x], 0) + (int64_t)b * kWave + lane; i < total; i += (int64_t)gridDim.x * kWave) {
     masks[i] = 0;
     depths[i] = 0;
   }
